@@ -170,6 +170,25 @@ def require_operand(t: torch.Tensor, like: torch.Tensor, name: str, numel: Optio
         torch._assert(t.numel() == numel, f"Invalid {name} shape: expected {numel} elements, got {t.numel()}")
 
 
+_ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def element_type(t: torch.Tensor, name: str = "the tensor") -> int:
+    """Code of a tensor's type for the entry points that take rows in float32, bfloat16 or float16."""
+    code = _ELEMENT_TYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+_no_switch = contextlib.nullcontext()
+
+
+def device_of(t: torch.Tensor):
+    """Context in which the device of `t` is the current one (nothing to do, and nothing done, when it is already)."""
+    return _no_switch if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
+
+
 def core() -> ctypes.CDLL:
     """The fixed-function library; (re)built on first use when nvcc is present and a source is newer."""
     global _core
@@ -226,13 +245,34 @@ def core() -> ctypes.CDLL:
         lib.e3b_gate_fwd_channels.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_void_p]
         lib.e3b_gate_bwd_channels.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_void_p]
         lib.e3b_gate_bwd.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p]
+        vp, i64, i, f = c_void_p, c_int64, c_int, c_float
+        lib.e3b_rms_norm_fwd.argtypes = [vp] * 4 + [i, i, f, vp, i64, i, i, vp]
+        lib.e3b_rms_norm_bwd.argtypes = [vp] * 6 + [i, i, i, f, vp, vp, vp, i64, i64, i, i, vp]
+        lib.e3b_norm_scratch_bytes.argtypes = [i64, i]
+        lib.e3b_norm_gate_residual_fwd.argtypes = [vp] * 10 + [i, f, vp, vp, i64, i, vp]
+        lib.e3b_norm_gate_residual_bwd.argtypes = [vp] * 15 + [i, f, vp, vp, vp, vp, i64, i64, i, vp]
+        lib.e3b_distance_buckets.argtypes = [vp] * 5 + [i, i64, i64, vp, vp, vp]
+        lib.e3b_relative_bias_fwd.argtypes = [vp, vp, i, i, i64, i, vp, vp, vp]
+        lib.e3b_relative_bias_scratch_bytes.argtypes = [i64, i, i]
+        lib.e3b_relative_bias_bwd.argtypes = [vp, vp, i, i, i64, i, vp, i, vp, i64, vp, vp]
+        lib.e3b_attention_scratch_bytes.argtypes = [i64, i64, i, i]
+        lib.e3b_attention_fwd.argtypes = [vp] * 3 + [i64] * 3 + [vp] * 5 + [i] + [vp] * 4 + [f, i64, i64, i64, i] + [vp] * 4 + [i64, vp, vp]
+        lib.e3b_attention_bwd_scratch_bytes.argtypes = [i64, i64, i]
+        lib.e3b_attention_bwd.argtypes = [vp] * 4 + [i64] * 3 + [vp] * 7 + [i] + [vp] * 4 + [f, i64, i64, i64, i] + [vp] * 8 + [i64, vp, vp]
+        lib.e3b_attention_bwd_src_scratch_bytes.argtypes = [i64, i64, i, i]
+        lib.e3b_attention_bwd_src.argtypes = [vp] * 2 + [i64] + [vp] * 8 + [f, i64, i64, i64, i] + [vp] * 3 + [i64, vp, vp]
+        for name in ("e3b_norm_scratch_bytes", "e3b_relative_bias_scratch_bytes", "e3b_attention_scratch_bytes",
+                     "e3b_attention_bwd_scratch_bytes", "e3b_attention_bwd_src_scratch_bytes"):
+            getattr(lib, name).restype = i64
         lib.e3b_selftest_bounded_wait.argtypes = [c_void_p, ctypes.c_uint, c_void_p]
         lib.e3b_selftest_bounded_wait.restype = c_int
         for name in ("e3b_sh_fwd", "e3b_sh_bwd", "e3b_csr_from_dst", "e3b_dense_fwd", "e3b_dense_fwd_gate", "e3b_dense_bwd_w", "e3b_dense_bwd_x",
                      "e3b_dense_bwd_x_ordered", "e3b_dense_bwd_x_supported", "e3b_fill_columns",
                      "e3b_radial_embed_fwd", "e3b_radial_embed_bwd", "e3b_radial_embed_bwd_all", "e3b_matmul_tn", "e3b_neighbor_count", "e3b_neighbor_fill",
                      "e3b_neighbor_count_rows", "e3b_neighbor_fill_rows",
-                     "e3b_gate_fwd", "e3b_gate_fwd_channels", "e3b_gate_bwd", "e3b_gate_bwd_channels"):
+                     "e3b_gate_fwd", "e3b_gate_fwd_channels", "e3b_gate_bwd", "e3b_gate_bwd_channels",
+                     "e3b_rms_norm_fwd", "e3b_rms_norm_bwd", "e3b_norm_gate_residual_fwd", "e3b_norm_gate_residual_bwd", "e3b_distance_buckets",
+                     "e3b_relative_bias_fwd", "e3b_relative_bias_bwd", "e3b_attention_fwd", "e3b_attention_bwd", "e3b_attention_bwd_src"):
             getattr(lib, name).restype = c_int
         _core = lib
     return _core

@@ -1,0 +1,251 @@
+// Attention over the incoming edges of every node: gradients along the rows of destinations.
+//
+// With p = softmax(a) (computed again from q, k and the kept maximum and sum), g the cotangent of the output:
+//   dp[e, h] = <g[dst], v[src]>_h     delta[n, h] = <g[n], out[n]>_h     da = p (dp - delta)
+//   grad_q[n] = scale sum_e da k[src]      grad_k = scale da q[dst]      grad_v = p g[dst]      grad bias = da
+// delta is taken from the unrounded fp32 output: dp - delta cancels, and in a row with one edge it is exactly zero.
+// k and v per edge: their gradients are written here, row by row.  k and v per node: p and da of every edge are kept and
+// attention_bwd_src.cu adds the terms of every source over its outgoing edges.  Bound like the forward kernel by the
+// gather of k and v (and by the write of their gradients per edge).
+#include "attention.cuh"
+
+namespace e3b {
+namespace {
+
+struct BwdArgs {
+    const void *q, *k, *v, *grad_out;
+    int64_t q_stride, k_stride, v_stride;
+    const float *out32, *stats;
+    void *grad_q, *grad_k, *grad_v;      // grad_k, grad_v: per edge, or null
+    float *p, *da;                       // [edges, heads] or null
+    int32_t* dst;                        // [edges] or null: destination of every edge
+    float scale;
+    Heads h;
+    Edges e;
+    Rows r;
+    Partials parts;
+};
+
+template <typename T, int VEC, int V, bool MERGE>
+__global__ void __launch_bounds__(256) attn_bwd_dst_kernel(const BwdArgs a) {
+    extern __shared__ float smem[];
+    constexpr int U = edges_in_flight(V, words_of<T, VEC>(), 64);
+    const int lane = threadIdx.x & 31, part = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    const int head = blockIdx.y * (32 / a.h.lanes) + lane / a.h.lanes;
+    const bool live = head < a.h.heads, leads = live && (lane & (a.h.lanes - 1)) == 0;
+    int cq[V], cv[V];
+    lane_columns<V>(a.h.qk, a.h.nqk, a.h.lanes, head, live, cq);
+    lane_columns<V>(a.h.v, a.h.nv, a.h.lanes, head, live, cv);
+    const T* k = static_cast<const T*>(a.k);
+    const T* v = static_cast<const T*>(a.v);
+    Sums<VEC, V, 1, false> s;
+    s.clear();
+    int64_t goes_on = -1;
+    int ended = -1;
+    if (part < a.r.parts) {
+        float qf[V][VEC], gf[V][VEC], delta = 0.0f, top = 0.0f, inv = 0.0f;
+        int row_now = 0;
+        walk_rows(
+            a.r, part,
+            [&](int64_t n) {
+                row_now = static_cast<int>(n);
+                load_row_f<T, VEC, V>(qf, static_cast<const T*>(a.q), n, a.q_stride, cq);
+                load_row_f<T, VEC, V>(gf, static_cast<const T*>(a.grad_out), n, a.h.dv, cv);
+                float d = 0.0f, o[V][VEC];
+                load_row_f<float, VEC, V>(o, a.out32, n, a.h.dv, cv);
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) d = fmaf(gf[j][i], o[j][i], d);
+                delta = head_sum(d, a.h.lanes);
+                if (live) {
+                    top = a.stats[(n * a.h.heads + head) * 2];
+                    inv = a.stats[(n * a.h.heads + head) * 2 + 1];
+                }
+                s.clear();
+            },
+            [&](int64_t first, int64_t last) {
+                for (int64_t base = first; base < last; base += 32) {
+                    EdgeMeta meta;
+                    meta.load(a.e, base + lane, last);
+                    if (a.dst && blockIdx.y == 0 && meta.edge >= 0) a.dst[meta.edge] = row_now;
+                    const int count = static_cast<int>(min(last - base, int64_t{32}));
+                    for (int u0 = 0; u0 < count; u0 += U) {
+                        Packed<T, VEC> kk[U][V], vv[U][V];
+                        float bias[U];
+                        int edge[U];
+                        bool use[U];
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {
+                            const int row = __shfl_sync(kAll, meta.row, u0 + u);
+                            edge[u] = __shfl_sync(kAll, meta.edge, u0 + u);
+                            use[u] = row >= 0;
+                            bias[u] = 0.0f;
+                            if (a.e.buckets) {
+                                const int b = __shfl_sync(kAll, meta.bucket, u0 + u);
+                                if (live) bias[u] = a.e.bias[b * a.h.heads + head];
+                            } else if (a.e.bias) {
+                                if (live && edge[u] >= 0) bias[u] = a.e.bias[static_cast<int64_t>(edge[u]) * a.h.heads + head];
+                                use[u] = use[u] && bias[u] != -INFINITY;
+                            }
+                            load_row<T, VEC, V>(kk[u], k, row, a.k_stride, cq, use[u]);
+                            load_row<T, VEC, V>(vv[u], v, row, a.v_stride, cv, use[u]);
+                        }
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {
+                            float d = 0.0f, dp = 0.0f, kf[V][VEC];
+#pragma unroll
+                            for (int j = 0; j < V; ++j) {
+                                float vf[VEC];
+                                kk[u][j].unpack(kf[j]);
+                                vv[u][j].unpack(vf);
+#pragma unroll
+                                for (int i = 0; i < VEC; ++i) {
+                                    d = fmaf(qf[j][i], kf[j][i], d);
+                                    dp = fmaf(gf[j][i], vf[i], dp);
+                                }
+                            }
+                            const float x = logit(head_sum(d, a.h.lanes), a.scale, bias[u], a.e.weight ? __shfl_sync(kAll, meta.log_weight, u0 + u) : 0.0f);
+                            dp = head_sum(dp, a.h.lanes);
+                            float p = 0.0f, da = 0.0f;
+                            if (use[u]) {
+                                p = __expf(x - top) * inv;
+                                da = p == 0.0f ? 0.0f : p * (dp - delta);
+                            }
+#pragma unroll
+                            for (int j = 0; j < V; ++j)
+#pragma unroll
+                                for (int i = 0; i < VEC; ++i) s.a[0][j][i] = fmaf(da, kf[j][i], s.a[0][j][i]);
+                            if (edge[u] < 0) continue;
+                            if (leads && a.p) a.p[static_cast<int64_t>(edge[u]) * a.h.heads + head] = p;
+                            if (leads && a.da) a.da[static_cast<int64_t>(edge[u]) * a.h.heads + head] = da;
+                            if (a.grad_k) {
+                                store_row<T, VEC, V>(static_cast<T*>(a.grad_k), edge[u], a.h.dqk, cq, qf, a.scale * da);
+                                store_row<T, VEC, V>(static_cast<T*>(a.grad_v), edge[u], a.h.dv, cv, gf, p);
+                            }
+                        }
+                    }
+                }
+            },
+            [&](int64_t n, bool started, bool ends) {
+                if (!ends) {
+                    goes_on = n;
+                } else if (started) {
+                    if (a.grad_q) store_row<T, VEC, V>(static_cast<T*>(a.grad_q), n, a.h.dqk, cq, s.a[0], a.scale);
+                } else {
+                    s.save(a.parts.at(part, 0), a.h, cq, cv, head, leads);
+                    ended = static_cast<int>(n);
+                }
+            },
+            // slots behind the last row take part in nothing: their gradients are zero
+            [&](int64_t first, int64_t last) {
+                float zero[V][VEC];
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) zero[j][i] = 0.0f;
+                for (int64_t slot = max(first, int64_t{0}); slot < min(last, a.r.edges); ++slot) {
+                    const int64_t e = a.e.perm ? a.e.perm[slot] : slot;
+                    if (e < 0 || e >= a.e.edges) continue;
+                    if (a.dst && blockIdx.y == 0 && lane == 0) a.dst[e] = -1;
+                    if (leads && a.p) a.p[e * a.h.heads + head] = 0.0f;
+                    if (leads && a.da) a.da[e * a.h.heads + head] = 0.0f;
+                    if (a.grad_k) {
+                        store_row<T, VEC, V>(static_cast<T*>(a.grad_k), e, a.h.dqk, cq, zero, 0.0f);
+                        store_row<T, VEC, V>(static_cast<T*>(a.grad_v), e, a.h.dv, cv, zero, 0.0f);
+                    }
+                }
+            });
+        if (blockIdx.y == 0 && lane == 0) a.parts.ended[part] = ended;
+    }
+    leave_part<MERGE>(s, goes_on, part, a.r.parts, a.parts, a.h, cq, cv, head, leads, smem);
+}
+
+template <typename T, int VEC, int V>
+__global__ void __launch_bounds__(256) attn_bwd_dst_join_kernel(const BwdArgs a) {
+    extern __shared__ float smem[];
+    const int lane = threadIdx.x & 31;
+    const int head = blockIdx.y * (32 / a.h.lanes) + lane / a.h.lanes;
+    const bool live = head < a.h.heads;
+    int cq[V];
+    lane_columns<V>(a.h.qk, a.h.nqk, a.h.lanes, head, live, cq);
+    Sums<VEC, V, 1, false> s;
+    int64_t n;
+    if (join_parts(s, a.r, blockIdx.x, a.parts, a.h, cq, cq, head, live, smem, &n)) store_row<T, VEC, V>(static_cast<T*>(a.grad_q), n, a.h.dqk, cq, s.a[0], a.scale);
+}
+
+// Gradient of the weight of every edge: share / weight = exp(logit without it) / sum, so it is sum_h da / weight; an edge that was
+// left out has none.
+__global__ void __launch_bounds__(256) attn_weight_grad_kernel(const float* __restrict__ da, const float* __restrict__ weight, int heads,
+                                                               int64_t edges, float* __restrict__ grad) {
+    for (int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; e < edges; e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+        const float w = weight[e];
+        float s = 0.0f;
+        for (int h = 0; h < heads; ++h) s += da[e * heads + h];
+        grad[e] = w <= 0.0f || s == 0.0f ? 0.0f : s / w;      // (s = 0: also an edge of no row, whatever its weight)
+    }
+}
+
+int dq_slot(int dqk) { return static_cast<int>(ceil_div(dqk, 4) * 4); }
+
+}  // namespace
+}  // namespace e3b
+
+using namespace e3b;
+
+extern "C" int64_t e3b_attention_bwd_scratch_bytes(int64_t num_dst, int64_t num_edges, int dim_qk) {
+    if (num_dst < 0 || num_edges < 0) return 0;
+    return partial_bytes(split_rows(num_dst, num_edges).parts, dq_slot(dim_qk));
+}
+
+extern "C" int e3b_attention_bwd(const void* q, const void* k, const void* v, const void* grad_out, int64_t q_stride, int64_t k_stride,
+                                 int64_t v_stride, const float* out32, const float* stats, const int64_t* rowptr, const int64_t* perm,
+                                 const int64_t* edge_src, const float* bias, const int32_t* buckets, int num_buckets,
+                                 const float* edge_weight, const int32_t* qk_table, const int32_t* v_table, const int32_t* layout,
+                                 float scale, int64_t num_dst, int64_t num_src, int64_t num_edges, int type, void* grad_q, void* grad_k,
+                                 void* grad_v, float* share, float* grad_logit, int32_t* edge_dst, float* grad_weight, void* scratch,
+                                 int64_t scratch_bytes, int32_t* status, void* stream) {
+    if (!layout || num_dst < 0 || num_src < 0 || num_edges < 0 || num_edges >= INT32_MAX || num_dst >= INT32_MAX || num_src >= INT32_MAX || !known_type(type))
+        return fail(E3B_ERR_ARG, "attention_bwd: bad size or type");
+    const int vec = layout[0], heads = layout[1], nqk = layout[2], nv = layout[3], dqk = layout[4], dv = layout[5];
+    if (heads < 1 || (vec != 1 && vec != 4)) return fail(E3B_ERR_ARG, "attention_bwd: bad head layout");
+    const int most = vec == 4 ? 8 : 32, lanes = lanes_of_head(heads, std::max(nqk, nv), most);
+    if (lanes == 0) return fail(E3B_ERR_UNSUPPORTED, "attention_bwd: a head of %d columns (at most 1024)", vec * std::max(nqk, nv));
+    if (num_dst == 0 && num_edges == 0) return E3B_OK;
+    const Split s = split_rows(num_dst, num_edges);
+    if ((num_dst > 0 && (!q || !grad_out || !out32 || !stats || !grad_q)) || !rowptr || (num_edges > 0 && num_src > 0 && (!k || !v)) || !qk_table ||
+        !v_table || !scratch || !status || (buckets && !bias) || !grad_k != !grad_v || (grad_weight && (!edge_weight || !grad_logit)))
+        return fail(E3B_ERR_ARG, "attention_bwd: null pointer");
+    if (scratch_bytes < e3b_attention_bwd_scratch_bytes(num_dst, num_edges, dqk))
+        return fail(E3B_ERR_ARG, "attention_bwd: scratch of %lld bytes is too small", static_cast<long long>(scratch_bytes));
+    BwdArgs a{q, k, v, grad_out, q_stride, k_stride, v_stride, out32, stats, grad_q, grad_k, grad_v, share, grad_logit, edge_dst, scale,
+              {qk_table, v_table, heads, nqk, nv, dqk, dv, lanes},
+              {perm, edge_src, bias, buckets, edge_weight, num_buckets, num_src, num_edges, status},
+              {rowptr, num_dst, num_edges, s.per_part, s.parts}, partials_in(scratch, s.parts, dq_slot(dqk))};
+    const int groups = static_cast<int>(ceil_div(heads, 32 / lanes));
+    const int v_lane = compiled_vectors(vec, static_cast<int>(ceil_div(std::max(nqk, nv), lanes)));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int rc = by_type_and_vectors(type, vec, v_lane, [&](auto t0, auto vec0, auto v0) -> int {
+        using T = decltype(t0);
+        constexpr int VEC = decltype(vec0)::value, V = decltype(v0)::value;
+        using S = Sums<VEC, V, 1, false>;
+        const dim3 grid(static_cast<unsigned>(ceil_div(s.parts, s.warps)), groups);
+        int r = E3B_OK;
+        if (s.merge) {
+            const size_t smem = sizeof(float) * 32 * S::kFloats * s.warps;
+            if ((r = allow_smem(attn_bwd_dst_kernel<T, VEC, V, true>, smem)) != E3B_OK) return r;
+            attn_bwd_dst_kernel<T, VEC, V, true><<<grid, 32 * s.warps, smem, st>>>(a);
+        } else {
+            attn_bwd_dst_kernel<T, VEC, V, false><<<grid, 32 * s.warps, 0, st>>>(a);
+        }
+        if ((r = check_launch("attention_bwd")) != E3B_OK || s.parts == 1) return r;
+        const size_t smem = s.join_warps > 1 ? sizeof(float) * 32 * S::kFloats * s.join_warps : 0;
+        if ((r = allow_smem(attn_bwd_dst_join_kernel<T, VEC, V>, smem)) != E3B_OK) return r;
+        attn_bwd_dst_join_kernel<T, VEC, V><<<dim3(s.parts, groups), 32 * s.join_warps, smem, st>>>(a);
+        return check_launch("attention_bwd join");
+    });
+    if (rc != E3B_OK || !grad_weight || num_edges == 0) return rc;
+    attn_weight_grad_kernel<<<static_cast<unsigned>(std::min<int64_t>(ceil_div(num_edges, 256), kNumSMs * 8)), 256, 0, st>>>(
+        grad_logit, edge_weight, heads, num_edges, grad_weight);
+    return check_launch("attention_bwd weights");
+}

@@ -1,0 +1,246 @@
+// Learned bias by distance buckets (the relative position bias of attention, on distances of atoms).
+//
+//   bucket[e] = number of thresholds t_i with t_i <= |pos[src[e]] - pos[dst[e]] + shift[e]|
+//   bias[e, h] = table[bucket[e], h];     grad_table[b, h] = sum over the edges of bucket b of grad[e, h]
+//
+// Buckets: squared distances and squared thresholds are compared in fp64, where the fp32 inputs and their differences are
+// exact to 2^-53, so that a distance next to a border falls on the side that it is on.  Bound by HBM (28 bytes of edge data in,
+// 4 out; the positions come from L2).
+// Bias: bound by the write of 4 H bytes an edge (2 H in 16 bits).
+// Gradient: every thread keeps one head and walks edges of its own; it adds into a table that it shares with no other
+// thread's (head, slice), so the order of the additions is fixed by the grid; slices, then thread blocks, are added in
+// order.  No atomics.
+#include <algorithm>
+
+#include "common.cuh"
+#include "typed.cuh"
+
+namespace e3b {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxBuckets = 1024;
+
+__global__ void __launch_bounds__(kThreads) distance_buckets_kernel(const float* __restrict__ pos, const int64_t* __restrict__ src,
+                                                                    const int64_t* __restrict__ dst, const float* __restrict__ shift,
+                                                                    const double* __restrict__ thresholds2, int num, int64_t edges,
+                                                                    int64_t nodes, int32_t* __restrict__ buckets, int32_t* status) {
+    __shared__ double t2[kMaxBuckets];
+    for (int i = threadIdx.x; i < num; i += kThreads) t2[i] = thresholds2[i];
+    __syncthreads();
+    for (int64_t e = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; e < edges; e += static_cast<int64_t>(gridDim.x) * kThreads) {
+        const int64_t a = src[e], b = dst[e];
+        if (a < 0 || a >= nodes || b < 0 || b >= nodes) {
+            *status = 2;
+            buckets[e] = 0;
+            continue;
+        }
+        double r2 = 0.0;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            double d = static_cast<double>(pos[3 * a + i]) - static_cast<double>(pos[3 * b + i]);
+            if (shift) d += static_cast<double>(shift[3 * e + i]);
+            r2 = __dadd_rn(r2, __dmul_rn(d, d));
+        }
+        int lo = 0, hi = num;                       // thresholds below lo are <= r, from hi on they are > r
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (t2[mid] <= r2) lo = mid + 1; else hi = mid;
+        }
+        buckets[e] = lo;
+    }
+}
+
+// Four outputs of the flat [edges * heads] array a thread.  RAW: the elements are copied as they are.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads) bias_fwd_kernel(const T* __restrict__ table, const int32_t* __restrict__ buckets, int num_buckets,
+                                                            int heads, int64_t total, T* __restrict__ out, int32_t* status) {
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * kThreads * VEC;
+    for (int64_t i0 = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * VEC; i0 < total; i0 += stride) {
+        float v[VEC];
+        int64_t e = i0 / heads;
+        int h = static_cast<int>(i0 - e * heads);
+        int b = buckets[e];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            if (i > 0 && ++h == heads) {
+                h = 0;
+                ++e;
+                if (i0 + i < total) b = buckets[e];
+            }
+            const bool ok = b >= 0 && b < num_buckets;
+            if (!ok && i0 + i < total) *status = 2;
+            v[i] = ok ? to_float(table[b * heads + h]) : 0.0f;
+        }
+        if (VEC == 1 || i0 + VEC <= total) {
+            Packed<T, VEC>::store(out + i0, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+                if (i0 + i < total) out[i0 + i] = from_float<T>(v[i]);
+        }
+    }
+}
+
+// Thread t of a block: head h0 + t % width, slice t / width; its block's edges in turns of `slices`.
+// Shared memory: [slices][num_buckets][width].
+template <typename T>
+__global__ void bias_bwd_kernel(const T* __restrict__ grad, const int32_t* __restrict__ buckets, int num_buckets, int heads, int width,
+                                int slices, int64_t edges, int64_t edges_per_block, float* __restrict__ partial, int32_t* status) {
+    extern __shared__ float acc[];
+    const int h = threadIdx.x % width, slice = threadIdx.x / width, head = blockIdx.y * width + h;
+    const int cells = num_buckets * width;
+    for (int i = threadIdx.x; i < slices * cells; i += blockDim.x) acc[i] = 0.0f;
+    __syncthreads();
+    const int64_t begin = static_cast<int64_t>(blockIdx.x) * edges_per_block, end = min(begin + edges_per_block, edges);
+    if (head < heads && slice < slices) {
+        float* mine = acc + slice * cells + h;
+        constexpr int U = 8;       // loads in flight a thread
+        for (int64_t e0 = begin + slice; e0 < end; e0 += U * slices) {
+            int b[U];
+            float g[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t e = e0 + u * slices;
+                b[u] = -1;
+                if (e >= end) continue;
+                b[u] = buckets[e];
+                g[u] = to_float(grad[e * heads + head]);
+                if (b[u] < 0 || b[u] >= num_buckets) { *status = 2; b[u] = -1; }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (b[u] >= 0) mine[b[u] * width] += g[u];
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < cells; i += blockDim.x) {
+        const int b = i / width, hh = i % width;
+        if (blockIdx.y * width + hh >= heads) continue;
+        float s = 0.0f;
+        for (int k = 0; k < slices; ++k) s += acc[k * cells + i];
+        partial[(static_cast<int64_t>(blockIdx.x) * num_buckets + b) * heads + blockIdx.y * width + hh] = s;
+    }
+}
+
+// 32 cells a block, 32 slices of the thread blocks' partial tables.
+template <typename T>
+__global__ void __launch_bounds__(1024) bias_sum_kernel(const float* __restrict__ partial, int cells, int parts, T* __restrict__ out) {
+    __shared__ float s[32][33];
+    const int i = blockIdx.x * 32 + threadIdx.x;
+    float a = 0.0f;
+    if (i < cells) {
+#pragma unroll 4
+        for (int p = threadIdx.y; p < parts; p += 32) a += partial[static_cast<int64_t>(p) * cells + i];
+    }
+    s[threadIdx.x][threadIdx.y] = a;
+    __syncthreads();
+    const float t = warp_sum(s[threadIdx.y][threadIdx.x]);
+    const int cell = blockIdx.x * 32 + threadIdx.y;
+    if (threadIdx.x == 0 && cell < cells) out[cell] = from_float<T>(t);
+}
+
+// How the table gradient is split: heads a block takes, slices of its edges, thread blocks.
+struct BiasSplit {
+    int width, slices, groups, parts;
+    int64_t per_block;
+    size_t smem;
+};
+BiasSplit bias_split(int64_t edges, int heads, int num_buckets) {
+    BiasSplit s;
+    s.width = std::min(heads, 32);
+    constexpr size_t kMostSmem = 200 * 1024;
+    while (s.width > 1 && sizeof(float) * num_buckets * s.width > kMostSmem) s.width = (s.width + 1) / 2;
+    const size_t table = sizeof(float) * num_buckets * s.width;
+    s.slices = static_cast<int>(std::max<size_t>(1, std::min<size_t>(kThreads / s.width, 64 * 1024 / table)));
+    s.groups = (heads + s.width - 1) / s.width;
+    s.smem = table * s.slices;
+    const int resident = static_cast<int>(std::max<size_t>(1, std::min<size_t>(8, kMostSmem / s.smem)));
+    // a block clears, sums and writes a table: it takes at least a few edges for every cell of it
+    const int64_t least = std::max<int64_t>(8 * s.slices, num_buckets);
+    s.parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ceil_div(edges, least), std::max(1, kNumSMs * resident / s.groups))));
+    s.per_block = ceil_div(std::max<int64_t>(edges, 1), s.parts);
+    return s;
+}
+
+int flat_grid(int64_t items) { return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ceil_div(items, kThreads), kNumSMs * 16))); }
+
+template <typename T>
+int bias_fwd(const void* table, const int32_t* buckets, int num_buckets, int heads, int64_t edges, void* out, int32_t* status, cudaStream_t st) {
+    const int64_t total = edges * heads;
+    const bool v4 = aligned_to(out, 4 * sizeof(T));
+    const T* tab = static_cast<const T*>(table);
+    T* o = static_cast<T*>(out);
+    if (v4) bias_fwd_kernel<T, 4><<<flat_grid(ceil_div(total, 4)), kThreads, 0, st>>>(tab, buckets, num_buckets, heads, total, o, status);
+    else bias_fwd_kernel<T, 1><<<flat_grid(total), kThreads, 0, st>>>(tab, buckets, num_buckets, heads, total, o, status);
+    return check_launch("relative_bias_fwd");
+}
+
+template <typename T>
+int bias_bwd(const void* grad, const int32_t* buckets, int num_buckets, int heads, int64_t edges, void* grad_table, float* partial,
+             int table_type, int32_t* status, cudaStream_t st) {
+    const BiasSplit s = bias_split(edges, heads, num_buckets);
+    if (s.smem > 48 * 1024) E3B_CUDA_TRY(cudaFuncSetAttribute(bias_bwd_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(s.smem)));
+    bias_bwd_kernel<T><<<dim3(s.parts, s.groups), s.width * s.slices, s.smem, st>>>(static_cast<const T*>(grad), buckets, num_buckets, heads, s.width,
+                                                                                   s.slices, edges, s.per_block, partial, status);
+    const int rc = check_launch("relative_bias_bwd");
+    if (rc != E3B_OK) return rc;
+    const int cells = num_buckets * heads;
+    const dim3 block(32, 32);
+    const int grid = (cells + 31) / 32;
+    if (table_type == kFloat32) bias_sum_kernel<<<grid, block, 0, st>>>(partial, cells, s.parts, static_cast<float*>(grad_table));
+    else if (table_type == kBFloat16) bias_sum_kernel<<<grid, block, 0, st>>>(partial, cells, s.parts, static_cast<__nv_bfloat16*>(grad_table));
+    else bias_sum_kernel<<<grid, block, 0, st>>>(partial, cells, s.parts, static_cast<__half*>(grad_table));
+    return check_launch("relative_bias_bwd sums");
+}
+
+}  // namespace
+}  // namespace e3b
+
+using namespace e3b;
+
+extern "C" int e3b_distance_buckets(const float* pos, const int64_t* edge_src, const int64_t* edge_dst, const float* shift,
+                                    const double* thresholds_squared, int num_thresholds, int64_t num_edges, int64_t num_nodes,
+                                    int32_t* buckets, int32_t* status, void* stream) {
+    if (num_edges < 0 || num_nodes < 0 || num_thresholds < 0 || num_thresholds >= kMaxBuckets) return fail(E3B_ERR_ARG, "distance_buckets: bad size");
+    if (num_edges == 0) return E3B_OK;
+    if ((num_nodes > 0 && !pos) || !edge_src || !edge_dst || (num_thresholds > 0 && !thresholds_squared) || !buckets || !status)
+        return fail(E3B_ERR_ARG, "distance_buckets: null pointer");
+    distance_buckets_kernel<<<flat_grid(num_edges), kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+        pos, edge_src, edge_dst, shift, thresholds_squared, num_thresholds, num_edges, num_nodes, buckets, status);
+    return check_launch("distance_buckets");
+}
+
+extern "C" int e3b_relative_bias_fwd(const void* table, const int32_t* buckets, int num_buckets, int num_heads, int64_t num_edges, int type,
+                                     void* bias, int32_t* status, void* stream) {
+    if (num_edges < 0 || num_buckets < 1 || num_buckets > kMaxBuckets || num_heads < 1 || !known_type(type)) return fail(E3B_ERR_ARG, "relative_bias_fwd: bad size or type");
+    if (num_edges == 0) return E3B_OK;
+    if (!table || !buckets || !bias || !status) return fail(E3B_ERR_ARG, "relative_bias_fwd: null pointer");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (type == kFloat32) return bias_fwd<float>(table, buckets, num_buckets, num_heads, num_edges, bias, status, st);
+    if (type == kBFloat16) return bias_fwd<__nv_bfloat16>(table, buckets, num_buckets, num_heads, num_edges, bias, status, st);
+    return bias_fwd<__half>(table, buckets, num_buckets, num_heads, num_edges, bias, status, st);
+}
+
+extern "C" int64_t e3b_relative_bias_scratch_bytes(int64_t num_edges, int num_buckets, int num_heads) {
+    if (num_edges < 0 || num_buckets < 1 || num_buckets > kMaxBuckets || num_heads < 1) return 0;
+    return sizeof(float) * static_cast<int64_t>(bias_split(num_edges, num_heads, num_buckets).parts) * num_buckets * num_heads;
+}
+
+extern "C" int e3b_relative_bias_bwd(const void* grad_bias, const int32_t* buckets, int num_buckets, int num_heads, int64_t num_edges, int type,
+                                     void* grad_table, int table_type, void* scratch, int64_t scratch_bytes, int32_t* status, void* stream) {
+    if (num_edges < 0 || num_buckets < 1 || num_buckets > kMaxBuckets || num_heads < 1 || !known_type(type) || !known_type(table_type))
+        return fail(E3B_ERR_ARG, "relative_bias_bwd: bad size or type");
+    if (!grad_table) return fail(E3B_ERR_ARG, "relative_bias_bwd: null pointer");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (num_edges == 0) {
+        E3B_CUDA_TRY(cudaMemsetAsync(grad_table, 0, static_cast<size_t>(element_size(table_type)) * num_buckets * num_heads, st));
+        return E3B_OK;
+    }
+    if (!grad_bias || !buckets || !scratch || !status) return fail(E3B_ERR_ARG, "relative_bias_bwd: null pointer");
+    if (scratch_bytes < e3b_relative_bias_scratch_bytes(num_edges, num_buckets, num_heads)) return fail(E3B_ERR_ARG, "relative_bias_bwd: scratch of %lld bytes is too small", static_cast<long long>(scratch_bytes));
+    float* partial = static_cast<float*>(scratch);
+    if (type == kFloat32) return bias_bwd<float>(grad_bias, buckets, num_buckets, num_heads, num_edges, grad_table, partial, table_type, status, st);
+    if (type == kBFloat16) return bias_bwd<__nv_bfloat16>(grad_bias, buckets, num_buckets, num_heads, num_edges, grad_table, partial, table_type, status, st);
+    return bias_bwd<__half>(grad_bias, buckets, num_buckets, num_heads, num_edges, grad_table, partial, table_type, status, st);
+}

@@ -1,0 +1,75 @@
+// Rows stored as fp32, bf16 or fp16 and computed in fp32: vector loads and stores, warp and block sums in a fixed order.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+namespace e3b {
+
+enum DataType { kFloat32 = 0, kBFloat16 = 1, kFloat16 = 2 };   // codes of the C entry points
+
+template <typename T> struct Pair;
+template <> struct Pair<__nv_bfloat16> {
+    static __device__ __forceinline__ float2 load(uint32_t u) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u)); }
+    static __device__ __forceinline__ uint32_t store(float a, float b) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+};
+template <> struct Pair<__half> {
+    static __device__ __forceinline__ float2 load(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+    static __device__ __forceinline__ uint32_t store(float a, float b) {
+        const __half2 v = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+};
+
+template <typename T> __device__ __forceinline__ float to_float(T v) { return static_cast<float>(v); }
+template <typename T> __device__ __forceinline__ T from_float(float v) { return T(v); }
+
+// VEC consecutive elements as they lie in memory (one load), and their fp32 values.
+template <typename T, int VEC> struct Packed;
+template <typename T> struct Packed<T, 1> {
+    T v;
+    __device__ __forceinline__ void load(const T* p) { v = *p; }
+    __device__ __forceinline__ void zero() { v = from_float<T>(0.0f); }
+    __device__ __forceinline__ void unpack(float* f) const { f[0] = to_float(v); }
+    static __device__ __forceinline__ void store(T* p, const float* f) { *p = from_float<T>(f[0]); }
+};
+template <> struct Packed<float, 4> {
+    float4 v;
+    __device__ __forceinline__ void load(const float* p) { v = *reinterpret_cast<const float4*>(p); }
+    __device__ __forceinline__ void zero() { v = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
+    __device__ __forceinline__ void unpack(float* f) const { f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
+    static __device__ __forceinline__ void store(float* p, const float* f) { *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]); }
+};
+template <typename T> struct Packed<T, 4> {
+    uint2 v;
+    __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint2*>(p); }
+    __device__ __forceinline__ void zero() { v = make_uint2(0u, 0u); }
+    __device__ __forceinline__ void unpack(float* f) const {
+        const float2 a = Pair<T>::load(v.x), b = Pair<T>::load(v.y);
+        f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
+    }
+    static __device__ __forceinline__ void store(T* p, const float* f) {
+        *reinterpret_cast<uint2*>(p) = make_uint2(Pair<T>::store(f[0], f[1]), Pair<T>::store(f[2], f[3]));
+    }
+};
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+template <int N> using Int = std::integral_constant<int, N>;   // a size handed to a generic lambda
+
+inline int element_size(int type) { return type == kFloat32 ? 4 : 2; }
+inline bool known_type(int type) { return type >= kFloat32 && type <= kFloat16; }
+// Whether vectors of `bytes` bytes may start at p.
+inline bool aligned_to(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+}  // namespace e3b

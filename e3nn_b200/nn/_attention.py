@@ -1,0 +1,257 @@
+"""Multi-head softmax attention over the incoming edges of every node, on irreps features.
+
+The attention of the reference's transformer example (``docs/guide/transformer.rst``: ``exp = cutoff * exp(dot(q, k))``,
+``alpha = exp / scatter(exp)``, ``scatter(alpha * v)``) as one pass over a destination-sorted CSR.  The dot product of two rows of
+irreps is invariant, so the shares are scalars and the output transforms like the values.
+"""
+from __future__ import annotations
+
+from typing import List, Optional, Tuple
+
+import ctypes
+
+import torch
+
+from .. import _lib
+from ..message_passing import csr_from_dst
+from ..o3 import Irreps, Linear
+from ._gate import Gate
+from ._norm import NormGateResidual
+from ._relative_bias import bias_table_grad
+
+MAX_HEAD_COLUMNS = 1024
+
+
+def _head_vectors(irreps: Irreps, heads: int, vec: int) -> torch.Tensor:
+    """``{column of head 0, columns from one head to the next}`` of every vector of ``vec`` columns of a head."""
+    out: List[Tuple[int, int]] = []
+    at = 0
+    for mul, ir in irreps:
+        run = mul // heads * ir.dim
+        out += [(at + c, run) for c in range(0, run, vec)]
+        at += mul * ir.dim
+    return torch.tensor(out, dtype=torch.int32).reshape(-1, 2)
+
+
+def _fits_fours(t: torch.Tensor) -> bool:
+    return t.data_ptr() % (4 * t.element_size()) == 0 and t.stride(0) % 4 == 0
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """Rows may lie apart (a slice of a wider tensor, an expanded row); their columns may not."""
+    return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
+
+
+class _Call:
+    """Everything of a call that is not differentiated."""
+
+    __slots__ = ("vec", "layout", "qk_tbl", "v_tbl", "scale", "rowptr", "perm", "src", "buckets", "transpose", "edges")
+
+
+class _AttentionFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, bias, weight, c, train):
+        N, (H, dv), dev, type_code = q.shape[0], (c.layout[1], c.layout[5]), q.device, _lib.element_type(q)
+        core = _lib.core()
+        out = torch.empty(N, dv, dtype=q.dtype, device=dev)
+        out32 = stats = None
+        if train:
+            stats = torch.empty(N, H, 2, dtype=torch.float32, device=dev)
+            out32 = torch.empty(N, dv, dtype=torch.float32, device=dev) if q.dtype != torch.float32 else None
+        nbytes = core.e3b_attention_scratch_bytes(N, c.edges, H, dv)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        with _lib.device_of(q), _lib.nvtx_range("e3b_attention_fwd"):
+            rc = core.e3b_attention_fwd(
+                _lib._ptr(q), _lib._ptr(k), _lib._ptr(v), q.stride(0), k.stride(0), v.stride(0), _lib._ptr(c.rowptr), _lib._ptr(c.perm), _lib._ptr(c.src),
+                _lib._ptr(bias), _lib._ptr(c.buckets), bias.shape[0] if c.buckets is not None else 0, _lib._ptr(weight), _lib._ptr(c.qk_tbl),
+                _lib._ptr(c.v_tbl), c.layout, c.scale, N, k.shape[0], c.edges, type_code, _lib._ptr(out), _lib._ptr(out32), _lib._ptr(stats),
+                _lib._ptr(scratch), nbytes, _lib._ptr(_lib.status_word(dev)), _lib.stream_ptr())
+        _lib.check(rc, "e3b_attention_fwd")
+        if train:
+            ctx.save_for_backward(q, k, v, bias, weight, out32 if out32 is not None else out, stats)
+            ctx.call = c
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        q, k, v, bias, weight, out32, stats = ctx.saved_tensors
+        c = ctx.call
+        _, H, _, _, dqk, dv = list(c.layout)
+        N, S, E, dev, type_code, core = q.shape[0], k.shape[0], c.edges, q.device, _lib.element_type(q), _lib.core()
+        _, need_k, need_v, need_bias, need_weight = ctx.needs_input_grad[:5]
+        grad = grad.contiguous()
+        if c.vec == 4 and not _fits_fours(grad):
+            grad = grad.clone()
+        per_node = c.src is not None and (need_k or need_v)
+        per_edge = c.src is None and (need_k or need_v)
+        gq = torch.empty(N, dqk, dtype=q.dtype, device=dev)
+        gk = torch.empty(S, dqk, dtype=q.dtype, device=dev) if need_k or need_v else None
+        gv = torch.empty(S, dv, dtype=q.dtype, device=dev) if need_k or need_v else None
+        share = torch.empty(E, H, dtype=torch.float32, device=dev) if per_node else None
+        da = torch.empty(E, H, dtype=torch.float32, device=dev) if per_node or need_bias or need_weight else None
+        dst = torch.empty(E, dtype=torch.int32, device=dev) if per_node else None
+        gweight = torch.empty(E, dtype=torch.float32, device=dev) if need_weight else None
+        nbytes = core.e3b_attention_bwd_scratch_bytes(N, E, dqk)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        status = _lib._ptr(_lib.status_word(dev))
+        with _lib.device_of(q), _lib.nvtx_range("e3b_attention_bwd"):
+            rc = core.e3b_attention_bwd(
+                _lib._ptr(q), _lib._ptr(k), _lib._ptr(v), _lib._ptr(grad), q.stride(0), k.stride(0), v.stride(0), _lib._ptr(out32), _lib._ptr(stats),
+                _lib._ptr(c.rowptr), _lib._ptr(c.perm), _lib._ptr(c.src), _lib._ptr(bias), _lib._ptr(c.buckets),
+                bias.shape[0] if c.buckets is not None else 0, _lib._ptr(weight), _lib._ptr(c.qk_tbl), _lib._ptr(c.v_tbl), c.layout, c.scale, N, S, E,
+                type_code, _lib._ptr(gq), _lib._ptr(gk) if per_edge else None, _lib._ptr(gv) if per_edge else None, _lib._ptr(share), _lib._ptr(da),
+                _lib._ptr(dst), _lib._ptr(gweight), _lib._ptr(scratch), nbytes, status, _lib.stream_ptr())
+        _lib.check(rc, "e3b_attention_bwd")
+        if per_node:
+            perm_t, rowptr_t = c.transpose if c.transpose is not None else csr_from_dst(c.src, S)
+            nbytes = core.e3b_attention_bwd_src_scratch_bytes(S, E, dqk, dv)
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            with _lib.device_of(q), _lib.nvtx_range("e3b_attention_bwd_src"):
+                rc = core.e3b_attention_bwd_src(
+                    _lib._ptr(q), _lib._ptr(grad), q.stride(0), _lib._ptr(share), _lib._ptr(da), _lib._ptr(dst), _lib._ptr(perm_t), _lib._ptr(rowptr_t),
+                    _lib._ptr(c.qk_tbl), _lib._ptr(c.v_tbl), c.layout, c.scale, N, S, E, type_code, _lib._ptr(gk), _lib._ptr(gv), _lib._ptr(scratch),
+                    nbytes, status, _lib.stream_ptr())
+            _lib.check(rc, "e3b_attention_bwd_src")
+        gbias = None
+        if need_bias:
+            gbias = bias_table_grad(da, c.buckets, bias.shape[0], torch.float32) if c.buckets is not None else da
+        return gq, gk if need_k else None, gv if need_v else None, gbias, gweight, None, None
+
+
+class NeighborAttention(torch.nn.Module):
+    """``out[n]_h = sum_e share[e, h] v[src_e]_h`` over the edges ``e`` of node ``n``, with
+    ``share = softmax_e(scale * <q[n], k[src_e]>_h + bias[e, h] + log(edge_weight[e]))``.
+
+    Head ``h`` owns channels ``h mul / H .. (h+1) mul / H`` of every block of the irreps, so ``num_heads`` divides all
+    multiplicities; a head has at most 1,024 columns of each of ``irreps_qk`` and ``irreps_v``.  ``scale`` defaults to the inverse root of
+    the columns of a head of ``irreps_qk``.
+    """
+
+    def __init__(self, irreps_qk, irreps_v, num_heads: int, scale: Optional[float] = None) -> None:
+        super().__init__()
+        self.irreps_qk, self.irreps_v, self.num_heads = Irreps(irreps_qk), Irreps(irreps_v), int(num_heads)
+        if self.num_heads < 1:
+            raise ValueError(f"num_heads must be positive, got {num_heads}")
+        for irreps in (self.irreps_qk, self.irreps_v):
+            if irreps.dim == 0 or any(mul % self.num_heads for mul, _ in irreps):
+                raise ValueError(f"{self.num_heads} heads must divide the multiplicities of {irreps}, which must not be empty")
+            if irreps.dim // self.num_heads > MAX_HEAD_COLUMNS:
+                raise NotImplementedError(f"{irreps.dim // self.num_heads} columns a head, at most {MAX_HEAD_COLUMNS} are supported")
+        self.scale = float(scale) if scale is not None else (self.irreps_qk.dim // self.num_heads) ** -0.5
+        self._fours = all(mul // self.num_heads * ir.dim % 4 == 0 for irreps in (self.irreps_qk, self.irreps_v) for mul, ir in irreps)
+        self._layouts = {}
+        for vec in (1, 4) if self._fours else (1,):
+            tables = [_head_vectors(irreps, self.num_heads, vec) for irreps in (self.irreps_qk, self.irreps_v)]
+            self.register_buffer(f"_qk{vec}", tables[0], persistent=False)
+            self.register_buffer(f"_v{vec}", tables[1], persistent=False)
+            self._layouts[vec] = [vec, self.num_heads, tables[0].shape[0], tables[1].shape[0], self.irreps_qk.dim, self.irreps_v.dim]
+
+    def __repr__(self) -> str:
+        return f"{self.__class__.__name__}(q, k: {self.irreps_qk}, v: {self.irreps_v}, {self.num_heads} heads)"
+
+    def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rowptr: torch.Tensor, edge_src: Optional[torch.Tensor] = None,
+                perm: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, buckets: Optional[torch.Tensor] = None,
+                edge_weight: Optional[torch.Tensor] = None, transpose: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
+                check_indices: bool = False) -> torch.Tensor:
+        """``q [N, irreps_qk.dim]``, ``k`` and ``v`` in one of float32, bfloat16 and float16 -> ``[N, irreps_v.dim]`` in that type.
+
+        Edge slot ``s`` in ``[rowptr[n], rowptr[n+1])`` belongs to node ``n`` and is edge ``perm[s]`` (``s`` itself without ``perm``;
+        `e3nn_b200.csr_from_dst` gives both).  ``edge_src [E]``: ``k`` and ``v`` are rows of nodes, edge ``e`` reads row ``edge_src[e]``;
+        without it they are rows of edges.  Slots from ``rowptr[N]`` on belong to no node.  A node without edges gets zeros.
+
+        ``bias``: ``[E, num_heads]``, or with ``buckets [E]`` (int32) a table ``[num_buckets, num_heads]`` (`RelativeBias`);
+        an entry ``-inf`` of the former masks its edge for that head, whatever ``k`` and ``v`` hold there.  ``edge_weight [E]``
+        multiplies the exponentials (a smooth cutoff); an edge with weight zero or below is left out, its rows are not read
+        and its gradients, that of the weight included, are zero.
+
+        Statistics and sums are fp32.  Gradients (first order, fixed order of summation) of ``q``, ``k``, ``v``, ``bias`` and ``edge_weight``;
+        those of node-wise ``k`` and ``v`` need the edges by source, ``transpose = csr_from_dst(edge_src, k.shape[0])``,
+        which is built in the backward pass (with a synchronisation: not while a graph is captured) if it is not given.
+        Indices out of range are reported like those of `conv_uvu` and their edges left out.
+        """
+        _lib.require_same_device(q, k, v, rowptr, edge_src, perm, bias, buckets, edge_weight, *(transpose or ()))
+        _lib.require_operand(self._qk1, q, "NeighborAttention's tables (move the module with .to(device))", None, torch.int32)
+        _lib.element_type(q, "q")
+        if not q.dtype == k.dtype == v.dtype:
+            raise TypeError(f"q, k and v must have one type, got {q.dtype}, {k.dtype} and {v.dtype}")
+        for t, name in ((rowptr, "rowptr"), (edge_src, "edge_src"), (perm, "perm"), *((t, "transpose") for t in transpose or ())):
+            if t is not None and t.dtype != torch.int64:
+                raise TypeError(f"{name} must be int64")
+            torch._assert(t is None or t.dim() == 1, f"Incorrect shape for {name}")
+        H, dqk, dv = self.num_heads, self.irreps_qk.dim, self.irreps_v.dim
+        E = k.shape[0] if edge_src is None else edge_src.shape[0]
+        torch._assert(q.dim() == 2 and q.shape[1] == dqk, "Incorrect shape for q")
+        torch._assert(k.dim() == 2 and k.shape[1] == dqk, "Incorrect shape for k")
+        torch._assert(v.dim() == 2 and v.shape == (k.shape[0], dv), "Incorrect shape for v")
+        torch._assert(rowptr.shape[0] == q.shape[0] + 1, "Incorrect shape for rowptr")
+        torch._assert(perm is None or perm.shape[0] == E, "Incorrect shape for perm")
+        if buckets is not None:
+            if bias is None:
+                raise ValueError("buckets need the table they index: bias=[num_buckets, num_heads]")
+            if buckets.dtype != torch.int32:
+                raise TypeError("buckets must be int32")
+            torch._assert(buckets.shape == (E,), "Incorrect shape for buckets")
+            torch._assert(bias.dim() == 2 and bias.shape[1] == H, "Incorrect shape for bias")
+        elif bias is not None:
+            torch._assert(bias.shape == (E, H), "Incorrect shape for bias")
+        torch._assert(edge_weight is None or edge_weight.shape == (E,), "Incorrect shape for edge_weight")
+        if transpose is not None:
+            torch._assert(len(transpose) == 2 and transpose[0].shape[0] == E and transpose[1].shape[0] == k.shape[0] + 1, "Incorrect shape for transpose")
+        for t, name in ((bias, "bias"), (edge_weight, "edge_weight")):
+            if t is not None:
+                _lib.element_type(t, name)
+        if max(E, q.shape[0], k.shape[0]) >= 2 ** 31 - 1:
+            raise NotImplementedError("at most 2^31 - 2 edges and rows")
+        _lib.poll_status(q.device)
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        c = _Call()
+        c.vec = 4 if self._fours and _fits_fours(q) and _fits_fours(k) and _fits_fours(v) else 1
+        c.layout = (ctypes.c_int32 * 6)(*self._layouts[c.vec])
+        c.qk_tbl, c.v_tbl = (self._qk4, self._v4) if c.vec == 4 else (self._qk1, self._v1)
+        c.scale, c.edges = self.scale, E
+        c.rowptr, c.src = rowptr.contiguous(), None if edge_src is None else edge_src.contiguous()
+        c.perm, c.buckets = None if perm is None else perm.contiguous(), None if buckets is None else buckets.contiguous()
+        c.transpose = None if transpose is None else (transpose[0].contiguous(), transpose[1].contiguous())
+        bias = None if bias is None else bias.to(torch.float32).contiguous()
+        weight = None if edge_weight is None else edge_weight.to(torch.float32).contiguous()
+        train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias, weight))
+        out = _AttentionFunction.apply(q, k, v, bias, weight, c, train)
+        if check_indices:
+            _lib.check_status(q.device, "NeighborAttention")
+        return out
+
+
+class AttentionBlock(torch.nn.Module):
+    """One residual attention block on node features, from the modules of this package::
+
+        q, k, v = Linear(h)
+        y       = Linear(NeighborAttention(q, k, v))
+        x', h'  = NormGateResidual(gate)(x, y)            h' = norm(x') is the next block's input
+
+    ``h`` is ``x`` after a norm: `RMSNorm` before the first block, the previous block's second output after it.  Scalars
+    of ``irreps_node`` are activated with ``act`` and all other channels gated with ``gate_act``."""
+
+    def __init__(self, irreps_node, num_heads: int, irreps_key=None, act=torch.nn.functional.silu, gate_act=torch.sigmoid,
+                 linear_math_mode: str = "tf32x3", eps: float = 1e-5, scale_init: float = 1.0) -> None:
+        super().__init__()
+        self.irreps_node = Irreps(irreps_node)
+        self.irreps_key = Irreps(irreps_key) if irreps_key is not None else self.irreps_node
+        scalars = Irreps([(mul, ir) for mul, ir in self.irreps_node if ir.l == 0])
+        gated = Irreps([(mul, ir) for mul, ir in self.irreps_node if ir.l > 0])
+        gates = Irreps([(mul, "0e") for mul, _ in gated])
+        gate = Gate(scalars, [act] * len(scalars), gates, [gate_act] * len(gates), gated)
+        if gate.irreps_out != self.irreps_node:
+            raise ValueError(f"irreps_node must be sorted, scalars first, and keep its parities under the activations: got {self.irreps_node}, "
+                             f"the gate gives {gate.irreps_out}")
+        self.attention = NeighborAttention(self.irreps_key, self.irreps_node, num_heads)
+        self.lin_qkv = Linear(self.irreps_node, self.irreps_key + self.irreps_key + self.irreps_node, math_mode=linear_math_mode)
+        self.lin_out = Linear(self.irreps_node, gate.irreps_in, math_mode=linear_math_mode)
+        self.post = NormGateResidual(gate, eps=eps, scale_init=scale_init)
+
+    def forward(self, x: torch.Tensor, h: torch.Tensor, rowptr: torch.Tensor, edge_src: torch.Tensor, **edges) -> Tuple[torch.Tensor, torch.Tensor]:
+        """``x`` and ``h`` ``[N, irreps_node.dim]`` float32; ``edges`` are the keyword arguments of `NeighborAttention`
+        (``perm``, ``bias``, ``buckets``, ``edge_weight``, ``transpose``)."""
+        dk = self.irreps_key.dim
+        q, k, v = self.lin_qkv(h).split([dk, dk, self.irreps_node.dim], dim=-1)
+        return self.post(x, self.lin_out(self.attention(q, k, v, rowptr, edge_src, **edges)))

@@ -1,0 +1,257 @@
+"""Norms on rows of irreps features and the boundary between two residual blocks.
+
+`RMSNorm` divides every block ``(mul, ir)`` of a row by the root of the mean square of its ``mul * (2l+1)`` columns (a
+rotation leaves that number alone) and multiplies every channel by a learned weight; the reference's ``BatchNorm``
+(``e3nn/nn/_batchnorm.py:8-50``) with ``normalization='component'`` takes the same mean over a batch and has no form per row.
+
+`NormGateResidual` is the run of steps between the last Linear of one residual block and the first of the next, in one
+kernel per direction (``e3b_norm_gate_residual_fwd`` / ``_bwd``)::
+
+    n = RMSNorm(y);  g = gate(n);  z = residual + scale * g;  h = RMSNorm(z)
+
+Rows are fp32, bf16 or fp16; sums, products and parameters are fp32, every output is rounded once (``h`` is taken from ``z``
+before ``z`` is rounded).  Gradients are first order and summed in a fixed order.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import List, Optional, Tuple, Union
+
+import torch
+
+from .. import _lib
+from ..o3 import Irreps
+from ._activation import Activation
+from ._gate import Gate
+
+
+def _blocks(irreps: Irreps) -> List[Tuple[int, int]]:
+    """``(channels, components)`` of the blocks that have columns."""
+    return [(mul, ir.dim) for mul, ir in irreps if mul > 0]
+
+
+def _column_blocks(blocks) -> List[Tuple[int, int]]:
+    """``(block, channel)`` of every column; channels are numbered through the row."""
+    out, chan = [], 0
+    for b, (mul, d) in enumerate(blocks):
+        out += [(b, chan + u) for u in range(mul) for _ in range(d)]
+        chan += mul
+    return out
+
+
+def _channel_columns(blocks) -> torch.Tensor:
+    """``{first column, components}`` of every channel."""
+    out, at = [], 0
+    for mul, d in blocks:
+        out += [(at + u * d, d) for u in range(mul)]
+        at += mul * d
+    return torch.tensor(out, dtype=torch.int32).reshape(-1, 2)
+
+
+def _inverse_counts(blocks) -> torch.Tensor:
+    return torch.tensor([1.0 / (mul * d) for mul, d in blocks], dtype=torch.float32)
+
+
+def _fours(blocks) -> bool:
+    """Whether vectors of four columns never straddle two blocks."""
+    return all(mul * d % 4 == 0 for mul, d in blocks)
+
+
+def _float_bits(value: float) -> int:
+    return ctypes.c_int32.from_buffer(ctypes.c_float(value)).value
+
+
+def _fp32(parameter: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return None if parameter is None else parameter.to(torch.float32).contiguous()
+
+
+def _flat_rows(x: torch.Tensor, dim: int, name: str) -> torch.Tensor:
+    _lib.element_type(x, name)
+    torch._assert(x.dim() > 0 and x.shape[-1] == dim, f"Incorrect last dimension for {name}")
+    return x.reshape(-1, dim).contiguous() if dim > 0 else x.reshape(x.shape[:-1].numel(), 0)
+
+
+class _RMSNormFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, tbl, inv, channels, fours, eps):
+        h = torch.empty_like(x)
+        with _lib.device_of(x):
+            rc = _lib.core().e3b_rms_norm_fwd(_lib._ptr(x), _lib._ptr(weight), _lib._ptr(tbl), _lib._ptr(inv), inv.shape[0], fours, eps,
+                                              _lib._ptr(h), x.shape[0], x.shape[1], _lib.element_type(x), _lib.stream_ptr())
+        _lib.check(rc, "e3b_rms_norm_fwd")
+        ctx.save_for_backward(x, weight, tbl, inv, channels)
+        ctx.meta = (fours, eps)
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, weight, tbl, inv, channels = ctx.saved_tensors
+        fours, eps = ctx.meta
+        core, (rows, dim), nch = _lib.core(), x.shape, channels.shape[0]
+        gx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
+        gw = scratch = None
+        nbytes = 0
+        if ctx.needs_input_grad[1]:
+            gw = torch.empty(nch, dtype=torch.float32, device=x.device)
+            nbytes = core.e3b_norm_scratch_bytes(rows, nch)
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        grad = grad.contiguous()
+        with _lib.device_of(x):
+            rc = core.e3b_rms_norm_bwd(_lib._ptr(x), _lib._ptr(grad), _lib._ptr(weight), _lib._ptr(tbl), _lib._ptr(inv), _lib._ptr(channels), nch,
+                                       inv.shape[0], fours, eps, _lib._ptr(gx), _lib._ptr(gw), _lib._ptr(scratch), nbytes, rows, dim,
+                                       _lib.element_type(x), _lib.stream_ptr())
+        _lib.check(rc, "e3b_rms_norm_bwd")
+        return gx, gw, None, None, None, None, None
+
+
+class RMSNorm(torch.nn.Module):
+    """``h[b, u, m] = weight[b, u] * x[b, u, m] / sqrt(mean_{u, m} x[b, u, m]^2 + eps)`` for every block ``b`` of ``irreps``.
+
+    ``affine=False``: without the weights (one per channel, ones at the start).  Input ``[..., irreps.dim]`` in float32,
+    bfloat16 or float16; the output has its type.  Blocks are normalised as they are written: ``"16x0e+16x0e"`` has two."""
+
+    def __init__(self, irreps, eps: float = 1e-5, affine: bool = True) -> None:
+        super().__init__()
+        self.irreps_in = self.irreps_out = Irreps(irreps)
+        self.eps = float(eps)
+        if not self.eps >= 0.0:
+            raise ValueError(f"eps must not be negative, got {eps}")
+        blocks = _blocks(self.irreps_in)
+        self._fours = int(_fours(blocks))
+        cols = _column_blocks(blocks)
+        tbl = torch.tensor([(b, c, 0, 0) for b, c in cols], dtype=torch.int32).reshape(-1, 4)
+        self.register_buffer("_tbl", tbl, persistent=False)
+        self.register_buffer("_inv_bits", _inverse_counts(blocks).view(torch.int32), persistent=False)
+        self.register_buffer("_channels", _channel_columns(blocks), persistent=False)
+        if affine:
+            self.weight = torch.nn.Parameter(torch.ones(self._channels.shape[0]))
+        else:
+            self.register_parameter("weight", None)
+
+    def __repr__(self) -> str:
+        return f"{self.__class__.__name__}({self.irreps_in}, eps={self.eps})"
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if not x.is_cuda:
+            raise NotImplementedError("RMSNorm runs on CUDA tensors only")
+        dim = self.irreps_in.dim
+        rows = _flat_rows(x, dim, "x")
+        _lib.require_operand(self._tbl, x, "RMSNorm's tables (move the module with .to(device))", None, torch.int32)
+        _lib.poll_status(x.device)
+        if self.weight is not None and self.weight.device != x.device:
+            raise RuntimeError(f"Expected all tensors to be on the same device, but weight is on {self.weight.device} and x on {x.device}")
+        out = _RMSNormFunction.apply(rows, _fp32(self.weight), self._tbl, self._inv_bits.view(torch.float32), self._channels, self._fours, self.eps)
+        return out.reshape(x.shape)
+
+
+class _NormGateFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, residual, y, w_post, scale, w_pre, tables, sizes, fours, eps):
+        in_tbl, out_tbl, _, _, _, in_inv, out_inv = tables
+        z = torch.empty_like(residual)
+        h = torch.empty_like(residual) if w_pre is not None else None
+        with _lib.device_of(y):
+            rc = _lib.core().e3b_norm_gate_residual_fwd(
+                _lib._ptr(residual), _lib._ptr(y), _lib._ptr(w_post), _lib._ptr(scale), _lib._ptr(w_pre), _lib._ptr(in_tbl), _lib._ptr(out_tbl),
+                _lib._ptr(in_inv), _lib._ptr(out_inv), sizes, fours, eps, _lib._ptr(z), _lib._ptr(h), y.shape[0], _lib.element_type(y),
+                _lib.stream_ptr())
+        _lib.check(rc, "e3b_norm_gate_residual_fwd")
+        ctx.save_for_backward(residual, y, w_post, scale, w_pre)
+        ctx.meta = (tables, sizes, fours, eps)
+        ctx.set_materialize_grads(False)
+        return z, h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_z, grad_h):
+        residual, y, w_post, scale, w_pre = ctx.saved_tensors
+        tables, sizes, fours, eps = ctx.meta
+        if grad_z is None and grad_h is None:
+            return (None,) * 9
+        core, rows = _lib.core(), y.shape[0]
+        grad_z = grad_z.contiguous() if grad_z is not None else None
+        grad_h = grad_h.contiguous() if grad_h is not None else None
+        g_residual = torch.empty_like(residual) if ctx.needs_input_grad[0] else None
+        gy = torch.empty_like(y) if ctx.needs_input_grad[1] else None
+        params = scratch = None
+        nbytes, n_in, n_out = 0, sizes[4], sizes[5]
+        if any(ctx.needs_input_grad[2:5]):
+            params = torch.empty(n_in + 2 * n_out, dtype=torch.float32, device=y.device)
+            nbytes = core.e3b_norm_scratch_bytes(rows, n_in + 2 * n_out)
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=y.device)
+        with _lib.device_of(y):
+            rc = core.e3b_norm_gate_residual_bwd(
+                _lib._ptr(residual), _lib._ptr(y), _lib._ptr(grad_z), _lib._ptr(grad_h), _lib._ptr(w_post), _lib._ptr(scale), _lib._ptr(w_pre),
+                *(_lib._ptr(t) for t in tables), sizes, fours, eps, _lib._ptr(g_residual), _lib._ptr(gy), _lib._ptr(params), _lib._ptr(scratch), nbytes,
+                rows, _lib.element_type(y), _lib.stream_ptr())
+        _lib.check(rc, "e3b_norm_gate_residual_bwd")
+        gw = params.split([n_in, n_out, n_out]) if params is not None else (None, None, None)
+        return (g_residual, gy, gw[0], gw[1], gw[2] if w_pre is not None else None, None, None, None, None)
+
+
+class NormGateResidual(torch.nn.Module):
+    """``z = residual + scale * gate(norm(y))`` and ``h = norm(z)``: the end of one residual block and the norm before the next.
+
+    ``gate``: a `Gate` or an `Activation`; or ``None`` with ``irreps``, and the row is added as it is.  ``y`` has the
+    gate's ``irreps_in``, ``residual``, ``z`` and ``h`` its ``irreps_out``.  Parameters: ``weight_post`` (one per channel
+    of ``y``, ones), ``scale`` (one per channel of ``z``, ``scale_init``) and ``weight_pre`` (one per channel of ``z``, ones);
+    ``pre_norm=False``: no second norm, ``forward`` returns ``z`` alone."""
+
+    def __init__(self, gate: Union[Gate, Activation, None] = None, irreps=None, eps: float = 1e-5, pre_norm: bool = True,
+                 scale_init: float = 1.0) -> None:
+        super().__init__()
+        if (gate is None) == (irreps is None):
+            raise ValueError("give either a gate or, without one, the irreps")
+        if gate is not None and not isinstance(gate, (Gate, Activation)):
+            raise TypeError(f"gate must be a Gate or an Activation, got {type(gate).__name__}")
+        self.eps, self.pre_norm = float(eps), bool(pre_norm)
+        if not self.eps >= 0.0:
+            raise ValueError(f"eps must not be negative, got {eps}")
+        self.irreps_in = Irreps(irreps) if gate is None else gate.irreps_in
+        self.irreps_out = Irreps(irreps) if gate is None else gate.irreps_out
+        ins, outs = _blocks(self.irreps_in), _blocks(self.irreps_out)
+        din, dout = self.irreps_in.dim, self.irreps_out.dim
+        if gate is None:
+            back, const = [[0, j, 1, 0, 3] for j in range(din)], [1.0] * din
+            forth = [[j, -1, 3] for j in range(dout)]
+        else:
+            back, const, forth = gate._in_tbl.tolist(), gate._in_cst.tolist(), gate._out_tbl.tolist()
+        # scalars (0) and gates (2) pass through their activation, gated components (1) and unused columns (3) do not
+        acts = [(row[4], _float_bits(c)) if row[0] in (0, 2) else (3, _float_bits(1.0)) for row, c in zip(back, const)]
+        in_tbl = [(b, u, *a) for (b, u), a in zip(_column_blocks(ins), acts)]
+        out_tbl = [(b, u, row[0], row[1]) for (b, u), row in zip(_column_blocks(outs), forth)]
+        for name, value in (("_in", in_tbl), ("_out", out_tbl), ("_back", [row[:4] for row in back])):
+            self.register_buffer(name, torch.tensor(value, dtype=torch.int32).reshape(-1, 4), persistent=False)
+        self.register_buffer("_in_channels", _channel_columns(ins), persistent=False)
+        self.register_buffer("_out_channels", _channel_columns(outs), persistent=False)
+        self.register_buffer("_in_inv_bits", _inverse_counts(ins).view(torch.int32), persistent=False)
+        self.register_buffer("_out_inv_bits", _inverse_counts(outs).view(torch.int32), persistent=False)
+        n_in, n_out = self._in_channels.shape[0], self._out_channels.shape[0]
+        self._sizes = [din, dout, len(ins), len(outs), n_in, n_out]
+        self._fours = int(_fours(ins) and _fours(outs))
+        self.weight_post = torch.nn.Parameter(torch.ones(n_in))
+        self.scale = torch.nn.Parameter(torch.full((n_out,), float(scale_init)))
+        if pre_norm:
+            self.weight_pre = torch.nn.Parameter(torch.ones(n_out))
+        else:
+            self.register_parameter("weight_pre", None)
+
+    def __repr__(self) -> str:
+        return f"{self.__class__.__name__}({self.irreps_in} -> {self.irreps_out}, eps={self.eps})"
+
+    def forward(self, residual: torch.Tensor, y: torch.Tensor):
+        if not (residual.is_cuda and y.is_cuda):
+            raise NotImplementedError("NormGateResidual runs on CUDA tensors only")
+        torch._assert(residual.shape[:-1] == y.shape[:-1], "residual and y must have the same leading dimensions")
+        if residual.dtype != y.dtype:
+            raise TypeError(f"residual and y must have one type, got {residual.dtype} and {y.dtype}")
+        _lib.require_same_device(y, residual, self.weight_post, self.scale, self.weight_pre)
+        r, x = _flat_rows(residual, self._sizes[1], "residual"), _flat_rows(y, self._sizes[0], "y")
+        _lib.require_operand(self._in, y, "NormGateResidual's tables (move the module with .to(device))", None, torch.int32)
+        _lib.poll_status(y.device)
+        tables = (self._in, self._out, self._back, self._in_channels, self._out_channels, self._in_inv_bits, self._out_inv_bits)
+        z, h = _NormGateFunction.apply(r, x, _fp32(self.weight_post), _fp32(self.scale), _fp32(self.weight_pre), tables,
+                                       (ctypes.c_int32 * 6)(*self._sizes), self._fours, self.eps)
+        z = z.reshape(residual.shape)
+        return (z, h.reshape(residual.shape)) if self.pre_norm else z

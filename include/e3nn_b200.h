@@ -280,6 +280,102 @@ int e3b_fill_columns(float* out, int64_t num_rows, int row_stride, int col0, int
                      void* stream);
 
 /*
+ * Norms on rows of irreps features and the boundary between two residual blocks (no counterpart in the reference, whose
+ * BatchNorm, e3nn/nn/_batchnorm.py, takes its means over a batch).  Rows are fp32 (type 0), bf16 (1) or fp16 (2);
+ * weights, statistics and parameter gradients are fp32.  A row is a list of irreps blocks of n_b = mul_b (2 l_b + 1) columns:
+ *   norm(x; w)[column] = w[channel] * x[column] / sqrt(mean of x^2 over the block + eps).
+ * e3b_rms_norm_fwd: h = norm(x; weight) (weight NULL: ones).  table [dim,4] = {block, channel, -, -}, inv_count [blocks] = 1 / n_b,
+ * vec4: no group of four consecutive columns, from column 0 on, straddles two blocks.
+ * e3b_rms_norm_bwd: channels [num_channels,2] = {first column, components}; grad_x and grad_weight may each be NULL, not both;
+ * grad_weight needs e3b_norm_scratch_bytes(rows, num_channels) bytes of scratch and is summed in a fixed order.
+ * e3b_norm_gate_residual_fwd: n = norm(y; weight_post), g = Gate(n), z = residual + scale[channel] g, and h = norm(z; weight_pre)
+ * unless h is NULL.  in_table [din,4] = {block, channel, activation (codes of e3b_gate_fwd), constant as float bits},
+ * out_table [dout,4] = {block, channel, input column, gate column or -1}, back_table [din,4] = {kind as in e3b_gate_bwd, first
+ * output column, count, partner column}; sizes: HOST array {din, dout, blocks in, blocks out, channels in, channels out}.
+ * e3b_norm_gate_residual_bwd: grad_z or grad_h may be NULL, each of the gradients too; grad_params [channels in + 2 channels out] =
+ * gradients of weight_post, scale, weight_pre, with e3b_norm_scratch_bytes(rows, its length) bytes of scratch.
+ * Rows of at most e3b_norm_max_columns(1) columns with vec4 and 16-byte (8-byte for 16-bit types) pointers, else
+ * e3b_norm_max_columns(0).
+ */
+int e3b_norm_max_columns(int aligned);
+int64_t e3b_norm_scratch_bytes(int64_t rows, int num_params);
+int e3b_rms_norm_fwd(const void* x, const float* weight, const int32_t* table, const float* inv_count, int num_blocks, int vec4,
+                     float eps, void* h, int64_t rows, int dim, int type, void* stream);
+int e3b_rms_norm_bwd(const void* x, const void* grad_h, const float* weight, const int32_t* table, const float* inv_count,
+                     const int32_t* channels, int num_channels, int num_blocks, int vec4, float eps, void* grad_x,
+                     float* grad_weight, void* scratch, int64_t scratch_bytes, int64_t rows, int dim, int type, void* stream);
+int e3b_norm_gate_residual_fwd(const void* residual, const void* y, const float* weight_post, const float* scale,
+                               const float* weight_pre, const int32_t* in_table, const int32_t* out_table, const float* in_inv,
+                               const float* out_inv, const int32_t* sizes, int vec4, float eps, void* z, void* h, int64_t rows,
+                               int type, void* stream);
+int e3b_norm_gate_residual_bwd(const void* residual, const void* y, const void* grad_z, const void* grad_h,
+                               const float* weight_post, const float* scale, const float* weight_pre, const int32_t* in_table,
+                               const int32_t* out_table, const int32_t* back_table, const int32_t* in_channels,
+                               const int32_t* out_channels, const float* in_inv, const float* out_inv, const int32_t* sizes,
+                               int vec4, float eps, void* grad_residual, void* grad_y, float* grad_params, void* scratch,
+                               int64_t scratch_bytes, int64_t rows, int type, void* stream);
+
+/*
+ * Learned bias by distance buckets (no counterpart in the reference).
+ * e3b_distance_buckets: buckets[e] = number of squared thresholds (ascending, at most 1,023) that are <= |pos[src] - pos[dst] + shift|^2,
+ * in fp64 from fp32 coordinates; shift may be NULL; an index out of range sets *status = 2 and gives bucket 0.
+ * e3b_relative_bias_fwd: bias[e, h] = table[buckets[e], h], both of `type`; a bucket out of range sets *status = 2 and gives 0.
+ * e3b_relative_bias_bwd: grad_table[b, h] = sum over the edges of bucket b of grad_bias[e, h], in fp32 and in a fixed order, with
+ * e3b_relative_bias_scratch_bytes(...) bytes of scratch.  At most 1,024 buckets.
+ */
+int e3b_distance_buckets(const float* pos, const int64_t* edge_src, const int64_t* edge_dst, const float* shift,
+                         const double* thresholds_squared, int num_thresholds, int64_t num_edges, int64_t num_nodes,
+                         int32_t* buckets, int32_t* status, void* stream);
+int e3b_relative_bias_fwd(const void* table, const int32_t* buckets, int num_buckets, int num_heads, int64_t num_edges, int type,
+                          void* bias, int32_t* status, void* stream);
+int64_t e3b_relative_bias_scratch_bytes(int64_t num_edges, int num_buckets, int num_heads);
+int e3b_relative_bias_bwd(const void* grad_bias, const int32_t* buckets, int num_buckets, int num_heads, int64_t num_edges, int type,
+                          void* grad_table, int table_type, void* scratch, int64_t scratch_bytes, int32_t* status, void* stream);
+
+/*
+ * Multi-head softmax attention over the incoming edges of every node (the transformer example of the reference,
+ * docs/guide/transformer.rst, as one pass):
+ *   a[e,h] = scale <q[n], k[r]>_h + bias[e,h] + log edge_weight[e],   out[n]_h = sum_e softmax_e(a[e,h]) v[r]_h
+ * over the slots s of row n (rowptr[n] <= s < rowptr[n+1]; rowptr[0] is taken as 0), e = perm[s] (perm NULL: s), r = edge_src[e]
+ * (edge_src NULL: e).  q [num_dst, .], k and v [num_src, .] of `type`, rows q_stride, k_stride, v_stride elements apart;
+ * out [num_dst, dv] dense.  bias NULL, [num_edges, heads] (-inf: masked, k and v unread), or with buckets [num_edges] a table
+ * [num_buckets, heads].  edge_weight NULL or [num_edges]; an edge with a weight <= 0 is left out and its rows are unread.
+ * A row without edges (or all left out) is zero.  An index out of range sets *status = 2, its edge is left out.
+ * layout: HOST array {vector width 1 or 4, heads, vectors of a head of q and k, of v, columns of q and k, of v}; qk_table, v_table:
+ * per vector {column of head 0, columns from one head to the next}; width 4 needs pointers and strides in multiples of four elements.
+ * A head has at most 1,024 columns (E3B_ERR_UNSUPPORTED).  Fewer than 2^31 - 1 edges and rows.
+ * out32 (NULL or the output in fp32) and stats [num_dst, heads, 2] (NULL or maximum and reciprocal of the sum) are what the
+ * gradient needs; with type 0 out itself serves as out32.
+ *
+ * e3b_attention_bwd: grad_q [num_dst, dqk]; k and v per edge (edge_src NULL): grad_k, grad_v per edge (both or neither).  Optional, per
+ * edge: share [num_edges, heads], grad_logit [num_edges, heads] (the gradient of bias), edge_dst [num_edges] (destination, -1: none),
+ * grad_weight [num_edges] (needs grad_logit).
+ * e3b_attention_bwd_src: grad_k and grad_v of nodes from share, grad_logit and edge_dst and the CSR by source (e3b_csr_from_dst of
+ * edge_src: src_perm, src_rowptr).  All sums have a fixed order.
+ */
+int64_t e3b_attention_scratch_bytes(int64_t num_dst, int64_t num_edges, int num_heads, int dim_v);
+int e3b_attention_fwd(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                      const int64_t* rowptr, const int64_t* perm, const int64_t* edge_src, const float* bias,
+                      const int32_t* buckets, int num_buckets, const float* edge_weight, const int32_t* qk_table,
+                      const int32_t* v_table, const int32_t* layout, float scale, int64_t num_dst, int64_t num_src,
+                      int64_t num_edges, int type, void* out, float* out32, float* stats, void* scratch, int64_t scratch_bytes,
+                      int32_t* status, void* stream);
+int64_t e3b_attention_bwd_scratch_bytes(int64_t num_dst, int64_t num_edges, int dim_qk);
+int e3b_attention_bwd(const void* q, const void* k, const void* v, const void* grad_out, int64_t q_stride, int64_t k_stride,
+                      int64_t v_stride, const float* out32, const float* stats, const int64_t* rowptr, const int64_t* perm,
+                      const int64_t* edge_src, const float* bias, const int32_t* buckets, int num_buckets,
+                      const float* edge_weight, const int32_t* qk_table, const int32_t* v_table, const int32_t* layout,
+                      float scale, int64_t num_dst, int64_t num_src, int64_t num_edges, int type, void* grad_q, void* grad_k,
+                      void* grad_v, float* share, float* grad_logit, int32_t* edge_dst, float* grad_weight, void* scratch,
+                      int64_t scratch_bytes, int32_t* status, void* stream);
+int64_t e3b_attention_bwd_src_scratch_bytes(int64_t num_src, int64_t num_edges, int dim_qk, int dim_v);
+int e3b_attention_bwd_src(const void* q, const void* grad_out, int64_t q_stride, const float* share, const float* grad_logit,
+                          const int32_t* edge_dst, const int64_t* src_perm, const int64_t* src_rowptr, const int32_t* qk_table,
+                          const int32_t* v_table, const int32_t* layout, float scale, int64_t num_dst, int64_t num_src,
+                          int64_t num_edges, int type, void* grad_k, void* grad_v, void* scratch, int64_t scratch_bytes,
+                          int32_t* status, void* stream);
+
+/*
  * Self-test of the bounded-wait convention of the pipelined kernels (no counterpart in the reference, which has
  * no device code): one small block waits on an mbarrier that nothing arrives at, gives up after `limit` polls
  * (1 .. 100000, each a try_wait with a short back-off), stores 3 in *status and returns.  The host reads the

@@ -1,0 +1,95 @@
+"""Host side of the transformer modules: constructors, tables and refusals that need no GPU."""
+import pytest
+import torch
+
+from e3nn_b200 import nn as bnn
+from e3nn_b200 import o3
+from e3nn_b200.nn._attention import _head_vectors
+from e3nn_b200.nn._norm import _channel_columns, _column_blocks
+
+
+@pytest.mark.parametrize("irreps,heads", [("8x0e+8x1o+4x2e", 4), ("3x0e+6x1o", 3), ("5x0e", 1), ("4x2e+0x1o+4x0e", 2)])
+def test_heads_own_every_column_once(irreps, heads):
+    irreps = o3.Irreps(irreps)
+    fours = all(mul // heads * ir.dim % 4 == 0 for mul, ir in irreps)
+    for vec in (1, 4) if fours else (1,):
+        tbl = _head_vectors(irreps, heads, vec).tolist()
+        cols = [c + h * run + i for h in range(heads) for c, run in tbl for i in range(vec)]
+        assert sorted(cols) == list(range(irreps.dim))
+        owner = {c + h * run + i: h for h in range(heads) for c, run in tbl for i in range(vec)}
+        at = 0
+        for mul, ir in irreps:
+            for u in range(mul):
+                for m in range(ir.dim):
+                    assert owner[at + u * ir.dim + m] == u * heads // mul
+            at += mul * ir.dim
+
+
+def test_columns_blocks_and_channels():
+    irreps = o3.Irreps("2x0e+0x3o+3x1o")
+    blocks = [(mul, ir.dim) for mul, ir in irreps if mul > 0]
+    assert _column_blocks(blocks) == [(0, 0), (0, 1), (1, 2), (1, 2), (1, 2), (1, 3), (1, 3), (1, 3), (1, 4), (1, 4), (1, 4)]
+    assert _channel_columns(blocks).tolist() == [[0, 1], [1, 1], [2, 3], [5, 3], [8, 3]]
+
+
+def test_gate_rows_name_every_column():
+    gate = bnn.Gate("4x0e+2x0o", [torch.nn.functional.silu, torch.tanh], "3x0e", [torch.sigmoid], "2x1o+1x2e")
+    mod = bnn.NormGateResidual(gate)
+    assert mod.irreps_in == gate.irreps_in and mod.irreps_out == gate.irreps_out
+    assert mod._in.shape == (gate.irreps_in.dim, 4) and mod._out.shape == (gate.irreps_out.dim, 4)
+    kinds = mod._back[:, 0]
+    assert (kinds == 2).sum() == 3 and (kinds == 0).sum() == 6 and (kinds == 1).sum() == 11
+    assert mod.weight_post.numel() == gate.irreps_in.num_irreps and mod.scale.numel() == mod.weight_pre.numel() == gate.irreps_out.num_irreps
+    assert bnn.NormGateResidual(gate, pre_norm=False).weight_pre is None
+
+
+@pytest.mark.parametrize("num,r_linear", [(1, None), (2, 1.0), (3, 1.0), (32, None), (33, 0.5), (1024, 2.0)])
+def test_lower_ends_ascend(num, r_linear):
+    mod = bnn.RelativeBias(num, 2, 5.0, r_linear=r_linear)
+    ends = mod.lower_ends
+    assert len(ends) == num and ends[0] == 0.0 and all(a < b for a, b in zip(ends, ends[1:])) and ends[-1] < 5.0
+    squares = mod._squares.view(torch.float64)
+    assert squares.tolist() == [t * t for t in ends[1:]]
+    assert mod.half()._squares.dtype == torch.int64
+
+
+def test_constructors_refuse():
+    with pytest.raises(ValueError):
+        bnn.RMSNorm("4x0e", eps=-1.0)
+    gate = bnn.Gate("4x0e", [torch.tanh], "2x0e", [torch.sigmoid], "2x1o")
+    with pytest.raises(ValueError):
+        bnn.NormGateResidual()
+    with pytest.raises(ValueError):
+        bnn.NormGateResidual(gate, irreps="4x0e")
+    with pytest.raises(TypeError):
+        bnn.NormGateResidual(torch.nn.SiLU())
+    for args in ((0, 1, 5.0), (1025, 1, 5.0), (4, 0, 5.0), (4, 1, 0.0), (4, 1, float("inf"))):
+        with pytest.raises(ValueError):
+            bnn.RelativeBias(*args)
+    with pytest.raises(ValueError):
+        bnn.RelativeBias(4, 1, 5.0, r_linear=6.0)
+    with pytest.raises(ValueError):
+        bnn.NeighborAttention("4x0e+2x1o", "4x0e", 4)
+    with pytest.raises(ValueError):
+        bnn.NeighborAttention("4x0e", "", 2)
+    with pytest.raises(ValueError):
+        bnn.NeighborAttention("4x0e", "4x0e", 0)
+    with pytest.raises(NotImplementedError):
+        bnn.NeighborAttention("1100x0e", "4x0e", 1)
+    with pytest.raises(ValueError):
+        bnn.AttentionBlock("4x1o+4x0e", 2)
+
+
+def test_host_tensors_are_refused():
+    x = torch.randn(4, 16)
+    with pytest.raises(NotImplementedError):
+        bnn.RMSNorm("4x0e+4x1o")(x)
+    with pytest.raises(NotImplementedError):
+        bnn.NormGateResidual(irreps="4x0e+4x1o")(x, x)
+    idx = torch.zeros(2, dtype=torch.int64)
+    with pytest.raises(NotImplementedError):
+        bnn.RelativeBias(4, 2, 5.0).buckets(x[:, :3], idx, idx)
+    with pytest.raises(NotImplementedError):
+        bnn.RelativeBias(4, 2, 5.0)(idx.int())
+    with pytest.raises(NotImplementedError):
+        bnn.NeighborAttention("4x0e+4x1o", "4x0e+4x1o", 2)(x, x, x, torch.zeros(5, dtype=torch.int64), idx)
