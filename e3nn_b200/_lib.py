@@ -260,7 +260,7 @@ def core() -> ctypes.CDLL:
         lib.e3b_attention_bwd_scratch_bytes.argtypes = [i64, i64, i]
         lib.e3b_attention_bwd.argtypes = [vp] * 4 + [i64] * 3 + [vp] * 7 + [i] + [vp] * 4 + [f, i64, i64, i64, i] + [vp] * 8 + [i64, vp, vp]
         lib.e3b_attention_bwd_src_scratch_bytes.argtypes = [i64, i64, i, i]
-        lib.e3b_attention_bwd_src.argtypes = [vp] * 2 + [i64] + [vp] * 8 + [f, i64, i64, i64, i] + [vp] * 3 + [i64, vp, vp]
+        lib.e3b_attention_bwd_src.argtypes = [vp] * 2 + [i64] + [vp] * 7 + [f, i64, i64, i64, i] + [vp] * 3 + [i64, vp, vp]
         for name in ("e3b_norm_scratch_bytes", "e3b_relative_bias_scratch_bytes", "e3b_attention_scratch_bytes",
                      "e3b_attention_bwd_scratch_bytes", "e3b_attention_bwd_src_scratch_bytes"):
             getattr(lib, name).restype = i64

@@ -24,6 +24,10 @@ struct FwdArgs {
     Edges e;
     Rows r;
     Partials p;
+    bool merge;
+    RingSource ring;
+    int depth;
+    uint32_t warp_smem;
 };
 
 template <typename T, int VEC, int V>
@@ -37,7 +41,7 @@ __device__ __forceinline__ void finish_row(const FwdArgs& a, const Sums<VEC, V, 
     }
 }
 
-template <typename T, int VEC, int V, bool MERGE>
+template <typename T, int VEC, int V>
 __global__ void __launch_bounds__(256) attn_fwd_kernel(const FwdArgs a) {
     extern __shared__ float smem[];
     constexpr int U = edges_in_flight(V, words_of<T, VEC>(), 80);
@@ -56,8 +60,9 @@ __global__ void __launch_bounds__(256) attn_fwd_kernel(const FwdArgs a) {
     int ended = -1;
     if (part < a.r.parts) {
         float qf[V][VEC];
+        const Part range = find_part(a.r, part);
         walk_rows(
-            a.r, part,
+            a.r, range,
             [&](int64_t n) {
                 load_row_f<T, VEC, V>(qf, q, n, a.q_stride, cq);
                 s.clear();
@@ -137,11 +142,101 @@ __global__ void __launch_bounds__(256) attn_fwd_kernel(const FwdArgs a) {
                     s.save(a.p.at(part, 0), a.h, cq, cv, head, leads);
                     ended = static_cast<int>(n);
                 }
-            },
-            [](int64_t, int64_t) {});
+            });
         if (blockIdx.y == 0 && lane == 0) a.p.ended[part] = ended;
     }
-    leave_part<MERGE>(s, goes_on, part, a.r.parts, a.p, a.h, cq, cv, head, leads, smem);
+    leave_part(a.merge, s, goes_on, part, a.r.parts, a.p, a.h, cq, cv, head, leads, smem);
+}
+
+// The same with k and v through the ring: the registers hold q, the sums and the row in hand, so more warps fit and all copies that
+// fit in shared memory are under way (about 200 KB an SM).
+template <typename T, int VEC, int V>
+__global__ void __launch_bounds__(128, 3) attn_fwd_ring_kernel(const FwdArgs a) {
+    extern __shared__ __align__(128) uint8_t memory[];
+    constexpr int U = V * VEC <= 12 ? 4 : 2;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = blockIdx.x * (blockDim.x >> 5) + warp;
+    const int head = lane / a.h.lanes;
+    const bool live = head < a.h.heads, leads = live && (lane & (a.h.lanes - 1)) == 0;
+    int cq[V], cv[V];
+    lane_columns<V>(a.h.qk, a.h.nqk, a.h.lanes, head, live, cq);
+    lane_columns<V>(a.h.v, a.h.nv, a.h.lanes, head, live, cv);
+    Sums<VEC, V, 1, true> s;
+    s.clear();
+    int64_t goes_on = -1;
+    int ended = -1;
+    if (part < a.r.parts) {
+        const Part range = find_part(a.r, part);
+        Ring<U, EdgeMeta> ring(a.ring, memory + warp * a.warp_smem, a.depth);
+        float qf[V][VEC], bias[U];
+        bool use[U];
+        walk_ring(
+            a.r, range, ring, a.e.status, [&](EdgeMeta& m, int i) { m.load(a.e, range.e0 + i, range.behind); },
+            [&](int64_t n) {
+                load_row_f<T, VEC, V>(qf, static_cast<const T*>(a.q), n, a.q_stride, cq);
+                s.clear();
+            },
+            [&](const EdgeMeta& meta, int at, int m) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int from = (at + u) & 31;
+                    use[u] = u < m && __shfl_sync(kAll, meta.row, from) >= 0;
+                    bias[u] = 0.0f;
+                    if (a.e.buckets) {
+                        const int b = __shfl_sync(kAll, meta.bucket, from);
+                        if (live) bias[u] = a.e.bias[b * a.h.heads + head];
+                    } else if (a.e.bias) {
+                        const int e = __shfl_sync(kAll, meta.edge, from);
+                        if (live && use[u]) bias[u] = a.e.bias[static_cast<int64_t>(e) * a.h.heads + head];
+                        use[u] = use[u] && bias[u] != -INFINITY;      // masked: whatever k and v hold there
+                    }
+                }
+            },
+            [&](const uint8_t* const (&slot)[U], const EdgeMeta& meta, int at, int m) {
+                float x[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) x[u] = dot_row<T, VEC, V>(slot[u], qf, cq);
+                head_sums<U>(x, a.h.lanes);
+                float top = s.m;
+                bool nan = false;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    x[u] = logit(x[u], a.scale, bias[u], a.e.weight ? __shfl_sync(kAll, meta.log_weight, (at + u) & 31) : 0.0f);
+                    if (!use[u]) x[u] = -INFINITY;
+                    nan = nan || x[u] != x[u];
+                    top = fmaxf(top, x[u]);
+                }
+                if (nan) top = NAN;
+                if (top != s.m) {         // a new maximum: rare after the first edges of a row
+                    const float keep = __expf(s.m - (top == -INFINITY ? 0.0f : top));
+                    s.m = top;
+                    s.l *= keep;
+#pragma unroll
+                    for (int j = 0; j < V; ++j)
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) s.a[0][j][i] *= keep;
+                }
+                const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const float w = __expf(x[u] - ref);
+                    if (w == 0.0f) continue;      // left out, or too small to count: its slot may hold anything
+                    s.l += w;
+                    add_row<T, VEC, V>(slot[u] + a.ring.a_bytes, w, s.a[0], cv);
+                }
+            },
+            [&](int64_t n, bool started, bool ends) {
+                if (!ends) {
+                    goes_on = n;
+                } else if (started) {
+                    finish_row<T, VEC, V>(a, s, n, cv, head, leads);
+                } else {
+                    s.save(a.p.at(part, 0), a.h, cq, cv, head, leads);
+                    ended = static_cast<int>(n);
+                }
+            });
+        if (lane == 0) a.p.ended[part] = ended;
+    }
+    leave_part(a.merge, s, goes_on, part, a.r.parts, a.p, a.h, cq, cv, head, leads, reinterpret_cast<float*>(memory));
 }
 
 template <typename T, int VEC, int V>
@@ -166,7 +261,7 @@ using namespace e3b;
 
 extern "C" int64_t e3b_attention_scratch_bytes(int64_t num_dst, int64_t num_edges, int num_heads, int dim_v) {
     if (num_dst < 0 || num_edges < 0) return 0;
-    return partial_bytes(split_rows(num_dst, num_edges).parts, fwd_slot(num_heads, dim_v));
+    return partial_bytes(most_parts(num_dst, num_edges), fwd_slot(num_heads, dim_v));
 }
 
 extern "C" int e3b_attention_fwd(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride,
@@ -179,37 +274,45 @@ extern "C" int e3b_attention_fwd(const void* q, const void* k, const void* v, in
         return fail(E3B_ERR_ARG, "attention_fwd: bad size or type");
     const int vec = layout[0], heads = layout[1], nqk = layout[2], nv = layout[3], dqk = layout[4], dv = layout[5];
     if (num_dst == 0) return E3B_OK;
-    if (heads < 1 || (vec != 1 && vec != 4)) return fail(E3B_ERR_ARG, "attention_fwd: bad head layout");
-    const int most = vec == 4 ? 8 : 32, lanes = lanes_of_head(heads, std::max(nqk, nv), most);
-    if (lanes == 0) return fail(E3B_ERR_UNSUPPORTED, "attention_fwd: a head of %d columns (at most 1024)", vec * std::max(nqk, nv));
-    const Split s = split_rows(num_dst, num_edges);
+    if (heads < 1 || (vec != 1 && vec != 4 && (vec != 8 || type == kFloat32))) return fail(E3B_ERR_ARG, "attention_fwd: bad head layout");
     if (!q || !rowptr || (num_edges > 0 && num_src > 0 && (!k || !v)) || !qk_table || !v_table || !out || !scratch || !status || (buckets && !bias))
         return fail(E3B_ERR_ARG, "attention_fwd: null pointer");
+    const int size = element_size(type);
+    const RingSource rows{static_cast<const char*>(k), static_cast<const char*>(v), nullptr, k_stride * size, v_stride * size,
+                          static_cast<uint32_t>(dqk * size), static_cast<uint32_t>(dv * size), 0};
+    Plan p;
+    const int planned = plan(&p, "attention_fwd", type, vec, heads, std::max(nqk, nv), num_dst, num_edges, rows, 3, 4, true);
+    if (planned != E3B_OK) return planned;
     if (scratch_bytes < e3b_attention_scratch_bytes(num_dst, num_edges, heads, dv))
         return fail(E3B_ERR_ARG, "attention_fwd: scratch of %lld bytes is too small", static_cast<long long>(scratch_bytes));
-    FwdArgs a{q, k, v, q_stride, k_stride, v_stride, out, out32, stats, scale, {qk_table, v_table, heads, nqk, nv, dqk, dv, lanes},
+    const Split& s = p.s;
+    FwdArgs a{q, k, v, q_stride, k_stride, v_stride, out, out32, stats, scale, {qk_table, v_table, heads, nqk, nv, dqk, dv, p.lanes},
               {perm, edge_src, bias, buckets, edge_weight, num_buckets, num_src, num_edges, status},
-              {rowptr, num_dst, num_edges, s.per_part, s.parts}, partials_in(scratch, s.parts, fwd_slot(heads, dv))};
-    const int groups = static_cast<int>(ceil_div(heads, 32 / lanes));
-    const int v_lane = compiled_vectors(vec, static_cast<int>(ceil_div(std::max(nqk, nv), lanes)));
+              {rowptr, num_dst, num_edges, s.per_part, s.parts}, partials_in(scratch, s.parts, fwd_slot(heads, dv)), s.merge, rows, p.depth,
+              static_cast<uint32_t>(p.warp_smem)};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return by_type_and_vectors(type, vec, v_lane, [&](auto t0, auto vec0, auto v0) -> int {
+    return by_type_and_vectors(type, vec, p.v, [&](auto t0, auto vec0, auto v0) -> int {
         using T = decltype(t0);
         constexpr int VEC = decltype(vec0)::value, V = decltype(v0)::value;
         using S = Sums<VEC, V, 1, true>;
-        const dim3 grid(static_cast<unsigned>(ceil_div(s.parts, s.warps)), groups);
+        const unsigned blocks = static_cast<unsigned>(ceil_div(s.parts, s.warps));
+        const size_t merge_smem = s.merge ? sizeof(float) * 32 * S::kFloats * s.warps : 0;
         int rc = E3B_OK;
-        if (s.merge) {
-            const size_t smem = sizeof(float) * 32 * S::kFloats * s.warps;
-            if ((rc = allow_smem(attn_fwd_kernel<T, VEC, V, true>, smem)) != E3B_OK) return rc;
-            attn_fwd_kernel<T, VEC, V, true><<<grid, 32 * s.warps, smem, st>>>(a);
-        } else {
-            attn_fwd_kernel<T, VEC, V, false><<<grid, 32 * s.warps, 0, st>>>(a);
+        if constexpr (VEC * sizeof(T) == 16) {
+            if (p.ring) {
+                const size_t smem = std::max(p.warp_smem * s.warps, merge_smem);
+                if ((rc = allow_smem(attn_fwd_ring_kernel<T, VEC, V>, smem)) != E3B_OK) return rc;
+                attn_fwd_ring_kernel<T, VEC, V><<<blocks, 32 * s.warps, smem, st>>>(a);
+            }
+        }
+        if (!p.ring) {
+            if ((rc = allow_smem(attn_fwd_kernel<T, VEC, V>, merge_smem)) != E3B_OK) return rc;
+            attn_fwd_kernel<T, VEC, V><<<dim3(blocks, p.groups), 32 * s.warps, merge_smem, st>>>(a);
         }
         if ((rc = check_launch("attention_fwd")) != E3B_OK || s.parts == 1) return rc;
         const size_t smem = s.join_warps > 1 ? sizeof(float) * 32 * S::kFloats * s.join_warps : 0;
         if ((rc = allow_smem(attn_fwd_join_kernel<T, VEC, V>, smem)) != E3B_OK) return rc;
-        attn_fwd_join_kernel<T, VEC, V><<<dim3(s.parts, groups), 32 * s.join_warps, smem, st>>>(a);
+        attn_fwd_join_kernel<T, VEC, V><<<dim3(s.parts, p.groups), 32 * s.join_warps, smem, st>>>(a);
         return check_launch("attention_fwd join");
     });
 }

@@ -15,8 +15,10 @@
 #pragma once
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
+#include "tc_common.cuh"
 #include "typed.cuh"
 
 namespace e3b {
@@ -34,39 +36,46 @@ struct Rows {
     __device__ __forceinline__ int64_t end(int64_t n) const { return min(max(rowptr[n + 1], int64_t{0}), edges); }
 };
 
-// First row whose end lies at item d or later (num: none); 32 probes a step.
-__device__ __forceinline__ int64_t find_row(const Rows& r, int64_t d) {
-    const int lane = threadIdx.x & 31;
+// The slots and rows of one part: rows n0 .. n1 - 1 end in it, row n1 (if there is one) goes on; slots e0 .. e1 - 1, of which those
+// from `behind` on lie behind the last row.
+struct Part {
+    int64_t n0, n1, e0, e1, behind;
+};
+
+// First rows whose end lies at item d0 or later, and at d1 or later (num: none).  Half a warp looks for each, 16 probes a step.
+__device__ __forceinline__ Part find_part(const Rows& r, int part) {
+    const int lane = threadIdx.x & 31, probe = lane & 15;
+    const int64_t d0 = part * r.per_part, d1 = min(d0 + r.per_part, r.num + r.edges), d = lane < 16 ? d0 : d1;
     int64_t lo = 0, hi = r.num;
-    while (lo < hi) {
-        const int64_t step = (hi - lo + 31) / 32, i = lo + lane * step;
-        const unsigned before = __ballot_sync(kAll, i < hi && r.end(i) + i < d);
-        const int c = before == kAll ? 32 : __ffs(~before) - 1;
-        if (c == 0) break;
-        hi = min(hi, lo + c * step);
-        lo += (c - 1) * step + 1;
+    while (__any_sync(kAll, lo < hi)) {
+        const int64_t step = max((hi - lo + 15) / 16, int64_t{1}), i = lo + probe * step;
+        const unsigned before = (__ballot_sync(kAll, i < hi && r.end(i) + i < d) >> (lane & 16)) & 0xffffu;
+        const int c = __ffs(~before) - 1;           // probes in front of the row (16: all)
+        hi = c == 0 ? lo : min(hi, lo + c * step);
+        if (c > 0) lo += (c - 1) * step + 1;
     }
-    return lo;
+    Part p;
+    p.n0 = __shfl_sync(kAll, lo, 0);
+    p.n1 = max(__shfl_sync(kAll, lo, 16), p.n0);
+    p.e0 = min(max(d0 - p.n0, int64_t{0}), r.edges);
+    p.e1 = min(max(d1 - p.n1, p.e0), r.edges);
+    p.behind = p.n1 < r.num ? p.e1 : min(max(r.num > 0 ? r.end(r.num - 1) : 0, p.e0), p.e1);
+    return p;
 }
 
-// The rows of part p: open(n), edges(first, last), close(n, started here, ended here); rest(first, last) are edge slots behind
-// the last row.
-template <typename Open, typename Edges, typename Close, typename Rest>
-__device__ __forceinline__ void walk_rows(const Rows& r, int part, Open&& open, Edges&& edges, Close&& close, Rest&& rest) {
-    int64_t d = part * r.per_part;
-    const int64_t d1 = min(d + r.per_part, r.num + r.edges);
-    int64_t n = find_row(r, d);
-    while (d < d1 && n < r.num) {
-        const int64_t first = r.begin(n), last = r.end(n);
-        const bool ends = last + n < d1;
-        const int64_t e0 = min(max(d - n, first), last), e1 = ends ? last : min(d1 - n, last);
+// The rows of a part in order: open(n), edges(first, last), close(n, started here, ended here).
+template <typename Open, typename Edges, typename Close>
+__device__ __forceinline__ void walk_rows(const Rows& r, const Part& p, Open&& open, Edges&& edges, Close&& close) {
+    int64_t s = p.e0;
+    for (int64_t n = p.n0; n < r.num && (n < p.n1 || s < p.behind); ++n) {
+        const bool ends = n < p.n1, started = n > p.n0 || r.begin(n) == p.e0;
+        const int64_t last = ends ? min(max(r.end(n), s), p.behind) : p.behind;
         open(n);
-        edges(e0, e1);
-        close(n, e0 == first, ends);
-        d = max(d + 1, last + n + 1);
-        ++n;
+        edges(s, last);
+        s = last;
+        close(n, started, ends);
+        if (!ends) break;
     }
-    if (n >= r.num && d < d1) rest(d - r.num, d1 - r.num);
 }
 
 struct Heads {
@@ -290,13 +299,13 @@ struct Sums {
 };
 
 // The end of a part: `sums` are those of the row that goes on (row, -1: none).  Where all warps of the block are inside one
-// row (MERGE: long rows only) their sums are added up here, in the order of the warps, and the first keeps them.
-template <bool MERGE, typename S, int V>
-__device__ __forceinline__ void leave_part(S& sums, int64_t row, int part, int parts, const Partials& out, const Heads& h, const int (&cq)[V],
+// row (looked for where rows are long) their sums are added up here, in the order of the warps, and the first keeps them.
+template <typename S, int V>
+__device__ __forceinline__ void leave_part(bool merge, S& sums, int64_t row, int part, int parts, const Partials& out, const Heads& h, const int (&cq)[V],
                                            const int (&cv)[V], int head, bool leads, float* smem) {
     const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     bool keeps = row >= 0;
-    if (MERGE) {
+    if (merge) {
         __shared__ int64_t row_of[32];
         if ((threadIdx.x & 31) == 0) row_of[warp] = row;
         __syncthreads();
@@ -344,6 +353,194 @@ __device__ __forceinline__ bool join_parts(S& sums, const Rows& r, int part, con
     return true;
 }
 
+// ------------------------------------------------------------------------------------------------- rows through shared memory
+// The two rows of every edge arrive by bulk copies (cp.async.bulk) in a ring of `depth` slots that belongs to one warp: one copy
+// instruction a row, issued by the lane that holds the edge's number, no registers and no address arithmetic of the other lanes
+// while it is under way.  The ring runs ahead over the ends of rows; a slot is refilled as soon as its edges have been used.
+// Every wait is bounded: one that gives up reports status 3, waits (bounded again) for the copies under way and ends the part.
+struct RingSource {
+    const char *a, *b, *c;               // rows by EdgeMeta::row (a, b) and by EdgeMeta::edge (c, may be null)
+    int64_t a_stride, b_stride;          // bytes
+    uint32_t a_bytes, b_bytes, c_bytes;  // of a row, multiples of 16
+    __host__ __device__ uint32_t slot() const { return (a_bytes + b_bytes + c_bytes + 127) / 128 * 128; }
+};
+
+__device__ __forceinline__ void bulk_copy(void* smem, const void* global, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::smem_u32(smem)),
+                 "l"(__cvta_generic_to_global(global)), "r"(bytes), "r"(tc::smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity) {
+    for (uint32_t it = 0; it < 400000u; ++it) {
+        if (tc::mbar_try_wait(bar, parity)) return true;
+        if ((it & 63u) == 63u) __nanosleep(64);
+    }
+    return false;
+}
+
+template <int U, typename Meta>
+struct Ring {
+    const RingSource src;
+    uint8_t* smem;
+    uint64_t* full;
+    int depth, total;             // slots; edges of the part
+    int used, issued;             // edges handed out, edges under way or there
+    int used_at, issued_at;       // their slots
+    uint32_t parity;              // of the slots from used_at on
+    Meta now, next;               // 32 edges each: those of the batch that is being used, and of the one after it
+
+    __device__ __forceinline__ Ring(const RingSource& source, uint8_t* memory, int slots) : src(source), smem(memory), depth(slots) {
+        full = reinterpret_cast<uint64_t*>(memory + static_cast<size_t>(slots) * source.slot());
+        const int lane = threadIdx.x & 31;
+        for (int i = lane; i < depth; i += 32) tc::mbar_init(&full[i], 1);
+        tc::mbar_init_fence();
+        __syncwarp();
+    }
+    // copies of the next m edges (one lane each)
+    __device__ __forceinline__ void issue(int m) {
+        const int lane = threadIdx.x & 31, t = (lane - issued) & 31, i = issued + t;
+        m = min(m, total - issued);
+        if (t < m) {
+            const bool same = (i >> 5) == (used >> 5);
+            const int64_t row = same ? now.row : next.row, edge = same ? now.edge : next.edge;
+            int at = issued_at + t;
+            if (at >= depth) at -= depth;
+            uint64_t* bar = &full[at];
+            if (row >= 0) {
+                uint8_t* slot = smem + static_cast<uint32_t>(at) * src.slot();
+                tc::fence_proxy_async_smem();
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc::smem_u32(bar)), "r"(src.a_bytes + src.b_bytes + src.c_bytes) : "memory");
+                bulk_copy(slot, src.a + row * src.a_stride, src.a_bytes, bar);
+                bulk_copy(slot + src.a_bytes, src.b + row * src.b_stride, src.b_bytes, bar);
+                if (src.c) bulk_copy(slot + src.a_bytes + src.b_bytes, src.c + edge * src.c_bytes, src.c_bytes, bar);
+            } else {
+                tc::mbar_arrive(bar);
+            }
+        }
+        issued += m;
+        issued_at += m;
+        if (issued_at >= depth) issued_at -= depth;
+    }
+    // `load(meta, i)` fetches what lane i & 31 has to know about edge i of the part (nothing from `count` on)
+    template <typename Load>
+    __device__ __forceinline__ void start(int count, Load&& load) {
+        total = count;
+        used = issued = used_at = issued_at = 0;
+        parity = 0;
+        const int lane = threadIdx.x & 31;
+        load(now, lane);
+        load(next, lane + 32);
+        __syncwarp();
+        issue(depth);
+    }
+    // The next m <= U edges, all of one batch: waits for their slots.  False: a wait gave up.
+    __device__ __forceinline__ bool wait(int m, const uint8_t* (&slot)[U]) {
+        bool ok = true;
+        int at = used_at;
+        uint32_t p = parity;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            slot[u] = smem + static_cast<uint32_t>(at) * src.slot();
+            if (u < m) {
+                ok = bounded_wait(&full[at], p) && ok;
+                if (++at == depth) { at = 0; p ^= 1u; }
+            }
+        }
+        return __all_sync(kAll, ok);
+    }
+    // They have been used: their slots take the next edges.
+    template <typename Load>
+    __device__ __forceinline__ void release(int m, Load&& load) {
+        __syncwarp();
+        const int batch = used >> 5;
+        used += m;
+        used_at += m;
+        if (used_at >= depth) { used_at -= depth; parity ^= 1u; }
+        if ((used >> 5) != batch) {
+            now = next;
+            load(next, ((used >> 5) + 1) * 32 + (threadIdx.x & 31));
+        }
+        if (issued < total) issue(m);
+    }
+    // After a wait that gave up: the copies under way must not outlive this warp's shared memory.
+    __device__ __forceinline__ void abandon(int32_t* status) {
+        if ((threadIdx.x & 31) == 0) *status = 3;
+        for (int i = used; i < issued; ++i) {
+            bounded_wait(&full[used_at], parity);
+            if (++used_at == depth) { used_at = 0; parity ^= 1u; }
+        }
+        used = issued = total;
+    }
+};
+
+// walk_rows over a ring: before(meta, lane of the first edge, m) runs ahead of the wait, group(slots, meta, lane, m) uses the edges.
+template <int U, typename Meta, typename Load, typename Open, typename Before, typename Group, typename Close>
+__device__ __forceinline__ void walk_ring(const Rows& r, const Part& p, Ring<U, Meta>& ring, int32_t* status, Load&& load, Open&& open, Before&& before,
+                                          Group&& group, Close&& close) {
+    ring.start(static_cast<int>(p.behind - p.e0), load);
+    bool failed = false;
+    walk_rows(
+        r, p, open,
+        [&](int64_t first, int64_t last) {
+            int left = static_cast<int>(last - first);
+            while (left > 0 && !failed) {
+                const int at = ring.used & 31, m = min(min(U, left), 32 - at);
+                const uint8_t* slot[U];
+                before(ring.now, at, m);
+                failed = !ring.wait(m, slot);
+                if (failed) break;
+                group(slot, ring.now, at, m);
+                ring.release(m, load);
+                left -= m;
+            }
+        },
+        [&](int64_t n, bool started, bool ends) {
+            if (!failed) close(n, started, ends);
+        });
+    if (failed) ring.abandon(status);
+}
+
+// Dots of the lane's columns of a row in shared memory, and products added to a lane's sums.  Columns a lane does not have are left
+// out by a test, not by a zero: what lies there belongs to another head and may be anything.
+template <typename T, int VEC, int V>
+__device__ __forceinline__ float dot_row(const uint8_t* row, const float (&f)[V][VEC], const int (&col)[V]) {
+    float d = 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        if (col[j] < 0) continue;
+        Packed<T, VEC> p;
+        float x[VEC];
+        p.load(reinterpret_cast<const T*>(row) + col[j]);
+        p.unpack(x);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) d = fmaf(f[j][i], x[i], d);
+    }
+    return d;
+}
+template <typename T, int VEC, int V>
+__device__ __forceinline__ void add_row(const uint8_t* row, float by, float (&sum)[V][VEC], const int (&col)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        if (col[j] < 0) continue;
+        Packed<T, VEC> p;
+        float x[VEC];
+        p.load(reinterpret_cast<const T*>(row) + col[j]);
+        p.unpack(x);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sum[j][i] = fmaf(by, x[i], sum[j][i]);
+    }
+}
+// Sums over the lanes of a head of U numbers side by side.
+template <int U>
+__device__ __forceinline__ void head_sums(float (&v)[U], int lanes) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        if (o >= lanes) continue;
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] += __shfl_xor_sync(kAll, v[u], o);
+    }
+}
+
 // ------------------------------------------------------------------------------------------------------------- host side
 struct Split {
     int64_t per_part;
@@ -352,13 +549,15 @@ struct Split {
     int join_warps;
 };
 
-// About four waves of warps; at least 32 items a part (a part costs a search for its row and up to two slots).
-inline Split split_rows(int64_t num, int64_t edges) {
+// Parts of equal size over whole waves of warps (`per_sm` run at a time on an SM), at most about 1,024 items each; at least 16 items a
+// part (a part costs a search for its row and up to two slots).
+inline Split split_rows(int64_t num, int64_t edges, int per_sm) {
     Split s;
-    const int64_t items = std::max<int64_t>(num + edges, 1);
-    s.per_part = std::min<int64_t>(256, std::max<int64_t>(32, ceil_div(items, static_cast<int64_t>(kNumSMs) * 16 * 4)));
+    const int64_t items = std::max<int64_t>(num + edges, 1), wave = static_cast<int64_t>(kNumSMs) * per_sm;
+    const int64_t waves = std::max<int64_t>(1, ceil_div(items, wave * 1024));
+    s.per_part = std::max<int64_t>(16, ceil_div(items, wave * waves));
     s.parts = static_cast<int>(ceil_div(items, s.per_part));
-    s.warps = s.parts >= kNumSMs * 8 ? 8 : 2;
+    s.warps = s.parts >= kNumSMs * 4 ? 4 : 1;
     const int64_t longest = num > 0 ? edges / num : 0;
     s.merge = longest > s.per_part * s.warps;
     s.join_warps = longest > 4 * s.per_part ? 8 : 1;
@@ -372,17 +571,57 @@ inline int lanes_of_head(int heads, int vectors, int most) {
     return vectors <= lanes * most ? lanes : 0;
 }
 
-struct Launch {
-    Heads h;
-    Rows r;
-    Split s;
-    int vec, v, groups;     // vector width, vectors a lane, head groups (grid.y)
-};
-
 // Vectors a lane that are compiled: the next one up is taken.
 inline int compiled_vectors(int vec, int v) {
-    if (vec == 4) return v <= 6 ? v : 8;
+    if (vec > 1) return v <= 6 ? v : 8;
     return v <= 4 ? 4 : v <= 8 ? 8 : v <= 16 ? 16 : 32;
+}
+
+constexpr int kWarpsPerSm[] = {16, 12, 8, 4};    // that the kernels may be launched with
+inline int most_parts(int64_t num, int64_t edges) {
+    int parts = 1;
+    for (int w : kWarpsPerSm) parts = std::max(parts, split_rows(num, edges, w).parts);
+    return parts;
+}
+
+// How a kernel is launched: through the ring where the rows can be copied in bulk (16-byte rows, strides and addresses, vectors of 16
+// bytes) and one warp holds all heads, else by loads into registers.
+struct Plan {
+    int lanes, v, groups;      // lanes of a head, vectors of a lane, head groups (grid.y)
+    bool ring;
+    int depth;
+    size_t warp_smem;          // of the ring
+    Split s;
+};
+
+// Slots of a warp's ring: as many blocks of four warps on an SM as leave `least` slots to a warp (fewer, deeper rings below that).
+inline bool ring_fits(uint32_t slot, int most_blocks, int least, int* blocks, int* depth) {
+    for (*blocks = most_blocks; *blocks >= 1; --*blocks) {
+        const int budget = (227 * 1024 / *blocks - 1024) / 4 - 128;
+        *depth = std::min<int>(16, budget / static_cast<int>(slot + 8));
+        if (*depth >= (*blocks > 1 ? least : 2)) return true;
+    }
+    return false;
+}
+
+inline int most_vectors(int vec) { return vec == 8 ? 4 : vec == 4 ? 8 : 32; }
+
+inline int plan(Plan* p, const char* what, int type, int vec, int heads, int vectors, int64_t num, int64_t edges, const RingSource& rows,
+                int most_blocks, int least, bool may_ring) {
+    p->lanes = lanes_of_head(heads, vectors, most_vectors(vec));
+    if (p->lanes == 0) return fail(E3B_ERR_UNSUPPORTED, "%s: a head of %d columns (at most 1024)", what, vec * vectors);
+    p->groups = static_cast<int>(ceil_div(heads, 32 / p->lanes));
+    p->v = compiled_vectors(vec, static_cast<int>(ceil_div(vectors, p->lanes)));
+    int blocks = 2;
+    p->ring = may_ring && vec * element_size(type) == 16 && p->groups == 1 && ((rows.a_bytes | rows.b_bytes | rows.c_bytes) & 15) == 0 &&
+              ((rows.a_stride | rows.b_stride) & 15) == 0 && aligned_to(rows.a, 16) && aligned_to(rows.b, 16) && aligned_to(rows.c, 16) &&
+              ring_fits(rows.slot(), most_blocks, least, &blocks, &p->depth);
+    p->s = split_rows(num, edges, p->ring ? 4 * blocks : 8);
+    if (p->ring) {
+        if (p->s.warps == 1) p->depth = std::min<int>(16, (200 * 1024) / static_cast<int>(rows.slot() + 8));
+        p->warp_smem = ceil_div(static_cast<int64_t>(p->depth) * (rows.slot() + 8), 128) * 128;
+    }
+    return E3B_OK;
 }
 
 template <typename T, typename F>
@@ -396,6 +635,16 @@ int by_vectors(int vec, int v, F&& f) {
             case 5: return f(T(), Int<4>(), Int<5>());
             case 6: return f(T(), Int<4>(), Int<6>());
             default: return f(T(), Int<4>(), Int<8>());
+        }
+    }
+    if constexpr (sizeof(T) == 2) {
+        if (vec == 8) {
+            switch (v) {
+                case 1: return f(T(), Int<8>(), Int<1>());
+                case 2: return f(T(), Int<8>(), Int<2>());
+                case 3: return f(T(), Int<8>(), Int<3>());
+                default: return f(T(), Int<8>(), Int<4>());
+            }
         }
     }
     switch (v) {

@@ -17,16 +17,64 @@ struct BwdArgs {
     int64_t q_stride, k_stride, v_stride;
     const float *out32, *stats;
     void *grad_q, *grad_k, *grad_v;      // grad_k, grad_v: per edge, or null
-    float *p, *da;                       // [edges, heads] or null
+    float2* share;                       // [edges, even(heads)] {p, da} or null
+    float* da;                           // [edges, heads] or null
     int32_t* dst;                        // [edges] or null: destination of every edge
     float scale;
     Heads h;
     Edges e;
     Rows r;
     Partials parts;
+    bool merge;
+    RingSource ring;
+    int depth;
+    uint32_t warp_smem;
+    __device__ __forceinline__ float2* share_of(int64_t edge) const { return share + edge * ((h.heads + 1) & ~1); }
 };
 
-template <typename T, int VEC, int V, bool MERGE>
+// q, cotangent and statistics of a row; returns delta.  (The output enters unrounded, in the order of the dots g v: an edge alone in
+// its row gives the same number.)
+template <typename T, int VEC, int V>
+__device__ __forceinline__ float open_row(const BwdArgs& a, int64_t n, const int (&cq)[V], const int (&cv)[V], int head, bool live, float (&qf)[V][VEC],
+                                          float (&gf)[V][VEC], float* top, float* inv) {
+    load_row_f<T, VEC, V>(qf, static_cast<const T*>(a.q), n, a.q_stride, cq);
+    load_row_f<T, VEC, V>(gf, static_cast<const T*>(a.grad_out), n, a.h.dv, cv);
+    float d = 0.0f, o[V][VEC];
+    load_row_f<float, VEC, V>(o, a.out32, n, a.h.dv, cv);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) d = fmaf(gf[j][i], o[j][i], d);
+    if (live) {
+        *top = a.stats[(n * a.h.heads + head) * 2];
+        *inv = a.stats[(n * a.h.heads + head) * 2 + 1];
+    }
+    return head_sum(d, a.h.lanes);
+}
+
+// Slots behind the last row take part in nothing: their gradients are zero.
+template <typename T, int VEC, int V>
+__device__ __forceinline__ void clear_behind(const BwdArgs& a, const Part& range, const int (&cq)[V], const int (&cv)[V], int head, bool leads) {
+    if (range.behind >= range.e1) return;
+    float zero[V][VEC];
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) zero[j][i] = 0.0f;
+    for (int64_t slot = range.behind; slot < range.e1; ++slot) {
+        const int64_t e = a.e.perm ? a.e.perm[slot] : slot;
+        if (e < 0 || e >= a.e.edges) continue;
+        if (a.dst && blockIdx.y == 0 && (threadIdx.x & 31) == 0) a.dst[e] = -1;
+        if (leads && a.share) a.share_of(e)[head] = make_float2(0.0f, 0.0f);
+        if (leads && a.da) a.da[e * a.h.heads + head] = 0.0f;
+        if (a.grad_k) {
+            store_row<T, VEC, V>(static_cast<T*>(a.grad_k), e, a.h.dqk, cq, zero, 0.0f);
+            store_row<T, VEC, V>(static_cast<T*>(a.grad_v), e, a.h.dv, cv, zero, 0.0f);
+        }
+    }
+}
+
+template <typename T, int VEC, int V>
 __global__ void __launch_bounds__(256) attn_bwd_dst_kernel(const BwdArgs a) {
     extern __shared__ float smem[];
     constexpr int U = edges_in_flight(V, words_of<T, VEC>(), 64);
@@ -45,23 +93,12 @@ __global__ void __launch_bounds__(256) attn_bwd_dst_kernel(const BwdArgs a) {
     if (part < a.r.parts) {
         float qf[V][VEC], gf[V][VEC], delta = 0.0f, top = 0.0f, inv = 0.0f;
         int row_now = 0;
+        const Part range = find_part(a.r, part);
         walk_rows(
-            a.r, part,
+            a.r, range,
             [&](int64_t n) {
                 row_now = static_cast<int>(n);
-                load_row_f<T, VEC, V>(qf, static_cast<const T*>(a.q), n, a.q_stride, cq);
-                load_row_f<T, VEC, V>(gf, static_cast<const T*>(a.grad_out), n, a.h.dv, cv);
-                float d = 0.0f, o[V][VEC];
-                load_row_f<float, VEC, V>(o, a.out32, n, a.h.dv, cv);
-#pragma unroll
-                for (int j = 0; j < V; ++j)
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) d = fmaf(gf[j][i], o[j][i], d);
-                delta = head_sum(d, a.h.lanes);
-                if (live) {
-                    top = a.stats[(n * a.h.heads + head) * 2];
-                    inv = a.stats[(n * a.h.heads + head) * 2 + 1];
-                }
+                delta = open_row<T, VEC, V>(a, n, cq, cv, head, live, qf, gf, &top, &inv);
                 s.clear();
             },
             [&](int64_t first, int64_t last) {
@@ -117,7 +154,7 @@ __global__ void __launch_bounds__(256) attn_bwd_dst_kernel(const BwdArgs a) {
 #pragma unroll
                                 for (int i = 0; i < VEC; ++i) s.a[0][j][i] = fmaf(da, kf[j][i], s.a[0][j][i]);
                             if (edge[u] < 0) continue;
-                            if (leads && a.p) a.p[static_cast<int64_t>(edge[u]) * a.h.heads + head] = p;
+                            if (leads && a.share) a.share_of(edge[u])[head] = make_float2(p, da);
                             if (leads && a.da) a.da[static_cast<int64_t>(edge[u]) * a.h.heads + head] = da;
                             if (a.grad_k) {
                                 store_row<T, VEC, V>(static_cast<T*>(a.grad_k), edge[u], a.h.dqk, cq, qf, a.scale * da);
@@ -136,29 +173,99 @@ __global__ void __launch_bounds__(256) attn_bwd_dst_kernel(const BwdArgs a) {
                     s.save(a.parts.at(part, 0), a.h, cq, cv, head, leads);
                     ended = static_cast<int>(n);
                 }
-            },
-            // slots behind the last row take part in nothing: their gradients are zero
-            [&](int64_t first, int64_t last) {
-                float zero[V][VEC];
-#pragma unroll
-                for (int j = 0; j < V; ++j)
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) zero[j][i] = 0.0f;
-                for (int64_t slot = max(first, int64_t{0}); slot < min(last, a.r.edges); ++slot) {
-                    const int64_t e = a.e.perm ? a.e.perm[slot] : slot;
-                    if (e < 0 || e >= a.e.edges) continue;
-                    if (a.dst && blockIdx.y == 0 && lane == 0) a.dst[e] = -1;
-                    if (leads && a.p) a.p[e * a.h.heads + head] = 0.0f;
-                    if (leads && a.da) a.da[e * a.h.heads + head] = 0.0f;
-                    if (a.grad_k) {
-                        store_row<T, VEC, V>(static_cast<T*>(a.grad_k), e, a.h.dqk, cq, zero, 0.0f);
-                        store_row<T, VEC, V>(static_cast<T*>(a.grad_v), e, a.h.dv, cv, zero, 0.0f);
-                    }
-                }
             });
+        clear_behind<T, VEC, V>(a, range, cq, cv, head, leads);
         if (blockIdx.y == 0 && lane == 0) a.parts.ended[part] = ended;
     }
-    leave_part<MERGE>(s, goes_on, part, a.r.parts, a.parts, a.h, cq, cv, head, leads, smem);
+    leave_part(a.merge, s, goes_on, part, a.r.parts, a.parts, a.h, cq, cv, head, leads, smem);
+}
+
+// The same with k and v through the ring.
+template <typename T, int VEC, int V>
+__global__ void __launch_bounds__(128, 3) attn_bwd_dst_ring_kernel(const BwdArgs a) {
+    extern __shared__ __align__(128) uint8_t memory[];
+    constexpr int U = V * VEC <= 12 ? 4 : 2;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = blockIdx.x * (blockDim.x >> 5) + warp;
+    const int head = lane / a.h.lanes;
+    const bool live = head < a.h.heads, leads = live && (lane & (a.h.lanes - 1)) == 0;
+    int cq[V], cv[V];
+    lane_columns<V>(a.h.qk, a.h.nqk, a.h.lanes, head, live, cq);
+    lane_columns<V>(a.h.v, a.h.nv, a.h.lanes, head, live, cv);
+    Sums<VEC, V, 1, false> s;
+    s.clear();
+    int64_t goes_on = -1;
+    int ended = -1;
+    if (part < a.r.parts) {
+        const Part range = find_part(a.r, part);
+        Ring<U, EdgeMeta> ring(a.ring, memory + warp * a.warp_smem, a.depth);
+        float qf[V][VEC], gf[V][VEC], delta = 0.0f, top = 0.0f, inv = 0.0f, bias[U];
+        int edge[U], row_now = 0;
+        bool use[U];
+        walk_ring(
+            a.r, range, ring, a.e.status, [&](EdgeMeta& m, int i) { m.load(a.e, range.e0 + i, range.behind); },
+            [&](int64_t n) {
+                row_now = static_cast<int>(n);
+                delta = open_row<T, VEC, V>(a, n, cq, cv, head, live, qf, gf, &top, &inv);
+                s.clear();
+            },
+            [&](const EdgeMeta& meta, int at, int m) {
+                if (a.dst && lane >= at && lane < at + m && meta.edge >= 0) a.dst[meta.edge] = row_now;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int from = (at + u) & 31;
+                    edge[u] = __shfl_sync(kAll, meta.edge, from);
+                    if (u >= m) edge[u] = -1;
+                    use[u] = __shfl_sync(kAll, meta.row, from) >= 0 && edge[u] >= 0;
+                    bias[u] = 0.0f;
+                    if (a.e.buckets) {
+                        const int b = __shfl_sync(kAll, meta.bucket, from);
+                        if (live) bias[u] = a.e.bias[b * a.h.heads + head];
+                    } else if (a.e.bias) {
+                        if (live && use[u]) bias[u] = a.e.bias[static_cast<int64_t>(edge[u]) * a.h.heads + head];
+                        use[u] = use[u] && bias[u] != -INFINITY;
+                    }
+                }
+            },
+            [&](const uint8_t* const (&slot)[U], const EdgeMeta& meta, int at, int m) {
+                float x[2 * U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    x[u] = dot_row<T, VEC, V>(slot[u], qf, cq);
+                    x[U + u] = dot_row<T, VEC, V>(slot[u] + a.ring.a_bytes, gf, cv);
+                }
+                head_sums<2 * U>(x, a.h.lanes);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const float lw = a.e.weight ? __shfl_sync(kAll, meta.log_weight, (at + u) & 31) : 0.0f;
+                    if (edge[u] < 0) continue;
+                    float p = 0.0f, da = 0.0f;
+                    if (use[u]) {
+                        p = __expf(logit(x[u], a.scale, bias[u], lw) - top) * inv;
+                        da = p == 0.0f ? 0.0f : p * (x[U + u] - delta);
+                    }
+                    if (da != 0.0f) add_row<T, VEC, V>(slot[u], da, s.a[0], cq);
+                    if (leads && a.share) a.share_of(edge[u])[head] = make_float2(p, da);
+                    if (leads && a.da) a.da[static_cast<int64_t>(edge[u]) * a.h.heads + head] = da;
+                    if (a.grad_k) {
+                        store_row<T, VEC, V>(static_cast<T*>(a.grad_k), edge[u], a.h.dqk, cq, qf, a.scale * da);
+                        store_row<T, VEC, V>(static_cast<T*>(a.grad_v), edge[u], a.h.dv, cv, gf, p);
+                    }
+                }
+            },
+            [&](int64_t n, bool started, bool ends) {
+                if (!ends) {
+                    goes_on = n;
+                } else if (started) {
+                    store_row<T, VEC, V>(static_cast<T*>(a.grad_q), n, a.h.dqk, cq, s.a[0], a.scale);
+                } else {
+                    s.save(a.parts.at(part, 0), a.h, cq, cv, head, leads);
+                    ended = static_cast<int>(n);
+                }
+            });
+        clear_behind<T, VEC, V>(a, range, cq, cv, head, leads);
+        if (lane == 0) a.parts.ended[part] = ended;
+    }
+    leave_part(a.merge, s, goes_on, part, a.r.parts, a.parts, a.h, cq, cv, head, leads, reinterpret_cast<float*>(memory));
 }
 
 template <typename T, int VEC, int V>
@@ -195,7 +302,7 @@ using namespace e3b;
 
 extern "C" int64_t e3b_attention_bwd_scratch_bytes(int64_t num_dst, int64_t num_edges, int dim_qk) {
     if (num_dst < 0 || num_edges < 0) return 0;
-    return partial_bytes(split_rows(num_dst, num_edges).parts, dq_slot(dim_qk));
+    return partial_bytes(most_parts(num_dst, num_edges), dq_slot(dim_qk));
 }
 
 extern "C" int e3b_attention_bwd(const void* q, const void* k, const void* v, const void* grad_out, int64_t q_stride, int64_t k_stride,
@@ -208,40 +315,48 @@ extern "C" int e3b_attention_bwd(const void* q, const void* k, const void* v, co
     if (!layout || num_dst < 0 || num_src < 0 || num_edges < 0 || num_edges >= INT32_MAX || num_dst >= INT32_MAX || num_src >= INT32_MAX || !known_type(type))
         return fail(E3B_ERR_ARG, "attention_bwd: bad size or type");
     const int vec = layout[0], heads = layout[1], nqk = layout[2], nv = layout[3], dqk = layout[4], dv = layout[5];
-    if (heads < 1 || (vec != 1 && vec != 4)) return fail(E3B_ERR_ARG, "attention_bwd: bad head layout");
-    const int most = vec == 4 ? 8 : 32, lanes = lanes_of_head(heads, std::max(nqk, nv), most);
-    if (lanes == 0) return fail(E3B_ERR_UNSUPPORTED, "attention_bwd: a head of %d columns (at most 1024)", vec * std::max(nqk, nv));
+    if (heads < 1 || (vec != 1 && vec != 4 && (vec != 8 || type == kFloat32))) return fail(E3B_ERR_ARG, "attention_bwd: bad head layout");
     if (num_dst == 0 && num_edges == 0) return E3B_OK;
-    const Split s = split_rows(num_dst, num_edges);
     if ((num_dst > 0 && (!q || !grad_out || !out32 || !stats || !grad_q)) || !rowptr || (num_edges > 0 && num_src > 0 && (!k || !v)) || !qk_table ||
-        !v_table || !scratch || !status || (buckets && !bias) || !grad_k != !grad_v || (grad_weight && (!edge_weight || !grad_logit)))
+        !v_table || !scratch || !status || (share && !aligned_to(share, 16)) || (buckets && !bias) || !grad_k != !grad_v || (grad_weight && (!edge_weight || !grad_logit)))
         return fail(E3B_ERR_ARG, "attention_bwd: null pointer");
     if (scratch_bytes < e3b_attention_bwd_scratch_bytes(num_dst, num_edges, dqk))
         return fail(E3B_ERR_ARG, "attention_bwd: scratch of %lld bytes is too small", static_cast<long long>(scratch_bytes));
-    BwdArgs a{q, k, v, grad_out, q_stride, k_stride, v_stride, out32, stats, grad_q, grad_k, grad_v, share, grad_logit, edge_dst, scale,
-              {qk_table, v_table, heads, nqk, nv, dqk, dv, lanes},
+    const int size = element_size(type);
+    const RingSource rows{static_cast<const char*>(k), static_cast<const char*>(v), nullptr, k_stride * size, v_stride * size,
+                          static_cast<uint32_t>(dqk * size), static_cast<uint32_t>(dv * size), 0};
+    Plan p;
+    const int planned = plan(&p, "attention_bwd", type, vec, heads, std::max(nqk, nv), num_dst, num_edges, rows, 3, 4, true);
+    if (planned != E3B_OK) return planned;
+    const Split& s = p.s;
+    BwdArgs a{q, k, v, grad_out, q_stride, k_stride, v_stride, out32, stats, grad_q, grad_k, grad_v, reinterpret_cast<float2*>(share), grad_logit,
+              edge_dst, scale, {qk_table, v_table, heads, nqk, nv, dqk, dv, p.lanes},
               {perm, edge_src, bias, buckets, edge_weight, num_buckets, num_src, num_edges, status},
-              {rowptr, num_dst, num_edges, s.per_part, s.parts}, partials_in(scratch, s.parts, dq_slot(dqk))};
-    const int groups = static_cast<int>(ceil_div(heads, 32 / lanes));
-    const int v_lane = compiled_vectors(vec, static_cast<int>(ceil_div(std::max(nqk, nv), lanes)));
+              {rowptr, num_dst, num_edges, s.per_part, s.parts}, partials_in(scratch, s.parts, dq_slot(dqk)), s.merge, rows, p.depth,
+              static_cast<uint32_t>(p.warp_smem)};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int rc = by_type_and_vectors(type, vec, v_lane, [&](auto t0, auto vec0, auto v0) -> int {
+    const int rc = by_type_and_vectors(type, vec, p.v, [&](auto t0, auto vec0, auto v0) -> int {
         using T = decltype(t0);
         constexpr int VEC = decltype(vec0)::value, V = decltype(v0)::value;
         using S = Sums<VEC, V, 1, false>;
-        const dim3 grid(static_cast<unsigned>(ceil_div(s.parts, s.warps)), groups);
+        const unsigned blocks = static_cast<unsigned>(ceil_div(s.parts, s.warps));
+        const size_t merge_smem = s.merge ? sizeof(float) * 32 * S::kFloats * s.warps : 0;
         int r = E3B_OK;
-        if (s.merge) {
-            const size_t smem = sizeof(float) * 32 * S::kFloats * s.warps;
-            if ((r = allow_smem(attn_bwd_dst_kernel<T, VEC, V, true>, smem)) != E3B_OK) return r;
-            attn_bwd_dst_kernel<T, VEC, V, true><<<grid, 32 * s.warps, smem, st>>>(a);
-        } else {
-            attn_bwd_dst_kernel<T, VEC, V, false><<<grid, 32 * s.warps, 0, st>>>(a);
+        if constexpr (VEC * sizeof(T) == 16) {
+            if (p.ring) {
+                const size_t smem = std::max(p.warp_smem * s.warps, merge_smem);
+                if ((r = allow_smem(attn_bwd_dst_ring_kernel<T, VEC, V>, smem)) != E3B_OK) return r;
+                attn_bwd_dst_ring_kernel<T, VEC, V><<<blocks, 32 * s.warps, smem, st>>>(a);
+            }
+        }
+        if (!p.ring) {
+            if ((r = allow_smem(attn_bwd_dst_kernel<T, VEC, V>, merge_smem)) != E3B_OK) return r;
+            attn_bwd_dst_kernel<T, VEC, V><<<dim3(blocks, p.groups), 32 * s.warps, merge_smem, st>>>(a);
         }
         if ((r = check_launch("attention_bwd")) != E3B_OK || s.parts == 1) return r;
         const size_t smem = s.join_warps > 1 ? sizeof(float) * 32 * S::kFloats * s.join_warps : 0;
         if ((r = allow_smem(attn_bwd_dst_join_kernel<T, VEC, V>, smem)) != E3B_OK) return r;
-        attn_bwd_dst_join_kernel<T, VEC, V><<<dim3(s.parts, groups), 32 * s.join_warps, smem, st>>>(a);
+        attn_bwd_dst_join_kernel<T, VEC, V><<<dim3(s.parts, p.groups), 32 * s.join_warps, smem, st>>>(a);
         return check_launch("attention_bwd join");
     });
     if (rc != E3B_OK || !grad_weight || num_edges == 0) return rc;

@@ -59,6 +59,35 @@ template <typename T> struct Packed<T, 4> {
     }
 };
 
+template <typename T> struct Packed<T, 8> {
+    uint4 v;
+    __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void zero() { v = make_uint4(0u, 0u, 0u, 0u); }
+    __device__ __forceinline__ void unpack(float* f) const {
+        const float2 a = Pair<T>::load(v.x), b = Pair<T>::load(v.y), c = Pair<T>::load(v.z), d = Pair<T>::load(v.w);
+        f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y; f[4] = c.x; f[5] = c.y; f[6] = d.x; f[7] = d.y;
+    }
+    static __device__ __forceinline__ void store(T* p, const float* f) {
+        *reinterpret_cast<uint4*>(p) = make_uint4(Pair<T>::store(f[0], f[1]), Pair<T>::store(f[2], f[3]), Pair<T>::store(f[4], f[5]),
+                                                  Pair<T>::store(f[6], f[7]));
+    }
+};
+template <> struct Packed<float, 8> {
+    float4 lo, hi;
+    __device__ __forceinline__ void load(const float* p) {
+        lo = *reinterpret_cast<const float4*>(p);
+        hi = *reinterpret_cast<const float4*>(p + 4);
+    }
+    __device__ __forceinline__ void zero() { lo = hi = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
+    __device__ __forceinline__ void unpack(float* f) const {
+        f[0] = lo.x; f[1] = lo.y; f[2] = lo.z; f[3] = lo.w; f[4] = hi.x; f[5] = hi.y; f[6] = hi.z; f[7] = hi.w;
+    }
+    static __device__ __forceinline__ void store(float* p, const float* f) {
+        *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+        *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+    }
+};
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

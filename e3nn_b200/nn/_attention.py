@@ -33,8 +33,9 @@ def _head_vectors(irreps: Irreps, heads: int, vec: int) -> torch.Tensor:
     return torch.tensor(out, dtype=torch.int32).reshape(-1, 2)
 
 
-def _fits_fours(t: torch.Tensor) -> bool:
-    return t.data_ptr() % (4 * t.element_size()) == 0 and t.stride(0) % 4 == 0
+def _fits(t: torch.Tensor, vec: int) -> bool:
+    """Whether every row starts on a vector of `vec` elements."""
+    return t.data_ptr() % (vec * t.element_size()) == 0 and t.stride(0) % vec == 0
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -81,15 +82,15 @@ class _AttentionFunction(torch.autograd.Function):
         N, S, E, dev, type_code, core = q.shape[0], k.shape[0], c.edges, q.device, _lib.element_type(q), _lib.core()
         _, need_k, need_v, need_bias, need_weight = ctx.needs_input_grad[:5]
         grad = grad.contiguous()
-        if c.vec == 4 and not _fits_fours(grad):
+        if not _fits(grad, c.vec):
             grad = grad.clone()
         per_node = c.src is not None and (need_k or need_v)
         per_edge = c.src is None and (need_k or need_v)
         gq = torch.empty(N, dqk, dtype=q.dtype, device=dev)
         gk = torch.empty(S, dqk, dtype=q.dtype, device=dev) if need_k or need_v else None
         gv = torch.empty(S, dv, dtype=q.dtype, device=dev) if need_k or need_v else None
-        share = torch.empty(E, H, dtype=torch.float32, device=dev) if per_node else None
-        da = torch.empty(E, H, dtype=torch.float32, device=dev) if per_node or need_bias or need_weight else None
+        share = torch.empty(E, (H + 1) // 2 * 2, 2, dtype=torch.float32, device=dev) if per_node else None
+        da = torch.empty(E, H, dtype=torch.float32, device=dev) if need_bias or need_weight else None
         dst = torch.empty(E, dtype=torch.int32, device=dev) if per_node else None
         gweight = torch.empty(E, dtype=torch.float32, device=dev) if need_weight else None
         nbytes = core.e3b_attention_bwd_scratch_bytes(N, E, dqk)
@@ -109,7 +110,7 @@ class _AttentionFunction(torch.autograd.Function):
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
             with _lib.device_of(q), _lib.nvtx_range("e3b_attention_bwd_src"):
                 rc = core.e3b_attention_bwd_src(
-                    _lib._ptr(q), _lib._ptr(grad), q.stride(0), _lib._ptr(share), _lib._ptr(da), _lib._ptr(dst), _lib._ptr(perm_t), _lib._ptr(rowptr_t),
+                    _lib._ptr(q), _lib._ptr(grad), q.stride(0), _lib._ptr(share), _lib._ptr(dst), _lib._ptr(perm_t), _lib._ptr(rowptr_t),
                     _lib._ptr(c.qk_tbl), _lib._ptr(c.v_tbl), c.layout, c.scale, N, S, E, type_code, _lib._ptr(gk), _lib._ptr(gv), _lib._ptr(scratch),
                     nbytes, status, _lib.stream_ptr())
             _lib.check(rc, "e3b_attention_bwd_src")
@@ -139,9 +140,11 @@ class NeighborAttention(torch.nn.Module):
             if irreps.dim // self.num_heads > MAX_HEAD_COLUMNS:
                 raise NotImplementedError(f"{irreps.dim // self.num_heads} columns a head, at most {MAX_HEAD_COLUMNS} are supported")
         self.scale = float(scale) if scale is not None else (self.irreps_qk.dim // self.num_heads) ** -0.5
-        self._fours = all(mul // self.num_heads * ir.dim % 4 == 0 for irreps in (self.irreps_qk, self.irreps_v) for mul, ir in irreps)
         self._layouts = {}
-        for vec in (1, 4) if self._fours else (1,):
+        runs = [mul // self.num_heads * ir.dim for irreps in (self.irreps_qk, self.irreps_v) for mul, ir in irreps]
+        for vec in (1, 4, 8):
+            if any(run % vec for run in runs):
+                break
             tables = [_head_vectors(irreps, self.num_heads, vec) for irreps in (self.irreps_qk, self.irreps_v)]
             self.register_buffer(f"_qk{vec}", tables[0], persistent=False)
             self.register_buffer(f"_v{vec}", tables[1], persistent=False)
@@ -206,9 +209,12 @@ class NeighborAttention(torch.nn.Module):
         _lib.poll_status(q.device)
         q, k, v = _rows(q), _rows(k), _rows(v)
         c = _Call()
-        c.vec = 4 if self._fours and _fits_fours(q) and _fits_fours(k) and _fits_fours(v) else 1
+        # vectors of 16 bytes where the layout and the rows allow them, else of four elements, else single elements
+        for c.vec in (4, 1) if q.dtype == torch.float32 else (8, 4, 1):
+            if c.vec in self._layouts and _fits(q, c.vec) and _fits(k, c.vec) and _fits(v, c.vec):
+                break
         c.layout = (ctypes.c_int32 * 6)(*self._layouts[c.vec])
-        c.qk_tbl, c.v_tbl = (self._qk4, self._v4) if c.vec == 4 else (self._qk1, self._v1)
+        c.qk_tbl, c.v_tbl = getattr(self, f"_qk{c.vec}"), getattr(self, f"_v{c.vec}")
         c.scale, c.edges = self.scale, E
         c.rowptr, c.src = rowptr.contiguous(), None if edge_src is None else edge_src.contiguous()
         c.perm, c.buckets = None if perm is None else perm.contiguous(), None if buckets is None else buckets.contiguous()

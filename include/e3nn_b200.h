@@ -341,16 +341,18 @@ int e3b_relative_bias_bwd(const void* grad_bias, const int32_t* buckets, int num
  * out [num_dst, dv] dense.  bias NULL, [num_edges, heads] (-inf: masked, k and v unread), or with buckets [num_edges] a table
  * [num_buckets, heads].  edge_weight NULL or [num_edges]; an edge with a weight <= 0 is left out and its rows are unread.
  * A row without edges (or all left out) is zero.  An index out of range sets *status = 2, its edge is left out.
- * layout: HOST array {vector width 1 or 4, heads, vectors of a head of q and k, of v, columns of q and k, of v}; qk_table, v_table:
- * per vector {column of head 0, columns from one head to the next}; width 4 needs pointers and strides in multiples of four elements.
+ * layout: HOST array {vector width 1, 4 or (16-bit types) 8, heads, vectors of a head of q and k, of v, columns of q and k, of v}; qk_table, v_table:
+ * per vector {column of head 0, columns from one head to the next}; a width
+ * above 1 needs pointers and strides in multiples of it.
  * A head has at most 1,024 columns (E3B_ERR_UNSUPPORTED).  Fewer than 2^31 - 1 edges and rows.
  * out32 (NULL or the output in fp32) and stats [num_dst, heads, 2] (NULL or maximum and reciprocal of the sum) are what the
  * gradient needs; with type 0 out itself serves as out32.
  *
  * e3b_attention_bwd: grad_q [num_dst, dqk]; k and v per edge (edge_src NULL): grad_k, grad_v per edge (both or neither).  Optional, per
- * edge: share [num_edges, heads], grad_logit [num_edges, heads] (the gradient of bias), edge_dst [num_edges] (destination, -1: none),
+ * edge: share [num_edges, heads rounded up to even, 2] {softmax, its gradient's logit part} (16-byte aligned), grad_logit [num_edges, heads]
+ * (the gradient of bias), edge_dst [num_edges] (destination, -1: none),
  * grad_weight [num_edges] (needs grad_logit).
- * e3b_attention_bwd_src: grad_k and grad_v of nodes from share, grad_logit and edge_dst and the CSR by source (e3b_csr_from_dst of
+ * e3b_attention_bwd_src: grad_k and grad_v of nodes from share and edge_dst and the CSR by source (e3b_csr_from_dst of
  * edge_src: src_perm, src_rowptr).  All sums have a fixed order.
  */
 int64_t e3b_attention_scratch_bytes(int64_t num_dst, int64_t num_edges, int num_heads, int dim_v);
@@ -369,8 +371,8 @@ int e3b_attention_bwd(const void* q, const void* k, const void* v, const void* g
                       void* grad_v, float* share, float* grad_logit, int32_t* edge_dst, float* grad_weight, void* scratch,
                       int64_t scratch_bytes, int32_t* status, void* stream);
 int64_t e3b_attention_bwd_src_scratch_bytes(int64_t num_src, int64_t num_edges, int dim_qk, int dim_v);
-int e3b_attention_bwd_src(const void* q, const void* grad_out, int64_t q_stride, const float* share, const float* grad_logit,
-                          const int32_t* edge_dst, const int64_t* src_perm, const int64_t* src_rowptr, const int32_t* qk_table,
+int e3b_attention_bwd_src(const void* q, const void* grad_out, int64_t q_stride, const float* share, const int32_t* edge_dst,
+                          const int64_t* src_perm, const int64_t* src_rowptr, const int32_t* qk_table,
                           const int32_t* v_table, const int32_t* layout, float scale, int64_t num_dst, int64_t num_src,
                           int64_t num_edges, int type, void* grad_k, void* grad_v, void* scratch, int64_t scratch_bytes,
                           int32_t* status, void* stream);
