@@ -65,6 +65,11 @@ def _fp32(parameter: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return None if parameter is None else parameter.to(torch.float32).contiguous()
 
 
+def _aligned(t: torch.Tensor, width: int) -> torch.Tensor:
+    """`t`, or a copy of it where it does not start on a vector of `width` elements."""
+    return t if t.data_ptr() % (width * t.element_size()) == 0 else t.clone()
+
+
 def _flat_rows(x: torch.Tensor, dim: int, name: str) -> torch.Tensor:
     _lib.element_type(x, name)
     torch._assert(x.dim() > 0 and x.shape[-1] == dim, f"Incorrect last dimension for {name}")
@@ -145,20 +150,44 @@ class RMSNorm(torch.nn.Module):
         return out.reshape(x.shape)
 
 
+def _gate_items(back, const, forth, ins, outs, width: int) -> Optional[List[List[int]]]:
+    """The row as items of `width` columns, `None` where it does not fall into such items (see ``e3b_norm_gate_residual_fwd``).
+    `back`, `const`: per input column {kind, first output column, count, partner column, activation} and constant; `forth`: per
+    output column {input column, gate column or -1, ..}."""
+    out_of = {row[0]: j for j, row in enumerate(forth)}                       # input column -> output column
+    slot_of = {c: n for n, c in enumerate(c for c, row in enumerate(back) if row[0] == 2)}
+    in_blk, out_blk = [b for b, _ in _column_blocks(ins)], [b for b, _ in _column_blocks(outs)]
+    if len(back) % width or len(forth) % width:
+        return None
+    items = []
+    for c in range(0, len(back), width):
+        cols = range(c, c + width)
+        kind, act = back[c][0], back[c][4] if back[c][0] in (0, 2) else 3
+        j = out_of.get(c, -1)
+        alike = all(back[x][0] == kind and in_blk[x] == in_blk[c] and out_of.get(x, -1) == (j + x - c if j >= 0 else -1)
+                    and (kind not in (0, 2) or (back[x][4] == act and const[x] == const[c])) for x in cols)
+        if not alike or (j >= 0 and (j % width or out_blk[j + width - 1] != out_blk[j])) or (kind == 2 and slot_of[c] % width):
+            return None
+        gates = [slot_of[forth[out_of[x]][1]] if kind == 1 else 0 for x in cols]
+        items.append([kind, c, j, in_blk[c], out_blk[j] if j >= 0 else -1, act, _float_bits(const[c] if kind in (0, 2) else 1.0),
+                      slot_of[c] if kind == 2 else 0, *gates])
+    return items
+
+
 class _NormGateFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, residual, y, w_post, scale, w_pre, tables, sizes, fours, eps):
-        in_tbl, out_tbl, _, _, _, in_inv, out_inv = tables
+    def forward(ctx, residual, y, w_post, scale, w_pre, tables, sizes, eps):
+        items, in_tbl, out_tbl, _, _, in_inv, out_inv = tables
         z = torch.empty_like(residual)
         h = torch.empty_like(residual) if w_pre is not None else None
         with _lib.device_of(y):
             rc = _lib.core().e3b_norm_gate_residual_fwd(
-                _lib._ptr(residual), _lib._ptr(y), _lib._ptr(w_post), _lib._ptr(scale), _lib._ptr(w_pre), _lib._ptr(in_tbl), _lib._ptr(out_tbl),
-                _lib._ptr(in_inv), _lib._ptr(out_inv), sizes, fours, eps, _lib._ptr(z), _lib._ptr(h), y.shape[0], _lib.element_type(y),
+                _lib._ptr(residual), _lib._ptr(y), _lib._ptr(w_post), _lib._ptr(scale), _lib._ptr(w_pre), _lib._ptr(items), _lib._ptr(in_tbl),
+                _lib._ptr(out_tbl), _lib._ptr(in_inv), _lib._ptr(out_inv), sizes, eps, _lib._ptr(z), _lib._ptr(h), y.shape[0], _lib.element_type(y),
                 _lib.stream_ptr())
         _lib.check(rc, "e3b_norm_gate_residual_fwd")
         ctx.save_for_backward(residual, y, w_post, scale, w_pre)
-        ctx.meta = (tables, sizes, fours, eps)
+        ctx.meta = (tables, sizes, eps)
         ctx.set_materialize_grads(False)
         return z, h
 
@@ -166,16 +195,15 @@ class _NormGateFunction(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_z, grad_h):
         residual, y, w_post, scale, w_pre = ctx.saved_tensors
-        tables, sizes, fours, eps = ctx.meta
+        tables, sizes, eps = ctx.meta
         if grad_z is None and grad_h is None:
-            return (None,) * 9
+            return (None,) * 8
         core, rows = _lib.core(), y.shape[0]
-        grad_z = grad_z.contiguous() if grad_z is not None else None
-        grad_h = grad_h.contiguous() if grad_h is not None else None
+        grad_z, grad_h = (None if g is None else _aligned(g.contiguous(), sizes[0]) for g in (grad_z, grad_h))
         g_residual = torch.empty_like(residual) if ctx.needs_input_grad[0] else None
         gy = torch.empty_like(y) if ctx.needs_input_grad[1] else None
         params = scratch = None
-        nbytes, n_in, n_out = 0, sizes[4], sizes[5]
+        nbytes, n_in, n_out = 0, sizes[7], sizes[8]
         if any(ctx.needs_input_grad[2:5]):
             params = torch.empty(n_in + 2 * n_out, dtype=torch.float32, device=y.device)
             nbytes = core.e3b_norm_scratch_bytes(rows, n_in + 2 * n_out)
@@ -183,11 +211,11 @@ class _NormGateFunction(torch.autograd.Function):
         with _lib.device_of(y):
             rc = core.e3b_norm_gate_residual_bwd(
                 _lib._ptr(residual), _lib._ptr(y), _lib._ptr(grad_z), _lib._ptr(grad_h), _lib._ptr(w_post), _lib._ptr(scale), _lib._ptr(w_pre),
-                *(_lib._ptr(t) for t in tables), sizes, fours, eps, _lib._ptr(g_residual), _lib._ptr(gy), _lib._ptr(params), _lib._ptr(scratch), nbytes,
+                *(_lib._ptr(t) for t in tables), sizes, eps, _lib._ptr(g_residual), _lib._ptr(gy), _lib._ptr(params), _lib._ptr(scratch), nbytes,
                 rows, _lib.element_type(y), _lib.stream_ptr())
         _lib.check(rc, "e3b_norm_gate_residual_bwd")
         gw = params.split([n_in, n_out, n_out]) if params is not None else (None, None, None)
-        return (g_residual, gy, gw[0], gw[1], gw[2] if w_pre is not None else None, None, None, None, None)
+        return (g_residual, gy, gw[0], gw[1], gw[2] if w_pre is not None else None, None, None, None)
 
 
 class NormGateResidual(torch.nn.Module):
@@ -217,19 +245,23 @@ class NormGateResidual(torch.nn.Module):
             forth = [[j, -1, 3] for j in range(dout)]
         else:
             back, const, forth = gate._in_tbl.tolist(), gate._in_cst.tolist(), gate._out_tbl.tolist()
-        # scalars (0) and gates (2) pass through their activation, gated components (1) and unused columns (3) do not
-        acts = [(row[4], _float_bits(c)) if row[0] in (0, 2) else (3, _float_bits(1.0)) for row, c in zip(back, const)]
-        in_tbl = [(b, u, *a) for (b, u), a in zip(_column_blocks(ins), acts)]
-        out_tbl = [(b, u, row[0], row[1]) for (b, u), row in zip(_column_blocks(outs), forth)]
-        for name, value in (("_in", in_tbl), ("_out", out_tbl), ("_back", [row[:4] for row in back])):
+        comps = [(row[1], row[2]) if row[0] == 2 else (0, 0) for row in back]
+        tables = {"_in": [(*bc, *n) for bc, n in zip(_column_blocks(ins), comps)], "_out": [(*bc, 0, 0) for bc in _column_blocks(outs)]}
+        for name, value in tables.items():
             self.register_buffer(name, torch.tensor(value, dtype=torch.int32).reshape(-1, 4), persistent=False)
         self.register_buffer("_in_channels", _channel_columns(ins), persistent=False)
         self.register_buffer("_out_channels", _channel_columns(outs), persistent=False)
         self.register_buffer("_in_inv_bits", _inverse_counts(ins).view(torch.int32), persistent=False)
         self.register_buffer("_out_inv_bits", _inverse_counts(outs).view(torch.int32), persistent=False)
         n_in, n_out = self._in_channels.shape[0], self._out_channels.shape[0]
-        self._sizes = [din, dout, len(ins), len(outs), n_in, n_out]
-        self._fours = int(_fours(ins) and _fours(outs))
+        self._dims = (din, dout)
+        self._sizes = {}
+        for width in (1, 4, 8):
+            items = _gate_items(back, const, forth, ins, outs, width)
+            if items is None:
+                break
+            self.register_buffer(f"_items{width}", torch.tensor(items, dtype=torch.int32).reshape(-1, 8 + width), persistent=False)
+            self._sizes[width] = (ctypes.c_int32 * 9)(width, len(items), sum(row[0] == 2 for row in back), din, dout, len(ins), len(outs), n_in, n_out)
         self.weight_post = torch.nn.Parameter(torch.ones(n_in))
         self.scale = torch.nn.Parameter(torch.full((n_out,), float(scale_init)))
         if pre_norm:
@@ -247,11 +279,13 @@ class NormGateResidual(torch.nn.Module):
         if residual.dtype != y.dtype:
             raise TypeError(f"residual and y must have one type, got {residual.dtype} and {y.dtype}")
         _lib.require_same_device(y, residual, self.weight_post, self.scale, self.weight_pre)
-        r, x = _flat_rows(residual, self._sizes[1], "residual"), _flat_rows(y, self._sizes[0], "y")
+        din, dout = self._dims
+        width = max(w for w in self._sizes if w <= (4 if y.dtype == torch.float32 else 8))      # vectors of 16 bytes if the row falls into such
+        r, x = _aligned(_flat_rows(residual, dout, "residual"), width), _aligned(_flat_rows(y, din, "y"), width)
         _lib.require_operand(self._in, y, "NormGateResidual's tables (move the module with .to(device))", None, torch.int32)
         _lib.poll_status(y.device)
-        tables = (self._in, self._out, self._back, self._in_channels, self._out_channels, self._in_inv_bits, self._out_inv_bits)
+        tables = (getattr(self, f"_items{width}"), self._in, self._out, self._in_channels, self._out_channels, self._in_inv_bits, self._out_inv_bits)
         z, h = _NormGateFunction.apply(r, x, _fp32(self.weight_post), _fp32(self.scale), _fp32(self.weight_pre), tables,
-                                       (ctypes.c_int32 * 6)(*self._sizes), self._fours, self.eps)
+                                       self._sizes[width], self.eps)
         z = z.reshape(residual.shape)
         return (z, h.reshape(residual.shape)) if self.pre_norm else z

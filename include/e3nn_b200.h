@@ -289,12 +289,16 @@ int e3b_fill_columns(float* out, int64_t num_rows, int row_stride, int col0, int
  * e3b_rms_norm_bwd: channels [num_channels,2] = {first column, components}; grad_x and grad_weight may each be NULL, not both;
  * grad_weight needs e3b_norm_scratch_bytes(rows, num_channels) bytes of scratch and is summed in a fixed order.
  * e3b_norm_gate_residual_fwd: n = norm(y; weight_post), g = Gate(n), z = residual + scale[channel] g, and h = norm(z; weight_pre)
- * unless h is NULL.  in_table [din,4] = {block, channel, activation (codes of e3b_gate_fwd), constant as float bits},
- * out_table [dout,4] = {block, channel, input column, gate column or -1}, back_table [din,4] = {kind as in e3b_gate_bwd, first
- * output column, count, partner column}; sizes: HOST array {din, dout, blocks in, blocks out, channels in, channels out}.
+ * unless h is NULL.  The row is described by items of w = 1, 4 or (16-bit types) 8 columns, in the order of their input columns: items
+ * [num_items, 8 + w] = {kind: 0 scalars, 1 gated components, 2 gates, 3 unused columns; first input column; first output column or -1;
+ * block of each (-1: none); activation (codes of e3b_gate_fwd); its constant as float bits; first gate slot (kind 2); then the gate
+ * slot of each column (kind 1)}; the w columns of an item are consecutive on both sides and of one block and one activation.
+ * in_table [din,4] = {block, channel, first output column, count} (the last two: of the components a gate column multiplies),
+ * out_table [dout,4] = {block, channel, -, -}; sizes: HOST array {w, num_items, gate slots, din, dout, blocks in, blocks out, channels in,
+ * channels out}.  Row pointers are aligned to w elements.  At most 2,048 items (4,096 of one column).
  * e3b_norm_gate_residual_bwd: grad_z or grad_h may be NULL, each of the gradients too; grad_params [channels in + 2 channels out] =
  * gradients of weight_post, scale, weight_pre, with e3b_norm_scratch_bytes(rows, its length) bytes of scratch.
- * Rows of at most e3b_norm_max_columns(1) columns with vec4 and 16-byte (8-byte for 16-bit types) pointers, else
+ * e3b_rms_norm: rows of at most e3b_norm_max_columns(1) columns with vec4 and pointers aligned to four elements, else
  * e3b_norm_max_columns(0).
  */
 int e3b_norm_max_columns(int aligned);
@@ -305,14 +309,14 @@ int e3b_rms_norm_bwd(const void* x, const void* grad_h, const float* weight, con
                      const int32_t* channels, int num_channels, int num_blocks, int vec4, float eps, void* grad_x,
                      float* grad_weight, void* scratch, int64_t scratch_bytes, int64_t rows, int dim, int type, void* stream);
 int e3b_norm_gate_residual_fwd(const void* residual, const void* y, const float* weight_post, const float* scale,
-                               const float* weight_pre, const int32_t* in_table, const int32_t* out_table, const float* in_inv,
-                               const float* out_inv, const int32_t* sizes, int vec4, float eps, void* z, void* h, int64_t rows,
-                               int type, void* stream);
+                               const float* weight_pre, const int32_t* items, const int32_t* in_table, const int32_t* out_table,
+                               const float* in_inv, const float* out_inv, const int32_t* sizes, float eps, void* z, void* h,
+                               int64_t rows, int type, void* stream);
 int e3b_norm_gate_residual_bwd(const void* residual, const void* y, const void* grad_z, const void* grad_h,
-                               const float* weight_post, const float* scale, const float* weight_pre, const int32_t* in_table,
-                               const int32_t* out_table, const int32_t* back_table, const int32_t* in_channels,
+                               const float* weight_post, const float* scale, const float* weight_pre, const int32_t* items,
+                               const int32_t* in_table, const int32_t* out_table, const int32_t* in_channels,
                                const int32_t* out_channels, const float* in_inv, const float* out_inv, const int32_t* sizes,
-                               int vec4, float eps, void* grad_residual, void* grad_y, float* grad_params, void* scratch,
+                               float eps, void* grad_residual, void* grad_y, float* grad_params, void* scratch,
                                int64_t scratch_bytes, int64_t rows, int type, void* stream);
 
 /*

@@ -37,8 +37,10 @@ def test_gate_rows_name_every_column():
     mod = bnn.NormGateResidual(gate)
     assert mod.irreps_in == gate.irreps_in and mod.irreps_out == gate.irreps_out
     assert mod._in.shape == (gate.irreps_in.dim, 4) and mod._out.shape == (gate.irreps_out.dim, 4)
-    kinds = mod._back[:, 0]
+    kinds = mod._items1[:, 0]
     assert (kinds == 2).sum() == 3 and (kinds == 0).sum() == 6 and (kinds == 1).sum() == 11
+    assert sorted(mod._items1[:, 1].tolist()) == list(range(gate.irreps_in.dim))
+    assert sorted(j for j in mod._items1[:, 2].tolist() if j >= 0) == list(range(gate.irreps_out.dim))
     assert mod.weight_post.numel() == gate.irreps_in.num_irreps and mod.scale.numel() == mod.weight_pre.numel() == gate.irreps_out.num_irreps
     assert bnn.NormGateResidual(gate, pre_norm=False).weight_pre is None
 
