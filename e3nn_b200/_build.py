@@ -23,7 +23,7 @@ CSRC = os.path.join(PKG, "csrc")
 LIB_DIR = os.path.join(PKG, "lib")
 LAYOUT_DIR = os.path.join(PKG, "_layouts")
 CORE_LIB = os.path.join(LIB_DIR, "libe3nn_b200.so")
-CORE_SOURCES = ["abi.cu", "sh.cu", "csr.cu", "dense.cu", "dense_tile.cu", "radial.cu", "matmul_tn.cu", "neighbor.cu", "gate.cu", "norm.cu", "rel_bias.cu", "attention.cu", "attention_bwd.cu",
+CORE_SOURCES = ["abi.cu", "sh.cu", "csr.cu", "dense.cu", "dense_tile.cu", "radial.cu", "matmul_tn.cu", "neighbor.cu", "gate.cu", "norm.cu", "norm_gate.cu", "norm_gate_bwd.cu", "rel_bias.cu", "attention.cu", "attention_bwd.cu",
                 "attention_bwd_src.cu", "selftest.cu"]
 
 NVCC_FLAGS = [

@@ -1,0 +1,103 @@
+// Shared by the norm kernels: sums over the blocks of the irreps, parameter gradients, launches.
+#pragma once
+#include <algorithm>
+
+#include "common.cuh"
+#include "gate_act.cuh"
+#include "typed.cuh"
+
+namespace e3b {
+namespace {
+
+constexpr int kMaxThreads = 512;
+
+// Sums over the irreps blocks of a row by the warps that touch a block.  share: [nblk][nw]; span: [nblk][2] first and last of those
+// warps (warps between them that do not touch the block leave the zero from the start of the kernel).
+struct BlockSums {
+    float* share;
+    int* span;
+    int nblk, nw;
+    __device__ __forceinline__ void clear() const {
+        for (int i = threadIdx.x; i < nblk * nw; i += blockDim.x) share[i] = 0.0f;
+        for (int i = threadIdx.x; i < nblk; i += blockDim.x) { span[2 * i] = 1 << 30; span[2 * i + 1] = -1; }
+    }
+    __device__ __forceinline__ void touch(unsigned blocks) const {      // the warp's
+        const int warp = threadIdx.x >> 5;
+        if ((threadIdx.x & 31) == 0)
+            for (; blocks; blocks &= blocks - 1) {
+                const int b = __ffs(blocks) - 1;
+                atomicMin(&span[2 * b], warp);
+                atomicMax(&span[2 * b + 1], warp);
+            }
+    }
+    // shares of this warp's items: K values of the blocks vb, M of the blocks wb (0 where there is no item)
+    template <int K, int M>
+    __device__ __forceinline__ void add(unsigned blocks, const float (&v)[K], const int (&vb)[K], const float (&w)[M], const int (&wb)[M]) const {
+        for (; blocks; blocks &= blocks - 1) {
+            const int b = __ffs(blocks) - 1;
+            float s = 0.0f;
+#pragma unroll
+            for (int k = 0; k < K; ++k) s += vb[k] == b ? v[k] : 0.0f;
+#pragma unroll
+            for (int j = 0; j < M; ++j) s += wb[j] == b ? w[j] : 0.0f;
+            s = warp_sum(s);
+            if ((threadIdx.x & 31) == 0) share[b * nw + (threadIdx.x >> 5)] = s;
+        }
+    }
+    __device__ __forceinline__ float get(int b) const {
+        const int w1 = span[2 * b + 1];
+        float s = 0.0f;
+        for (int w = span[2 * b]; w <= w1; ++w) s += share[b * nw + w];
+        return s;
+    }
+    __host__ __device__ static int floats(int nblk, int nw) { return (nblk * nw + 2 * nblk + 3) / 4 * 4; }
+};
+__device__ __forceinline__ BlockSums block_sums_at(float*& p, int nblk, int nw) {
+    BlockSums b{p, reinterpret_cast<int*>(p + nblk * nw), nblk, nw};
+    p += BlockSums::floats(nblk, nw);
+    return b;
+}
+
+// A thread block's row of the parameter gradients: columns already summed over its rows lie in `columns`, channel u has
+// chan[2u + 1] of them from chan[2u] on.
+__device__ __forceinline__ void store_channels(const float* columns, const int32_t* __restrict__ chan, int nchan, float* __restrict__ partial) {
+    for (int u = threadIdx.x; u < nchan; u += blockDim.x) {
+        float s = 0.0f;
+        const int first = chan[2 * u], n = chan[2 * u + 1];
+        for (int m = 0; m < n; ++m) s += columns[first + m];
+        partial[u] = s;
+    }
+}
+
+// Parameter gradient: the thread blocks' partial rows added in a fixed order.  32 channels a block, 32 slices of the rows.
+static __global__ void __launch_bounds__(1024) add_partials_kernel(const float* __restrict__ partial, int n, int parts, float* __restrict__ out) {
+    __shared__ float s[32][33];
+    const int u = blockIdx.x * 32 + threadIdx.x;
+    float a = 0.0f;
+    if (u < n) {
+#pragma unroll 4
+        for (int p = threadIdx.y; p < parts; p += 32) a += partial[static_cast<int64_t>(p) * n + u];
+    }
+    s[threadIdx.x][threadIdx.y] = a;
+    __syncthreads();
+    const float t = warp_sum(s[threadIdx.y][threadIdx.x]);      // channel threadIdx.y, its slices across the lanes
+    if (threadIdx.x == 0 && blockIdx.x * 32 + threadIdx.y < n) out[blockIdx.x * 32 + threadIdx.y] = t;
+}
+
+template <typename F>
+int resident_blocks(F kernel, int threads, size_t smem, int64_t rows, int* grid) {
+    if (smem > 48 * 1024) E3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    int per_sm = 0;
+    E3B_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem));
+    if (per_sm < 1) return fail(E3B_ERR_UNSUPPORTED, "norm: the row does not fit a thread block");
+    *grid = static_cast<int>(std::min<int64_t>(rows, static_cast<int64_t>(per_sm) * kNumSMs));
+    return E3B_OK;
+}
+
+inline int max_parts(int64_t rows) { return static_cast<int>(std::min<int64_t>(rows, 32 * kNumSMs)); }
+inline int64_t norm_scratch_bytes(int64_t rows, int num_params) {
+    return rows < 0 || num_params < 0 ? 0 : sizeof(float) * static_cast<int64_t>(max_parts(rows)) * num_params;
+}
+
+}  // namespace
+}  // namespace e3b

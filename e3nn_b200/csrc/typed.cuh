@@ -39,6 +39,21 @@ template <typename T> struct Packed<T, 1> {
     __device__ __forceinline__ void unpack(float* f) const { f[0] = to_float(v); }
     static __device__ __forceinline__ void store(T* p, const float* f) { *p = from_float<T>(f[0]); }
 };
+template <> struct Packed<float, 2> {
+    float2 v;
+    __device__ __forceinline__ void load(const float* p) { v = *reinterpret_cast<const float2*>(p); }
+    __device__ __forceinline__ void unpack(float* f) const { f[0] = v.x; f[1] = v.y; }
+    static __device__ __forceinline__ void store(float* p, const float* f) { *reinterpret_cast<float2*>(p) = make_float2(f[0], f[1]); }
+};
+template <typename T> struct Packed<T, 2> {
+    uint32_t v;
+    __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint32_t*>(p); }
+    __device__ __forceinline__ void unpack(float* f) const {
+        const float2 a = Pair<T>::load(v);
+        f[0] = a.x; f[1] = a.y;
+    }
+    static __device__ __forceinline__ void store(T* p, const float* f) { *reinterpret_cast<uint32_t*>(p) = Pair<T>::store(f[0], f[1]); }
+};
 template <> struct Packed<float, 4> {
     float4 v;
     __device__ __forceinline__ void load(const float* p) { v = *reinterpret_cast<const float4*>(p); }

@@ -150,40 +150,52 @@ class RMSNorm(torch.nn.Module):
         return out.reshape(x.shape)
 
 
-def _gate_items(back, const, forth, ins, outs, width: int) -> Optional[List[List[int]]]:
-    """The row as items of `width` columns, `None` where it does not fall into such items (see ``e3b_norm_gate_residual_fwd``).
-    `back`, `const`: per input column {kind, first output column, count, partner column, activation} and constant; `forth`: per
-    output column {input column, gate column or -1, ..}."""
+def _gate_items(back, const, forth, ins, outs, width: int, narrow: int):
+    """The row as wide items of `width` columns and narrow ones of `narrow` (see ``e3b_norm_gate_residual_fwd``), `None` where it does
+    not fall into such items.  `back`, `const`: per input column {kind, first output column, count, partner column, activation} and
+    constant; `forth`: per output column {input column, gate column or -1, ..}."""
     out_of = {row[0]: j for j, row in enumerate(forth)}                       # input column -> output column
     slot_of = {c: n for n, c in enumerate(c for c, row in enumerate(back) if row[0] == 2)}
     in_blk, out_blk = [b for b, _ in _column_blocks(ins)], [b for b, _ in _column_blocks(outs)]
     if len(back) % width or len(forth) % width:
         return None
-    items = []
-    for c in range(0, len(back), width):
-        cols = range(c, c + width)
-        kind, act = back[c][0], back[c][4] if back[c][0] in (0, 2) else 3
-        j = out_of.get(c, -1)
-        alike = all(back[x][0] == kind and in_blk[x] == in_blk[c] and out_of.get(x, -1) == (j + x - c if j >= 0 else -1)
-                    and (kind not in (0, 2) or (back[x][4] == act and const[x] == const[c])) for x in cols)
-        if not alike or (j >= 0 and (j % width or out_blk[j + width - 1] != out_blk[j])) or (kind == 2 and slot_of[c] % width):
+    # gated components, and scalars that nothing is applied to, need no activation
+    plain = [row[0] == 1 or (row[0] == 0 and row[4] == 3) for row in back]
+    wides, narrows, c = [], [], 0
+    while c < len(back):
+        n = width if plain[c] else narrow
+        cols, j = range(c, c + n), out_of.get(c, -1)
+        if c % n or c + n > len(back) or (j >= 0 and (j % n or j + n > len(forth) or out_blk[j + n - 1] != out_blk[j])):
             return None
-        gates = [slot_of[forth[out_of[x]][1]] if kind == 1 else 0 for x in cols]
-        items.append([kind, c, j, in_blk[c], out_blk[j] if j >= 0 else -1, act, _float_bits(const[c] if kind in (0, 2) else 1.0),
-                      slot_of[c] if kind == 2 else 0, *gates])
-    return items
+        for x in cols:
+            if plain[x] != plain[c] or in_blk[x] != in_blk[c] or out_of.get(x, -1) != (j + x - c if j >= 0 else -1):
+                return None
+            if not plain[c] and (back[x][0] != back[c][0] or back[x][4] != back[c][4] or const[x] != const[c]):
+                return None
+        if plain[c]:
+            if any(const[x] != 1.0 for x in cols if back[x][0] == 0):
+                return None
+            wides.append([c, j, in_blk[c], out_blk[j], *(slot_of[forth[out_of[x]][1]] if back[x][0] == 1 else len(slot_of) for x in cols)])
+        else:
+            kind = back[c][0]
+            if kind == 2 and slot_of[c] % n:
+                return None
+            narrows.append([kind, c, j, in_blk[c], out_blk[j] if j >= 0 else 0, back[c][4] if kind != 3 else 3,
+                            _float_bits(const[c] if kind != 3 else 1.0), slot_of[c] if kind == 2 else 0])
+        c += n
+    return (torch.tensor(wides, dtype=torch.int32).reshape(-1, 4 + width), torch.tensor(narrows, dtype=torch.int32).reshape(-1, 8), len(slot_of))
 
 
 class _NormGateFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, residual, y, w_post, scale, w_pre, tables, sizes, eps):
-        items, in_tbl, out_tbl, _, _, in_inv, out_inv = tables
+        wide, narrow, in_tbl, out_tbl, _, _, in_inv, out_inv = tables
         z = torch.empty_like(residual)
         h = torch.empty_like(residual) if w_pre is not None else None
         with _lib.device_of(y):
             rc = _lib.core().e3b_norm_gate_residual_fwd(
-                _lib._ptr(residual), _lib._ptr(y), _lib._ptr(w_post), _lib._ptr(scale), _lib._ptr(w_pre), _lib._ptr(items), _lib._ptr(in_tbl),
-                _lib._ptr(out_tbl), _lib._ptr(in_inv), _lib._ptr(out_inv), sizes, eps, _lib._ptr(z), _lib._ptr(h), y.shape[0], _lib.element_type(y),
+                _lib._ptr(residual), _lib._ptr(y), _lib._ptr(w_post), _lib._ptr(scale), _lib._ptr(w_pre), _lib._ptr(wide), _lib._ptr(narrow),
+                _lib._ptr(in_tbl), _lib._ptr(out_tbl), _lib._ptr(in_inv), _lib._ptr(out_inv), sizes, eps, _lib._ptr(z), _lib._ptr(h), y.shape[0], _lib.element_type(y),
                 _lib.stream_ptr())
         _lib.check(rc, "e3b_norm_gate_residual_fwd")
         ctx.save_for_backward(residual, y, w_post, scale, w_pre)
@@ -203,7 +215,7 @@ class _NormGateFunction(torch.autograd.Function):
         g_residual = torch.empty_like(residual) if ctx.needs_input_grad[0] else None
         gy = torch.empty_like(y) if ctx.needs_input_grad[1] else None
         params = scratch = None
-        nbytes, n_in, n_out = 0, sizes[7], sizes[8]
+        nbytes, n_in, n_out = 0, sizes[9], sizes[10]
         if any(ctx.needs_input_grad[2:5]):
             params = torch.empty(n_in + 2 * n_out, dtype=torch.float32, device=y.device)
             nbytes = core.e3b_norm_scratch_bytes(rows, n_in + 2 * n_out)
@@ -255,13 +267,16 @@ class NormGateResidual(torch.nn.Module):
         self.register_buffer("_out_inv_bits", _inverse_counts(outs).view(torch.int32), persistent=False)
         n_in, n_out = self._in_channels.shape[0], self._out_channels.shape[0]
         self._dims = (din, dout)
+        if max(len(ins), len(outs)) > 32:
+            raise NotImplementedError(f"at most 32 blocks of irreps are supported, got {self.irreps_in} -> {self.irreps_out}")
         self._sizes = {}
-        for width in (1, 4, 8):
-            items = _gate_items(back, const, forth, ins, outs, width)
-            if items is None:
-                break
-            self.register_buffer(f"_items{width}", torch.tensor(items, dtype=torch.int32).reshape(-1, 8 + width), persistent=False)
-            self._sizes[width] = (ctypes.c_int32 * 9)(width, len(items), sum(row[0] == 2 for row in back), din, dout, len(ins), len(outs), n_in, n_out)
+        for width, narrow in ((1, 1), (4, 1), (4, 2), (8, 2)):
+            items = _gate_items(back, const, forth, ins, outs, width, narrow)
+            if items is not None:
+                self.register_buffer(f"_wide{width}{narrow}", items[0], persistent=False)
+                self.register_buffer(f"_narrow{width}{narrow}", items[1], persistent=False)
+                self._sizes[width, narrow] = (ctypes.c_int32 * 11)(width, narrow, len(items[0]), len(items[1]), items[2], din, dout, len(ins),
+                                                                   len(outs), n_in, n_out)
         self.weight_post = torch.nn.Parameter(torch.ones(n_in))
         self.scale = torch.nn.Parameter(torch.full((n_out,), float(scale_init)))
         if pre_norm:
@@ -280,12 +295,17 @@ class NormGateResidual(torch.nn.Module):
             raise TypeError(f"residual and y must have one type, got {residual.dtype} and {y.dtype}")
         _lib.require_same_device(y, residual, self.weight_post, self.scale, self.weight_pre)
         din, dout = self._dims
-        width = max(w for w in self._sizes if w <= (4 if y.dtype == torch.float32 else 8))      # vectors of 16 bytes if the row falls into such
+        # vectors of 16 bytes if the row falls into such
+        for key in ((4, 1), (1, 1)) if y.dtype == torch.float32 else ((8, 2), (4, 2), (1, 1)):
+            if key in self._sizes:
+                break
+        width = key[0]
         r, x = _aligned(_flat_rows(residual, dout, "residual"), width), _aligned(_flat_rows(y, din, "y"), width)
         _lib.require_operand(self._in, y, "NormGateResidual's tables (move the module with .to(device))", None, torch.int32)
         _lib.poll_status(y.device)
-        tables = (getattr(self, f"_items{width}"), self._in, self._out, self._in_channels, self._out_channels, self._in_inv_bits, self._out_inv_bits)
+        wide, narrow = getattr(self, f"_wide{key[0]}{key[1]}"), getattr(self, f"_narrow{key[0]}{key[1]}")
+        tables = (wide, narrow, self._in, self._out, self._in_channels, self._out_channels, self._in_inv_bits, self._out_inv_bits)
         z, h = _NormGateFunction.apply(r, x, _fp32(self.weight_post), _fp32(self.scale), _fp32(self.weight_pre), tables,
-                                       self._sizes[width], self.eps)
+                                       self._sizes[key], self.eps)
         z = z.reshape(residual.shape)
         return (z, h.reshape(residual.shape)) if self.pre_norm else z

@@ -289,13 +289,14 @@ int e3b_fill_columns(float* out, int64_t num_rows, int row_stride, int col0, int
  * e3b_rms_norm_bwd: channels [num_channels,2] = {first column, components}; grad_x and grad_weight may each be NULL, not both;
  * grad_weight needs e3b_norm_scratch_bytes(rows, num_channels) bytes of scratch and is summed in a fixed order.
  * e3b_norm_gate_residual_fwd: n = norm(y; weight_post), g = Gate(n), z = residual + scale[channel] g, and h = norm(z; weight_pre)
- * unless h is NULL.  The row is described by items of w = 1, 4 or (16-bit types) 8 columns, in the order of their input columns: items
- * [num_items, 8 + w] = {kind: 0 scalars, 1 gated components, 2 gates, 3 unused columns; first input column; first output column or -1;
- * block of each (-1: none); activation (codes of e3b_gate_fwd); its constant as float bits; first gate slot (kind 2); then the gate
- * slot of each column (kind 1)}; the w columns of an item are consecutive on both sides and of one block and one activation.
+ * unless h is NULL.  The row is described by items.  wide [num_wide, 4 + w]: w columns that are multiplied by gates or by nothing,
+ * {first input column, first output column, block of each, gate slot of each column (num_gates: none)}.  narrow [num_narrow, 8]: n columns
+ * with an activation, {kind: 0 scalars, 2 gates, 3 unused columns; first input column; first output column or -1; block of each (0: none);
+ * activation (codes of e3b_gate_fwd); its constant as float bits; first gate slot (kind 2)}.  The columns of an item are consecutive on
+ * both sides and of one block and one activation.  (w, n) = (1, 1), for fp32 (4, 1), for 16-bit types (4, 2) or (8, 2).
  * in_table [din,4] = {block, channel, first output column, count} (the last two: of the components a gate column multiplies),
- * out_table [dout,4] = {block, channel, -, -}; sizes: HOST array {w, num_items, gate slots, din, dout, blocks in, blocks out, channels in,
- * channels out}.  Row pointers are aligned to w elements.  At most 2,048 items (4,096 of one column).
+ * out_table [dout,4] = {block, channel, -, -}; sizes: HOST array {w, n, num_wide, num_narrow, num_gates, din, dout, blocks in,
+ * blocks out, channels in, channels out}.  Row pointers are aligned to w elements.  At most 4,096 items of each sort and 32 blocks.
  * e3b_norm_gate_residual_bwd: grad_z or grad_h may be NULL, each of the gradients too; grad_params [channels in + 2 channels out] =
  * gradients of weight_post, scale, weight_pre, with e3b_norm_scratch_bytes(rows, its length) bytes of scratch.
  * e3b_rms_norm: rows of at most e3b_norm_max_columns(1) columns with vec4 and pointers aligned to four elements, else
@@ -309,12 +310,12 @@ int e3b_rms_norm_bwd(const void* x, const void* grad_h, const float* weight, con
                      const int32_t* channels, int num_channels, int num_blocks, int vec4, float eps, void* grad_x,
                      float* grad_weight, void* scratch, int64_t scratch_bytes, int64_t rows, int dim, int type, void* stream);
 int e3b_norm_gate_residual_fwd(const void* residual, const void* y, const float* weight_post, const float* scale,
-                               const float* weight_pre, const int32_t* items, const int32_t* in_table, const int32_t* out_table,
-                               const float* in_inv, const float* out_inv, const int32_t* sizes, float eps, void* z, void* h,
-                               int64_t rows, int type, void* stream);
+                               const float* weight_pre, const int32_t* wide, const int32_t* narrow, const int32_t* in_table,
+                               const int32_t* out_table, const float* in_inv, const float* out_inv, const int32_t* sizes, float eps,
+                               void* z, void* h, int64_t rows, int type, void* stream);
 int e3b_norm_gate_residual_bwd(const void* residual, const void* y, const void* grad_z, const void* grad_h,
-                               const float* weight_post, const float* scale, const float* weight_pre, const int32_t* items,
-                               const int32_t* in_table, const int32_t* out_table, const int32_t* in_channels,
+                               const float* weight_post, const float* scale, const float* weight_pre, const int32_t* wide,
+                               const int32_t* narrow, const int32_t* in_table, const int32_t* out_table, const int32_t* in_channels,
                                const int32_t* out_channels, const float* in_inv, const float* out_inv, const int32_t* sizes,
                                float eps, void* grad_residual, void* grad_y, float* grad_params, void* scratch,
                                int64_t scratch_bytes, int64_t rows, int type, void* stream);

@@ -37,10 +37,15 @@ def test_gate_rows_name_every_column():
     mod = bnn.NormGateResidual(gate)
     assert mod.irreps_in == gate.irreps_in and mod.irreps_out == gate.irreps_out
     assert mod._in.shape == (gate.irreps_in.dim, 4) and mod._out.shape == (gate.irreps_out.dim, 4)
-    kinds = mod._items1[:, 0]
-    assert (kinds == 2).sum() == 3 and (kinds == 0).sum() == 6 and (kinds == 1).sum() == 11
-    assert sorted(mod._items1[:, 1].tolist()) == list(range(gate.irreps_in.dim))
-    assert sorted(j for j in mod._items1[:, 2].tolist() if j >= 0) == list(range(gate.irreps_out.dim))
+    for width, narrow in mod._sizes:
+        w, n = getattr(mod, f"_wide{width}{narrow}").tolist(), getattr(mod, f"_narrow{width}{narrow}").tolist()
+        assert sorted([e[0] + i for e in w for i in range(width)] + [e[1] + i for e in n for i in range(narrow)]) == list(range(gate.irreps_in.dim))
+        assert sorted([e[1] + i for e in w for i in range(width)] + [e[2] + i for e in n for i in range(narrow) if e[2] >= 0]) == list(range(gate.irreps_out.dim))
+        for e in w:       # gates in the order of the channels they multiply
+            for i, slot in enumerate(e[4:]):
+                assert slot == (e[1] + i - 6) // 3 if e[1] + i < 12 else slot == 2
+    assert (1, 1) in mod._sizes and sum(e[0] == 2 for e in mod._narrow11.tolist()) == 3
+    assert set(bnn.NormGateResidual(bnn.Gate("8x0e", [torch.tanh], "16x0e", [torch.sigmoid], "8x1o+8x2e"))._sizes) == {(1, 1), (4, 1), (4, 2), (8, 2)}
     assert mod.weight_post.numel() == gate.irreps_in.num_irreps and mod.scale.numel() == mod.weight_pre.numel() == gate.irreps_out.num_irreps
     assert bnn.NormGateResidual(gate, pre_norm=False).weight_pre is None
 
@@ -58,6 +63,8 @@ def test_lower_ends_ascend(num, r_linear):
 def test_constructors_refuse():
     with pytest.raises(ValueError):
         bnn.RMSNorm("4x0e", eps=-1.0)
+    with pytest.raises(NotImplementedError):
+        bnn.NormGateResidual(irreps="+".join(f"1x{l}e" for l in range(33)))
     gate = bnn.Gate("4x0e", [torch.tanh], "2x0e", [torch.sigmoid], "2x1o")
     with pytest.raises(ValueError):
         bnn.NormGateResidual()
