@@ -181,12 +181,40 @@ def element_type(t: torch.Tensor, name: str = "the tensor") -> int:
     return code
 
 
+def address(t: Optional[torch.Tensor]) -> int:
+    """Pointer argument of an entry point (a plain integer: ctypes converts it without an object in between)."""
+    return 0 if t is None else t.data_ptr()
+
+
+def raw_stream(t: torch.Tensor) -> int:
+    """The current stream of the device of `t`."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def status_address(t: torch.Tensor) -> int:
+    """Pointer of the status word of the device of `t`."""
+    st = _status.get(t.get_device())
+    return (st if st is not None else _device_status(t.device)).word.data_ptr()
+
+
+def check_earlier(t: torch.Tensor) -> None:
+    """`poll_status` of the device of `t`, for the many calls that find nothing."""
+    st = _status.get(t.get_device())
+    if st is not None and st.value.value != 0:
+        poll_status(t.device)
+
+
+def wants_grad(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether a call has to be recorded for a backward pass."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 _no_switch = contextlib.nullcontext()
 
 
 def device_of(t: torch.Tensor):
     """Context in which the device of `t` is the current one (nothing to do, and nothing done, when it is already)."""
-    return _no_switch if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
+    return _no_switch if torch._C._cuda_getDevice() == t.get_device() else torch.cuda.device(t.device)
 
 
 def core() -> ctypes.CDLL:

@@ -661,11 +661,5 @@ int by_type_and_vectors(int type, int vec, int v, F&& f) {
     return by_vectors<__half>(vec, v, f);
 }
 
-template <typename K>
-int allow_smem(K kernel, size_t smem) {
-    if (smem > 48 * 1024) E3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-    return E3B_OK;
-}
-
 }  // namespace
 }  // namespace e3b

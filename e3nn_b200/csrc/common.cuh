@@ -37,6 +37,16 @@ inline int check_launch(const char* what) {
 
 constexpr int kNumSMs = 148;  // B200
 
+// Lets a kernel be launched with `smem` bytes of dynamic shared memory.  Always the same large limit, so that no call lowers the
+// one that another thread is about to launch with.
+template <typename K>
+int allow_smem(K kernel, size_t smem) {
+    constexpr int kMost = 226 * 1024;
+    if (smem > kMost) return fail(E3B_ERR_UNSUPPORTED, "%lld bytes of shared memory are needed", static_cast<long long>(smem));
+    if (smem > 48 * 1024) E3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
+    return E3B_OK;
+}
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace e3b

@@ -84,13 +84,33 @@ static __global__ void __launch_bounds__(1024) add_partials_kernel(const float* 
     if (threadIdx.x == 0 && blockIdx.x * 32 + threadIdx.y < n) out[blockIdx.x * 32 + threadIdx.y] = t;
 }
 
+// Thread blocks of a persistent launch: all that fit on the GPU, at most one a row.  The query of the last shape is kept, one
+// per kernel and host thread (it costs about as much as the launch).
 template <typename F>
 int resident_blocks(F kernel, int threads, size_t smem, int64_t rows, int* grid) {
-    if (smem > 48 * 1024) E3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-    int per_sm = 0;
-    E3B_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem));
-    if (per_sm < 1) return fail(E3B_ERR_UNSUPPORTED, "norm: the row does not fit a thread block");
-    *grid = static_cast<int>(std::min<int64_t>(rows, static_cast<int64_t>(per_sm) * kNumSMs));
+    struct Last {
+        F kernel;
+        int threads, per_sm, device;
+        size_t smem;
+    };
+    static thread_local Last last[8] = {};
+    static thread_local int next = 0;
+    int device = 0;
+    E3B_CUDA_TRY(cudaGetDevice(&device));
+    const Last* hit = nullptr;
+    for (const Last& l : last)
+        if (l.kernel == kernel && l.threads == threads && l.smem == smem && l.device == device) hit = &l;
+    if (!hit) {
+        int per_sm = 0;
+        const int rc = allow_smem(kernel, smem);
+        if (rc != E3B_OK) return rc;
+        E3B_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem));
+        if (per_sm < 1) return fail(E3B_ERR_UNSUPPORTED, "norm: the row does not fit a thread block");
+        last[next] = {kernel, threads, per_sm, device, smem};
+        hit = &last[next];
+        next = (next + 1) % 8;
+    }
+    *grid = static_cast<int>(std::min<int64_t>(rows, static_cast<int64_t>(hit->per_sm) * kNumSMs));
     return E3B_OK;
 }
 

@@ -180,7 +180,8 @@ template <typename T>
 int bias_bwd(const void* grad, const int32_t* buckets, int num_buckets, int heads, int64_t edges, void* grad_table, float* partial,
              int table_type, int32_t* status, cudaStream_t st) {
     const BiasSplit s = bias_split(edges, heads, num_buckets);
-    if (s.smem > 48 * 1024) E3B_CUDA_TRY(cudaFuncSetAttribute(bias_bwd_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(s.smem)));
+    const int allowed = allow_smem(bias_bwd_kernel<T>, s.smem);
+    if (allowed != E3B_OK) return allowed;
     bias_bwd_kernel<T><<<dim3(s.parts, s.groups), s.width * s.slices, s.smem, st>>>(static_cast<const T*>(grad), buckets, num_buckets, heads, s.width,
                                                                                    s.slices, edges, s.per_block, partial, status);
     const int rc = check_launch("relative_bias_bwd");

@@ -49,28 +49,34 @@ class _Call:
     __slots__ = ("vec", "layout", "qk_tbl", "v_tbl", "scale", "rowptr", "perm", "src", "buckets", "transpose", "edges")
 
 
+def _attend(q, k, v, bias, weight, c: _Call, keep: bool):
+    """The output, and for the backward pass its fp32 form and the statistics of every row."""
+    N, (H, dv), type_code, dev = q.shape[0], (c.layout[1], c.layout[5]), _lib.element_type(q), q.device
+    core, address = _lib.core(), _lib.address
+    out = torch.empty(N, dv, dtype=q.dtype, device=dev)
+    out32 = stats = None
+    if keep:
+        stats = torch.empty(N, H, 2, dtype=torch.float32, device=dev)
+        out32 = torch.empty(N, dv, dtype=torch.float32, device=dev) if type_code else None
+    nbytes = core.e3b_attention_scratch_bytes(N, c.edges, H, dv)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    with _lib.device_of(q):
+        rc = core.e3b_attention_fwd(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), k.stride(0), v.stride(0), c.rowptr.data_ptr(), address(c.perm), address(c.src),
+            address(bias), address(c.buckets), bias.shape[0] if c.buckets is not None else 0, address(weight), c.qk_tbl.data_ptr(), c.v_tbl.data_ptr(),
+            c.layout, c.scale, N, k.shape[0], c.edges, type_code, out.data_ptr(), address(out32), address(stats), scratch.data_ptr(), nbytes,
+            _lib.status_address(q), _lib.raw_stream(q))
+    if rc:
+        _lib.check(rc, "e3b_attention_fwd")
+    return out, out32 if out32 is not None else out, stats
+
+
 class _AttentionFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, bias, weight, c, train):
-        N, (H, dv), dev, type_code = q.shape[0], (c.layout[1], c.layout[5]), q.device, _lib.element_type(q)
-        core = _lib.core()
-        out = torch.empty(N, dv, dtype=q.dtype, device=dev)
-        out32 = stats = None
-        if train:
-            stats = torch.empty(N, H, 2, dtype=torch.float32, device=dev)
-            out32 = torch.empty(N, dv, dtype=torch.float32, device=dev) if q.dtype != torch.float32 else None
-        nbytes = core.e3b_attention_scratch_bytes(N, c.edges, H, dv)
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        with _lib.device_of(q), _lib.nvtx_range("e3b_attention_fwd"):
-            rc = core.e3b_attention_fwd(
-                _lib._ptr(q), _lib._ptr(k), _lib._ptr(v), q.stride(0), k.stride(0), v.stride(0), _lib._ptr(c.rowptr), _lib._ptr(c.perm), _lib._ptr(c.src),
-                _lib._ptr(bias), _lib._ptr(c.buckets), bias.shape[0] if c.buckets is not None else 0, _lib._ptr(weight), _lib._ptr(c.qk_tbl),
-                _lib._ptr(c.v_tbl), c.layout, c.scale, N, k.shape[0], c.edges, type_code, _lib._ptr(out), _lib._ptr(out32), _lib._ptr(stats),
-                _lib._ptr(scratch), nbytes, _lib._ptr(_lib.status_word(dev)), _lib.stream_ptr())
-        _lib.check(rc, "e3b_attention_fwd")
-        if train:
-            ctx.save_for_backward(q, k, v, bias, weight, out32 if out32 is not None else out, stats)
-            ctx.call = c
+    def forward(ctx, q, k, v, bias, weight, c):
+        out, out32, stats = _attend(q, k, v, bias, weight, c, True)
+        ctx.save_for_backward(q, k, v, bias, weight, out32, stats)
+        ctx.call = c
         return out
 
     @staticmethod
@@ -95,29 +101,31 @@ class _AttentionFunction(torch.autograd.Function):
         gweight = torch.empty(E, dtype=torch.float32, device=dev) if need_weight else None
         nbytes = core.e3b_attention_bwd_scratch_bytes(N, E, dqk)
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        status = _lib._ptr(_lib.status_word(dev))
-        with _lib.device_of(q), _lib.nvtx_range("e3b_attention_bwd"):
+        status = _lib.status_address(q)
+        with _lib.device_of(q):
             rc = core.e3b_attention_bwd(
-                _lib._ptr(q), _lib._ptr(k), _lib._ptr(v), _lib._ptr(grad), q.stride(0), k.stride(0), v.stride(0), _lib._ptr(out32), _lib._ptr(stats),
-                _lib._ptr(c.rowptr), _lib._ptr(c.perm), _lib._ptr(c.src), _lib._ptr(bias), _lib._ptr(c.buckets),
-                bias.shape[0] if c.buckets is not None else 0, _lib._ptr(weight), _lib._ptr(c.qk_tbl), _lib._ptr(c.v_tbl), c.layout, c.scale, N, S, E,
-                type_code, _lib._ptr(gq), _lib._ptr(gk) if per_edge else None, _lib._ptr(gv) if per_edge else None, _lib._ptr(share), _lib._ptr(da),
-                _lib._ptr(dst), _lib._ptr(gweight), _lib._ptr(scratch), nbytes, status, _lib.stream_ptr())
-        _lib.check(rc, "e3b_attention_bwd")
+                _lib.address(q), _lib.address(k), _lib.address(v), _lib.address(grad), q.stride(0), k.stride(0), v.stride(0), _lib.address(out32), _lib.address(stats),
+                _lib.address(c.rowptr), _lib.address(c.perm), _lib.address(c.src), _lib.address(bias), _lib.address(c.buckets),
+                bias.shape[0] if c.buckets is not None else 0, _lib.address(weight), _lib.address(c.qk_tbl), _lib.address(c.v_tbl), c.layout, c.scale, N, S, E,
+                type_code, _lib.address(gq), _lib.address(gk) if per_edge else None, _lib.address(gv) if per_edge else None, _lib.address(share), _lib.address(da),
+                _lib.address(dst), _lib.address(gweight), _lib.address(scratch), nbytes, status, _lib.raw_stream(q))
+        if rc:
+            _lib.check(rc, "e3b_attention_bwd")
         if per_node:
             perm_t, rowptr_t = c.transpose if c.transpose is not None else csr_from_dst(c.src, S)
             nbytes = core.e3b_attention_bwd_src_scratch_bytes(S, E, dqk, dv)
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            with _lib.device_of(q), _lib.nvtx_range("e3b_attention_bwd_src"):
+            with _lib.device_of(q):
                 rc = core.e3b_attention_bwd_src(
-                    _lib._ptr(q), _lib._ptr(grad), q.stride(0), _lib._ptr(share), _lib._ptr(dst), _lib._ptr(perm_t), _lib._ptr(rowptr_t),
-                    _lib._ptr(c.qk_tbl), _lib._ptr(c.v_tbl), c.layout, c.scale, N, S, E, type_code, _lib._ptr(gk), _lib._ptr(gv), _lib._ptr(scratch),
-                    nbytes, status, _lib.stream_ptr())
-            _lib.check(rc, "e3b_attention_bwd_src")
+                    _lib.address(q), _lib.address(grad), q.stride(0), _lib.address(share), _lib.address(dst), _lib.address(perm_t), _lib.address(rowptr_t),
+                    _lib.address(c.qk_tbl), _lib.address(c.v_tbl), c.layout, c.scale, N, S, E, type_code, _lib.address(gk), _lib.address(gv), _lib.address(scratch),
+                    nbytes, status, _lib.raw_stream(q))
+            if rc:
+                _lib.check(rc, "e3b_attention_bwd_src")
         gbias = None
         if need_bias:
             gbias = bias_table_grad(da, c.buckets, bias.shape[0], torch.float32) if c.buckets is not None else da
-        return gq, gk if need_k else None, gv if need_v else None, gbias, gweight, None, None
+        return gq, gk if need_k else None, gv if need_v else None, gbias, gweight, None
 
 
 class NeighborAttention(torch.nn.Module):
@@ -140,7 +148,7 @@ class NeighborAttention(torch.nn.Module):
             if irreps.dim // self.num_heads > MAX_HEAD_COLUMNS:
                 raise NotImplementedError(f"{irreps.dim // self.num_heads} columns a head, at most {MAX_HEAD_COLUMNS} are supported")
         self.scale = float(scale) if scale is not None else (self.irreps_qk.dim // self.num_heads) ** -0.5
-        self._layouts = {}
+        self._layouts, self._dims = {}, (self.irreps_qk.dim, self.irreps_v.dim)
         runs = [mul // self.num_heads * ir.dim for irreps in (self.irreps_qk, self.irreps_v) for mul, ir in irreps]
         for vec in (1, 4, 8):
             if any(run % vec for run in runs):
@@ -148,7 +156,7 @@ class NeighborAttention(torch.nn.Module):
             tables = [_head_vectors(irreps, self.num_heads, vec) for irreps in (self.irreps_qk, self.irreps_v)]
             self.register_buffer(f"_qk{vec}", tables[0], persistent=False)
             self.register_buffer(f"_v{vec}", tables[1], persistent=False)
-            self._layouts[vec] = [vec, self.num_heads, tables[0].shape[0], tables[1].shape[0], self.irreps_qk.dim, self.irreps_v.dim]
+            self._layouts[vec] = (ctypes.c_int32 * 6)(vec, self.num_heads, tables[0].shape[0], tables[1].shape[0], *self._dims)
 
     def __repr__(self) -> str:
         return f"{self.__class__.__name__}(q, k: {self.irreps_qk}, v: {self.irreps_v}, {self.num_heads} heads)"
@@ -173,56 +181,57 @@ class NeighborAttention(torch.nn.Module):
         which is built in the backward pass (with a synchronisation: not while a graph is captured) if it is not given.
         Indices out of range are reported like those of `conv_uvu` and their edges left out.
         """
+        buffers = self._buffers
         _lib.require_same_device(q, k, v, rowptr, edge_src, perm, bias, buckets, edge_weight, *(transpose or ()))
-        _lib.require_operand(self._qk1, q, "NeighborAttention's tables (move the module with .to(device))", None, torch.int32)
+        if buffers["_qk1"].get_device() != q.get_device():
+            raise RuntimeError(f"Expected all tensors to be on the same device, but NeighborAttention's tables are on {buffers['_qk1'].device} and q is on "
+                               f"{q.device} (move the module with .to(device))")
         _lib.element_type(q, "q")
         if not q.dtype == k.dtype == v.dtype:
             raise TypeError(f"q, k and v must have one type, got {q.dtype}, {k.dtype} and {v.dtype}")
         for t, name in ((rowptr, "rowptr"), (edge_src, "edge_src"), (perm, "perm"), *((t, "transpose") for t in transpose or ())):
-            if t is not None and t.dtype != torch.int64:
-                raise TypeError(f"{name} must be int64")
-            torch._assert(t is None or t.dim() == 1, f"Incorrect shape for {name}")
-        H, dqk, dv = self.num_heads, self.irreps_qk.dim, self.irreps_v.dim
-        E = k.shape[0] if edge_src is None else edge_src.shape[0]
-        torch._assert(q.dim() == 2 and q.shape[1] == dqk, "Incorrect shape for q")
-        torch._assert(k.dim() == 2 and k.shape[1] == dqk, "Incorrect shape for k")
-        torch._assert(v.dim() == 2 and v.shape == (k.shape[0], dv), "Incorrect shape for v")
-        torch._assert(rowptr.shape[0] == q.shape[0] + 1, "Incorrect shape for rowptr")
-        torch._assert(perm is None or perm.shape[0] == E, "Incorrect shape for perm")
+            if t is not None and (t.dtype != torch.int64 or t.dim() != 1):
+                if t.dtype != torch.int64:
+                    raise TypeError(f"{name} must be int64")
+                torch._assert(False, f"Incorrect shape for {name}")
+        H, dqk, dv = self.num_heads, self._dims[0], self._dims[1]
+        N, S = q.shape[0] if q.dim() == 2 else -1, k.shape[0] if k.dim() == 2 else -1
+        E = S if edge_src is None else edge_src.shape[0]
+        wrong = [name for name, bad in (
+            ("q", q.shape != (N, dqk)), ("k", k.shape != (S, dqk)), ("v", v.shape != (S, dv)), ("rowptr", rowptr.shape[0] != N + 1),
+            ("perm", perm is not None and perm.shape[0] != E), ("buckets", buckets is not None and buckets.shape != (E,)),
+            ("bias", bias is not None and (bias.dim() != 2 or bias.shape[1] != H or (buckets is None and bias.shape[0] != E))),
+            ("edge_weight", edge_weight is not None and edge_weight.shape != (E,)),
+            ("transpose", transpose is not None and (len(transpose) != 2 or transpose[0].shape[0] != E or transpose[1].shape[0] != S + 1))) if bad]
+        if wrong:
+            torch._assert(False, f"Incorrect shape for {wrong[0]}")
         if buckets is not None:
             if bias is None:
                 raise ValueError("buckets need the table they index: bias=[num_buckets, num_heads]")
             if buckets.dtype != torch.int32:
                 raise TypeError("buckets must be int32")
-            torch._assert(buckets.shape == (E,), "Incorrect shape for buckets")
-            torch._assert(bias.dim() == 2 and bias.shape[1] == H, "Incorrect shape for bias")
-        elif bias is not None:
-            torch._assert(bias.shape == (E, H), "Incorrect shape for bias")
-        torch._assert(edge_weight is None or edge_weight.shape == (E,), "Incorrect shape for edge_weight")
-        if transpose is not None:
-            torch._assert(len(transpose) == 2 and transpose[0].shape[0] == E and transpose[1].shape[0] == k.shape[0] + 1, "Incorrect shape for transpose")
         for t, name in ((bias, "bias"), (edge_weight, "edge_weight")):
             if t is not None:
                 _lib.element_type(t, name)
-        if max(E, q.shape[0], k.shape[0]) >= 2 ** 31 - 1:
+        if max(E, N, S) >= 2 ** 31 - 1:
             raise NotImplementedError("at most 2^31 - 2 edges and rows")
-        _lib.poll_status(q.device)
+        _lib.check_earlier(q)
         q, k, v = _rows(q), _rows(k), _rows(v)
         c = _Call()
         # vectors of 16 bytes where the layout and the rows allow them, else of four elements, else single elements
         for c.vec in (4, 1) if q.dtype == torch.float32 else (8, 4, 1):
             if c.vec in self._layouts and _fits(q, c.vec) and _fits(k, c.vec) and _fits(v, c.vec):
                 break
-        c.layout = (ctypes.c_int32 * 6)(*self._layouts[c.vec])
-        c.qk_tbl, c.v_tbl = getattr(self, f"_qk{c.vec}"), getattr(self, f"_v{c.vec}")
+        c.layout, c.qk_tbl, c.v_tbl = self._layouts[c.vec], buffers[f"_qk{c.vec}"], buffers[f"_v{c.vec}"]
         c.scale, c.edges = self.scale, E
-        c.rowptr, c.src = rowptr.contiguous(), None if edge_src is None else edge_src.contiguous()
-        c.perm, c.buckets = None if perm is None else perm.contiguous(), None if buckets is None else buckets.contiguous()
+        c.rowptr, c.src, c.perm, c.buckets = (t if t is None or t.is_contiguous() else t.contiguous() for t in (rowptr, edge_src, perm, buckets))
         c.transpose = None if transpose is None else (transpose[0].contiguous(), transpose[1].contiguous())
         bias = None if bias is None else bias.to(torch.float32).contiguous()
         weight = None if edge_weight is None else edge_weight.to(torch.float32).contiguous()
-        train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias, weight))
-        out = _AttentionFunction.apply(q, k, v, bias, weight, c, train)
+        if _lib.wants_grad(q, k, v, bias, weight):
+            out = _AttentionFunction.apply(q, k, v, bias, weight, c)
+        else:
+            out = _attend(q, k, v, bias, weight, c, False)[0]
         if check_indices:
             _lib.check_status(q.device, "NeighborAttention")
         return out

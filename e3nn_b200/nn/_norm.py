@@ -62,7 +62,9 @@ def _float_bits(value: float) -> int:
 
 
 def _fp32(parameter: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return None if parameter is None else parameter.to(torch.float32).contiguous()
+    if parameter is None or (parameter.dtype == torch.float32 and parameter.is_contiguous()):
+        return parameter
+    return parameter.to(torch.float32).contiguous()
 
 
 def _aligned(t: torch.Tensor, width: int) -> torch.Tensor:
@@ -71,28 +73,43 @@ def _aligned(t: torch.Tensor, width: int) -> torch.Tensor:
 
 
 def _flat_rows(x: torch.Tensor, dim: int, name: str) -> torch.Tensor:
-    _lib.element_type(x, name)
-    torch._assert(x.dim() > 0 and x.shape[-1] == dim, f"Incorrect last dimension for {name}")
+    if x.dim() < 1 or x.shape[-1] != dim:
+        torch._assert(False, f"Incorrect last dimension for {name}")
+    if x.dim() == 2 and x.is_contiguous():
+        return x
     return x.reshape(-1, dim).contiguous() if dim > 0 else x.reshape(x.shape[:-1].numel(), 0)
+
+
+def _on_device_of(x: torch.Tensor, module: torch.nn.Module, table: torch.Tensor, *parameters: Optional[torch.Tensor]) -> None:
+    device = x.get_device()
+    if table.get_device() != device or any(p is not None and p.get_device() != device for p in parameters):
+        raise RuntimeError(f"Expected all tensors to be on the same device, but the input is on {x.device} and {type(module).__name__}'s tables or "
+                           "parameters are not (move the module with .to(device))")
+
+
+def _rms_norm(x, weight, tables, fours: int, eps: float) -> torch.Tensor:
+    tbl, inv, _ = tables
+    h = torch.empty_like(x)
+    with _lib.device_of(x):
+        rc = _lib.core().e3b_rms_norm_fwd(x.data_ptr(), _lib.address(weight), tbl.data_ptr(), inv.data_ptr(), inv.shape[0], fours, eps, h.data_ptr(),
+                                          x.shape[0], x.shape[1], _lib.element_type(x), _lib.raw_stream(x))
+    if rc:
+        _lib.check(rc, "e3b_rms_norm_fwd")
+    return h
 
 
 class _RMSNormFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, tbl, inv, channels, fours, eps):
-        h = torch.empty_like(x)
-        with _lib.device_of(x):
-            rc = _lib.core().e3b_rms_norm_fwd(_lib._ptr(x), _lib._ptr(weight), _lib._ptr(tbl), _lib._ptr(inv), inv.shape[0], fours, eps,
-                                              _lib._ptr(h), x.shape[0], x.shape[1], _lib.element_type(x), _lib.stream_ptr())
-        _lib.check(rc, "e3b_rms_norm_fwd")
-        ctx.save_for_backward(x, weight, tbl, inv, channels)
-        ctx.meta = (fours, eps)
-        return h
+    def forward(ctx, x, weight, tables, fours, eps):
+        ctx.save_for_backward(x, weight)
+        ctx.meta = (tables, fours, eps)
+        return _rms_norm(x, weight, tables, fours, eps)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        x, weight, tbl, inv, channels = ctx.saved_tensors
-        fours, eps = ctx.meta
+        x, weight = ctx.saved_tensors
+        (tbl, inv, channels), fours, eps = ctx.meta
         core, (rows, dim), nch = _lib.core(), x.shape, channels.shape[0]
         gx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
         gw = scratch = None
@@ -103,11 +120,12 @@ class _RMSNormFunction(torch.autograd.Function):
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
         grad = grad.contiguous()
         with _lib.device_of(x):
-            rc = core.e3b_rms_norm_bwd(_lib._ptr(x), _lib._ptr(grad), _lib._ptr(weight), _lib._ptr(tbl), _lib._ptr(inv), _lib._ptr(channels), nch,
-                                       inv.shape[0], fours, eps, _lib._ptr(gx), _lib._ptr(gw), _lib._ptr(scratch), nbytes, rows, dim,
-                                       _lib.element_type(x), _lib.stream_ptr())
-        _lib.check(rc, "e3b_rms_norm_bwd")
-        return gx, gw, None, None, None, None, None
+            rc = core.e3b_rms_norm_bwd(x.data_ptr(), grad.data_ptr(), _lib.address(weight), tbl.data_ptr(), inv.data_ptr(), channels.data_ptr(), nch,
+                                       inv.shape[0], fours, eps, _lib.address(gx), _lib.address(gw), _lib.address(scratch), nbytes, rows, dim,
+                                       _lib.element_type(x), _lib.raw_stream(x))
+        if rc:
+            _lib.check(rc, "e3b_rms_norm_bwd")
+        return gx, gw, None, None, None
 
 
 class RMSNorm(torch.nn.Module):
@@ -123,6 +141,7 @@ class RMSNorm(torch.nn.Module):
         if not self.eps >= 0.0:
             raise ValueError(f"eps must not be negative, got {eps}")
         blocks = _blocks(self.irreps_in)
+        self._dim = self.irreps_in.dim
         self._fours = int(_fours(blocks))
         cols = _column_blocks(blocks)
         tbl = torch.tensor([(b, c, 0, 0) for b, c in cols], dtype=torch.int32).reshape(-1, 4)
@@ -140,14 +159,18 @@ class RMSNorm(torch.nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if not x.is_cuda:
             raise NotImplementedError("RMSNorm runs on CUDA tensors only")
-        dim = self.irreps_in.dim
-        rows = _flat_rows(x, dim, "x")
-        _lib.require_operand(self._tbl, x, "RMSNorm's tables (move the module with .to(device))", None, torch.int32)
-        _lib.poll_status(x.device)
-        if self.weight is not None and self.weight.device != x.device:
-            raise RuntimeError(f"Expected all tensors to be on the same device, but weight is on {self.weight.device} and x on {x.device}")
-        out = _RMSNormFunction.apply(rows, _fp32(self.weight), self._tbl, self._inv_bits.view(torch.float32), self._channels, self._fours, self.eps)
-        return out.reshape(x.shape)
+        buffers, weight = self._buffers, self._parameters["weight"]
+        tables = (buffers["_tbl"], buffers["_inv_bits"], buffers["_channels"])
+        _on_device_of(x, self, tables[0], weight)
+        _lib.element_type(x, "x")
+        rows = _flat_rows(x, self._dim, "x")
+        _lib.check_earlier(x)
+        weight = _fp32(weight)
+        if _lib.wants_grad(rows, weight):
+            out = _RMSNormFunction.apply(rows, weight, tables, self._fours, self.eps)
+        else:
+            out = _rms_norm(rows, weight, tables, self._fours, self.eps)
+        return out if x.dim() == 2 else out.reshape(x.shape)
 
 
 def _gate_items(back, const, forth, ins, outs, width: int, narrow: int):
@@ -186,22 +209,27 @@ def _gate_items(back, const, forth, ins, outs, width: int, narrow: int):
     return (torch.tensor(wides, dtype=torch.int32).reshape(-1, 4 + width), torch.tensor(narrows, dtype=torch.int32).reshape(-1, 8), len(slot_of))
 
 
+def _norm_gate(residual, y, w_post, scale, w_pre, tables, sizes, eps: float):
+    wide, narrow, in_tbl, out_tbl, _, _, in_inv, out_inv = tables
+    z = torch.empty_like(residual)
+    h = torch.empty_like(residual) if w_pre is not None else None
+    with _lib.device_of(y):
+        rc = _lib.core().e3b_norm_gate_residual_fwd(
+            residual.data_ptr(), y.data_ptr(), w_post.data_ptr(), scale.data_ptr(), _lib.address(w_pre), wide.data_ptr(), narrow.data_ptr(),
+            in_tbl.data_ptr(), out_tbl.data_ptr(), in_inv.data_ptr(), out_inv.data_ptr(), sizes, eps, z.data_ptr(), _lib.address(h), y.shape[0],
+            _lib.element_type(y), _lib.raw_stream(y))
+    if rc:
+        _lib.check(rc, "e3b_norm_gate_residual_fwd")
+    return z, h
+
+
 class _NormGateFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, residual, y, w_post, scale, w_pre, tables, sizes, eps):
-        wide, narrow, in_tbl, out_tbl, _, _, in_inv, out_inv = tables
-        z = torch.empty_like(residual)
-        h = torch.empty_like(residual) if w_pre is not None else None
-        with _lib.device_of(y):
-            rc = _lib.core().e3b_norm_gate_residual_fwd(
-                _lib._ptr(residual), _lib._ptr(y), _lib._ptr(w_post), _lib._ptr(scale), _lib._ptr(w_pre), _lib._ptr(wide), _lib._ptr(narrow),
-                _lib._ptr(in_tbl), _lib._ptr(out_tbl), _lib._ptr(in_inv), _lib._ptr(out_inv), sizes, eps, _lib._ptr(z), _lib._ptr(h), y.shape[0], _lib.element_type(y),
-                _lib.stream_ptr())
-        _lib.check(rc, "e3b_norm_gate_residual_fwd")
         ctx.save_for_backward(residual, y, w_post, scale, w_pre)
         ctx.meta = (tables, sizes, eps)
         ctx.set_materialize_grads(False)
-        return z, h
+        return _norm_gate(residual, y, w_post, scale, w_pre, tables, sizes, eps)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -210,7 +238,7 @@ class _NormGateFunction(torch.autograd.Function):
         tables, sizes, eps = ctx.meta
         if grad_z is None and grad_h is None:
             return (None,) * 8
-        core, rows = _lib.core(), y.shape[0]
+        core, rows, address = _lib.core(), y.shape[0], _lib.address
         grad_z, grad_h = (None if g is None else _aligned(g.contiguous(), sizes[0]) for g in (grad_z, grad_h))
         g_residual = torch.empty_like(residual) if ctx.needs_input_grad[0] else None
         gy = torch.empty_like(y) if ctx.needs_input_grad[1] else None
@@ -222,10 +250,11 @@ class _NormGateFunction(torch.autograd.Function):
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=y.device)
         with _lib.device_of(y):
             rc = core.e3b_norm_gate_residual_bwd(
-                _lib._ptr(residual), _lib._ptr(y), _lib._ptr(grad_z), _lib._ptr(grad_h), _lib._ptr(w_post), _lib._ptr(scale), _lib._ptr(w_pre),
-                *(_lib._ptr(t) for t in tables), sizes, eps, _lib._ptr(g_residual), _lib._ptr(gy), _lib._ptr(params), _lib._ptr(scratch), nbytes,
-                rows, _lib.element_type(y), _lib.stream_ptr())
-        _lib.check(rc, "e3b_norm_gate_residual_bwd")
+                residual.data_ptr(), y.data_ptr(), address(grad_z), address(grad_h), w_post.data_ptr(), scale.data_ptr(), address(w_pre),
+                *(t.data_ptr() for t in tables), sizes, eps, address(g_residual), address(gy), address(params), address(scratch), nbytes, rows,
+                _lib.element_type(y), _lib.raw_stream(y))
+        if rc:
+            _lib.check(rc, "e3b_norm_gate_residual_bwd")
         gw = params.split([n_in, n_out, n_out]) if params is not None else (None, None, None)
         return (g_residual, gy, gw[0], gw[1], gw[2] if w_pre is not None else None, None, None, None)
 
@@ -269,12 +298,14 @@ class NormGateResidual(torch.nn.Module):
         self._dims = (din, dout)
         if max(len(ins), len(outs)) > 32:
             raise NotImplementedError(f"at most 32 blocks of irreps are supported, got {self.irreps_in} -> {self.irreps_out}")
-        self._sizes = {}
+        self._sizes, self._table_names = {}, {}
         for width, narrow in ((1, 1), (4, 1), (4, 2), (8, 2)):
             items = _gate_items(back, const, forth, ins, outs, width, narrow)
             if items is not None:
                 self.register_buffer(f"_wide{width}{narrow}", items[0], persistent=False)
                 self.register_buffer(f"_narrow{width}{narrow}", items[1], persistent=False)
+                self._table_names[width, narrow] = (f"_wide{width}{narrow}", f"_narrow{width}{narrow}", "_in", "_out", "_in_channels", "_out_channels",
+                                                    "_in_inv_bits", "_out_inv_bits")
                 self._sizes[width, narrow] = (ctypes.c_int32 * 11)(width, narrow, len(items[0]), len(items[1]), items[2], din, dout, len(ins),
                                                                    len(outs), n_in, n_out)
         self.weight_post = torch.nn.Parameter(torch.ones(n_in))
@@ -290,22 +321,25 @@ class NormGateResidual(torch.nn.Module):
     def forward(self, residual: torch.Tensor, y: torch.Tensor):
         if not (residual.is_cuda and y.is_cuda):
             raise NotImplementedError("NormGateResidual runs on CUDA tensors only")
-        torch._assert(residual.shape[:-1] == y.shape[:-1], "residual and y must have the same leading dimensions")
+        if residual.shape[:-1] != y.shape[:-1]:
+            torch._assert(False, "residual and y must have the same leading dimensions")
         if residual.dtype != y.dtype:
             raise TypeError(f"residual and y must have one type, got {residual.dtype} and {y.dtype}")
-        _lib.require_same_device(y, residual, self.weight_post, self.scale, self.weight_pre)
-        din, dout = self._dims
+        _lib.element_type(y, "y")
+        buffers, parameters = self._buffers, self._parameters
+        w_post, scale, w_pre = parameters["weight_post"], parameters["scale"], parameters["weight_pre"]
+        _on_device_of(y, self, buffers["_in"], residual, w_post, scale, w_pre)
+        (din, dout), sizes = self._dims, self._sizes
         # vectors of 16 bytes if the row falls into such
         for key in ((4, 1), (1, 1)) if y.dtype == torch.float32 else ((8, 2), (4, 2), (1, 1)):
-            if key in self._sizes:
+            if key in sizes:
                 break
-        width = key[0]
-        r, x = _aligned(_flat_rows(residual, dout, "residual"), width), _aligned(_flat_rows(y, din, "y"), width)
-        _lib.require_operand(self._in, y, "NormGateResidual's tables (move the module with .to(device))", None, torch.int32)
-        _lib.poll_status(y.device)
-        wide, narrow = getattr(self, f"_wide{key[0]}{key[1]}"), getattr(self, f"_narrow{key[0]}{key[1]}")
-        tables = (wide, narrow, self._in, self._out, self._in_channels, self._out_channels, self._in_inv_bits, self._out_inv_bits)
-        z, h = _NormGateFunction.apply(r, x, _fp32(self.weight_post), _fp32(self.scale), _fp32(self.weight_pre), tables,
-                                       self._sizes[key], self.eps)
-        z = z.reshape(residual.shape)
-        return (z, h.reshape(residual.shape)) if self.pre_norm else z
+        r, x = _aligned(_flat_rows(residual, dout, "residual"), key[0]), _aligned(_flat_rows(y, din, "y"), key[0])
+        _lib.check_earlier(y)
+        tables = (*(buffers[name] for name in self._table_names[key]),)
+        args = (r, x, _fp32(w_post), _fp32(scale), _fp32(w_pre))
+        apply = _NormGateFunction.apply if _lib.wants_grad(*args) else _norm_gate
+        z, h = apply(*args, tables, sizes[key], self.eps)
+        if residual.dim() == 2:
+            return (z, h) if self.pre_norm else z
+        return (z.reshape(residual.shape), h.reshape(residual.shape)) if self.pre_norm else z.reshape(residual.shape)

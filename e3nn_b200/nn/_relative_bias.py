@@ -16,25 +16,29 @@ import torch
 from .. import _lib
 
 
+def _look_up(weight: torch.Tensor, buckets: torch.Tensor) -> torch.Tensor:
+    num, heads = weight.shape
+    out = torch.empty(buckets.shape[0], heads, dtype=weight.dtype, device=weight.device)
+    with _lib.device_of(weight):
+        rc = _lib.core().e3b_relative_bias_fwd(weight.data_ptr(), buckets.data_ptr(), num, heads, buckets.shape[0], _lib.element_type(weight), out.data_ptr(),
+                                               _lib.status_address(weight), _lib.raw_stream(weight))
+    if rc:
+        _lib.check(rc, "e3b_relative_bias_fwd")
+    return out
+
+
 class _RelativeBiasFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weight, buckets):
-        out = torch.empty(buckets.shape[0], weight.shape[1], dtype=weight.dtype, device=weight.device)
-        with _lib.device_of(weight):
-            rc = _lib.core().e3b_relative_bias_fwd(_lib._ptr(weight), _lib._ptr(buckets), weight.shape[0], weight.shape[1], buckets.shape[0],
-                                                   _lib.element_type(weight), _lib._ptr(out), _lib._ptr(_lib.status_word(weight.device)),
-                                                   _lib.stream_ptr())
-        _lib.check(rc, "e3b_relative_bias_fwd")
         ctx.save_for_backward(buckets)
-        ctx.meta = (weight.shape, weight.dtype)
-        return out
+        ctx.meta = (weight.shape[0], weight.dtype)
+        return _look_up(weight, buckets)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         (buckets,) = ctx.saved_tensors
-        shape, dtype = ctx.meta
-        return bias_table_grad(grad, buckets, shape[0], dtype), None
+        return bias_table_grad(grad, buckets, *ctx.meta), None
 
 
 def bias_table_grad(grad: torch.Tensor, buckets: torch.Tensor, num_buckets: int, dtype: torch.dtype) -> torch.Tensor:
@@ -46,9 +50,10 @@ def bias_table_grad(grad: torch.Tensor, buckets: torch.Tensor, num_buckets: int,
     nbytes = core.e3b_relative_bias_scratch_bytes(edges, num_buckets, heads)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=grad.device)
     with _lib.device_of(grad):
-        rc = core.e3b_relative_bias_bwd(_lib._ptr(grad), _lib._ptr(buckets), num_buckets, heads, edges, _lib.element_type(grad), _lib._ptr(out),
-                                        _lib.element_type(out), _lib._ptr(scratch), nbytes, _lib._ptr(_lib.status_word(grad.device)), _lib.stream_ptr())
-    _lib.check(rc, "e3b_relative_bias_bwd")
+        rc = core.e3b_relative_bias_bwd(grad.data_ptr(), buckets.data_ptr(), num_buckets, heads, edges, _lib.element_type(grad), _lib.address(out),
+                                        _lib.element_type(out), _lib.address(scratch), nbytes, _lib.status_address(grad), _lib.raw_stream(grad))
+    if rc:
+        _lib.check(rc, "e3b_relative_bias_bwd")
     return out
 
 
@@ -80,34 +85,38 @@ class RelativeBias(torch.nn.Module):
         if not pos.is_cuda:
             raise NotImplementedError("RelativeBias runs on CUDA tensors only")
         _lib.require_same_device(pos, edge_src, edge_dst, shift)
-        _lib.require_operand(self._squares, pos, "RelativeBias's tables (move the module with .to(device))", None, torch.int64)
-        E = edge_src.numel()
+        squares, E = self._buffers["_squares"], edge_src.shape[0] if edge_src.dim() == 1 else -1
+        _lib.require_operand(squares, pos, "RelativeBias's tables (move the module with .to(device))", None, torch.int64)
         if pos.dtype != torch.float32 or (shift is not None and shift.dtype != torch.float32):
             raise TypeError("pos and shift must be float32")
         if edge_src.dtype != torch.int64 or edge_dst.dtype != torch.int64:
             raise TypeError("edge_src and edge_dst must be int64")
-        torch._assert(pos.dim() == 2 and pos.shape[1] == 3, "Incorrect shape for pos")
-        torch._assert(edge_src.shape == edge_dst.shape == (E,), "Incorrect shape for edge_src or edge_dst")
-        torch._assert(shift is None or shift.shape == (E, 3), "Incorrect shape for shift")
-        _lib.poll_status(pos.device)
+        if pos.dim() != 2 or pos.shape[1] != 3:
+            torch._assert(False, "Incorrect shape for pos")
+        if E < 0 or edge_dst.shape != (E,) or (shift is not None and shift.shape != (E, 3)):
+            torch._assert(False, "Incorrect shape for edge_src, edge_dst or shift")
+        _lib.check_earlier(pos)
         out = torch.empty(E, dtype=torch.int32, device=pos.device)
-        pos, edge_src, edge_dst = pos.detach().contiguous(), edge_src.contiguous(), edge_dst.contiguous()
-        shift = shift.detach().contiguous() if shift is not None else None
+        pos, edge_src, edge_dst = pos.contiguous(), edge_src.contiguous(), edge_dst.contiguous()
+        shift = shift.contiguous() if shift is not None else None
         with _lib.device_of(pos):
-            rc = _lib.core().e3b_distance_buckets(_lib._ptr(pos), _lib._ptr(edge_src), _lib._ptr(edge_dst), _lib._ptr(shift), _lib._ptr(self._squares),
-                                                  self.num_buckets - 1, E, pos.shape[0], _lib._ptr(out), _lib._ptr(_lib.status_word(pos.device)),
-                                                  _lib.stream_ptr())
-        _lib.check(rc, "e3b_distance_buckets")
+            rc = _lib.core().e3b_distance_buckets(pos.data_ptr(), edge_src.data_ptr(), edge_dst.data_ptr(), _lib.address(shift), squares.data_ptr(),
+                                                  self.num_buckets - 1, E, pos.shape[0], out.data_ptr(), _lib.status_address(pos), _lib.raw_stream(pos))
+        if rc:
+            _lib.check(rc, "e3b_distance_buckets")
         return out
 
     def forward(self, buckets: torch.Tensor) -> torch.Tensor:
         if not buckets.is_cuda:
             raise NotImplementedError("RelativeBias runs on CUDA tensors only")
-        if self.weight.device != buckets.device:
-            raise RuntimeError(f"Expected all tensors to be on the same device, but weight is on {self.weight.device} and buckets on {buckets.device}")
+        weight = self._parameters["weight"]
+        if weight.get_device() != buckets.get_device():
+            raise RuntimeError(f"Expected all tensors to be on the same device, but weight is on {weight.device} and buckets on {buckets.device}")
         if buckets.dtype != torch.int32:
             raise TypeError("buckets must be int32")
-        torch._assert(buckets.dim() == 1, "Incorrect shape for buckets")
-        _lib.element_type(self.weight, "weight")
-        _lib.poll_status(buckets.device)
-        return _RelativeBiasFunction.apply(self.weight.contiguous(), buckets.contiguous())
+        if buckets.dim() != 1:
+            torch._assert(False, "Incorrect shape for buckets")
+        _lib.element_type(weight, "weight")
+        _lib.check_earlier(buckets)
+        apply = _RelativeBiasFunction.apply if _lib.wants_grad(weight) else _look_up
+        return apply(weight.contiguous(), buckets.contiguous())
