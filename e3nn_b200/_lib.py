@@ -277,7 +277,7 @@ def core() -> ctypes.CDLL:
         lib.e3b_rms_norm_fwd.argtypes = [vp] * 4 + [i, i, f, vp, i64, i, i, vp]
         lib.e3b_rms_norm_bwd.argtypes = [vp] * 6 + [i, i, i, f, vp, vp, vp, i64, i64, i, i, vp]
         lib.e3b_norm_scratch_bytes.argtypes = [i64, i]
-        lib.e3b_norm_gate_residual_fwd.argtypes = [vp] * 12 + [f, vp, vp, i64, i, vp]
+        lib.e3b_norm_gate_residual_fwd.argtypes = [vp] * 13 + [f, vp, vp, i64, i, vp]
         lib.e3b_norm_gate_residual_bwd.argtypes = [vp] * 16 + [f, vp, vp, vp, vp, i64, i64, i, vp]
         lib.e3b_distance_buckets.argtypes = [vp] * 5 + [i, i64, i64, vp, vp, vp]
         lib.e3b_relative_bias_fwd.argtypes = [vp, vp, i, i, i64, i, vp, vp, vp]

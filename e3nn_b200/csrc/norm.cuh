@@ -11,26 +11,15 @@ namespace {
 
 constexpr int kMaxThreads = 512;
 
-// Sums over the irreps blocks of a row by the warps that touch a block.  share: [nblk][nw]; span: [nblk][2] first and last of those
-// warps (warps between them that do not touch the block leave the zero from the start of the kernel).
+// Sums over the irreps blocks of a row by the warps that touch a block.  share: [nblk][nw], nw the number of warps rounded up to a power
+// of two; what a warp does not touch stays at the zero from the start of the kernel.
 struct BlockSums {
     float* share;
-    int* span;
     int nblk, nw;
     __device__ __forceinline__ void clear() const {
         for (int i = threadIdx.x; i < nblk * nw; i += blockDim.x) share[i] = 0.0f;
-        for (int i = threadIdx.x; i < nblk; i += blockDim.x) { span[2 * i] = 1 << 30; span[2 * i + 1] = -1; }
     }
-    __device__ __forceinline__ void touch(unsigned blocks) const {      // the warp's
-        const int warp = threadIdx.x >> 5;
-        if ((threadIdx.x & 31) == 0)
-            for (; blocks; blocks &= blocks - 1) {
-                const int b = __ffs(blocks) - 1;
-                atomicMin(&span[2 * b], warp);
-                atomicMax(&span[2 * b + 1], warp);
-            }
-    }
-    // shares of this warp's items: K values of the blocks vb, M of the blocks wb (0 where there is no item)
+    // shares of this warp's items: K values of the blocks vb, M of the blocks wb (0 where there is no item); `blocks`: what it touches
     template <int K, int M>
     __device__ __forceinline__ void add(unsigned blocks, const float (&v)[K], const int (&vb)[K], const float (&w)[M], const int (&wb)[M]) const {
         for (; blocks; blocks &= blocks - 1) {
@@ -44,16 +33,37 @@ struct BlockSums {
             if ((threadIdx.x & 31) == 0) share[b * nw + (threadIdx.x >> 5)] = s;
         }
     }
-    __device__ __forceinline__ float get(int b) const {
-        const int w1 = span[2 * b + 1];
-        float s = 0.0f;
-        for (int w = span[2 * b]; w <= w1; ++w) s += share[b * nw + w];
-        return s;
+    // sums of the blocks vb and wb (whole warps; after a barrier): 32 / nw blocks at a time, nw lanes each
+    template <int K, int M>
+    __device__ __forceinline__ void get(const int (&vb)[K], float (&v)[K], const int (&wb)[M], float (&w)[M]) const {
+        const int lane = threadIdx.x & 31, at_once = 32 / nw;
+        for (int b0 = 0; b0 < nblk; b0 += at_once) {
+            const int i = b0 * nw + lane;
+            float s = i < nblk * nw ? share[i] : 0.0f;
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1)
+                if (o < nw) s += __shfl_xor_sync(0xffffffffu, s, o);
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const float t = __shfl_sync(0xffffffffu, s, (vb[k] - b0) * nw & 31);
+                if (vb[k] >= b0 && vb[k] < b0 + at_once) v[k] = t;
+            }
+#pragma unroll
+            for (int j = 0; j < M; ++j) {
+                const float t = __shfl_sync(0xffffffffu, s, (wb[j] - b0) * nw & 31);
+                if (wb[j] >= b0 && wb[j] < b0 + at_once) w[j] = t;
+            }
+        }
     }
-    __host__ __device__ static int floats(int nblk, int nw) { return (nblk * nw + 2 * nblk + 3) / 4 * 4; }
+    __host__ __device__ static int floats(int nblk, int nw) { return (nblk * nw + 3) / 4 * 4; }
 };
+inline int warps_pow2(int threads) {
+    int n = 1;
+    while (n * 32 < threads) n *= 2;
+    return n;
+}
 __device__ __forceinline__ BlockSums block_sums_at(float*& p, int nblk, int nw) {
-    BlockSums b{p, reinterpret_cast<int*>(p + nblk * nw), nblk, nw};
+    BlockSums b{p, nblk, nw};
     p += BlockSums::floats(nblk, nw);
     return b;
 }

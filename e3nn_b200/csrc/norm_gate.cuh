@@ -10,6 +10,8 @@
 //           the others waited at the next barrier: 1,443 us of 262,144 rows in bf16 against what norm_gate.cu states).
 // Only the activated gates, and backward the products whose sums are the gates' gradients, go through shared memory.
 #pragma once
+#include <cstring>
+
 #include "norm.cuh"
 
 namespace e3b {
@@ -83,34 +85,276 @@ struct Items {
     }
 };
 
-// The next rows of A arrays on their way to shared memory (cp.async), kAhead rows in front of the one in hand.  Every thread
+// The next rows of A arrays on their way: by cp.async to shared memory, two rows in front of the one in hand.  Every thread
 // fetches its own columns and reads nothing else, so the only wait is for its own copies.  Single 16-bit columns are too
-// small for such a copy: they are loaded when they are needed.
-constexpr int kAhead = 2;
+// small for such a copy: they are loaded into registers, one row in front.
+__host__ __device__ constexpr int rows_ahead(int bytes) { return bytes >= 4 ? 2 : 1; }
 template <typename T, int WIDTH, int N, int A>
 struct RowAhead {
     static constexpr int kBytes = WIDTH * static_cast<int>(sizeof(T));
     static constexpr bool kAsync = kBytes >= 4;
-    static constexpr int kThread = kAsync ? kAhead * A * N * kBytes : 0;      // bytes a thread
-    char* mine;            // this thread's place: [kAhead][A][N] of kBytes, a block of threads apart
+    static constexpr int kThread = kAsync ? rows_ahead(kBytes) * A * N * kBytes : 0;      // bytes a thread
+    char* mine;            // this thread's place: [rows ahead][A][N] of kBytes, a block of threads apart
+    Packed<T, WIDTH> reg[kAsync ? 1 : A][kAsync ? 1 : N];
     __device__ __forceinline__ explicit RowAhead(void* smem) : mine(static_cast<char*>(smem) + threadIdx.x * kBytes) {}
     __device__ __forceinline__ char* at(int stage, int a, int n) const { return mine + ((stage * A + a) * N + n) * static_cast<int>(blockDim.x) * kBytes; }
-    __device__ __forceinline__ void fetch(int stage, int a, int n, const T* from) const {
+    __device__ __forceinline__ void fetch(int stage, int a, int n, const T* from) {
         if constexpr (kAsync) {
             const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(at(stage, a, n)));
             if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(__cvta_generic_to_global(from)) : "memory");
             else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(__cvta_generic_to_global(from)), "n"(kBytes) : "memory");
+        } else {
+            reg[a][n].load(from);
         }
     }
-    __device__ __forceinline__ void read(int stage, int a, int n, const T* from, float (&f)[WIDTH]) const {
-        Packed<T, WIDTH> p;
-        if constexpr (kAsync) p.load(reinterpret_cast<const T*>(at(stage, a, n)));
-        else p.load(from);
-        p.unpack(f);
+    __device__ __forceinline__ void read(int stage, int a, int n, float (&f)[WIDTH]) const {
+        if constexpr (kAsync) {
+            Packed<T, WIDTH> p;
+            p.load(reinterpret_cast<const T*>(at(stage, a, n)));
+            p.unpack(f);
+        } else {
+            reg[a][n].unpack(f);
+        }
     }
 };
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_row() { asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory"); }
+__device__ __forceinline__ void wait_for_row() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }      // two groups under way
+
+// ------------------------------------------------------------------------------------------------- one warp a row
+// Rows of ordinary width are taken by one warp each: no barriers, sums by shuffles, and the work that does not depend on the
+// width (sums, roots, addresses) is done once a row and not once a warp of it.  The columns fall into slots of 32 items that lie
+// side by side in the input and in the output row and belong to one irreps block, so everything about a slot but the lane's place in it
+// is the same for all lanes and comes from the kernel's parameters.
+constexpr int kMaxWide = 9, kMaxNarrow = 8, kMaxBlocks = 8;
+struct WideSlot {
+    int in, out, count;        // first columns, items
+    int bi, bo;                // irreps blocks
+    int gates;                 // place of the first column's gate in the row of gates per column, -1: no gate
+};
+struct NarrowSlot {
+    int kind, in, out, count, bi, bo, act;
+    float cst;
+    int spread, comps;         // gates: place of the first gate's copies, copies of each (components of its channel)
+};
+struct RowPlan {
+    WideSlot w[kMaxWide];
+    NarrowSlot n[kMaxNarrow];
+    int num_wide, num_narrow, din, dout, nblk_in, nblk_out, num_spread;      // num_spread: length of the row of gates per column
+    float inv_in[kMaxBlocks], inv_out[kMaxBlocks];           // 1 / columns, in the order in which the slots come to the blocks
+    unsigned wide_in_ends, narrow_in_ends, wide_out_ends, narrow_out_ends;
+};
+constexpr int kPlanHead = 9, kPlanSlot = 10;     // host array: {vec, narrow, wide slots, narrow slots, din, dout, blocks in, blocks out, spread}, slots
+
+// The kernel's parameters from the host's array.  False: more slots or blocks than a warp's registers take.
+inline bool row_plan(const int32_t* host, const int32_t* in_count, const int32_t* out_count, RowPlan* p) {
+    *p = {};
+    p->num_wide = host[2];
+    p->num_narrow = host[3];
+    p->din = host[4];
+    p->dout = host[5];
+    p->nblk_in = host[6];
+    p->nblk_out = host[7];
+    p->num_spread = host[8];
+    if (p->num_wide > kMaxWide || p->num_narrow > kMaxNarrow || p->nblk_in > kMaxBlocks || p->nblk_out > kMaxBlocks) return false;
+    const int32_t* s = host + kPlanHead;
+    for (int i = 0; i < p->num_wide; ++i, s += kPlanSlot) p->w[i] = {s[0], s[1], s[2], s[3], s[4], s[5]};
+    for (int i = 0; i < p->num_narrow; ++i, s += kPlanSlot) {
+        float cst;
+        memcpy(&cst, &s[7], sizeof(cst));
+        p->n[i] = {s[0], s[1], s[2], s[3], s[4], s[5], s[6], cst, s[8], s[9]};
+    }
+    // blocks numbered in the order of the slots; a block whose slots do not come together is not for this kernel
+    int in_seen[32], out_seen[32], n_in = 0, n_out = 0;
+    auto visit = [](int block, int* seen, int* n) {
+        if (*n > 0 && seen[*n - 1] == block) return true;
+        for (int i = 0; i < *n; ++i)
+            if (seen[i] == block) return false;
+        seen[(*n)++] = block;
+        return true;
+    };
+    int last_in = -1, last_out = -1;          // slot (narrow ones from 0, wide ones from kMaxNarrow on) that ends the present block
+    auto mark = [](int slot, unsigned* narrow, unsigned* wide) {
+        if (slot < 0) return;
+        if (slot < kMaxNarrow) *narrow |= 1u << slot;
+        else *wide |= 1u << (slot - kMaxNarrow);
+    };
+    auto slot = [&](int number, int* bi, int* bo, bool has_out) {
+        const int before_in = n_in, before_out = n_out;
+        if (!visit(*bi, in_seen, &n_in) || (has_out && !visit(*bo, out_seen, &n_out))) return false;
+        if (n_in != before_in) mark(last_in, &p->narrow_in_ends, &p->wide_in_ends);
+        last_in = number;
+        *bi = n_in - 1;
+        if (has_out) {
+            if (n_out != before_out) mark(last_out, &p->narrow_out_ends, &p->wide_out_ends);
+            last_out = number;
+            *bo = n_out - 1;
+        }
+        return true;
+    };
+    for (int j = 0; j < p->num_narrow; ++j)
+        if (!slot(j, &p->n[j].bi, &p->n[j].bo, p->n[j].out >= 0)) return false;
+    for (int k = 0; k < p->num_wide; ++k)
+        if (!slot(kMaxNarrow + k, &p->w[k].bi, &p->w[k].bo, true)) return false;
+    mark(last_in, &p->narrow_in_ends, &p->wide_in_ends);
+    mark(last_out, &p->narrow_out_ends, &p->wide_out_ends);
+    for (int i = 0; i < n_in; ++i) p->inv_in[i] = 1.0f / static_cast<float>(in_count[in_seen[i]]);
+    for (int i = 0; i < n_out; ++i) p->inv_out[i] = 1.0f / static_cast<float>(out_count[out_seen[i]]);
+    return true;
+}
+
+// Activations of a narrow item: silu and sigmoid on the hardware's exponential and division (relative error below 2^-22 + |x| 2^-23, where
+// gate_act costs five times the instructions), the others as in gate_act.
+template <int N>
+__device__ __forceinline__ void activate(int act, float cst, const float (&x)[N], float (&y)[N]) {
+    if (act == kGSilu || act == kGSigmoid) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float s = cst * __fdividef(1.0f, 1.0f + __expf(-x[i]));
+            y[i] = act == kGSilu ? x[i] * s : s;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) y[i] = cst * gate_act(act, x[i]);
+    }
+}
+
+// The same with the derivative (y may be x).
+template <int N>
+__device__ __forceinline__ void activate_and_derive(int act, float cst, const float (&x)[N], float (&y)[N], float (&dy)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float v = x[i];
+        if (act == kGSilu || act == kGSigmoid) {
+            const float s = __fdividef(1.0f, 1.0f + __expf(-v)), ds = s * (1.0f - s);
+            y[i] = cst * (act == kGSilu ? v * s : s);
+            dy[i] = cst * (act == kGSilu ? fmaf(v, ds, s) : ds);
+        } else {
+            y[i] = cst * gate_act(act, v);
+            dy[i] = cst * gate_act_grad(act, v);
+        }
+    }
+}
+
+// Sums over the irreps blocks of a row.  The slots come block by block, the narrow ones of a block before the wide ones: bit j of
+// narrow_ends (k of wide_ends) is set where a block ends with slot j (k); out receives the blocks in that order:
+// rsqrt(sum * inv + eps) or, with MEAN, sum * inv.  In shared memory of the warp.
+template <bool MEAN, int K, int M>
+__device__ __forceinline__ void row_sums(const float (&wv)[K], const float (&nv)[M], unsigned wide_ends, unsigned narrow_ends, const float* inv, float eps,
+                                         float* out) {
+    float s = 0.0f;
+    int b = 0;
+    auto end = [&]() {
+        s = warp_sum(s);
+        if ((threadIdx.x & 31) == 0) out[b] = MEAN ? s * inv[b] : rsqrtf(fmaf(s, inv[b], eps));
+        s = 0.0f;
+        ++b;
+    };
+#pragma unroll
+    for (int j = 0; j < M; ++j) {
+        s += nv[j];
+        if (narrow_ends >> j & 1u) end();
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        s += wv[k];
+        if (wide_ends >> k & 1u) end();
+    }
+    __syncwarp();
+}
+
+// Two fp32 operations an instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return d;
+}
+// d = a * b + c and d = a * b over N columns (N even: by pairs)
+template <int N>
+__device__ __forceinline__ void fma_n(const float (&a)[N], const float (&b)[N], const float (&c)[N], float (&d)[N]) {
+    if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float2 r = fma2(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]), make_float2(c[i], c[i + 1]));
+            d[i] = r.x;
+            d[i + 1] = r.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) d[i] = fmaf(a[i], b[i], c[i]);
+    }
+}
+template <int N>
+__device__ __forceinline__ void mul_n(const float (&a)[N], const float (&b)[N], float (&d)[N]) {
+    if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float2 r = mul2(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]));
+            d[i] = r.x;
+            d[i + 1] = r.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) d[i] = a[i] * b[i];
+    }
+}
+template <int N>
+__device__ __forceinline__ void scale_n(const float (&a)[N], float by, float (&d)[N]) {
+    float b[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) b[i] = by;
+    mul_n<N>(a, b, d);
+}
+// sum of a * b
+template <int N>
+__device__ __forceinline__ float dot_n(const float (&a)[N], const float (&b)[N]) {
+    if constexpr (N % 2 == 0) {
+        float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int i = 0; i < N; i += 2) s = fma2(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]), s);
+        return s.x + s.y;
+    } else {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) s = fmaf(a[i], b[i], s);
+        return s;
+    }
+}
+template <int N>
+__device__ __forceinline__ void load_n(const float* p, float (&f)[N]) {
+    Packed<float, N> v;
+    v.load(p);
+    v.unpack(f);
+}
+// N gates into the row of gates per column, each for the components of its channel
+template <int COMPS, int N>
+__device__ __forceinline__ void spread_gates(float* to, const float (&g)[N], int comps) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (COMPS > 0) {
+#pragma unroll
+            for (int m = 0; m < COMPS; ++m) to[i * COMPS + m] = g[i];
+        } else {
+            for (int m = 0; m < comps; ++m) to[i * comps + m] = g[i];
+        }
+    }
+}
+template <int N>
+__device__ __forceinline__ void spread_gates(float* row, int lane, const float (&g)[N], int comps) {
+    float* to = row + lane * N * comps;
+    switch (comps) {
+        case 3: spread_gates<3, N>(to, g, comps); break;
+        case 5: spread_gates<5, N>(to, g, comps); break;
+        case 7: spread_gates<7, N>(to, g, comps); break;
+        default: spread_gates<0, N>(to, g, comps); break;
+    }
+}
 
 // ----------------------------------------------------------------------------------------------------------- host side
 struct RowShape {
@@ -162,7 +406,7 @@ inline int gate_row(const char* what, int type, const int32_t* sizes, const int3
     if (n > 2 * kMaxThreads || m > 4 * kMaxThreads) s->k = s->m = 8;
     if (std::max(n, m) > 8 * kMaxThreads) return fail(E3B_ERR_UNSUPPORTED, "%s: %d items, at most %d", what, std::max(n, m), 8 * kMaxThreads);
     s->threads = static_cast<int>(std::max<int64_t>(1, ceil_div(std::max(ceil_div(n, s->k), ceil_div(m, s->m)), 32)) * 32);
-    t->nw = s->threads / 32;
+    t->nw = warps_pow2(s->threads);
     return E3B_OK;
 }
 

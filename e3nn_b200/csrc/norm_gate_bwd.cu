@@ -23,8 +23,9 @@ __global__ void __launch_bounds__(MAXT, BLOCKS) norm_gate_bwd_kernel(const T* __
     const BlockSums outs = block_sums_at(at, t.nblk_out, t.nw), ghs = block_sums_at(at, t.nblk_out, t.nw);
     float* gates = at;                                        // [num_gates + 1] activated gates
     float* prod = gates + (t.num_gates + 4) / 4 * 4;          // [dout] cotangent of the gated row times the normalised row
-    const RowAhead<T, VEC, K, 4> wide(prod + (t.dout + 3) / 4 * 4);
-    const RowAhead<T, NW, M, 4> narrow(wide.mine - threadIdx.x * wide.kBytes + static_cast<int>(blockDim.x) * wide.kThread);
+    RowAhead<T, VEC, K, 4> wide(prod + (t.dout + 3) / 4 * 4);
+    constexpr int AHEAD = rows_ahead(NW * sizeof(T));
+    RowAhead<T, NW, M, 4> narrow(wide.mine - threadIdx.x * wide.kBytes + static_cast<int>(blockDim.x) * wide.kThread);
     Items<VEC, NW, K, M> it;
     it.init(t);
     auto fetch = [&](int64_t z, int stage) {
@@ -51,17 +52,13 @@ __global__ void __launch_bounds__(MAXT, BLOCKS) norm_gate_bwd_kernel(const T* __
     };
     int64_t z = blockIdx.x;
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) fetch(z + static_cast<int64_t>(i) * gridDim.x, i);
+    for (int i = 0; i < AHEAD; ++i) fetch(z + static_cast<int64_t>(i) * gridDim.x, i);
     in.clear();
     dots.clear();
     outs.clear();
     ghs.clear();
     if (threadIdx.x == 0) gates[t.num_gates] = 1.0f;
     __syncthreads();
-    in.touch(it.in_blocks);
-    dots.touch(it.in_blocks);
-    outs.touch(it.out_blocks);
-    ghs.touch(it.out_blocks);
     float wp[K][VEC], sc[K][VEC], wn[K][VEC], w_inv_i[K], w_inv_o[K];
     float n_wp[M][NW], n_sc[M][NW], n_wn[M][NW], n_inv_i[M], n_inv_o[M];
     float a_post[K][VEC], a_scale[K][VEC], a_pre[K][VEC], n_post[M][NW], n_scale[M][NW], n_pre[M][NW];
@@ -94,7 +91,7 @@ __global__ void __launch_bounds__(MAXT, BLOCKS) norm_gate_bwd_kernel(const T* __
         }
     }
     __syncthreads();
-    for (int stage = 0; z < rows; z += gridDim.x, stage = stage + 1 == kAhead ? 0 : stage + 1) {
+    for (int stage = 0; z < rows; z += gridDim.x, stage = stage + 1 == AHEAD ? 0 : stage + 1) {
         const int64_t zi = z * t.din, zo = z * t.dout;
         // v: y, then normalised; x: residual, then z; g0: cotangent of z; g1: of h, then of the normalised row
         float v[K][VEC], x[K][VEC], g0[K][VEC], g1[K][VEC], sq[K], dot[K];
@@ -106,10 +103,10 @@ __global__ void __launch_bounds__(MAXT, BLOCKS) norm_gate_bwd_kernel(const T* __
             if (it.win[k] < 0) continue;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) g0[k][i] = g1[k][i] = 0.0f;
-            wide.read(stage, 0, k, y + zi + it.win[k], v[k]);
-            wide.read(stage, 1, k, residual + zo + it.wout[k], x[k]);
-            if (gz) wide.read(stage, 2, k, gz + zo + it.wout[k], g0[k]);
-            if (gh) wide.read(stage, 3, k, gh + zo + it.wout[k], g1[k]);
+            wide.read(stage, 0, k, v[k]);
+            wide.read(stage, 1, k, x[k]);
+            if (gz) wide.read(stage, 2, k, g0[k]);
+            if (gh) wide.read(stage, 3, k, g1[k]);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) sq[k] = fmaf(v[k][i], v[k][i], sq[k]);
         }
@@ -119,29 +116,31 @@ __global__ void __launch_bounds__(MAXT, BLOCKS) norm_gate_bwd_kernel(const T* __
             if (it.nin[j] < 0) continue;
 #pragma unroll
             for (int i = 0; i < NW; ++i) n0[j][i] = n1[j][i] = nx[j][i] = 0.0f;
-            narrow.read(stage, 0, j, y + zi + it.nin[j], nv[j]);
+            narrow.read(stage, 0, j, nv[j]);
             if (it.nout[j] >= 0) {
-                narrow.read(stage, 1, j, residual + zo + it.nout[j], nx[j]);
-                if (gz) narrow.read(stage, 2, j, gz + zo + it.nout[j], n0[j]);
-                if (gh) narrow.read(stage, 3, j, gh + zo + it.nout[j], n1[j]);
+                narrow.read(stage, 1, j, nx[j]);
+                if (gz) narrow.read(stage, 2, j, n0[j]);
+                if (gh) narrow.read(stage, 3, j, n1[j]);
             }
 #pragma unroll
             for (int i = 0; i < NW; ++i) nsq[j] = fmaf(nv[j][i], nv[j][i], nsq[j]);
         }
-        fetch(z + static_cast<int64_t>(kAhead) * gridDim.x, stage);
+        fetch(z + static_cast<int64_t>(AHEAD) * gridDim.x, stage);
         in.add(it.in_blocks, sq, it.wbi, nsq, it.nbi);
         __syncthreads();
-        float s_in[K], ns_in[M], act[M][NW];       // act: activated columns of the narrow items
+        float s_in[K], ns_in[M], act[M][NW], slope[M][NW];       // activated columns of the narrow items and their derivatives
+        in.get(it.wbi, s_in, it.nbi, ns_in);
 #pragma unroll
         for (int j = 0; j < M; ++j) {
             nsq[j] = ndot[j] = 0.0f;
             if (it.nin[j] < 0) continue;
-            ns_in[j] = rsqrtf(fmaf(in.get(it.nbi[j]), n_inv_i[j], eps));
+            ns_in[j] = rsqrtf(fmaf(ns_in[j], n_inv_i[j], eps));
 #pragma unroll
             for (int i = 0; i < NW; ++i) {
                 nv[j][i] *= ns_in[j];
-                act[j][i] = it.cst[j] * gate_act(it.act[j], nv[j][i] * n_wp[j][i]);
+                act[j][i] = nv[j][i] * n_wp[j][i];
             }
+            activate_and_derive<NW>(it.act[j], it.cst[j], act[j], act[j], slope[j]);
             if (it.kind[j] == kGates) Packed<float, NW>::store(gates + it.slot[j], act[j]);
             if (it.nout[j] < 0) continue;
 #pragma unroll
@@ -154,7 +153,7 @@ __global__ void __launch_bounds__(MAXT, BLOCKS) norm_gate_bwd_kernel(const T* __
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             if (it.win[k] < 0) continue;
-            s_in[k] = rsqrtf(fmaf(in.get(it.wbi[k]), w_inv_i[k], eps));
+            s_in[k] = rsqrtf(fmaf(s_in[k], w_inv_i[k], eps));
 #pragma unroll
             for (int i = 0; i < VEC; ++i) v[k][i] *= s_in[k];
         }
@@ -176,12 +175,14 @@ __global__ void __launch_bounds__(MAXT, BLOCKS) norm_gate_bwd_kernel(const T* __
             outs.add(it.out_blocks, sq, it.wbo, nsq, it.nbo);
             ghs.add(it.out_blocks, dot, it.wbo, ndot, it.nbo);
             __syncthreads();
+            outs.get(it.wbo, sq, it.nbo, nsq);
+            ghs.get(it.wbo, dot, it.nbo, ndot);
         }
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             if (it.win[k] < 0) continue;
             if (gh) {
-                const float s = rsqrtf(fmaf(outs.get(it.wbo[k]), w_inv_o[k], eps)), mean = ghs.get(it.wbo[k]) * w_inv_o[k] * s * s;
+                const float s = rsqrtf(fmaf(sq[k], w_inv_o[k], eps)), mean = dot[k] * w_inv_o[k] * s * s;
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
                     a_pre[k][i] = fmaf(g1[k][i], x[k][i] * s, a_pre[k][i]);
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(MAXT, BLOCKS) norm_gate_bwd_kernel(const T* __
         for (int j = 0; j < M; ++j) {
             if (it.nout[j] < 0) continue;
             if (gh) {
-                const float s = rsqrtf(fmaf(outs.get(it.nbo[j]), n_inv_o[j], eps)), mean = ghs.get(it.nbo[j]) * n_inv_o[j] * s * s;
+                const float s = rsqrtf(fmaf(nsq[j], n_inv_o[j], eps)), mean = ndot[j] * n_inv_o[j] * s * s;
 #pragma unroll
                 for (int i = 0; i < NW; ++i) {
                     n_pre[j][i] = fmaf(n1[j][i], nx[j][i] * s, n_pre[j][i]);
@@ -229,7 +230,7 @@ __global__ void __launch_bounds__(MAXT, BLOCKS) norm_gate_bwd_kernel(const T* __
                     n1[j][i] = 0.0f;
                     for (int m = 0; m < e[3]; ++m) n1[j][i] += prod[e[2] + m];
                 }
-                n1[j][i] = it.kind[j] == kUnused ? 0.0f : n1[j][i] * it.cst[j] * gate_act_grad(it.act[j], nv[j][i] * n_wp[j][i]);
+                n1[j][i] = it.kind[j] == kUnused ? 0.0f : n1[j][i] * slope[j][i];
                 n_post[j][i] = fmaf(n1[j][i], nv[j][i], n_post[j][i]);
                 n1[j][i] *= n_wp[j][i];
                 ndot[j] = fmaf(n1[j][i], nv[j][i], ndot[j]);
@@ -249,10 +250,11 @@ __global__ void __launch_bounds__(MAXT, BLOCKS) norm_gate_bwd_kernel(const T* __
         if (gy) {
             dots.add(it.in_blocks, dot, it.wbi, ndot, it.nbi);
             __syncthreads();
+            dots.get(it.wbi, dot, it.nbi, ndot);
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 if (it.win[k] < 0) continue;
-                const float mean = dots.get(it.wbi[k]) * w_inv_i[k];
+                const float mean = dot[k] * w_inv_i[k];
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) g1[k][i] = s_in[k] * (g1[k][i] - v[k][i] * mean);
                 Packed<T, VEC>::store(gy + zi + it.win[k], g1[k]);
@@ -260,7 +262,7 @@ __global__ void __launch_bounds__(MAXT, BLOCKS) norm_gate_bwd_kernel(const T* __
 #pragma unroll
             for (int j = 0; j < M; ++j) {
                 if (it.nin[j] < 0) continue;
-                const float mean = dots.get(it.nbi[j]) * n_inv_i[j];
+                const float mean = ndot[j] * n_inv_i[j];
 #pragma unroll
                 for (int i = 0; i < NW; ++i) n1[j][i] = ns_in[j] * (n1[j][i] - nv[j][i] * mean);
                 Packed<T, NW>::store(gy + zi + it.nin[j], n1[j]);

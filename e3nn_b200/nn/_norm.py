@@ -87,6 +87,44 @@ def _on_device_of(x: torch.Tensor, module: torch.nn.Module, table: torch.Tensor,
                            "parameters are not (move the module with .to(device))")
 
 
+def _row_plan(wides, narrows, back, ins, outs, width: int, narrow: int):
+    """The items of `_gate_items` as slots of at most 32 neighbours (see ``plan`` of ``e3b_norm_gate_residual_fwd``), a ctypes array."""
+    place, length = {}, 0                             # gate column -> place of its copies, one per component
+    for c, row in enumerate(back):
+        if row[0] == 2:
+            length += -length % 4 if c == 0 or back[c - 1][0] != 2 or back[c - 1][2] != row[2] else 0
+            place[c] = length
+            length += row[2]
+    gate_of = {row[3] + m: place[c] + m for c, row in enumerate(back) if row[0] == 2 for m in range(row[2])}
+    slots = []
+    for c, j, bi, bo, *_ in wides:
+        g, last = gate_of.get(c, -1), slots[-1] if slots else None
+        n = last[2] if last else 0
+        if last and n < 32 and last[:2] == [c - n * width, j - n * width] and last[3:5] == [bi, bo] and last[5] == (g - n * width if g >= 0 else -1):
+            last[2] += 1
+        else:
+            slots.append([c, j, 1, bi, bo, g, 0, 0, 0, 0])
+        if (g >= 0 and any(gate_of[c + i] != g + i for i in range(width))) or (g >= 0 and g % min(width, 4)):
+            return None
+    num_wide = len(slots)
+    for kind, c, j, bi, bo, act, bits, _ in narrows:
+        comps = back[c][2] if kind == 2 else 0
+        at = place[c] if kind == 2 else 0
+        if kind == 2 and any(back[c + i][2] != comps or place[c + i] != at + i * comps for i in range(narrow)):
+            return None
+        last = slots[-1] if len(slots) > num_wide else None
+        n = last[3] if last else 0
+        if (last and n < 32 and last[0] == kind and last[1] == c - n * narrow and last[2] == (j - n * narrow if j >= 0 else -1)
+                and last[4:8] == [bi, bo, act, bits] and last[9] == comps and (kind != 2 or last[8] == at - n * narrow * comps)):
+            last[3] += 1
+        else:
+            slots.append([kind, c, j, 1, bi, bo, act, bits, at, comps])
+    din, dout = (sum(mul * d for mul, d in b) for b in (ins, outs))
+    flat = [width, narrow, num_wide, len(slots) - num_wide, din, dout, len(ins), len(outs), length]
+    flat += [x for slot in slots for x in slot] + [mul * d for mul, d in ins] + [mul * d for mul, d in outs]
+    return (ctypes.c_int32 * len(flat))(*flat)
+
+
 def _rms_norm(x, weight, tables, fours: int, eps: float) -> torch.Tensor:
     tbl, inv, _ = tables
     h = torch.empty_like(x)
@@ -209,14 +247,15 @@ def _gate_items(back, const, forth, ins, outs, width: int, narrow: int):
     return (torch.tensor(wides, dtype=torch.int32).reshape(-1, 4 + width), torch.tensor(narrows, dtype=torch.int32).reshape(-1, 8), len(slot_of))
 
 
-def _norm_gate(residual, y, w_post, scale, w_pre, tables, sizes, eps: float):
+def _norm_gate(residual, y, w_post, scale, w_pre, tables, shape, eps: float):
+    sizes, plan = shape
     wide, narrow, in_tbl, out_tbl, _, _, in_inv, out_inv = tables
     z = torch.empty_like(residual)
     h = torch.empty_like(residual) if w_pre is not None else None
     with _lib.device_of(y):
         rc = _lib.core().e3b_norm_gate_residual_fwd(
             residual.data_ptr(), y.data_ptr(), w_post.data_ptr(), scale.data_ptr(), _lib.address(w_pre), wide.data_ptr(), narrow.data_ptr(),
-            in_tbl.data_ptr(), out_tbl.data_ptr(), in_inv.data_ptr(), out_inv.data_ptr(), sizes, eps, z.data_ptr(), _lib.address(h), y.shape[0],
+            in_tbl.data_ptr(), out_tbl.data_ptr(), in_inv.data_ptr(), out_inv.data_ptr(), sizes, plan, eps, z.data_ptr(), _lib.address(h), y.shape[0],
             _lib.element_type(y), _lib.raw_stream(y))
     if rc:
         _lib.check(rc, "e3b_norm_gate_residual_fwd")
@@ -225,17 +264,17 @@ def _norm_gate(residual, y, w_post, scale, w_pre, tables, sizes, eps: float):
 
 class _NormGateFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, residual, y, w_post, scale, w_pre, tables, sizes, eps):
+    def forward(ctx, residual, y, w_post, scale, w_pre, tables, shape, eps):
         ctx.save_for_backward(residual, y, w_post, scale, w_pre)
-        ctx.meta = (tables, sizes, eps)
+        ctx.meta = (tables, shape, eps)
         ctx.set_materialize_grads(False)
-        return _norm_gate(residual, y, w_post, scale, w_pre, tables, sizes, eps)
+        return _norm_gate(residual, y, w_post, scale, w_pre, tables, shape, eps)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_z, grad_h):
         residual, y, w_post, scale, w_pre = ctx.saved_tensors
-        tables, sizes, eps = ctx.meta
+        tables, (sizes, plan), eps = ctx.meta
         if grad_z is None and grad_h is None:
             return (None,) * 8
         core, rows, address = _lib.core(), y.shape[0], _lib.address
@@ -306,8 +345,11 @@ class NormGateResidual(torch.nn.Module):
                 self.register_buffer(f"_narrow{width}{narrow}", items[1], persistent=False)
                 self._table_names[width, narrow] = (f"_wide{width}{narrow}", f"_narrow{width}{narrow}", "_in", "_out", "_in_channels", "_out_channels",
                                                     "_in_inv_bits", "_out_inv_bits")
-                self._sizes[width, narrow] = (ctypes.c_int32 * 11)(width, narrow, len(items[0]), len(items[1]), items[2], din, dout, len(ins),
-                                                                   len(outs), n_in, n_out)
+                sizes = (ctypes.c_int32 * 11)(width, narrow, len(items[0]), len(items[1]), items[2], din, dout, len(ins), len(outs), n_in, n_out)
+                pair = 2 if width == 4 else narrow        # by warps, two columns an item where rows are wide enough for it
+                rows = items if pair == narrow else _gate_items(back, const, forth, ins, outs, width, pair)
+                plan = None if rows is None else _row_plan(rows[0].tolist(), rows[1].tolist(), back, ins, outs, width, pair)
+                self._sizes[width, narrow] = (sizes, plan)
         self.weight_post = torch.nn.Parameter(torch.ones(n_in))
         self.scale = torch.nn.Parameter(torch.full((n_out,), float(scale_init)))
         if pre_norm:

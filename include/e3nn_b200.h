@@ -297,6 +297,12 @@ int e3b_fill_columns(float* out, int64_t num_rows, int row_stride, int col0, int
  * in_table [din,4] = {block, channel, first output column, count} (the last two: of the components a gate column multiplies),
  * out_table [dout,4] = {block, channel, -, -}; sizes: HOST array {w, n, num_wide, num_narrow, num_gates, din, dout, blocks in,
  * blocks out, channels in, channels out}.  Row pointers are aligned to w elements.  At most 4,096 items of each sort and 32 blocks.
+ * plan: HOST array or NULL.  The same row as slots of at most 32 items that are consecutive on both sides, in one block, and (gates) of
+ * channels with the same number of components: {w, n, wide slots, narrow slots, din, dout, blocks in, blocks out, length of the row of gates per
+ * column}, per wide slot ten integers {first input column, first output column, items, blocks of both, place of the first column's gate
+ * or -1}, per narrow slot {kind, first input column, first output column or -1, items, blocks of both, activation, constant, place of the
+ * first gate, components}, the columns of the blocks in, of the blocks out.  Rows of at most 9 wide and 8 narrow slots and 8 blocks are
+ * taken by one warp each.
  * e3b_norm_gate_residual_bwd: grad_z or grad_h may be NULL, each of the gradients too; grad_params [channels in + 2 channels out] =
  * gradients of weight_post, scale, weight_pre, with e3b_norm_scratch_bytes(rows, its length) bytes of scratch.
  * e3b_rms_norm: rows of at most e3b_norm_max_columns(1) columns with vec4 and pointers aligned to four elements, else
@@ -311,8 +317,8 @@ int e3b_rms_norm_bwd(const void* x, const void* grad_h, const float* weight, con
                      float* grad_weight, void* scratch, int64_t scratch_bytes, int64_t rows, int dim, int type, void* stream);
 int e3b_norm_gate_residual_fwd(const void* residual, const void* y, const float* weight_post, const float* scale,
                                const float* weight_pre, const int32_t* wide, const int32_t* narrow, const int32_t* in_table,
-                               const int32_t* out_table, const float* in_inv, const float* out_inv, const int32_t* sizes, float eps,
-                               void* z, void* h, int64_t rows, int type, void* stream);
+                               const int32_t* out_table, const float* in_inv, const float* out_inv, const int32_t* sizes,
+                               const int32_t* plan, float eps, void* z, void* h, int64_t rows, int type, void* stream);
 int e3b_norm_gate_residual_bwd(const void* residual, const void* y, const void* grad_z, const void* grad_h,
                                const float* weight_post, const float* scale, const float* weight_pre, const int32_t* wide,
                                const int32_t* narrow, const int32_t* in_table, const int32_t* out_table, const int32_t* in_channels,
