@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(256) attn_fwd_kernel(const FwdArgs a) {
 // The same with k and v through the ring: the registers hold q, the sums and the row in hand, so more warps fit and all copies that
 // fit in shared memory are under way (about 200 KB an SM).
 template <typename T, int VEC, int V>
-__global__ void __launch_bounds__(128, 3) attn_fwd_ring_kernel(const FwdArgs a) {
+__global__ void __launch_bounds__(384, 1) attn_fwd_ring_kernel(const FwdArgs a) {
     extern __shared__ __align__(128) uint8_t memory[];
     constexpr int U = V * VEC <= 12 ? 4 : 2;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = blockIdx.x * (blockDim.x >> 5) + warp;
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(128, 3) attn_fwd_ring_kernel(const FwdArgs a) 
 }
 
 template <typename T, int VEC, int V>
-__global__ void __launch_bounds__(256) attn_fwd_join_kernel(const FwdArgs a) {
+__global__ void __launch_bounds__(512) attn_fwd_join_kernel(const FwdArgs a) {
     extern __shared__ float smem[];
     const int lane = threadIdx.x & 31;
     const int head = blockIdx.y * (32 / a.h.lanes) + lane / a.h.lanes;

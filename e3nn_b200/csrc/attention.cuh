@@ -500,11 +500,12 @@ __device__ __forceinline__ void walk_ring(const Rows& r, const Part& p, Ring<U, 
     if (failed) ring.abandon(status);
 }
 
-// Dots of the lane's columns of a row in shared memory, and products added to a lane's sums.  Columns a lane does not have are left
-// out by a test, not by a zero: what lies there belongs to another head and may be anything.
+// Dots of the lane's columns of a row in shared memory, and products added to a lane's sums, two columns an instruction.  Columns a
+// lane does not have are left out by a test, not by a zero: what lies there belongs to another head and may be anything.
 template <typename T, int VEC, int V>
 __device__ __forceinline__ float dot_row(const uint8_t* row, const float (&f)[V][VEC], const int (&col)[V]) {
-    float d = 0.0f;
+    static_assert(VEC % 2 == 0, "rows in shared memory are read in vectors of 16 bytes");
+    float2 d = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         if (col[j] < 0) continue;
@@ -513,9 +514,9 @@ __device__ __forceinline__ float dot_row(const uint8_t* row, const float (&f)[V]
         p.load(reinterpret_cast<const T*>(row) + col[j]);
         p.unpack(x);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) d = fmaf(f[j][i], x[i], d);
+        for (int i = 0; i < VEC; i += 2) d = fma2(make_float2(f[j][i], f[j][i + 1]), make_float2(x[i], x[i + 1]), d);
     }
-    return d;
+    return d.x + d.y;
 }
 template <typename T, int VEC, int V>
 __device__ __forceinline__ void add_row(const uint8_t* row, float by, float (&sum)[V][VEC], const int (&col)[V]) {
@@ -527,7 +528,11 @@ __device__ __forceinline__ void add_row(const uint8_t* row, float by, float (&su
         p.load(reinterpret_cast<const T*>(row) + col[j]);
         p.unpack(x);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sum[j][i] = fmaf(by, x[i], sum[j][i]);
+        for (int i = 0; i < VEC; i += 2) {
+            const float2 s = fma2(make_float2(by, by), make_float2(x[i], x[i + 1]), make_float2(sum[j][i], sum[j][i + 1]));
+            sum[j][i] = s.x;
+            sum[j][i + 1] = s.y;
+        }
     }
 }
 // Sums over the lanes of a head of U numbers side by side.
@@ -559,8 +564,10 @@ inline Split split_rows(int64_t num, int64_t edges, int per_sm) {
     s.parts = static_cast<int>(ceil_div(items, s.per_part));
     s.warps = s.parts >= kNumSMs * 4 ? 4 : 1;
     const int64_t longest = num > 0 ? edges / num : 0;
-    s.merge = longest > s.per_part * s.warps;
-    s.join_warps = longest > 4 * s.per_part ? 8 : 1;
+    // rows longer than the parts of an SM: all its warps are one block, which leaves one sum
+    s.merge = s.warps > 1 && longest > s.per_part * per_sm;
+    if (s.merge) s.warps = per_sm;
+    s.join_warps = longest > 4 * s.per_part ? 16 : 1;
     return s;
 }
 
@@ -577,7 +584,7 @@ inline int compiled_vectors(int vec, int v) {
     return v <= 4 ? 4 : v <= 8 ? 8 : v <= 16 ? 16 : 32;
 }
 
-constexpr int kWarpsPerSm[] = {16, 12, 8, 4};    // that the kernels may be launched with
+constexpr int kWarpsPerSm[] = {12, 8, 4};    // that the kernels may be launched with
 inline int most_parts(int64_t num, int64_t edges) {
     int parts = 1;
     for (int w : kWarpsPerSm) parts = std::max(parts, split_rows(num, edges, w).parts);
@@ -618,6 +625,7 @@ inline int plan(Plan* p, const char* what, int type, int vec, int heads, int vec
               ring_fits(rows.slot(), most_blocks, least, &blocks, &p->depth);
     p->s = split_rows(num, edges, p->ring ? 4 * blocks : 8);
     if (p->ring) {
+        if (p->s.warps > 4) p->depth = std::min(p->depth, (226 * 1024 / p->s.warps - 128) / static_cast<int>(rows.slot() + 8));
         if (p->s.warps == 1) p->depth = std::min<int>(16, (200 * 1024) / static_cast<int>(rows.slot() + 8));
         p->warp_smem = ceil_div(static_cast<int64_t>(p->depth) * (rows.slot() + 8), 128) * 128;
     }

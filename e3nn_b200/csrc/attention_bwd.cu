@@ -32,19 +32,28 @@ struct BwdArgs {
     __device__ __forceinline__ float2* share_of(int64_t edge) const { return share + edge * ((h.heads + 1) & ~1); }
 };
 
-// q, cotangent and statistics of a row; returns delta.  (The output enters unrounded, in the order of the dots g v: an edge alone in
-// its row gives the same number.)
-template <typename T, int VEC, int V>
+// q, cotangent and statistics of a row; returns delta.  The output enters unrounded, in the order of the dots g v of the kernel (PAIRS: of
+// dot_row): an edge alone in its row gives the same number.
+template <bool PAIRS, typename T, int VEC, int V>
 __device__ __forceinline__ float open_row(const BwdArgs& a, int64_t n, const int (&cq)[V], const int (&cv)[V], int head, bool live, float (&qf)[V][VEC],
                                           float (&gf)[V][VEC], float* top, float* inv) {
     load_row_f<T, VEC, V>(qf, static_cast<const T*>(a.q), n, a.q_stride, cq);
     load_row_f<T, VEC, V>(gf, static_cast<const T*>(a.grad_out), n, a.h.dv, cv);
     float d = 0.0f, o[V][VEC];
     load_row_f<float, VEC, V>(o, a.out32, n, a.h.dv, cv);
+    if constexpr (PAIRS) {
+        float2 pair = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int j = 0; j < V; ++j)
+        for (int j = 0; j < V; ++j)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) d = fmaf(gf[j][i], o[j][i], d);
+            for (int i = 0; i < VEC; i += 2) pair = fma2(make_float2(gf[j][i], gf[j][i + 1]), make_float2(o[j][i], o[j][i + 1]), pair);
+        d = pair.x + pair.y;
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) d = fmaf(gf[j][i], o[j][i], d);
+    }
     if (live) {
         *top = a.stats[(n * a.h.heads + head) * 2];
         *inv = a.stats[(n * a.h.heads + head) * 2 + 1];
@@ -98,7 +107,7 @@ __global__ void __launch_bounds__(256) attn_bwd_dst_kernel(const BwdArgs a) {
             a.r, range,
             [&](int64_t n) {
                 row_now = static_cast<int>(n);
-                delta = open_row<T, VEC, V>(a, n, cq, cv, head, live, qf, gf, &top, &inv);
+                delta = open_row<false, T, VEC, V>(a, n, cq, cv, head, live, qf, gf, &top, &inv);
                 s.clear();
             },
             [&](int64_t first, int64_t last) {
@@ -182,7 +191,7 @@ __global__ void __launch_bounds__(256) attn_bwd_dst_kernel(const BwdArgs a) {
 
 // The same with k and v through the ring.
 template <typename T, int VEC, int V>
-__global__ void __launch_bounds__(128, 3) attn_bwd_dst_ring_kernel(const BwdArgs a) {
+__global__ void __launch_bounds__(384, 1) attn_bwd_dst_ring_kernel(const BwdArgs a) {
     extern __shared__ __align__(128) uint8_t memory[];
     constexpr int U = V * VEC <= 12 ? 4 : 2;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = blockIdx.x * (blockDim.x >> 5) + warp;
@@ -205,7 +214,7 @@ __global__ void __launch_bounds__(128, 3) attn_bwd_dst_ring_kernel(const BwdArgs
             a.r, range, ring, a.e.status, [&](EdgeMeta& m, int i) { m.load(a.e, range.e0 + i, range.behind); },
             [&](int64_t n) {
                 row_now = static_cast<int>(n);
-                delta = open_row<T, VEC, V>(a, n, cq, cv, head, live, qf, gf, &top, &inv);
+                delta = open_row<true, T, VEC, V>(a, n, cq, cv, head, live, qf, gf, &top, &inv);
                 s.clear();
             },
             [&](const EdgeMeta& meta, int at, int m) {
@@ -269,7 +278,7 @@ __global__ void __launch_bounds__(128, 3) attn_bwd_dst_ring_kernel(const BwdArgs
 }
 
 template <typename T, int VEC, int V>
-__global__ void __launch_bounds__(256) attn_bwd_dst_join_kernel(const BwdArgs a) {
+__global__ void __launch_bounds__(512) attn_bwd_dst_join_kernel(const BwdArgs a) {
     extern __shared__ float smem[];
     const int lane = threadIdx.x & 31;
     const int head = blockIdx.y * (32 / a.h.lanes) + lane / a.h.lanes;

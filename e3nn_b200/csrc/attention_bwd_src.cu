@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(256) attn_bwd_src_kernel(const SrcArgs a) {
 
 // The same with the rows of q and g, and the shares of the edge, through the ring.
 template <typename T, int VEC, int V>
-__global__ void __launch_bounds__(128, 3) attn_bwd_src_ring_kernel(const SrcArgs a) {
+__global__ void __launch_bounds__(384, 1) attn_bwd_src_ring_kernel(const SrcArgs a) {
     extern __shared__ __align__(128) uint8_t memory[];
     constexpr int U = V * VEC <= 12 ? 4 : 2;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = blockIdx.x * (blockDim.x >> 5) + warp;
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(128, 3) attn_bwd_src_ring_kernel(const SrcArgs
 }
 
 template <typename T, int VEC, int V>
-__global__ void __launch_bounds__(256) attn_bwd_src_join_kernel(const SrcArgs a) {
+__global__ void __launch_bounds__(512) attn_bwd_src_join_kernel(const SrcArgs a) {
     extern __shared__ float smem[];
     const int lane = threadIdx.x & 31;
     const int head = blockIdx.y * (32 / a.h.lanes) + lane / a.h.lanes;

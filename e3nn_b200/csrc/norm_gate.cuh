@@ -262,76 +262,6 @@ __device__ __forceinline__ void row_sums(const float (&wv)[K], const float (&nv)
     __syncwarp();
 }
 
-// Two fp32 operations an instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;"
-        : "=l"(reinterpret_cast<uint64_t&>(d))
-        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
-    return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-    return d;
-}
-// d = a * b + c and d = a * b over N columns (N even: by pairs)
-template <int N>
-__device__ __forceinline__ void fma_n(const float (&a)[N], const float (&b)[N], const float (&c)[N], float (&d)[N]) {
-    if constexpr (N % 2 == 0) {
-#pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            const float2 r = fma2(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]), make_float2(c[i], c[i + 1]));
-            d[i] = r.x;
-            d[i + 1] = r.y;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) d[i] = fmaf(a[i], b[i], c[i]);
-    }
-}
-template <int N>
-__device__ __forceinline__ void mul_n(const float (&a)[N], const float (&b)[N], float (&d)[N]) {
-    if constexpr (N % 2 == 0) {
-#pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            const float2 r = mul2(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]));
-            d[i] = r.x;
-            d[i + 1] = r.y;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) d[i] = a[i] * b[i];
-    }
-}
-template <int N>
-__device__ __forceinline__ void scale_n(const float (&a)[N], float by, float (&d)[N]) {
-    float b[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) b[i] = by;
-    mul_n<N>(a, b, d);
-}
-// sum of a * b
-template <int N>
-__device__ __forceinline__ float dot_n(const float (&a)[N], const float (&b)[N]) {
-    if constexpr (N % 2 == 0) {
-        float2 s = make_float2(0.0f, 0.0f);
-#pragma unroll
-        for (int i = 0; i < N; i += 2) s = fma2(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]), s);
-        return s.x + s.y;
-    } else {
-        float s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) s = fmaf(a[i], b[i], s);
-        return s;
-    }
-}
-template <int N>
-__device__ __forceinline__ void load_n(const float* p, float (&f)[N]) {
-    Packed<float, N> v;
-    v.load(p);
-    v.unpack(f);
-}
 // N gates into the row of gates per column, each for the components of its channel
 template <int COMPS, int N>
 __device__ __forceinline__ void spread_gates(float* to, const float (&g)[N], int comps) {

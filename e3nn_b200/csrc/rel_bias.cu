@@ -7,9 +7,9 @@
 // exact to 2^-53, so that a distance next to a border falls on the side that it is on.  Bound by HBM (28 bytes of edge data in,
 // 4 out; the positions come from L2).
 // Bias: bound by the write of 4 H bytes an edge (2 H in 16 bits).
-// Gradient: every thread keeps one head and walks edges of its own; it adds into a table that it shares with no other
-// thread's (head, slice), so the order of the additions is fixed by the grid; slices, then thread blocks, are added in
-// order.  No atomics.
+// Gradient: every thread keeps its heads and walks edges of its own; it adds into cells of a table in shared memory that no other
+// thread touches, so the order of the additions is fixed by the grid; slices, then thread blocks, are added in order.  No atomics.
+// Bound by the loads in flight: a table per slice limits the threads, sixteen 16-byte loads each make up for it.
 #include <algorithm>
 
 #include "common.cuh"
@@ -20,6 +20,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxBuckets = 1024;
+constexpr int kSumThreads = 512;       // of a block of the table gradient, at most
 
 __global__ void __launch_bounds__(kThreads) distance_buckets_kernel(const float* __restrict__ pos, const int64_t* __restrict__ src,
                                                                     const int64_t* __restrict__ dst, const float* __restrict__ shift,
@@ -28,37 +29,54 @@ __global__ void __launch_bounds__(kThreads) distance_buckets_kernel(const float*
     __shared__ double t2[kMaxBuckets];
     for (int i = threadIdx.x; i < num; i += kThreads) t2[i] = thresholds2[i];
     __syncthreads();
-    for (int64_t e = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; e < edges; e += static_cast<int64_t>(gridDim.x) * kThreads) {
-        const int64_t a = src[e], b = dst[e];
-        if (a < 0 || a >= nodes || b < 0 || b >= nodes) {
-            *status = 2;
-            buckets[e] = 0;
-            continue;
-        }
-        double r2 = 0.0;
+    constexpr int U = 2;       // edges a thread looks at side by side
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * kThreads;
+    for (int64_t e0 = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; e0 < edges; e0 += U * stride) {
+        double r2[U];
+        bool bad[U];
 #pragma unroll
-        for (int i = 0; i < 3; ++i) {
-            double d = static_cast<double>(pos[3 * a + i]) - static_cast<double>(pos[3 * b + i]);
-            if (shift) d += static_cast<double>(shift[3 * e + i]);
-            r2 = __dadd_rn(r2, __dmul_rn(d, d));
+        for (int u = 0; u < U; ++u) {
+            const int64_t e = min(e0 + u * stride, edges - 1);
+            int64_t a = src[e], b = dst[e];
+            bad[u] = a < 0 || a >= nodes || b < 0 || b >= nodes;
+            if (bad[u]) a = b = -1;
+            r2[u] = 0.0;
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                double d = bad[u] ? 0.0 : static_cast<double>(pos[3 * a + i]) - static_cast<double>(pos[3 * b + i]);
+                if (shift) d += static_cast<double>(shift[3 * e + i]);
+                r2[u] = __dadd_rn(r2[u], __dmul_rn(d, d));
+            }
         }
-        int lo = 0, hi = num;                       // thresholds below lo are <= r, from hi on they are > r
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (t2[mid] <= r2) lo = mid + 1; else hi = mid;
+        int lo[U], hi[U];                           // thresholds below lo are <= r, from hi on they are > r
+#pragma unroll
+        for (int u = 0; u < U; ++u) { lo[u] = 0; hi[u] = num; }
+        for (int left = num; left > 0; left >>= 1) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (lo[u] >= hi[u]) continue;
+                const int mid = (lo[u] + hi[u]) >> 1;
+                if (t2[mid] <= r2[u]) lo[u] = mid + 1; else hi[u] = mid;
+            }
         }
-        buckets[e] = lo;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t e = e0 + u * stride;
+            if (e >= edges) continue;
+            buckets[e] = bad[u] ? 0 : lo[u];
+            if (bad[u]) *status = 2;
+        }
     }
 }
 
-// Four outputs of the flat [edges * heads] array a thread.  RAW: the elements are copied as they are.
-template <typename T, int VEC>
+// VEC outputs of the flat [edges * heads] array a thread.  INDEX: 32 bits where they hold it (a division of 64-bit numbers costs more than the rest).
+template <typename T, int VEC, typename INDEX>
 __global__ void __launch_bounds__(kThreads) bias_fwd_kernel(const T* __restrict__ table, const int32_t* __restrict__ buckets, int num_buckets,
                                                             int heads, int64_t total, T* __restrict__ out, int32_t* status) {
     const int64_t stride = static_cast<int64_t>(gridDim.x) * kThreads * VEC;
     for (int64_t i0 = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * VEC; i0 < total; i0 += stride) {
         float v[VEC];
-        int64_t e = i0 / heads;
+        int64_t e = static_cast<INDEX>(i0) / static_cast<INDEX>(heads);
         int h = static_cast<int>(i0 - e * heads);
         int b = buckets[e];
 #pragma unroll
@@ -82,41 +100,57 @@ __global__ void __launch_bounds__(kThreads) bias_fwd_kernel(const T* __restrict_
     }
 }
 
-// Thread t of a block: head h0 + t % width, slice t / width; its block's edges in turns of `slices`.
+// Thread t of a block: HV heads from HV (t % lanes) on (lanes = width / HV), slice t / lanes; its block's edges in turns of `slices`.
 // Shared memory: [slices][num_buckets][width].
-template <typename T>
-__global__ void bias_bwd_kernel(const T* __restrict__ grad, const int32_t* __restrict__ buckets, int num_buckets, int heads, int width,
-                                int slices, int64_t edges, int64_t edges_per_block, float* __restrict__ partial, int32_t* status) {
-    extern __shared__ float acc[];
-    const int h = threadIdx.x % width, slice = threadIdx.x / width, head = blockIdx.y * width + h;
+template <typename T, int HV>
+__global__ void __launch_bounds__(kSumThreads, 1) bias_bwd_kernel(const T* __restrict__ grad, const int32_t* __restrict__ buckets, int num_buckets,
+                                                                  int heads, int width, int slices, int64_t edges, int64_t edges_per_block,
+                                                                  float* __restrict__ partial, int32_t* status) {
+    extern __shared__ __align__(16) float acc[];
+    const int lanes = width / HV, h = threadIdx.x % lanes * HV, slice = threadIdx.x / lanes, head = blockIdx.y * width + h;
     const int cells = num_buckets * width;
     for (int i = threadIdx.x; i < slices * cells; i += blockDim.x) acc[i] = 0.0f;
     __syncthreads();
-    const int64_t begin = static_cast<int64_t>(blockIdx.x) * edges_per_block, end = min(begin + edges_per_block, edges);
+    const int64_t begin = static_cast<int64_t>(blockIdx.x) * edges_per_block;
+    const int count = static_cast<int>(min(edges_per_block, edges - begin));
     if (head < heads && slice < slices) {
         float* mine = acc + slice * cells + h;
-        constexpr int U = 8;       // loads in flight a thread
-        for (int64_t e0 = begin + slice; e0 < end; e0 += U * slices) {
+        const T* from = grad + begin * heads + head;
+        const int32_t* which = buckets + begin;
+        constexpr int U = 16;       // edges in flight a thread
+        bool bad = false;
+        for (int e0 = slice; e0 < count; e0 += U * slices) {
             int b[U];
-            float g[U];
+            Packed<T, HV> g[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int64_t e = e0 + u * slices;
-                b[u] = -1;
-                if (e >= end) continue;
-                b[u] = buckets[e];
-                g[u] = to_float(grad[e * heads + head]);
-                if (b[u] < 0 || b[u] >= num_buckets) { *status = 2; b[u] = -1; }
+                const int e = min(e0 + u * slices, count - 1);
+                b[u] = which[e];
+                g[u].load(from + static_cast<int64_t>(e) * heads);
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (b[u] >= 0) mine[b[u] * width] += g[u];
+            for (int u = 0; u < U; ++u) {
+                if (e0 + u * slices >= count) break;
+                if (b[u] < 0 || b[u] >= num_buckets) {
+                    bad = true;
+                    continue;
+                }
+                float x[HV], y[HV];
+                Packed<float, HV> sum;
+                sum.load(mine + b[u] * width);
+                sum.unpack(x);
+                g[u].unpack(y);
+#pragma unroll
+                for (int i = 0; i < HV; ++i) x[i] += y[i];
+                Packed<float, HV>::store(mine + b[u] * width, x);
+            }
         }
+        if (bad) *status = 2;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < cells; i += blockDim.x) {
         const int b = i / width, hh = i % width;
-        if (blockIdx.y * width + hh >= heads) continue;
+        if (static_cast<int>(blockIdx.y) * width + hh >= heads) continue;
         float s = 0.0f;
         for (int k = 0; k < slices; ++k) s += acc[k * cells + i];
         partial[(static_cast<int64_t>(blockIdx.x) * num_buckets + b) * heads + blockIdx.y * width + hh] = s;
@@ -140,25 +174,29 @@ __global__ void __launch_bounds__(1024) bias_sum_kernel(const float* __restrict_
     if (threadIdx.x == 0 && cell < cells) out[cell] = from_float<T>(t);
 }
 
-// How the table gradient is split: heads a block takes, slices of its edges, thread blocks.
+// How the table gradient is split: heads a thread and a block take, slices of a block's edges, thread blocks.  The tables of the
+// slices fill the shared memory of an SM; a wide vector of heads a thread keeps the loads in flight when that leaves few threads.
 struct BiasSplit {
-    int width, slices, groups, parts;
+    int vec, width, slices, groups, parts;
     int64_t per_block;
     size_t smem;
 };
-BiasSplit bias_split(int64_t edges, int heads, int num_buckets) {
+BiasSplit bias_split(int64_t edges, int heads, int num_buckets, int element) {
     BiasSplit s;
+    constexpr size_t kMostSmem = 208 * 1024;
+    s.vec = element == 2 && heads % 8 == 0 ? 8 : heads % 4 == 0 ? 4 : 1;
     s.width = std::min(heads, 32);
-    constexpr size_t kMostSmem = 200 * 1024;
-    while (s.width > 1 && sizeof(float) * num_buckets * s.width > kMostSmem) s.width = (s.width + 1) / 2;
+    while (s.width > s.vec && sizeof(float) * num_buckets * s.width > kMostSmem) s.width = static_cast<int>(ceil_div(s.width / 2, s.vec)) * s.vec;
     const size_t table = sizeof(float) * num_buckets * s.width;
-    s.slices = static_cast<int>(std::max<size_t>(1, std::min<size_t>(kThreads / s.width, 64 * 1024 / table)));
-    s.groups = (heads + s.width - 1) / s.width;
+    s.groups = static_cast<int>(ceil_div(heads, s.width));
+    // a block clears, sums and writes its tables: every slice takes at least some edges
+    const int64_t a_block = ceil_div(edges, kNumSMs);
+    s.slices = static_cast<int>(std::max<size_t>(1, std::min<size_t>(kSumThreads * s.vec / s.width, kMostSmem / table)));
+    s.slices = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(s.slices, ceil_div(a_block, 16))));
+    while (s.vec > 1 && s.slices * s.width / s.vec < 128) s.vec = s.vec == 8 ? 4 : 1;      // few slices: more threads, each with fewer heads
     s.smem = table * s.slices;
-    const int resident = static_cast<int>(std::max<size_t>(1, std::min<size_t>(8, kMostSmem / s.smem)));
-    // a block clears, sums and writes a table: it takes at least a few edges for every cell of it
-    const int64_t least = std::max<int64_t>(8 * s.slices, num_buckets);
-    s.parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ceil_div(edges, least), std::max(1, kNumSMs * resident / s.groups))));
+    const int64_t least = std::max<int64_t>(16 * s.slices, num_buckets / 4);
+    s.parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ceil_div(edges, least), kNumSMs)));
     s.per_block = ceil_div(std::max<int64_t>(edges, 1), s.parts);
     return s;
 }
@@ -171,20 +209,29 @@ int bias_fwd(const void* table, const int32_t* buckets, int num_buckets, int hea
     const bool v4 = aligned_to(out, 4 * sizeof(T));
     const T* tab = static_cast<const T*>(table);
     T* o = static_cast<T*>(out);
-    if (v4) bias_fwd_kernel<T, 4><<<flat_grid(ceil_div(total, 4)), kThreads, 0, st>>>(tab, buckets, num_buckets, heads, total, o, status);
-    else bias_fwd_kernel<T, 1><<<flat_grid(total), kThreads, 0, st>>>(tab, buckets, num_buckets, heads, total, o, status);
+    const int grid = flat_grid(v4 ? ceil_div(total, 4) : total);
+    if (v4 && total < UINT32_MAX) bias_fwd_kernel<T, 4, uint32_t><<<grid, kThreads, 0, st>>>(tab, buckets, num_buckets, heads, total, o, status);
+    else if (v4) bias_fwd_kernel<T, 4, int64_t><<<grid, kThreads, 0, st>>>(tab, buckets, num_buckets, heads, total, o, status);
+    else bias_fwd_kernel<T, 1, int64_t><<<grid, kThreads, 0, st>>>(tab, buckets, num_buckets, heads, total, o, status);
     return check_launch("relative_bias_fwd");
 }
 
 template <typename T>
 int bias_bwd(const void* grad, const int32_t* buckets, int num_buckets, int heads, int64_t edges, void* grad_table, float* partial,
              int table_type, int32_t* status, cudaStream_t st) {
-    const BiasSplit s = bias_split(edges, heads, num_buckets);
-    const int allowed = allow_smem(bias_bwd_kernel<T>, s.smem);
-    if (allowed != E3B_OK) return allowed;
-    bias_bwd_kernel<T><<<dim3(s.parts, s.groups), s.width * s.slices, s.smem, st>>>(static_cast<const T*>(grad), buckets, num_buckets, heads, s.width,
-                                                                                   s.slices, edges, s.per_block, partial, status);
-    const int rc = check_launch("relative_bias_bwd");
+    const BiasSplit s = bias_split(edges, heads, num_buckets, sizeof(T));
+    auto launch = [&](auto v0) -> int {
+        constexpr int HV = decltype(v0)::value;
+        const int allowed = allow_smem(bias_bwd_kernel<T, HV>, s.smem);
+        if (allowed != E3B_OK) return allowed;
+        bias_bwd_kernel<T, HV><<<dim3(s.parts, s.groups), s.width / HV * s.slices, s.smem, st>>>(
+            static_cast<const T*>(grad), buckets, num_buckets, heads, s.width, s.slices, edges, s.per_block, partial, status);
+        return check_launch("relative_bias_bwd");
+    };
+    if (!aligned_to(grad, s.vec * sizeof(T))) return fail(E3B_ERR_ARG, "relative_bias_bwd: the gradient must start on %d bytes", static_cast<int>(s.vec * sizeof(T)));
+    int rc;
+    if constexpr (sizeof(T) == 2) rc = s.vec == 8 ? launch(Int<8>()) : s.vec == 4 ? launch(Int<4>()) : launch(Int<1>());
+    else rc = s.vec == 4 ? launch(Int<4>()) : launch(Int<1>());
     if (rc != E3B_OK) return rc;
     const int cells = num_buckets * heads;
     const dim3 block(32, 32);
@@ -207,7 +254,7 @@ extern "C" int e3b_distance_buckets(const float* pos, const int64_t* edge_src, c
     if (num_edges == 0) return E3B_OK;
     if ((num_nodes > 0 && !pos) || !edge_src || !edge_dst || (num_thresholds > 0 && !thresholds_squared) || !buckets || !status)
         return fail(E3B_ERR_ARG, "distance_buckets: null pointer");
-    distance_buckets_kernel<<<flat_grid(num_edges), kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+    distance_buckets_kernel<<<flat_grid(ceil_div(num_edges, 2)), kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
         pos, edge_src, edge_dst, shift, thresholds_squared, num_thresholds, num_edges, num_nodes, buckets, status);
     return check_launch("distance_buckets");
 }
@@ -225,7 +272,8 @@ extern "C" int e3b_relative_bias_fwd(const void* table, const int32_t* buckets, 
 
 extern "C" int64_t e3b_relative_bias_scratch_bytes(int64_t num_edges, int num_buckets, int num_heads) {
     if (num_edges < 0 || num_buckets < 1 || num_buckets > kMaxBuckets || num_heads < 1) return 0;
-    return sizeof(float) * static_cast<int64_t>(bias_split(num_edges, num_heads, num_buckets).parts) * num_buckets * num_heads;
+    const int parts = std::max(bias_split(num_edges, num_heads, num_buckets, 2).parts, bias_split(num_edges, num_heads, num_buckets, 4).parts);
+    return sizeof(float) * static_cast<int64_t>(parts) * num_buckets * num_heads;
 }
 
 extern "C" int e3b_relative_bias_bwd(const void* grad_bias, const int32_t* buckets, int num_buckets, int num_heads, int64_t num_edges, int type,

@@ -44,6 +44,8 @@ class _RelativeBiasFunction(torch.autograd.Function):
 def bias_table_grad(grad: torch.Tensor, buckets: torch.Tensor, num_buckets: int, dtype: torch.dtype) -> torch.Tensor:
     """``out[b, h] = sum of grad[e, h] over the edges of bucket b`` in fp32, in a fixed order, rounded once to ``dtype``."""
     grad = grad.contiguous()
+    if grad.data_ptr() % 16:
+        grad = grad.clone()
     edges, heads = grad.shape
     out = torch.empty(num_buckets, heads, dtype=dtype, device=grad.device)
     core = _lib.core()
