@@ -151,15 +151,18 @@ __global__ void __launch_bounds__(256) attn_fwd_kernel(const FwdArgs a) {
 // The same with k and v through the ring: the registers hold q, the sums and the row in hand, so more warps fit and all copies that
 // fit in shared memory are under way (about 200 KB an SM).
 template <typename T, int VEC, int V>
-__global__ void __launch_bounds__(384, 1) attn_fwd_ring_kernel(const FwdArgs a) {
+__global__ void __launch_bounds__(512, 1) attn_fwd_ring_kernel(const FwdArgs a) {
     extern __shared__ __align__(128) uint8_t memory[];
-    constexpr int U = V * VEC <= 12 ? 4 : 2;
+    constexpr int U = edges_together(V * VEC);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = blockIdx.x * (blockDim.x >> 5) + warp;
     const int head = lane / a.h.lanes;
     const bool live = head < a.h.heads, leads = live && (lane & (a.h.lanes - 1)) == 0;
     int cq[V], cv[V];
     lane_columns<V>(a.h.qk, a.h.nqk, a.h.lanes, head, live, cq);
     lane_columns<V>(a.h.v, a.h.nv, a.h.lanes, head, live, cv);
+    uint32_t pq[V], pv[V];
+    slot_places<T, V>(cq, 0, a.ring.zeros(), pq);
+    slot_places<T, V>(cv, a.ring.a_bytes, a.ring.zeros(), pv);
     Sums<VEC, V, 1, true> s;
     s.clear();
     int64_t goes_on = -1;
@@ -194,7 +197,7 @@ __global__ void __launch_bounds__(384, 1) attn_fwd_ring_kernel(const FwdArgs a) 
             [&](const uint8_t* const (&slot)[U], const EdgeMeta& meta, int at, int m) {
                 float x[U];
 #pragma unroll
-                for (int u = 0; u < U; ++u) x[u] = dot_row<T, VEC, V>(slot[u], qf, cq);
+                for (int u = 0; u < U; ++u) x[u] = dot_row<T, VEC, V>(slot[u], qf, pq);
                 head_sums<U>(x, a.h.lanes);
                 float top = s.m;
                 bool nan = false;
@@ -221,7 +224,7 @@ __global__ void __launch_bounds__(384, 1) attn_fwd_ring_kernel(const FwdArgs a) 
                     const float w = __expf(x[u] - ref);
                     if (w == 0.0f) continue;      // left out, or too small to count: its slot may hold anything
                     s.l += w;
-                    add_row<T, VEC, V>(slot[u] + a.ring.a_bytes, w, s.a[0], cv);
+                    add_row<T, VEC, V>(slot[u], w, s.a[0], pv);
                 }
             },
             [&](int64_t n, bool started, bool ends) {
@@ -281,7 +284,7 @@ extern "C" int e3b_attention_fwd(const void* q, const void* k, const void* v, in
     const RingSource rows{static_cast<const char*>(k), static_cast<const char*>(v), nullptr, k_stride * size, v_stride * size,
                           static_cast<uint32_t>(dqk * size), static_cast<uint32_t>(dv * size), 0};
     Plan p;
-    const int planned = plan(&p, "attention_fwd", type, vec, heads, std::max(nqk, nv), num_dst, num_edges, rows, 3, 4, true);
+    const int planned = plan(&p, "attention_fwd", type, vec, heads, std::max(nqk, nv), num_dst, num_edges, rows, 4, 3, true);
     if (planned != E3B_OK) return planned;
     if (scratch_bytes < e3b_attention_scratch_bytes(num_dst, num_edges, heads, dv))
         return fail(E3B_ERR_ARG, "attention_fwd: scratch of %lld bytes is too small", static_cast<long long>(scratch_bytes));

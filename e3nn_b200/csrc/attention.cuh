@@ -362,7 +362,8 @@ struct RingSource {
     const char *a, *b, *c;               // rows by EdgeMeta::row (a, b) and by EdgeMeta::edge (c, may be null)
     int64_t a_stride, b_stride;          // bytes
     uint32_t a_bytes, b_bytes, c_bytes;  // of a row, multiples of 16
-    __host__ __device__ uint32_t slot() const { return (a_bytes + b_bytes + c_bytes + 127) / 128 * 128; }
+    __host__ __device__ uint32_t zeros() const { return a_bytes + b_bytes + c_bytes; }      // a slot ends with 16 bytes of zeros
+    __host__ __device__ uint32_t slot() const { return (zeros() + 16 + 127) / 128 * 128; }
 };
 
 __device__ __forceinline__ void bulk_copy(void* smem, const void* global, uint32_t bytes, uint64_t* bar) {
@@ -378,6 +379,10 @@ __device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity) {
     return false;
 }
 
+// Edges used together.  (Four everywhere: 5 to 15 % slower on rows of 26 to 32 edges of 576 and 1,024 columns, whose last group is
+// then half empty and whose ring holds few more.)
+__host__ __device__ constexpr int edges_together(int columns) { return columns <= 12 ? 4 : 2; }
+
 template <int U, typename Meta>
 struct Ring {
     const RingSource src;
@@ -392,7 +397,10 @@ struct Ring {
     __device__ __forceinline__ Ring(const RingSource& source, uint8_t* memory, int slots) : src(source), smem(memory), depth(slots) {
         full = reinterpret_cast<uint64_t*>(memory + static_cast<size_t>(slots) * source.slot());
         const int lane = threadIdx.x & 31;
-        for (int i = lane; i < depth; i += 32) tc::mbar_init(&full[i], 1);
+        for (int i = lane; i < depth; i += 32) {
+            tc::mbar_init(&full[i], 1);
+            *reinterpret_cast<uint4*>(memory + static_cast<uint32_t>(i) * source.slot() + source.zeros()) = make_uint4(0u, 0u, 0u, 0u);
+        }
         tc::mbar_init_fence();
         __syncwarp();
     }
@@ -409,7 +417,7 @@ struct Ring {
             if (row >= 0) {
                 uint8_t* slot = smem + static_cast<uint32_t>(at) * src.slot();
                 tc::fence_proxy_async_smem();
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc::smem_u32(bar)), "r"(src.a_bytes + src.b_bytes + src.c_bytes) : "memory");
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc::smem_u32(bar)), "r"(src.zeros()) : "memory");
                 bulk_copy(slot, src.a + row * src.a_stride, src.a_bytes, bar);
                 bulk_copy(slot + src.a_bytes, src.b + row * src.b_stride, src.b_bytes, bar);
                 if (src.c) bulk_copy(slot + src.a_bytes + src.b_bytes, src.c + edge * src.c_bytes, src.c_bytes, bar);
@@ -484,7 +492,7 @@ __device__ __forceinline__ void walk_ring(const Rows& r, const Part& p, Ring<U, 
         [&](int64_t first, int64_t last) {
             int left = static_cast<int>(last - first);
             while (left > 0 && !failed) {
-                const int at = ring.used & 31, m = min(min(U, left), 32 - at);
+                const int at = ring.used & 31, m = min(min(min(U, left), 32 - at), ring.issued - ring.used);
                 const uint8_t* slot[U];
                 before(ring.now, at, m);
                 failed = !ring.wait(m, slot);
@@ -500,11 +508,49 @@ __device__ __forceinline__ void walk_ring(const Rows& r, const Part& p, Ring<U, 
     if (failed) ring.abandon(status);
 }
 
-// Dots of the lane's columns of a row in shared memory, and products added to a lane's sums, two columns an instruction.  Columns a
-// lane does not have are left out by a test, not by a zero: what lies there belongs to another head and may be anything.
+// Places of a lane's vectors in a slot, in bytes; vectors that it does not have are the zeros at the slot's end, so that no product
+// has to be left out (a multiplication by zero would not do: what lies in the row belongs to another head and may be anything).
+template <typename T, int V>
+__device__ __forceinline__ void slot_places(const int (&col)[V], uint32_t row, uint32_t zeros, uint32_t (&place)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) place[j] = col[j] >= 0 ? row + static_cast<uint32_t>(col[j]) * static_cast<uint32_t>(sizeof(T)) : zeros;
+}
+// Dots with the lane's columns of a row in a slot, and products added to a lane's sums; two columns an instruction.
 template <typename T, int VEC, int V>
-__device__ __forceinline__ float dot_row(const uint8_t* row, const float (&f)[V][VEC], const int (&col)[V]) {
+__device__ __forceinline__ float dot_row(const uint8_t* slot, const float (&f)[V][VEC], const uint32_t (&place)[V]) {
     static_assert(VEC % 2 == 0, "rows in shared memory are read in vectors of 16 bytes");
+    float2 d = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        Packed<T, VEC> p;
+        float x[VEC];
+        p.load(reinterpret_cast<const T*>(slot + place[j]));
+        p.unpack(x);
+#pragma unroll
+        for (int i = 0; i < VEC; i += 2) d = fma2(make_float2(f[j][i], f[j][i + 1]), make_float2(x[i], x[i + 1]), d);
+    }
+    return d.x + d.y;
+}
+template <typename T, int VEC, int V>
+__device__ __forceinline__ void add_row(const uint8_t* slot, float by, float (&sum)[V][VEC], const uint32_t (&place)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        Packed<T, VEC> p;
+        float x[VEC];
+        p.load(reinterpret_cast<const T*>(slot + place[j]));
+        p.unpack(x);
+#pragma unroll
+        for (int i = 0; i < VEC; i += 2) {
+            const float2 s = fma2(make_float2(by, by), make_float2(x[i], x[i + 1]), make_float2(sum[j][i], sum[j][i + 1]));
+            sum[j][i] = s.x;
+            sum[j][i + 1] = s.y;
+        }
+    }
+}
+// The same by columns, testing each: for the kernel whose registers have no room for the places (with them, 700 us in place of 470
+// on 425,984 edges of 1,024 columns in bf16: it spills).  Same order of additions.
+template <typename T, int VEC, int V>
+__device__ __forceinline__ float dot_columns(const uint8_t* row, const float (&f)[V][VEC], const int (&col)[V]) {
     float2 d = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -519,7 +565,7 @@ __device__ __forceinline__ float dot_row(const uint8_t* row, const float (&f)[V]
     return d.x + d.y;
 }
 template <typename T, int VEC, int V>
-__device__ __forceinline__ void add_row(const uint8_t* row, float by, float (&sum)[V][VEC], const int (&col)[V]) {
+__device__ __forceinline__ void add_columns(const uint8_t* row, float by, float (&sum)[V][VEC], const int (&col)[V]) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         if (col[j] < 0) continue;
@@ -584,7 +630,7 @@ inline int compiled_vectors(int vec, int v) {
     return v <= 4 ? 4 : v <= 8 ? 8 : v <= 16 ? 16 : 32;
 }
 
-constexpr int kWarpsPerSm[] = {12, 8, 4};    // that the kernels may be launched with
+constexpr int kWarpsPerSm[] = {16, 12, 8, 4};    // that the kernels may be launched with
 inline int most_parts(int64_t num, int64_t edges) {
     int parts = 1;
     for (int w : kWarpsPerSm) parts = std::max(parts, split_rows(num, edges, w).parts);

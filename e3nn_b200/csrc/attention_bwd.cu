@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(256) attn_bwd_dst_kernel(const BwdArgs a) {
 template <typename T, int VEC, int V>
 __global__ void __launch_bounds__(384, 1) attn_bwd_dst_ring_kernel(const BwdArgs a) {
     extern __shared__ __align__(128) uint8_t memory[];
-    constexpr int U = V * VEC <= 12 ? 4 : 2;
+    constexpr int U = edges_together(V * VEC);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = blockIdx.x * (blockDim.x >> 5) + warp;
     const int head = lane / a.h.lanes;
     const bool live = head < a.h.heads, leads = live && (lane & (a.h.lanes - 1)) == 0;
@@ -239,8 +239,8 @@ __global__ void __launch_bounds__(384, 1) attn_bwd_dst_ring_kernel(const BwdArgs
                 float x[2 * U];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    x[u] = dot_row<T, VEC, V>(slot[u], qf, cq);
-                    x[U + u] = dot_row<T, VEC, V>(slot[u] + a.ring.a_bytes, gf, cv);
+                    x[u] = dot_columns<T, VEC, V>(slot[u], qf, cq);
+                    x[U + u] = dot_columns<T, VEC, V>(slot[u] + a.ring.a_bytes, gf, cv);
                 }
                 head_sums<2 * U>(x, a.h.lanes);
 #pragma unroll
@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(384, 1) attn_bwd_dst_ring_kernel(const BwdArgs
                         p = __expf(logit(x[u], a.scale, bias[u], lw) - top) * inv;
                         da = p == 0.0f ? 0.0f : p * (x[U + u] - delta);
                     }
-                    if (da != 0.0f) add_row<T, VEC, V>(slot[u], da, s.a[0], cq);
+                    if (da != 0.0f) add_columns<T, VEC, V>(slot[u], da, s.a[0], cq);
                     if (leads && a.share) a.share_of(edge[u])[head] = make_float2(p, da);
                     if (leads && a.da) a.da[static_cast<int64_t>(edge[u]) * a.h.heads + head] = da;
                     if (a.grad_k) {

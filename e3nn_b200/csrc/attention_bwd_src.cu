@@ -118,15 +118,18 @@ __global__ void __launch_bounds__(256) attn_bwd_src_kernel(const SrcArgs a) {
 
 // The same with the rows of q and g, and the shares of the edge, through the ring.
 template <typename T, int VEC, int V>
-__global__ void __launch_bounds__(384, 1) attn_bwd_src_ring_kernel(const SrcArgs a) {
+__global__ void __launch_bounds__(512, 1) attn_bwd_src_ring_kernel(const SrcArgs a) {
     extern __shared__ __align__(128) uint8_t memory[];
-    constexpr int U = V * VEC <= 12 ? 4 : 2;
+    constexpr int U = edges_together(V * VEC);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = blockIdx.x * (blockDim.x >> 5) + warp;
     const int head = lane / a.h.lanes;
     const bool live = head < a.h.heads, leads = live && (lane & (a.h.lanes - 1)) == 0;
     int cq[V], cv[V];
     lane_columns<V>(a.h.qk, a.h.nqk, a.h.lanes, head, live, cq);
     lane_columns<V>(a.h.v, a.h.nv, a.h.lanes, head, live, cv);
+    uint32_t pq[V], pv[V];
+    slot_places<T, V>(cq, 0, a.ring.zeros(), pq);
+    slot_places<T, V>(cv, a.ring.a_bytes, a.ring.zeros(), pv);
     Sums<VEC, V, 2, false> s;
     s.clear();
     int64_t goes_on = -1;
@@ -146,8 +149,8 @@ __global__ void __launch_bounds__(384, 1) attn_bwd_src_ring_kernel(const SrcArgs
                 for (int u = 0; u < U; ++u) {
                     if (!use[u] || !live) continue;
                     const float2 x = reinterpret_cast<const float2*>(slot[u] + a.ring.a_bytes + a.ring.b_bytes)[head];
-                    if (x.y != 0.0f) add_row<T, VEC, V>(slot[u], x.y, s.a[0], cq);
-                    if (x.x != 0.0f) add_row<T, VEC, V>(slot[u] + a.ring.a_bytes, x.x, s.a[1], cv);
+                    if (x.y != 0.0f) add_row<T, VEC, V>(slot[u], x.y, s.a[0], pq);
+                    if (x.x != 0.0f) add_row<T, VEC, V>(slot[u], x.x, s.a[1], pv);
                 }
             },
             [&](int64_t n, bool started, bool ends) {
@@ -214,7 +217,7 @@ extern "C" int e3b_attention_bwd_src(const void* q, const void* grad_out, int64_
                           static_cast<int64_t>(dv) * size, static_cast<uint32_t>(dqk * size), static_cast<uint32_t>(dv * size),
                           static_cast<uint32_t>(((heads + 1) & ~1) * sizeof(float2))};
     Plan p;
-    const int planned = plan(&p, "attention_bwd_src", type, vec, heads, std::max(nqk, nv), num_src, num_edges, rows, 3, 4, true);
+    const int planned = plan(&p, "attention_bwd_src", type, vec, heads, std::max(nqk, nv), num_src, num_edges, rows, 4, 3, true);
     if (planned != E3B_OK) return planned;
     const Split& s = p.s;
     SrcArgs a{q, grad_out, q_stride, reinterpret_cast<const float2*>(share), edge_dst, src_perm, grad_k, grad_v, num_dst, scale,

@@ -41,9 +41,9 @@ constexpr int kNumSMs = 148;  // B200
 // one that another thread is about to launch with.
 template <typename K>
 int allow_smem(K kernel, size_t smem) {
-    constexpr int kMost = 226 * 1024;
+    constexpr int kMost = 226 * 1024;      // (what is static counts against the 48 KB of a plain launch too)
     if (smem > kMost) return fail(E3B_ERR_UNSUPPORTED, "%lld bytes of shared memory are needed", static_cast<long long>(smem));
-    if (smem > 48 * 1024) E3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
+    if (smem > 32 * 1024) E3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
     return E3B_OK;
 }
 
