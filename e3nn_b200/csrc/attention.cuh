@@ -362,8 +362,8 @@ struct RingSource {
     const char *a, *b, *c;               // rows by EdgeMeta::row (a, b) and by EdgeMeta::edge (c, may be null)
     int64_t a_stride, b_stride;          // bytes
     uint32_t a_bytes, b_bytes, c_bytes;  // of a row, multiples of 16
-    __host__ __device__ uint32_t zeros() const { return a_bytes + b_bytes + c_bytes; }      // a slot ends with 16 bytes of zeros
-    __host__ __device__ uint32_t slot() const { return (zeros() + 16 + 127) / 128 * 128; }
+    __host__ __device__ uint32_t zeros() const { return a_bytes + b_bytes + c_bytes; }      // a slot ends with 16 bytes of zeros (and no padding: it would cost a slot of wide rows)
+    __host__ __device__ uint32_t slot() const { return zeros() + 16; }
 };
 
 __device__ __forceinline__ void bulk_copy(void* smem, const void* global, uint32_t bytes, uint64_t* bar) {
