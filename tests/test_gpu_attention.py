@@ -169,7 +169,7 @@ def test_transposed_edges_are_built_when_they_are_not_given():
 
 
 @pytest.mark.parametrize("irreps,heads", [("256x0e+256x1o", 1), ("1023x0e", 1), ("64x0e+64x1o+64x2e+64x3o", 8), ("64x0e+64x1o+64x2e+64x3o", 16),
-                                          ("20x0e+20x1o+20x2e", 2)])
+                                          ("20x0e+20x1o+20x2e", 2), ("4096x0e", 8)])
 def test_wide_heads(irreps, heads):
     t = make(irreps, irreps, heads, [3, 0, 40], torch.float32, False, "table", False, False)
     t["q"] *= 0.3                                       # logits of a few units, as the bound assumes
@@ -177,6 +177,49 @@ def test_wide_heads(irreps, heads):
     ref = attention64(irreps, irreps, heads, *(t[n].double() for n in "qkv"), t["rowptr"], t["src"], None, t["bias"].double(), t["buckets"])
     out = mod(*(t[n].cuda() for n in "qkv"), t["rowptr"].cuda(), t["src"].cuda(), bias=t["bias"].cuda(), buckets=t["buckets"].cuda())
     close(out, ref, torch.float32, 64 + 40 + o3.Irreps(irreps).dim // heads, t["v"].double().abs().max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("irreps,heads", [("8x0e+8x1o", 4), ("6x0e+3x1o", 3), ("64x0e+64x1o+64x2e+64x3o", 8)])
+@pytest.mark.parametrize("per_edge", [False, True])
+def test_large_graph(irreps, heads, per_edge, dtype):
+    """Enough edges for whole blocks of warps, uneven rows and one hub: the formula in 64 bits over all edges at once."""
+    gen = torch.Generator().manual_seed(heads)
+    N, D = 900, o3.Irreps(irreps).dim
+    degrees = (torch.rand(N, generator=gen) ** 3 * 40).long()
+    degrees[17], degrees[400:420] = 900, 0
+    rowptr = torch.cat([torch.zeros(1, dtype=torch.int64), degrees.cumsum(0)])
+    E = int(rowptr[-1])
+    S = E if per_edge else 700
+    src = None if per_edge else torch.randint(S, (E,), generator=gen)
+    q, k, v, g = (torch.randn(n, D, generator=gen).to(dtype).cuda() for n in (N, S, S, N))
+    weight = (0.1 + 0.9 * torch.rand(E, generator=gen)).cuda()
+    table, buckets = torch.randn(7, heads, generator=gen).cuda(), torch.randint(7, (E,), generator=gen, dtype=torch.int32).cuda()
+    dst = torch.repeat_interleave(torch.arange(N), degrees).cuda()
+    mod = bnn.NeighborAttention(irreps, irreps, heads).cuda()
+    leaves = [t.clone().requires_grad_() for t in (q, k, v, table, weight)]
+    src_d = None if src is None else src.cuda()
+    out = mod(*leaves[:3], rowptr.cuda(), src_d, bias=leaves[3], buckets=buckets, edge_weight=leaves[4],
+              transpose=None if src is None else e3nn_b200.csr_from_dst(src_d, S))
+    got = torch.autograd.grad(out, leaves, g)
+    e3nn_b200.check_status()
+    cols = torch.tensor(head_columns(irreps, heads)).cuda()
+    x = [t.double().requires_grad_() for t in (q, k, v, table, weight)]
+    r = torch.arange(S, device="cuda") if src is None else src_d
+    a = (x[0][:, cols][dst] * x[1][:, cols][r]).sum(2) * cols.shape[1] ** -0.5 + x[3][buckets.long()] + torch.log(x[4])[:, None]
+    top = torch.full((N, heads), -math.inf, dtype=torch.float64, device="cuda").scatter_reduce(0, dst[:, None].expand(-1, heads), a.detach(), "amax")
+    p = torch.exp(a - top[dst])
+    p = p / torch.zeros(N, heads, dtype=torch.float64, device="cuda").index_add(0, dst, p)[dst]
+    o = torch.zeros(N, *cols.shape, dtype=torch.float64, device="cuda").index_add(0, dst, p[:, :, None] * x[2][:, cols][r])
+    ref = torch.zeros(N, D, dtype=torch.float64, device="cuda").index_copy(1, cols.flatten(), o.reshape(N, D))
+    refs = torch.autograd.grad(ref, x, g.double())
+    n, d = 900, D // heads
+    out_deg = 1 if src is None else int(torch.bincount(src).max())
+    close(out.detach(), ref.detach().cpu(), dtype, 64 + n, v.abs().max().item())
+    da = 2 * g.abs().max().item() * v.abs().max().item() * d
+    sizes = (da * k.abs().max().item() * d ** -0.5, da * q.abs().max().item() * d ** -0.5 * out_deg, g.abs().max().item() * out_deg, da * E, da * heads / 0.1)
+    for a, b, size, t in zip(got, refs, sizes, (dtype, dtype, dtype, torch.float32, torch.float32)):
+        close(a, b.cpu(), t, 256 + max(n, out_deg), size)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])

@@ -99,16 +99,29 @@ def gates():
         "wide": bnn.Gate("600x0e", [silu], "500x0e", [sig], "300x1o+200x2e"),
         "wide odd": bnn.Gate("601x0e", [silu], "500x0e", [sig], "299x1o+201x2e"),
         "none": None,
+        "l3": bnn.Gate("64x0e", [silu], "192x0e", [sig], "64x1o+64x2e+64x3o"),
     }
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("name", list(gates()))
+@pytest.mark.parametrize("name", [n for n in gates() if n != "l3"])
 @pytest.mark.parametrize("rows", [1, 77])
 @pytest.mark.parametrize("pre", [True, False])
 def test_norm_gate_residual(name, rows, dtype, pre):
     if pre is False and (dtype != torch.float32 or rows == 1):
         pytest.skip("one form of it is enough")
+    check_norm_gate(name, rows, dtype, pre)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", [n for n in gates() if not n.startswith("wide")] + ["l3"])
+@pytest.mark.parametrize("pre", [True, False])
+def test_many_rows(name, dtype, pre):
+    """From 1,184 rows on the forward pass takes a row per warp."""
+    check_norm_gate(name, 1301, dtype, pre)
+
+
+def check_norm_gate(name, rows, dtype, pre):
     gen = torch.Generator().manual_seed(len(name) + rows)
     gate = gates()[name]
     mod = bnn.NormGateResidual(gate, irreps="6x0e+3x1o" if gate is None else None, eps=1e-5, pre_norm=pre, scale_init=0.7)
