@@ -19,9 +19,9 @@ __global__ void __launch_bounds__(MAXT, BLOCKS) norm_gate_fwd_kernel(const T* __
     float* at = smem;
     const BlockSums in = block_sums_at(at, t.nblk_in, t.nw), outs = block_sums_at(at, t.nblk_out, t.nw);
     float* gates = at;                                   // [num_gates + 1]
-    RowAhead<T, VEC, K, 2> wide(gates + (t.num_gates + 4) / 4 * 4);
-    constexpr int AHEAD = rows_ahead(NW * sizeof(T));
-    RowAhead<T, NW, M, 2> narrow(wide.mine - threadIdx.x * wide.kBytes + static_cast<int>(blockDim.x) * wide.kThread);
+    constexpr int AHEAD = rows_ahead(NW * sizeof(T), K > M ? K : M);
+    RowAhead<T, VEC, K, 2, AHEAD> wide(gates + (t.num_gates + 4) / 4 * 4);
+    RowAhead<T, NW, M, 2, AHEAD> narrow(wide.mine - threadIdx.x * wide.kBytes + static_cast<int>(blockDim.x) * wide.kThread);
     Items<VEC, NW, K, M> it;
     it.init(t);
     auto fetch = [&](int64_t z, int stage) {
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(MAXT, BLOCKS) norm_gate_fwd_kernel(const T* __
     __syncthreads();
     for (int stage = 0; z < rows; z += gridDim.x, stage = stage + 1 == AHEAD ? 0 : stage + 1) {
         float v[K][VEC], o[K][VEC], nv[M][NW], no[M][NW], sq[K], nsq[M];
-        wait_for_row();
+        wait_for_row<AHEAD>();
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             sq[k] = 0.0f;
@@ -403,9 +403,9 @@ extern "C" int e3b_norm_gate_residual_fwd(const void* residual, const void* y, c
     const int64_t floats = BlockSums::floats(t.nblk_in, t.nw) + BlockSums::floats(t.nblk_out, t.nw) + (t.num_gates + 4) / 4 * 4;
     return by_type_and_items(type, s, [&](auto t0, auto v0, auto n0, auto k0, auto m0, auto x0) -> int {
         using T = decltype(t0);
-        constexpr int VEC = decltype(v0)::value, NW = decltype(n0)::value, K = decltype(k0)::value, M = decltype(m0)::value, MAXT = decltype(x0)::value;
+        constexpr int VEC = decltype(v0)::value, NW = decltype(n0)::value, K = decltype(k0)::value, M = decltype(m0)::value, MAXT = decltype(x0)::value, AHEAD = rows_ahead(NW * sizeof(T), K > M ? K : M);
         constexpr int BLOCKS = MAXT == 128 ? 6 : MAXT == 256 ? 3 : 1;
-        const size_t smem = sizeof(float) * floats + static_cast<size_t>(RowAhead<T, VEC, K, 2>::kThread + RowAhead<T, NW, M, 2>::kThread) * s.threads;
+        const size_t smem = sizeof(float) * floats + static_cast<size_t>(RowAhead<T, VEC, K, 2, AHEAD>::kThread + RowAhead<T, NW, M, 2, AHEAD>::kThread) * s.threads;
         int grid = 0;
         const int e = resident_blocks(norm_gate_fwd_kernel<T, VEC, NW, K, M, MAXT, BLOCKS>, s.threads, smem, rows, &grid);
         if (e != E3B_OK) return e;

@@ -85,15 +85,15 @@ struct Items {
     }
 };
 
-// The next rows of A arrays on their way: by cp.async to shared memory, two rows in front of the one in hand.  Every thread
+// The next rows of A arrays on their way: by cp.async to shared memory, two rows in front of the one in hand (one where a thread has eight items).  Every thread
 // fetches its own columns and reads nothing else, so the only wait is for its own copies.  Single 16-bit columns are too
 // small for such a copy: they are loaded into registers, one row in front.
-__host__ __device__ constexpr int rows_ahead(int bytes) { return bytes >= 4 ? 2 : 1; }
-template <typename T, int WIDTH, int N, int A>
+__host__ __device__ constexpr int rows_ahead(int bytes, int items) { return bytes >= 4 && items < 8 ? 2 : 1; }      // (eight items: one, for their shared memory)
+template <typename T, int WIDTH, int N, int A, int AHEAD>
 struct RowAhead {
     static constexpr int kBytes = WIDTH * static_cast<int>(sizeof(T));
     static constexpr bool kAsync = kBytes >= 4;
-    static constexpr int kThread = kAsync ? rows_ahead(kBytes) * A * N * kBytes : 0;      // bytes a thread
+    static constexpr int kThread = kAsync ? AHEAD * A * N * kBytes : 0;      // bytes a thread
     char* mine;            // this thread's place: [rows ahead][A][N] of kBytes, a block of threads apart
     Packed<T, WIDTH> reg[kAsync ? 1 : A][kAsync ? 1 : N];
     __device__ __forceinline__ explicit RowAhead(void* smem) : mine(static_cast<char*>(smem) + threadIdx.x * kBytes) {}
@@ -118,7 +118,8 @@ struct RowAhead {
     }
 };
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_row() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }      // two groups under way
+template <int AHEAD>
+__device__ __forceinline__ void wait_for_row() { asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory"); }
 
 // ------------------------------------------------------------------------------------------------- one warp a row
 // Rows of ordinary width are taken by one warp each: no barriers, sums by shuffles, and the work that does not depend on the
@@ -287,6 +288,7 @@ __device__ __forceinline__ void spread_gates(float* row, int lane, const float (
 }
 
 // ----------------------------------------------------------------------------------------------------------- host side
+constexpr int kMostColumns = 4096;      // of a row: what the registers and the shared memory of 512 threads take in both directions
 struct RowShape {
     int vec, narrow, k, m, threads;
 };
@@ -300,8 +302,11 @@ int by_items(const RowShape& s, F&& f) {
             if (s.threads <= 256) return f(T(), v0, n0, Int<1>(), Int<1>(), Int<256>());
         }
         if (s.k == 1) return f(T(), v0, n0, Int<1>(), Int<2>(), Int<512>());
-        if (s.k == 2) return f(T(), v0, n0, Int<2>(), Int<4>(), Int<512>());
-        return f(T(), v0, n0, Int<8>(), Int<8>(), Int<512>());
+        if constexpr (decltype(v0)::value == 1) {
+            if (s.k == 8) return f(T(), v0, n0, Int<8>(), Int<8>(), Int<512>());
+        }
+        if (s.m == 8) return f(T(), v0, n0, Int<2>(), Int<8>(), Int<512>());
+        return f(T(), v0, n0, Int<2>(), Int<4>(), Int<512>());
     };
     if constexpr (sizeof(T) == 2) {
         if (s.vec == 8) return with_km(Int<8>(), Int<2>());
@@ -333,8 +338,9 @@ inline int gate_row(const char* what, int type, const int32_t* sizes, const int3
     s->k = s->m = 1;
     if (std::max(n, m) > 256) s->m = 2;
     if (n > kMaxThreads || m > 2 * kMaxThreads) s->k = 2, s->m = 4;
-    if (n > 2 * kMaxThreads || m > 4 * kMaxThreads) s->k = s->m = 8;
-    if (std::max(n, m) > 8 * kMaxThreads) return fail(E3B_ERR_UNSUPPORTED, "%s: %d items, at most %d", what, std::max(n, m), 8 * kMaxThreads);
+    if (m > 4 * kMaxThreads) s->m = 8;
+    if (n > 2 * kMaxThreads) s->k = s->m = 8;
+    if (std::max(t->din, t->dout) > kMostColumns) return fail(E3B_ERR_UNSUPPORTED, "%s: rows of %d columns, at most %d", what, std::max(t->din, t->dout), kMostColumns);
     s->threads = static_cast<int>(std::max<int64_t>(1, ceil_div(std::max(ceil_div(n, s->k), ceil_div(m, s->m)), 32)) * 32);
     t->nw = warps_pow2(s->threads);
     return E3B_OK;

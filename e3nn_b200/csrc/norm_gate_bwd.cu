@@ -25,9 +25,9 @@ __global__ void __launch_bounds__(MAXT, BLOCKS) norm_gate_bwd_kernel(const T* __
     const BlockSums outs = block_sums_at(at, t.nblk_out, t.nw), ghs = block_sums_at(at, t.nblk_out, t.nw);
     float* gates = at;                                        // [num_gates + 1] activated gates
     float* prod = gates + (t.num_gates + 4) / 4 * 4;          // [dout] cotangent of the gated row times the normalised row
-    RowAhead<T, VEC, K, 4> wide(prod + (t.dout + 3) / 4 * 4);
-    constexpr int AHEAD = rows_ahead(NW * sizeof(T));
-    RowAhead<T, NW, M, 4> narrow(wide.mine - threadIdx.x * wide.kBytes + static_cast<int>(blockDim.x) * wide.kThread);
+    constexpr int AHEAD = rows_ahead(NW * sizeof(T), K > M ? K : M);
+    RowAhead<T, VEC, K, 4, AHEAD> wide(prod + (t.dout + 3) / 4 * 4);
+    RowAhead<T, NW, M, 4, AHEAD> narrow(wide.mine - threadIdx.x * wide.kBytes + static_cast<int>(blockDim.x) * wide.kThread);
     Items<VEC, NW, K, M> it;
     it.init(t);
     auto fetch = [&](int64_t z, int stage) {
@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(MAXT, BLOCKS) norm_gate_bwd_kernel(const T* __
         // v: y, then normalised; x: residual, then z; g0: cotangent of z; g1: of h, then of the normalised row
         float v[K][VEC], x[K][VEC], g0[K][VEC], g1[K][VEC], sq[K], dot[K];
         float nv[M][NW], nx[M][NW], n0[M][NW], n1[M][NW], nsq[M], ndot[M];
-        wait_for_row();
+        wait_for_row<AHEAD>();
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             sq[k] = 0.0f;
@@ -331,9 +331,9 @@ extern "C" int e3b_norm_gate_residual_bwd(const void* residual, const void* y, c
     int grid = 0;
     const int rc = by_type_and_items(type, s, [&](auto t0, auto v0, auto n0, auto k0, auto m0, auto x0) -> int {
         using T = decltype(t0);
-        constexpr int VEC = decltype(v0)::value, NW = decltype(n0)::value, K = decltype(k0)::value, M = decltype(m0)::value, MAXT = decltype(x0)::value;
+        constexpr int VEC = decltype(v0)::value, NW = decltype(n0)::value, K = decltype(k0)::value, M = decltype(m0)::value, MAXT = decltype(x0)::value, AHEAD = rows_ahead(NW * sizeof(T), K > M ? K : M);
         constexpr int BLOCKS = MAXT == 128 ? 4 : MAXT == 256 ? 2 : 1;
-        const size_t smem = std::max<size_t>(sizeof(float) * floats + static_cast<size_t>(RowAhead<T, VEC, K, 4>::kThread + RowAhead<T, NW, M, 4>::kThread) * s.threads,
+        const size_t smem = std::max<size_t>(sizeof(float) * floats + static_cast<size_t>(RowAhead<T, VEC, K, 4, AHEAD>::kThread + RowAhead<T, NW, M, 4, AHEAD>::kThread) * s.threads,
                                              sizeof(float) * std::max(t.din, t.dout));
         const int e = resident_blocks(norm_gate_bwd_kernel<T, VEC, NW, K, M, MAXT, BLOCKS>, s.threads, smem, rows, &grid);
         if (e != E3B_OK) return e;

@@ -305,8 +305,7 @@ class NormGateResidual(torch.nn.Module):
     ``gate``: a `Gate` or an `Activation`; or ``None`` with ``irreps``, and the row is added as it is.  ``y`` has the
     gate's ``irreps_in``, ``residual``, ``z`` and ``h`` its ``irreps_out``.  Parameters: ``weight_post`` (one per channel
     of ``y``, ones), ``scale`` (one per channel of ``z``, ``scale_init``) and ``weight_pre`` (one per channel of ``z``, ones);
-    ``pre_norm=False``: no second norm, ``forward`` returns ``z`` alone.  At most 32 blocks of irreps, and 4,096 columns (four times as many
-    where all multiplicities allow vectors of four)."""
+    ``pre_norm=False``: no second norm, ``forward`` returns ``z`` alone.  At most 32 blocks of irreps, and rows of 4,096 columns."""
 
     def __init__(self, gate: Union[Gate, Activation, None] = None, irreps=None, eps: float = 1e-5, pre_norm: bool = True,
                  scale_init: float = 1.0) -> None:
@@ -352,6 +351,8 @@ class NormGateResidual(torch.nn.Module):
                 rows = items if pair == narrow else _gate_items(back, const, forth, ins, outs, width, pair)
                 plan = None if rows is None else _row_plan(rows[0].tolist(), rows[1].tolist(), back, ins, outs, width, pair)
                 self._sizes[width, narrow] = (sizes, plan)
+        if max(din, dout) > 4096:
+            raise NotImplementedError(f"rows of {max(din, dout)} columns are not supported, at most 4096")
         self.weight_post = torch.nn.Parameter(torch.ones(n_in))
         self.scale = torch.nn.Parameter(torch.full((n_out,), float(scale_init)))
         if pre_norm:

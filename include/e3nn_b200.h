@@ -296,7 +296,7 @@ int e3b_fill_columns(float* out, int64_t num_rows, int row_stride, int col0, int
  * both sides and of one block and one activation.  (w, n) = (1, 1), for fp32 (4, 1), for 16-bit types (4, 2) or (8, 2).
  * in_table [din,4] = {block, channel, first output column, count} (the last two: of the components a gate column multiplies),
  * out_table [dout,4] = {block, channel, -, -}; sizes: HOST array {w, n, num_wide, num_narrow, num_gates, din, dout, blocks in,
- * blocks out, channels in, channels out}.  Row pointers are aligned to w elements.  At most 4,096 items of each sort and 32 blocks.
+ * blocks out, channels in, channels out}.  Row pointers are aligned to w elements.  At most 4,096 columns and 32 blocks.
  * plan: HOST array or NULL.  The same row as slots of at most 32 items that are consecutive on both sides, in one block, and (gates) of
  * channels with the same number of components: {w, n, wide slots, narrow slots, din, dout, blocks in, blocks out, length of the row of gates per
  * column}, per wide slot ten integers {first input column, first output column, items, blocks of both, place of the first column's gate

@@ -167,6 +167,26 @@ def check_norm_gate(name, rows, dtype, pre):
         close(a, b, torch.float32, terms=64 + rows, size=size)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("gate", ["4096x0e", "4095x0e", "4093x0e activated", "4096x0e activated"])
+def test_widest_rows(gate, dtype):
+    """What the constructor takes has to fit both directions."""
+    irreps = gate.split()[0]
+    act = bnn.Activation(irreps, [torch.nn.functional.silu]) if "activated" in gate else None
+    mod = bnn.NormGateResidual(act, irreps=None if act else irreps).cuda()
+    gen = torch.Generator().manual_seed(0)
+    r, y, gz, gh = (rows_of(3, mod.irreps_out.dim, dtype, gen) for _ in range(4))
+    rd, yd = r.cuda().requires_grad_(), y.cuda().requires_grad_()
+    z, h = mod(rd, yd)
+    grads = torch.autograd.grad((z, h), (rd, yd, mod.scale), (gz.cuda(), gh.cuda()))
+    n = norm64(y.double(), torch.ones(mod.scale.numel(), dtype=torch.float64), irreps, 1e-5)
+    z64 = r.double() + (n if act is None else gate64(act, n))
+    close(z, z64, dtype, terms=64)
+    h64 = norm64(z64, torch.ones(mod.scale.numel(), dtype=torch.float64), irreps, 1e-5)
+    close(h, h64, dtype, terms=64, size=2 * h64.abs().amax(1, keepdim=True))
+    assert all(torch.isfinite(g).all() for g in grads)
+
+
 def test_gradients_of_one_output_alone_and_of_some_inputs():
     gen = torch.Generator().manual_seed(3)
     gate = gates()["l2"]

@@ -65,6 +65,9 @@ def test_constructors_refuse():
         bnn.RMSNorm("4x0e", eps=-1.0)
     with pytest.raises(NotImplementedError):
         bnn.NormGateResidual(irreps="+".join(f"1x{l}e" for l in range(33)))
+    for irreps in ("4097x0e", "4100x0e"):
+        with pytest.raises(NotImplementedError):
+            bnn.NormGateResidual(irreps=irreps)
     gate = bnn.Gate("4x0e", [torch.tanh], "2x0e", [torch.sigmoid], "2x1o")
     with pytest.raises(ValueError):
         bnn.NormGateResidual()
