@@ -224,8 +224,6 @@ bool row_fits(int widest, bool vec4) { return widest <= (vec4 ? 4 * 4 : 8) * kMa
 
 using namespace e3b;
 
-extern "C" int e3b_norm_max_columns(int aligned) { return (aligned ? 4 * 4 : 8) * kMaxThreads; }
-
 extern "C" int e3b_rms_norm_fwd(const void* x, const float* weight, const int32_t* table, const float* inv_count, int num_blocks,
                                 int vec4, float eps, void* h, int64_t rows, int dim, int type, void* stream) {
     if (rows < 0 || dim < 0 || num_blocks < 0 || !known_type(type)) return fail(E3B_ERR_ARG, "rms_norm_fwd: bad size or type");
