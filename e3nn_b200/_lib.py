@@ -13,6 +13,7 @@ from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64
 from typing import Dict, List, Optional
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _build
 
@@ -204,9 +205,17 @@ def check_earlier(t: torch.Tensor) -> None:
         poll_status(t.device)
 
 
-def wants_grad(*tensors: Optional[torch.Tensor]) -> bool:
-    """Whether a call has to be recorded for a backward pass."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def wants_function(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether a call has to go through its autograd function: it is recorded for a backward pass, or someone else follows it.  A
+    kernel launched past the function leaves no trace for a forward-mode level (the result would lose its tangent; the
+    function raises), a transform of `torch.func`, or the tracer of `torch.jit` (which would record the empty output alone)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return _forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active() or is_tracing()
+
+
+def is_tracing() -> bool:
+    return torch._C._get_tracing_state() is not None
 
 
 _no_switch = contextlib.nullcontext()

@@ -228,7 +228,7 @@ class NeighborAttention(torch.nn.Module):
         c.transpose = None if transpose is None else (transpose[0].contiguous(), transpose[1].contiguous())
         bias = None if bias is None else bias.to(torch.float32).contiguous()
         weight = None if edge_weight is None else edge_weight.to(torch.float32).contiguous()
-        if _lib.wants_grad(q, k, v, bias, weight):
+        if _lib.wants_function(q, k, v, bias, weight):
             out = _AttentionFunction.apply(q, k, v, bias, weight, c)
         else:
             out = _attend(q, k, v, bias, weight, c, False)[0]

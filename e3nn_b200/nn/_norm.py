@@ -75,7 +75,7 @@ def _aligned(t: torch.Tensor, width: int) -> torch.Tensor:
 def _flat_rows(x: torch.Tensor, dim: int, name: str) -> torch.Tensor:
     if x.dim() < 1 or x.shape[-1] != dim:
         torch._assert(False, f"Incorrect last dimension for {name}")
-    if x.dim() == 2 and x.is_contiguous():
+    if x.dim() == 2 and x.is_contiguous() and not _lib.is_tracing():      # (a tracer has to see the calls: its next input may lie otherwise)
         return x
     return x.reshape(-1, dim).contiguous() if dim > 0 else x.reshape(x.shape[:-1].numel(), 0)
 
@@ -125,8 +125,8 @@ def _row_plan(wides, narrows, back, ins, outs, width: int, narrow: int):
     return (ctypes.c_int32 * len(flat))(*flat)
 
 
-def _rms_norm(x, weight, tables, fours: int, eps: float) -> torch.Tensor:
-    tbl, inv, _ = tables
+def _rms_norm(x, weight, fours: int, eps: float, tbl, inv, _channels) -> torch.Tensor:
+    torch._assert(x.shape[1] == tbl.shape[0], "Incorrect last dimension for x")      # (of a traced call: checked nowhere else)
     h = torch.empty_like(x)
     with _lib.device_of(x):
         rc = _lib.core().e3b_rms_norm_fwd(x.data_ptr(), _lib.address(weight), tbl.data_ptr(), inv.data_ptr(), inv.shape[0], fours, eps, h.data_ptr(),
@@ -138,10 +138,10 @@ def _rms_norm(x, weight, tables, fours: int, eps: float) -> torch.Tensor:
 
 class _RMSNormFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, tables, fours, eps):
+    def forward(ctx, x, weight, fours, eps, *tables):
         ctx.save_for_backward(x, weight)
         ctx.meta = (tables, fours, eps)
-        return _rms_norm(x, weight, tables, fours, eps)
+        return _rms_norm(x, weight, fours, eps, *tables)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -163,7 +163,7 @@ class _RMSNormFunction(torch.autograd.Function):
                                        _lib.element_type(x), _lib.raw_stream(x))
         if rc:
             _lib.check(rc, "e3b_rms_norm_bwd")
-        return gx, gw, None, None, None
+        return gx, gw, *(None,) * 5
 
 
 class RMSNorm(torch.nn.Module):
@@ -205,10 +205,10 @@ class RMSNorm(torch.nn.Module):
         rows = _flat_rows(x, self._dim, "x")
         _lib.check_earlier(x)
         weight = _fp32(weight)
-        if _lib.wants_grad(rows, weight):
-            out = _RMSNormFunction.apply(rows, weight, tables, self._fours, self.eps)
+        if _lib.wants_function(rows, weight):
+            out = _RMSNormFunction.apply(rows, weight, self._fours, self.eps, *tables)
         else:
-            out = _rms_norm(rows, weight, tables, self._fours, self.eps)
+            out = _rms_norm(rows, weight, self._fours, self.eps, *tables)
         return out if x.dim() == 2 else out.reshape(x.shape)
 
 
@@ -248,9 +248,11 @@ def _gate_items(back, const, forth, ins, outs, width: int, narrow: int):
     return (torch.tensor(wides, dtype=torch.int32).reshape(-1, 4 + width), torch.tensor(narrows, dtype=torch.int32).reshape(-1, 8), len(slot_of))
 
 
-def _norm_gate(residual, y, w_post, scale, w_pre, tables, shape, eps: float):
+def _norm_gate(residual, y, w_post, scale, w_pre, shape, eps: float, *tables):
     sizes, plan = shape
     wide, narrow, in_tbl, out_tbl, _, _, in_inv, out_inv = tables
+    if residual.shape != (y.shape[0], out_tbl.shape[0]) or y.shape[1] != in_tbl.shape[0] or residual.dtype != y.dtype:      # (a traced call)
+        torch._assert(False, "residual and y do not fit the module")
     z = torch.empty_like(residual)
     h = torch.empty_like(residual) if w_pre is not None else None
     with _lib.device_of(y):
@@ -265,11 +267,11 @@ def _norm_gate(residual, y, w_post, scale, w_pre, tables, shape, eps: float):
 
 class _NormGateFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, residual, y, w_post, scale, w_pre, tables, shape, eps):
+    def forward(ctx, residual, y, w_post, scale, w_pre, shape, eps, *tables):
         ctx.save_for_backward(residual, y, w_post, scale, w_pre)
         ctx.meta = (tables, shape, eps)
         ctx.set_materialize_grads(False)
-        return _norm_gate(residual, y, w_post, scale, w_pre, tables, shape, eps)
+        return _norm_gate(residual, y, w_post, scale, w_pre, shape, eps, *tables)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -277,7 +279,7 @@ class _NormGateFunction(torch.autograd.Function):
         residual, y, w_post, scale, w_pre = ctx.saved_tensors
         tables, (sizes, plan), eps = ctx.meta
         if grad_z is None and grad_h is None:
-            return (None,) * 8
+            return (None,) * 15
         core, rows, address = _lib.core(), y.shape[0], _lib.address
         grad_z, grad_h = (None if g is None else _aligned(g.contiguous(), sizes[0]) for g in (grad_z, grad_h))
         g_residual = torch.empty_like(residual) if ctx.needs_input_grad[0] else None
@@ -296,7 +298,7 @@ class _NormGateFunction(torch.autograd.Function):
         if rc:
             _lib.check(rc, "e3b_norm_gate_residual_bwd")
         gw = params.split([n_in, n_out, n_out]) if params is not None else (None, None, None)
-        return (g_residual, gy, gw[0], gw[1], gw[2] if w_pre is not None else None, None, None, None)
+        return (g_residual, gy, gw[0], gw[1], gw[2] if w_pre is not None else None, *(None,) * 10)
 
 
 class NormGateResidual(torch.nn.Module):
@@ -383,8 +385,8 @@ class NormGateResidual(torch.nn.Module):
         _lib.check_earlier(y)
         tables = (*(buffers[name] for name in self._table_names[key]),)
         args = (r, x, _fp32(w_post), _fp32(scale), _fp32(w_pre))
-        apply = _NormGateFunction.apply if _lib.wants_grad(*args) else _norm_gate
-        z, h = apply(*args, tables, sizes[key], self.eps)
+        apply = _NormGateFunction.apply if _lib.wants_function(*args) else _norm_gate
+        z, h = apply(*args, sizes[key], self.eps, *tables)
         if residual.dim() == 2:
             return (z, h) if self.pre_norm else z
         return (z.reshape(residual.shape), h.reshape(residual.shape)) if self.pre_norm else z.reshape(residual.shape)

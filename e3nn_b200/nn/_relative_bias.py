@@ -16,6 +16,33 @@ import torch
 from .. import _lib
 
 
+def _distance_buckets(pos, edge_src, edge_dst, shift, squares):
+    E = edge_src.shape[0]
+    if pos.shape[1] != 3 or edge_dst.shape != (E,) or (shift is not None and shift.shape != (E, 3)):      # (of a traced call: checked nowhere else)
+        torch._assert(False, "Incorrect shape for pos, edge_src, edge_dst or shift")
+    out = torch.empty(E, dtype=torch.int32, device=pos.device)
+    with _lib.device_of(pos):
+        rc = _lib.core().e3b_distance_buckets(pos.data_ptr(), edge_src.data_ptr(), edge_dst.data_ptr(), _lib.address(shift), squares.data_ptr(),
+                                              squares.shape[0], E, pos.shape[0], out.data_ptr(), _lib.status_address(pos), _lib.raw_stream(pos))
+    if rc:
+        _lib.check(rc, "e3b_distance_buckets")
+    return out
+
+
+class _DistanceBucketsFunction(torch.autograd.Function):
+    """What a tracer records: whole numbers have no derivatives."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        out = _distance_buckets(*args)
+        ctx.mark_non_differentiable(out)
+        return out
+
+    @staticmethod
+    def backward(ctx, grad):
+        return (None,) * 5
+
+
 def _look_up(weight: torch.Tensor, buckets: torch.Tensor) -> torch.Tensor:
     num, heads = weight.shape
     out = torch.empty(buckets.shape[0], heads, dtype=weight.dtype, device=weight.device)
@@ -98,15 +125,8 @@ class RelativeBias(torch.nn.Module):
         if E < 0 or edge_dst.shape != (E,) or (shift is not None and shift.shape != (E, 3)):
             torch._assert(False, "Incorrect shape for edge_src, edge_dst or shift")
         _lib.check_earlier(pos)
-        out = torch.empty(E, dtype=torch.int32, device=pos.device)
-        pos, edge_src, edge_dst = pos.contiguous(), edge_src.contiguous(), edge_dst.contiguous()
-        shift = shift.contiguous() if shift is not None else None
-        with _lib.device_of(pos):
-            rc = _lib.core().e3b_distance_buckets(pos.data_ptr(), edge_src.data_ptr(), edge_dst.data_ptr(), _lib.address(shift), squares.data_ptr(),
-                                                  self.num_buckets - 1, E, pos.shape[0], out.data_ptr(), _lib.status_address(pos), _lib.raw_stream(pos))
-        if rc:
-            _lib.check(rc, "e3b_distance_buckets")
-        return out
+        args = (pos.contiguous(), edge_src.contiguous(), edge_dst.contiguous(), shift.contiguous() if shift is not None else None, squares)
+        return _DistanceBucketsFunction.apply(*args) if _lib.is_tracing() else _distance_buckets(*args)
 
     def forward(self, buckets: torch.Tensor) -> torch.Tensor:
         if not buckets.is_cuda:
@@ -120,5 +140,5 @@ class RelativeBias(torch.nn.Module):
             torch._assert(False, "Incorrect shape for buckets")
         _lib.element_type(weight, "weight")
         _lib.check_earlier(buckets)
-        apply = _RelativeBiasFunction.apply if _lib.wants_grad(weight) else _look_up
+        apply = _RelativeBiasFunction.apply if _lib.wants_function(weight) else _look_up
         return apply(weight.contiguous(), buckets.contiguous())

@@ -1,0 +1,99 @@
+"""Calls of the transformer modules that someone else follows although no backward pass is asked for: forward-mode levels,
+transforms of `torch.func` and the tracer of `torch.jit`.  A module may refuse them; it may not answer without their knowledge."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fw
+
+import e3nn_b200
+from e3nn_b200 import nn as bnn
+
+pytestmark = pytest.mark.gpu
+
+
+def modules():
+    """{name: (module, inputs, another set of inputs of another size)}"""
+    gen = torch.Generator().manual_seed(0)
+    def rows(n, d):
+        return torch.randn(n, d, generator=gen).cuda()
+    def edges(N, E, S):
+        dst = torch.randint(N, (E,), generator=gen).sort().values
+        rowptr = torch.cat([torch.zeros(1, dtype=torch.int64), torch.bincount(dst, minlength=N).cumsum(0)])
+        return rowptr.cuda(), torch.randint(S, (E,), generator=gen).cuda()
+    def attention(N, E, S):
+        return (rows(N, 16), rows(S, 16), rows(S, 16), *edges(N, E, S))
+    gate = bnn.Gate("4x0e", [torch.tanh], "4x0e", [torch.sigmoid], "4x1o")
+    return {
+        "rms": (bnn.RMSNorm("4x0e+4x1o"), (rows(5, 16),), (rows(9, 16),)),
+        "norm": (bnn.NormGateResidual(gate), (rows(5, 16), rows(5, 20)), (rows(9, 16), rows(9, 20))),
+        "norm alone": (bnn.NormGateResidual(gate, pre_norm=False), (rows(5, 16), rows(5, 20)), (rows(9, 16), rows(9, 20))),
+        "attention": (bnn.NeighborAttention("4x0e+4x1o", "4x0e+4x1o", 2), attention(6, 20, 7), attention(11, 33, 5)),
+    }
+
+
+def flat(out):
+    return out if isinstance(out, tuple) else (out,)
+
+
+@pytest.mark.parametrize("name", list(modules()))
+@pytest.mark.parametrize("recorded", [False, True])
+def test_a_tangent_is_not_lost(name, recorded):
+    mod, inputs, _ = modules()[name]
+    mod = mod.cuda()
+    for p in mod.parameters():
+        p.requires_grad_(recorded)
+    with torch.set_grad_enabled(recorded), fw.dual_level():
+        x = fw.make_dual(inputs[0], torch.ones_like(inputs[0]))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            mod(x, *inputs[1:])
+        mod(*inputs)                              # nothing to lose
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(lambda x: mod(x, *inputs[1:]), (inputs[0],), (torch.ones_like(inputs[0]),))
+
+
+def test_a_tangent_of_a_table_is_not_lost():
+    mod = bnn.RelativeBias(4, 2, 5.0).cuda()
+    buckets = torch.tensor([0, 3, 1], dtype=torch.int32, device="cuda")
+    weight = mod.weight.detach()
+    del mod.weight
+    with torch.no_grad(), fw.dual_level():
+        mod.register_parameter("weight", None)
+        mod._parameters["weight"] = fw.make_dual(weight, torch.ones_like(weight))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            mod(buckets)
+
+
+@pytest.mark.parametrize("name", [n for n in modules() if n != "attention"])
+@pytest.mark.parametrize("recorded", [False, True])
+def test_a_traced_module_computes(name, recorded):
+    mod, inputs, others = modules()[name]
+    mod = mod.cuda()
+    for p in mod.parameters():
+        p.requires_grad_(recorded)
+    with torch.set_grad_enabled(recorded):
+        traced = torch.jit.trace(mod, inputs)
+        wide = tuple(torch.randn(x.shape[0], 2 * x.shape[1], device="cuda")[:, ::2].copy_(x) if x.is_floating_point() else x for x in others)
+        for args in (inputs, others, wide):       # (the last one: columns apart)
+            junk = torch.full((4096,), float("nan"), device="cuda")
+            del junk                              # what an output that is never written would show
+            for a, b in zip(flat(traced(*args)), flat(mod(*args))):
+                assert torch.equal(a, b)
+
+
+def test_traced_buckets_and_bias():
+    class Both(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.bias = bnn.RelativeBias(8, 2, 5.0)
+        def forward(self, pos, src, dst):
+            buckets = self.bias.buckets(pos, src, dst)
+            return buckets, self.bias(buckets)
+    mod = Both().cuda()
+    gen = torch.Generator().manual_seed(1)
+    def graph(N, E):
+        return (5 * torch.rand(N, 3, generator=gen).cuda(), torch.randint(N, (E,), generator=gen).cuda(), torch.randint(N, (E,), generator=gen).cuda())
+    with torch.no_grad():
+        traced = torch.jit.trace(mod, graph(10, 30))
+        args = graph(20, 77)
+        for a, b in zip(traced(*args), mod(*args)):
+            assert torch.equal(a, b)
+    e3nn_b200.check_status()

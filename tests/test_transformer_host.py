@@ -105,3 +105,22 @@ def test_host_tensors_are_refused():
         bnn.RelativeBias(4, 2, 5.0)(idx.int())
     with pytest.raises(NotImplementedError):
         bnn.NeighborAttention("4x0e+4x1o", "4x0e+4x1o", 2)(x, x, x, torch.zeros(5, dtype=torch.int64), idx)
+
+
+def test_calls_that_someone_follows_go_through_autograd():
+    import torch.autograd.forward_ad as fw
+    from e3nn_b200 import _lib
+
+    x, seen = torch.zeros(2), []
+    assert not _lib.wants_function(x, None) and _lib.wants_function(x, torch.zeros(2, requires_grad=True))
+    with torch.no_grad():
+        assert not _lib.wants_function(torch.zeros(2, requires_grad=True))
+        with fw.dual_level():
+            assert _lib.wants_function(x)
+        def f(t):
+            seen.append(_lib.wants_function(t))
+            return t + 1
+        torch.jit.trace(f, x, check_trace=False)
+        torch.func.jvp(f, (x,), (x,))
+        torch.func.vmap(f)(x)
+    assert seen == [True] * 3 and not _lib.wants_function(x)
