@@ -44,13 +44,14 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 class _Call:
-    """Everything of a call that is not differentiated."""
+    """A checked call: its tensors as the kernels take them, and the layout that serves them."""
 
-    __slots__ = ("vec", "layout", "qk_tbl", "v_tbl", "scale", "rowptr", "perm", "src", "buckets", "transpose", "edges")
+    __slots__ = ("q", "k", "v", "bias", "weight", "rowptr", "src", "perm", "buckets", "perm_t", "rowptr_t", "vec", "layout", "qk_tbl", "v_tbl", "scale", "edges")
 
 
-def _attend(q, k, v, bias, weight, c: _Call, keep: bool):
+def _attend(c: _Call, keep: bool):
     """The output, and for the backward pass its fp32 form and the statistics of every row."""
+    q, k, v = c.q, c.k, c.v
     N, (H, dv), type_code, dev = q.shape[0], (c.layout[1], c.layout[5]), _lib.element_type(q), q.device
     core, address = _lib.core(), _lib.address
     out = torch.empty(N, dv, dtype=q.dtype, device=dev)
@@ -63,7 +64,7 @@ def _attend(q, k, v, bias, weight, c: _Call, keep: bool):
     with _lib.device_of(q):
         rc = core.e3b_attention_fwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), k.stride(0), v.stride(0), c.rowptr.data_ptr(), address(c.perm), address(c.src),
-            address(bias), address(c.buckets), bias.shape[0] if c.buckets is not None else 0, address(weight), c.qk_tbl.data_ptr(), c.v_tbl.data_ptr(),
+            address(c.bias), address(c.buckets), c.bias.shape[0] if c.buckets is not None else 0, address(c.weight), c.qk_tbl.data_ptr(), c.v_tbl.data_ptr(),
             c.layout, c.scale, N, k.shape[0], c.edges, type_code, out.data_ptr(), address(out32), address(stats), scratch.data_ptr(), nbytes,
             _lib.status_address(q), _lib.raw_stream(q))
     if rc:
@@ -72,26 +73,30 @@ def _attend(q, k, v, bias, weight, c: _Call, keep: bool):
 
 
 class _AttentionFunction(torch.autograd.Function):
+    """Every tensor of a call is an argument: what the backward pass reads again is watched for changes in between, and a traced call
+    takes its next graph."""
+
     @staticmethod
-    def forward(ctx, q, k, v, bias, weight, c):
-        out, out32, stats = _attend(q, k, v, bias, weight, c, True)
-        ctx.save_for_backward(q, k, v, bias, weight, out32, stats)
-        ctx.call = c
+    def forward(ctx, module, *tensors):
+        c = module._checked(*tensors)
+        out, out32, stats = _attend(c, True)
+        ctx.save_for_backward(c.q, c.k, c.v, c.bias, c.weight, out32, stats, c.rowptr, c.src, c.perm, c.buckets, c.perm_t, c.rowptr_t)
+        ctx.call = (c.vec, c.layout, c.qk_tbl, c.v_tbl, c.scale, c.edges)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        q, k, v, bias, weight, out32, stats = ctx.saved_tensors
-        c = ctx.call
-        _, H, _, _, dqk, dv = list(c.layout)
-        N, S, E, dev, type_code, core = q.shape[0], k.shape[0], c.edges, q.device, _lib.element_type(q), _lib.core()
-        _, need_k, need_v, need_bias, need_weight = ctx.needs_input_grad[:5]
+        q, k, v, bias, weight, out32, stats, rowptr, src, perm, buckets, perm_t, rowptr_t = ctx.saved_tensors
+        vec, layout, qk_tbl, v_tbl, scale, E = ctx.call
+        _, H, _, _, dqk, dv = list(layout)
+        N, S, dev, type_code, core, address = q.shape[0], k.shape[0], q.device, _lib.element_type(q), _lib.core(), _lib.address
+        _, need_k, need_v, need_bias, need_weight = ctx.needs_input_grad[1:6]
         grad = grad.contiguous()
-        if not _fits(grad, c.vec):
+        if not _fits(grad, vec):
             grad = grad.clone()
-        per_node = c.src is not None and (need_k or need_v)
-        per_edge = c.src is None and (need_k or need_v)
+        per_node = src is not None and (need_k or need_v)
+        per_edge = src is None and (need_k or need_v)
         gq = torch.empty(N, dqk, dtype=q.dtype, device=dev)
         gk = torch.empty(S, dqk, dtype=q.dtype, device=dev) if need_k or need_v else None
         gv = torch.empty(S, dv, dtype=q.dtype, device=dev) if need_k or need_v else None
@@ -104,28 +109,28 @@ class _AttentionFunction(torch.autograd.Function):
         status = _lib.status_address(q)
         with _lib.device_of(q):
             rc = core.e3b_attention_bwd(
-                _lib.address(q), _lib.address(k), _lib.address(v), _lib.address(grad), q.stride(0), k.stride(0), v.stride(0), _lib.address(out32), _lib.address(stats),
-                _lib.address(c.rowptr), _lib.address(c.perm), _lib.address(c.src), _lib.address(bias), _lib.address(c.buckets),
-                bias.shape[0] if c.buckets is not None else 0, _lib.address(weight), _lib.address(c.qk_tbl), _lib.address(c.v_tbl), c.layout, c.scale, N, S, E,
-                type_code, _lib.address(gq), _lib.address(gk) if per_edge else None, _lib.address(gv) if per_edge else None, _lib.address(share), _lib.address(da),
-                _lib.address(dst), _lib.address(gweight), _lib.address(scratch), nbytes, status, _lib.raw_stream(q))
+                address(q), address(k), address(v), address(grad), q.stride(0), k.stride(0), v.stride(0), address(out32), address(stats),
+                address(rowptr), address(perm), address(src), address(bias), address(buckets), bias.shape[0] if buckets is not None else 0, address(weight),
+                address(qk_tbl), address(v_tbl), layout, scale, N, S, E, type_code, address(gq), address(gk) if per_edge else None,
+                address(gv) if per_edge else None, address(share), address(da), address(dst), address(gweight), address(scratch), nbytes, status,
+                _lib.raw_stream(q))
         if rc:
             _lib.check(rc, "e3b_attention_bwd")
         if per_node:
-            perm_t, rowptr_t = c.transpose if c.transpose is not None else csr_from_dst(c.src, S)
+            if perm_t is None:
+                perm_t, rowptr_t = csr_from_dst(src, S)
             nbytes = core.e3b_attention_bwd_src_scratch_bytes(S, E, dqk, dv)
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
             with _lib.device_of(q):
                 rc = core.e3b_attention_bwd_src(
-                    _lib.address(q), _lib.address(grad), q.stride(0), _lib.address(share), _lib.address(dst), _lib.address(perm_t), _lib.address(rowptr_t),
-                    _lib.address(c.qk_tbl), _lib.address(c.v_tbl), c.layout, c.scale, N, S, E, type_code, _lib.address(gk), _lib.address(gv), _lib.address(scratch),
-                    nbytes, status, _lib.raw_stream(q))
+                    address(q), address(grad), q.stride(0), address(share), address(dst), address(perm_t), address(rowptr_t), address(qk_tbl), address(v_tbl),
+                    layout, scale, N, S, E, type_code, address(gk), address(gv), address(scratch), nbytes, status, _lib.raw_stream(q))
             if rc:
                 _lib.check(rc, "e3b_attention_bwd_src")
         gbias = None
         if need_bias:
-            gbias = bias_table_grad(da, c.buckets, bias.shape[0], torch.float32) if c.buckets is not None else da
-        return gq, gk if need_k else None, gv if need_v else None, gbias, gweight, None
+            gbias = bias_table_grad(da, buckets, bias.shape[0], torch.float32) if buckets is not None else da
+        return None, gq, gk if need_k else None, gv if need_v else None, gbias, gweight, *(None,) * 6
 
 
 class NeighborAttention(torch.nn.Module):
@@ -181,15 +186,27 @@ class NeighborAttention(torch.nn.Module):
         which is built in the backward pass (with a synchronisation: not while a graph is captured) if it is not given.
         Indices out of range are reported like those of `conv_uvu` and their edges left out.
         """
+        if transpose is not None and len(transpose) != 2:
+            torch._assert(False, "Incorrect shape for transpose")
+        tensors = (q, k, v, bias, edge_weight, rowptr, edge_src, perm, buckets, *(transpose or (None, None)))
+        if _lib.wants_function(q, k, v, bias, edge_weight):
+            out = _AttentionFunction.apply(self, *tensors)
+        else:
+            out = _attend(self._checked(*tensors), False)[0]
+        if check_indices:
+            _lib.check_status(q.device, "NeighborAttention")
+        return out
+
+    def _checked(self, q, k, v, bias, edge_weight, rowptr, edge_src, perm, buckets, perm_t, rowptr_t) -> _Call:
         buffers = self._buffers
-        _lib.require_same_device(q, k, v, rowptr, edge_src, perm, bias, buckets, edge_weight, *(transpose or ()))
+        _lib.require_same_device(q, k, v, rowptr, edge_src, perm, bias, buckets, edge_weight, perm_t, rowptr_t)
         if buffers["_qk1"].get_device() != q.get_device():
             raise RuntimeError(f"Expected all tensors to be on the same device, but NeighborAttention's tables are on {buffers['_qk1'].device} and q is on "
                                f"{q.device} (move the module with .to(device))")
         _lib.element_type(q, "q")
         if not q.dtype == k.dtype == v.dtype:
             raise TypeError(f"q, k and v must have one type, got {q.dtype}, {k.dtype} and {v.dtype}")
-        for t, name in ((rowptr, "rowptr"), (edge_src, "edge_src"), (perm, "perm"), *((t, "transpose") for t in transpose or ())):
+        for t, name in ((rowptr, "rowptr"), (edge_src, "edge_src"), (perm, "perm"), (perm_t, "transpose"), (rowptr_t, "transpose")):
             if t is not None and (t.dtype != torch.int64 or t.dim() != 1):
                 if t.dtype != torch.int64:
                     raise TypeError(f"{name} must be int64")
@@ -202,7 +219,7 @@ class NeighborAttention(torch.nn.Module):
             ("perm", perm is not None and perm.shape[0] != E), ("buckets", buckets is not None and buckets.shape != (E,)),
             ("bias", bias is not None and (bias.dim() != 2 or bias.shape[1] != H or (buckets is None and bias.shape[0] != E))),
             ("edge_weight", edge_weight is not None and edge_weight.shape != (E,)),
-            ("transpose", transpose is not None and (len(transpose) != 2 or transpose[0].shape[0] != E or transpose[1].shape[0] != S + 1))) if bad]
+            ("transpose", (perm_t is None) != (rowptr_t is None) or (perm_t is not None and (perm_t.shape[0] != E or rowptr_t.shape[0] != S + 1)))) if bad]
         if wrong:
             torch._assert(False, f"Incorrect shape for {wrong[0]}")
         if buckets is not None:
@@ -216,25 +233,19 @@ class NeighborAttention(torch.nn.Module):
         if max(E, N, S) >= 2 ** 31 - 1:
             raise NotImplementedError("at most 2^31 - 2 edges and rows")
         _lib.check_earlier(q)
-        q, k, v = _rows(q), _rows(k), _rows(v)
         c = _Call()
+        c.q, c.k, c.v = _rows(q), _rows(k), _rows(v)
         # vectors of 16 bytes where the layout and the rows allow them, else of four elements, else single elements
         for c.vec in (4, 1) if q.dtype == torch.float32 else (8, 4, 1):
-            if c.vec in self._layouts and _fits(q, c.vec) and _fits(k, c.vec) and _fits(v, c.vec):
+            if c.vec in self._layouts and _fits(c.q, c.vec) and _fits(c.k, c.vec) and _fits(c.v, c.vec):
                 break
         c.layout, c.qk_tbl, c.v_tbl = self._layouts[c.vec], buffers[f"_qk{c.vec}"], buffers[f"_v{c.vec}"]
         c.scale, c.edges = self.scale, E
-        c.rowptr, c.src, c.perm, c.buckets = (t if t is None or t.is_contiguous() else t.contiguous() for t in (rowptr, edge_src, perm, buckets))
-        c.transpose = None if transpose is None else (transpose[0].contiguous(), transpose[1].contiguous())
-        bias = None if bias is None else bias.to(torch.float32).contiguous()
-        weight = None if edge_weight is None else edge_weight.to(torch.float32).contiguous()
-        if _lib.wants_function(q, k, v, bias, weight):
-            out = _AttentionFunction.apply(q, k, v, bias, weight, c)
-        else:
-            out = _attend(q, k, v, bias, weight, c, False)[0]
-        if check_indices:
-            _lib.check_status(q.device, "NeighborAttention")
-        return out
+        c.rowptr, c.src, c.perm, c.buckets, c.perm_t, c.rowptr_t = (t if t is None or t.is_contiguous() else t.contiguous()
+                                                                    for t in (rowptr, edge_src, perm, buckets, perm_t, rowptr_t))
+        c.bias = None if bias is None else bias.to(torch.float32).contiguous()
+        c.weight = None if edge_weight is None else edge_weight.to(torch.float32).contiguous()
+        return c
 
 
 class AttentionBlock(torch.nn.Module):

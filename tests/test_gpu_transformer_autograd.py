@@ -65,7 +65,7 @@ def test_a_tangent_of_a_table_is_not_lost():
             mod(buckets)
 
 
-@pytest.mark.parametrize("name", NAMES[:3])
+@pytest.mark.parametrize("name", NAMES)
 @pytest.mark.parametrize("recorded", [False, True])
 def test_a_traced_module_computes(name, recorded):
     mod, inputs, others = modules()[name]
@@ -100,3 +100,34 @@ def test_traced_buckets_and_bias():
         for a, b in zip(traced(*args), mod(*args)):
             assert torch.equal(a, b)
     e3nn_b200.check_status()
+
+
+@pytest.mark.parametrize("changed", ["rowptr", "src", "perm", "buckets", "transpose", "q", "bias"])
+def test_what_the_backward_pass_reads_again_may_not_change(changed):
+    gen = torch.Generator().manual_seed(2)
+    N, E, S = 4, 12, 5
+    mod = bnn.NeighborAttention("4x0e+4x1o", "4x0e+4x1o", 2).cuda()
+    q, k, v = (torch.randn(n, 16, generator=gen).cuda().requires_grad_() for n in (N, S, S))
+    bias = torch.randn(6, 2, generator=gen).cuda().requires_grad_()
+    src, perm, buckets = torch.randint(S, (E,), generator=gen).cuda(), torch.randperm(E, generator=gen).cuda(), torch.randint(6, (E,), generator=gen).int().cuda()
+    rowptr = torch.tensor([0, 3, 3, 8, E]).cuda()
+    transpose = e3nn_b200.csr_from_dst(src, S)
+    out = mod(q, k, v, rowptr, src, perm=perm, bias=bias, buckets=buckets, transpose=transpose)
+    out.sum().backward(retain_graph=True)
+    with torch.no_grad():
+        {"rowptr": rowptr, "src": src, "perm": perm, "buckets": buckets, "transpose": transpose[0], "q": q, "bias": bias}[changed].zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
+def test_gradients_come_in_the_types_of_the_inputs():
+    gen = torch.Generator().manual_seed(3)
+    mod = bnn.NeighborAttention("4x0e+4x1o", "4x0e+4x1o", 2).cuda()
+    q, k, v = (torch.randn(3, 16, generator=gen).cuda().requires_grad_() for _ in range(3))
+    bias, weight = torch.randn(3, 2, generator=gen).cuda().bfloat16().requires_grad_(), torch.rand(3, generator=gen).cuda().half().requires_grad_()
+    rowptr = torch.tensor([0, 0, 1, 3]).cuda()
+    grads = torch.autograd.grad(mod(q, k, v, rowptr, bias=bias, edge_weight=weight).pow(2).sum(), (bias, weight))
+    exact = [t.detach().float().requires_grad_() for t in (bias, weight)]
+    full = torch.autograd.grad(mod(q, k, v, rowptr, bias=exact[0], edge_weight=exact[1]).pow(2).sum(), exact)
+    for a, b, t in zip(grads, full, (bias, weight)):
+        assert a.dtype == t.dtype and torch.equal(a, b.to(t.dtype))
