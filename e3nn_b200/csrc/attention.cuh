@@ -8,7 +8,7 @@
 // The host's table gives, per vector of a head, {column of head 0, distance between heads}.
 //
 // Parts.  Rows differ in length (an isolated atom, a hub, one query over a long list), so the unit is not the row: the edges of row
-// n followed by one item for its end, row after row, are numbered, item (rowptr[n + 1] + n) being the end of row n, and
+// n followed by one item for its end, row after row, are numbered (slots in front of the first row with it), item (rowptr[n + 1] + n) being the end of row n, and
 // every warp takes `per_part` consecutive items.  A row that lies inside one part is finished there.  Of a longer row each part
 // leaves its sums in scratch memory (slot 1: the row goes on in the next part; slot 0: it ended here) and a second
 // kernel adds them in the order of the parts.  The split depends on the sizes alone, so results do not depend on scheduling.
@@ -28,18 +28,19 @@ constexpr unsigned kAll = 0xffffffffu;
 
 // One row space (destinations of the edges, or their sources) and its split.
 struct Rows {
-    const int64_t* rowptr;   // [num + 1]; values are clamped to [0, edges], rowptr[0] is taken as 0
+    const int64_t* rowptr;   // [num + 1]; values are clamped to [0, edges]
     int64_t num, edges;
     int64_t per_part;        // items a warp takes
     int parts;
-    __device__ __forceinline__ int64_t begin(int64_t n) const { return n == 0 ? 0 : min(max(rowptr[n], int64_t{0}), edges); }
+    __device__ __forceinline__ int64_t begin(int64_t n) const { return min(max(rowptr[n], int64_t{0}), edges); }
     __device__ __forceinline__ int64_t end(int64_t n) const { return min(max(rowptr[n + 1], int64_t{0}), edges); }
 };
 
-// The slots and rows of one part: rows n0 .. n1 - 1 end in it, row n1 (if there is one) goes on; slots e0 .. e1 - 1, of which those
-// from `behind` on lie behind the last row.
+// The slots and rows of one part: rows n0 .. n1 - 1 end in it, row n1 (if there is one) goes on; slots first .. e1 - 1, of which those
+// before e0 lie in front of the first row (a row pointer may start anywhere: a range of rows of a larger graph) and those from
+// `behind` on behind the last.
 struct Part {
-    int64_t n0, n1, e0, e1, behind;
+    int64_t n0, n1, first, e0, e1, behind;
 };
 
 // First rows whose end lies at item d0 or later, and at d1 or later (num: none).  Half a warp looks for each, 16 probes a step.
@@ -57,8 +58,9 @@ __device__ __forceinline__ Part find_part(const Rows& r, int part) {
     Part p;
     p.n0 = __shfl_sync(kAll, lo, 0);
     p.n1 = max(__shfl_sync(kAll, lo, 16), p.n0);
-    p.e0 = min(max(d0 - p.n0, int64_t{0}), r.edges);
-    p.e1 = min(max(d1 - p.n1, p.e0), r.edges);
+    p.first = min(max(d0 - p.n0, int64_t{0}), r.edges);
+    p.e1 = min(max(d1 - p.n1, p.first), r.edges);
+    p.e0 = r.num > 0 && p.n0 == 0 ? min(max(p.first, r.begin(0)), p.e1) : p.first;
     p.behind = p.n1 < r.num ? p.e1 : min(max(r.num > 0 ? r.end(r.num - 1) : 0, p.e0), p.e1);
     return p;
 }

@@ -62,26 +62,30 @@ __device__ __forceinline__ float open_row(const BwdArgs& a, int64_t n, const int
     return head_sum(d, a.h.lanes);
 }
 
-// Slots behind the last row take part in nothing: their gradients are zero.
+// Slots in front of the first row and behind the last take part in nothing: their gradients are zero.
 template <typename T, int VEC, int V>
-__device__ __forceinline__ void clear_behind(const BwdArgs& a, const Part& range, const int (&cq)[V], const int (&cv)[V], int head, bool leads) {
-    if (range.behind >= range.e1) return;
+__device__ __forceinline__ void clear_outside(const BwdArgs& a, const Part& range, const int (&cq)[V], const int (&cv)[V], int head, bool leads) {
+    if (range.first >= range.e0 && range.behind >= range.e1) return;
     float zero[V][VEC];
 #pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) zero[j][i] = 0.0f;
-    for (int64_t slot = range.behind; slot < range.e1; ++slot) {
-        const int64_t e = a.e.perm ? a.e.perm[slot] : slot;
-        if (e < 0 || e >= a.e.edges) continue;
-        if (a.dst && blockIdx.y == 0 && (threadIdx.x & 31) == 0) a.dst[e] = -1;
-        if (leads && a.share) a.share_of(e)[head] = make_float2(0.0f, 0.0f);
-        if (leads && a.da) a.da[e * a.h.heads + head] = 0.0f;
-        if (a.grad_k) {
-            store_row<T, VEC, V>(static_cast<T*>(a.grad_k), e, a.h.dqk, cq, zero, 0.0f);
-            store_row<T, VEC, V>(static_cast<T*>(a.grad_v), e, a.h.dv, cv, zero, 0.0f);
+    auto clear = [&](int64_t from, int64_t to) {
+        for (int64_t slot = from; slot < to; ++slot) {
+            const int64_t e = a.e.perm ? a.e.perm[slot] : slot;
+            if (e < 0 || e >= a.e.edges) continue;
+            if (a.dst && blockIdx.y == 0 && (threadIdx.x & 31) == 0) a.dst[e] = -1;
+            if (leads && a.share) a.share_of(e)[head] = make_float2(0.0f, 0.0f);
+            if (leads && a.da) a.da[e * a.h.heads + head] = 0.0f;
+            if (a.grad_k) {
+                store_row<T, VEC, V>(static_cast<T*>(a.grad_k), e, a.h.dqk, cq, zero, 0.0f);
+                store_row<T, VEC, V>(static_cast<T*>(a.grad_v), e, a.h.dv, cv, zero, 0.0f);
+            }
         }
-    }
+    };
+    clear(range.first, range.e0);
+    clear(range.behind, range.e1);
 }
 
 template <typename T, int VEC, int V>
@@ -184,7 +188,7 @@ __global__ void __launch_bounds__(256) attn_bwd_dst_kernel(const BwdArgs a) {
                     ended = static_cast<int>(n);
                 }
             });
-        clear_behind<T, VEC, V>(a, range, cq, cv, head, leads);
+        clear_outside<T, VEC, V>(a, range, cq, cv, head, leads);
         if (blockIdx.y == 0 && lane == 0) a.parts.ended[part] = ended;
     }
     leave_part(a.merge, s, goes_on, part, a.r.parts, a.parts, a.h, cq, cv, head, leads, smem);
@@ -272,7 +276,7 @@ __global__ void __launch_bounds__(384, 1) attn_bwd_dst_ring_kernel(const BwdArgs
                     ended = static_cast<int>(n);
                 }
             });
-        clear_behind<T, VEC, V>(a, range, cq, cv, head, leads);
+        clear_outside<T, VEC, V>(a, range, cq, cv, head, leads);
         if (lane == 0) a.parts.ended[part] = ended;
     }
     leave_part(a.merge, s, goes_on, part, a.r.parts, a.parts, a.h, cq, cv, head, leads, reinterpret_cast<float*>(memory));

@@ -174,7 +174,8 @@ class NeighborAttention(torch.nn.Module):
 
         Edge slot ``s`` in ``[rowptr[n], rowptr[n+1])`` belongs to node ``n`` and is edge ``perm[s]`` (``s`` itself without ``perm``;
         `e3nn_b200.csr_from_dst` gives both).  ``edge_src [E]``: ``k`` and ``v`` are rows of nodes, edge ``e`` reads row ``edge_src[e]``;
-        without it they are rows of edges.  Slots from ``rowptr[N]`` on belong to no node.  A node without edges gets zeros.
+        without it they are rows of edges.  Slots before ``rowptr[0]`` and from ``rowptr[N]`` on belong to no node (``rowptr[a:b+1]`` gives
+        the nodes ``a .. b-1`` of a graph alone); their gradients are zero.  A node without edges gets zeros.
 
         ``bias``: ``[E, num_heads]``, or with ``buckets [E]`` (int32) a table ``[num_buckets, num_heads]`` (`RelativeBias`);
         an entry ``-inf`` of the former masks its edge for that head, whatever ``k`` and ``v`` hold there.  ``edge_weight [E]``

@@ -345,7 +345,7 @@ int e3b_relative_bias_bwd(const void* grad_bias, const int32_t* buckets, int num
  * Multi-head softmax attention over the incoming edges of every node (the transformer example of the reference,
  * docs/guide/transformer.rst, as one pass):
  *   a[e,h] = scale <q[n], k[r]>_h + bias[e,h] + log edge_weight[e],   out[n]_h = sum_e softmax_e(a[e,h]) v[r]_h
- * over the slots s of row n (rowptr[n] <= s < rowptr[n+1]; rowptr[0] is taken as 0), e = perm[s] (perm NULL: s), r = edge_src[e]
+ * over the slots s of row n (rowptr[n] <= s < rowptr[n+1]; rowptr[0] may be above 0), e = perm[s] (perm NULL: s), r = edge_src[e]
  * (edge_src NULL: e).  q [num_dst, .], k and v [num_src, .] of `type`, rows q_stride, k_stride, v_stride elements apart;
  * out [num_dst, dv] dense.  bias NULL, [num_edges, heads] (-inf: masked, k and v unread), or with buckets [num_edges] a table
  * [num_buckets, heads].  edge_weight NULL or [num_edges]; an edge with a weight <= 0 is left out and its rows are unread.

@@ -1,0 +1,98 @@
+"""NeighborAttention on layouts of every kind of kernel, against the formula in 64 bits with bounds on every number (attention_formula)."""
+import math
+
+import pytest
+import torch
+
+import e3nn_b200
+from attention_formula import compare, formula
+from e3nn_b200 import nn as bnn
+from e3nn_b200 import o3
+
+pytestmark = pytest.mark.gpu
+
+# layout, heads -> vector widths in fp32 and in 16 bits; 16-byte vectors (4, 8) travel in bulk copies, the others are loaded one by one
+LAYOUTS = {"bulk": ("16x0e+16x1o", 2, 4, 8), "bulk in fp32": ("8x0e+8x1o+8x2e", 2, 4, 4), "loads": ("6x0e+3x1o", 3, 1, 1)}
+DEGREES = {"ragged": [0, 3, 1, 0, 0, 37, 2, 5, 33, 0], "hub": [2, 1, 600, 0, 3] + [4] * 40, "one edge": [1] * 7}
+NAMES = ("q", "k", "v", "bias", "weight")
+
+
+def make(irreps, heads, degrees, dtype, per_edge, bias=None, weight=False, perm=False, sources=23, front=0, behind=0, seed=0):
+    """Edges of the rows, and `front` and `behind` edges that belong to no row."""
+    gen = torch.Generator().manual_seed(seed + heads + len(degrees))
+    N, E, D = len(degrees), front + sum(degrees) + behind, o3.Irreps(irreps).dim
+    S = E if per_edge else sources
+    t = {"rowptr": front + torch.tensor([0] + degrees).cumsum(0), "src": None if per_edge else torch.randint(S, (E,), generator=gen),
+         "perm": torch.randperm(E, generator=gen) if perm else None, "buckets": None, "bias": None, "weight": None}
+    for name, rows in (("q", N), ("k", S), ("v", S), ("g", N)):
+        t[name] = torch.randn(rows, D, generator=gen).to(dtype)
+    if bias == "table":
+        t["buckets"], t["bias"] = torch.randint(9, (E,), generator=gen, dtype=torch.int32), torch.randn(9, heads, generator=gen)
+    elif bias == "edges":
+        t["bias"] = torch.randn(E, heads, generator=gen)
+        t["bias"][torch.rand(E, heads, generator=gen) < 0.2] = -math.inf
+    if weight:
+        t["weight"] = 0.05 + 0.95 * torch.rand(E, generator=gen)
+        t["weight"][torch.rand(E, generator=gen) < 0.2] = 0.0
+    return {n: None if x is None else x.cuda() for n, x in t.items()}
+
+
+def module(layout, dtype, t):
+    irreps, heads, wide, narrow = LAYOUTS[layout]
+    mod = bnn.NeighborAttention(irreps, irreps, heads).cuda()
+    call = mod._checked(*(t[n] for n in ("q", "k", "v", "bias", "weight", "rowptr", "src", "perm", "buckets")), None, None)
+    assert call.vec == (wide if dtype == torch.float32 else narrow)
+    return mod
+
+
+def run(mod, t, transposed=True):
+    leaves = {n: t[n].detach().requires_grad_() for n in NAMES if t[n] is not None}
+    x = {**t, **leaves}
+    transpose = e3nn_b200.csr_from_dst(t["src"], t["k"].shape[0]) if t["src"] is not None and transposed else None
+    out = mod(x["q"], x["k"], x["v"], t["rowptr"], t["src"], perm=t["perm"], bias=x["bias"], buckets=t["buckets"], edge_weight=x["weight"], transpose=transpose)
+    grads = torch.autograd.grad(out, list(leaves.values()), t["g"])
+    return {"out": out.detach(), **dict(zip(leaves, grads))}
+
+
+def check(layout, t, dtype, sharp=0.25):
+    mod = module(layout, dtype, t)
+    got = run(mod, t)
+    compare(got, formula(*LAYOUTS[layout][:1], *LAYOUTS[layout][:2], t, dtype), sharp)
+    e3nn_b200.check_status()
+    return mod, got
+
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+@pytest.mark.parametrize("per_edge", [False, True])
+@pytest.mark.parametrize("perm", [False, True])
+def test_rows_in_a_window_of_the_edges(layout, per_edge, perm, dtype):
+    """A row pointer that starts above zero: slots before it belong to no row, whatever they hold."""
+    for front, behind in ((1, 0), (300, 0), (77, 250)):
+        t = make(*LAYOUTS[layout][:2], DEGREES["ragged"], dtype, per_edge, "table", True, perm, front=front, behind=behind)
+        _, got = check(layout, t, dtype)
+        if not per_edge or perm:
+            continue
+        outside = torch.ones(t["k"].shape[0], dtype=torch.bool, device="cuda")
+        outside[front:front + sum(DEGREES["ragged"])] = False
+        x = {n: None if y is None else y.clone() for n, y in t.items()}
+        for n in ("k", "v", "weight"):
+            x[n][outside] = float("nan")
+        again = run(module(layout, dtype, x), x)
+        assert all(torch.equal(again[n], got[n]) for n in got)
+        assert all(not got[n][outside].any() for n in ("k", "v", "weight"))
+
+
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+def test_nodes_of_a_graph_alone(layout):
+    """rowptr[a:b+1] gives the nodes a .. b-1 as the whole graph does."""
+    t = make(*LAYOUTS[layout][:2], DEGREES["hub"], torch.float32, False, "table", True)
+    whole = module(layout, torch.float32, t)(t["q"], t["k"], t["v"], t["rowptr"], t["src"], bias=t["bias"], buckets=t["buckets"], edge_weight=t["weight"])
+    for a, b in ((1, 4), (3, 20), (44, 45), (4, 4)):
+        x = {**t, "q": t["q"][a:b], "g": t["g"][a:b], "rowptr": t["rowptr"][a:b + 1]}
+        _, got = check(layout, x, torch.float32, None if a == b else 0.25)
+        want = formula(*LAYOUTS[layout][:1], *LAYOUTS[layout][:2], t, torch.float32)["out"]
+        assert ((got["out"].double() - whole[a:b].double()).abs() <= 2 * want[1][a:b]).all()
