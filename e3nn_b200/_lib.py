@@ -62,7 +62,7 @@ def require_cuda(*tensors: torch.Tensor) -> None:
 # ------------------------------------------------------------------------------------------- kernel status
 # Kernels report conditions they cannot raise themselves through a status word: 1 = a destination index out of range
 # (CSR builder), 2 = a source / edge index out of range (the access was skipped), 3 = a bounded wait on an mbarrier gave
-# up (the kernel returned early, its output is incomplete).  One word per device lives for the life of the process, in
+# up (the kernel returned early, its output is incomplete), 4 = a permutation names an edge twice.  One word per device lives for the life of the process, in
 # pinned host memory that the device addresses directly: a kernel writes it only when something is wrong, the next call
 # of any op on that device looks at it (no synchronisation while it is 0) and raises; `check_status` synchronises and raises.
 # A code stays until it is raised once: the word is cleared when the device is idle, because a launch that has reported one
@@ -109,6 +109,8 @@ def _raise_status(code: int, what: str) -> None:
         raise IndexError(f"{what}: a destination index was outside [0, num_nodes)")
     if code == 3:
         raise E3BError(f"{what}: a bounded wait inside a kernel gave up (status 3); the output of that launch is incomplete")
+    if code == 4:
+        raise IndexError(f"{what}: a permutation of edges names an edge twice (its gradients are those of one of the two)")
     raise E3BError(f"{what}: kernel status {code}")
 
 

@@ -20,7 +20,7 @@ struct BwdArgs {
     void *grad_q, *grad_k, *grad_v;      // grad_k, grad_v: per edge, or null
     float2* share;                       // [edges, even(heads)] {p, da} or null
     float* da;                           // [edges, heads] or null
-    int32_t* dst;                        // [edges] or null: destination of every edge
+    int32_t* dst;                        // [edges] or null: destination of every edge; with a permutation -1 beforehand
     float scale;
     Heads h;
     Edges e;
@@ -31,6 +31,11 @@ struct BwdArgs {
     int depth;
     uint32_t warp_smem;
     __device__ __forceinline__ float2* share_of(int64_t edge) const { return share + edge * ((h.heads + 1) & ~1); }
+    // Notes the destination of an edge.  A permutation may name an edge twice: two rows would write its gradients.
+    __device__ __forceinline__ void visit(int edge, int row) const {
+        if (!e.perm) dst[edge] = row;
+        else if (atomicCAS(dst + edge, -1, row) != -1) *e.status = 4;
+    }
 };
 
 // q, cotangent and statistics of a row; returns delta.  The output enters unrounded, in the order of the dots g v of the kernel (PAIRS: of
@@ -62,19 +67,19 @@ __device__ __forceinline__ float open_row(const BwdArgs& a, int64_t n, const int
     return head_sum(d, a.h.lanes);
 }
 
-// Slots in front of the first row and behind the last take part in nothing: their gradients are zero.
+// Slots in front of the first row and behind the last take part in nothing: their gradients are zero.  With a permutation the
+// edges that no row has visited are cleared afterwards (clear_unvisited_kernel): slots outside may name any edge, and not every
+// edge need be named.
 template <typename T, int VEC, int V>
 __device__ __forceinline__ void clear_outside(const BwdArgs& a, const Part& range, const int (&cq)[V], const int (&cv)[V], int head, bool leads) {
-    if (range.first >= range.e0 && range.behind >= range.e1) return;
+    if (a.e.perm || (range.first >= range.e0 && range.behind >= range.e1)) return;
     float zero[V][VEC];
 #pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) zero[j][i] = 0.0f;
     auto clear = [&](int64_t from, int64_t to) {
-        for (int64_t slot = from; slot < to; ++slot) {
-            const int64_t e = a.e.perm ? a.e.perm[slot] : slot;
-            if (e < 0 || e >= a.e.edges) continue;
+        for (int64_t e = from; e < to; ++e) {
             if (a.dst && blockIdx.y == 0 && (threadIdx.x & 31) == 0) a.dst[e] = -1;
             if (leads && a.share) a.share_of(e)[head] = make_float2(0.0f, 0.0f);
             if (leads && a.da) a.da[e * a.h.heads + head] = 0.0f;
@@ -119,7 +124,7 @@ __global__ void __launch_bounds__(256) attn_bwd_dst_kernel(const BwdArgs a) {
                 for (int64_t base = first; base < last; base += 32) {
                     EdgeMeta meta;
                     meta.load(a.e, base + lane, last);
-                    if (a.dst && blockIdx.y == 0 && meta.edge >= 0) a.dst[meta.edge] = row_now;
+                    if (a.dst && blockIdx.y == 0 && meta.edge >= 0) a.visit(meta.edge, row_now);
                     const int count = static_cast<int>(min(last - base, int64_t{32}));
                     for (int u0 = 0; u0 < count; u0 += U) {
                         Packed<T, VEC> kk[U][V], vv[U][V];
@@ -223,7 +228,7 @@ __global__ void __launch_bounds__(384, 1) attn_bwd_dst_ring_kernel(const BwdArgs
                 s.clear();
             },
             [&](const EdgeMeta& meta, int at, int m) {
-                if (a.dst && lane >= at && lane < at + m && meta.edge >= 0) a.dst[meta.edge] = row_now;
+                if (a.dst && lane >= at && lane < at + m && meta.edge >= 0) a.visit(meta.edge, row_now);
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     const int from = (at + u) & 31;
@@ -295,6 +300,25 @@ __global__ void __launch_bounds__(512) attn_bwd_dst_join_kernel(const BwdArgs a)
     if (join_parts(s, a.r, blockIdx.x, a.parts, a.h, cq, cq, head, live, smem, &n)) store_row<T, VEC, V>(static_cast<T*>(a.grad_q), n, a.h.dqk, cq, s.a[0], a.scale);
 }
 
+// Gradients of the edges that no row has visited (dst -1) are zero.  A warp looks at 32 edges.
+template <typename T>
+__global__ void __launch_bounds__(256) clear_unvisited_kernel(const int32_t* __restrict__ dst, int64_t edges, int heads, int dqk, int dv, float* __restrict__ da,
+                                                              T* __restrict__ grad_k, T* __restrict__ grad_v) {
+    const int lane = threadIdx.x & 31;
+    const int64_t warps = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
+    for (int64_t base = (static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5)) * 32; base < edges; base += warps * 32) {
+        unsigned left = __ballot_sync(kAll, base + lane < edges && dst[base + lane] < 0);
+        for (; left; left &= left - 1) {
+            const int64_t e = base + __ffs(left) - 1;
+            if (da)
+                for (int i = lane; i < heads; i += 32) da[e * heads + i] = 0.0f;
+            if (!grad_k) continue;
+            for (int i = lane; i < dqk; i += 32) grad_k[e * dqk + i] = from_float<T>(0.0f);
+            for (int i = lane; i < dv; i += 32) grad_v[e * dv + i] = from_float<T>(0.0f);
+        }
+    }
+}
+
 // Gradient of the weight of every edge: share / weight = exp(logit without it) / sum, so it is sum_h da / weight; an edge that was
 // left out has none.
 __global__ void __launch_bounds__(256) attn_weight_grad_kernel(const float* __restrict__ da, const float* __restrict__ weight, int heads,
@@ -332,7 +356,8 @@ extern "C" int e3b_attention_bwd(const void* q, const void* k, const void* v, co
     if (heads < 1 || (vec != 1 && vec != 4 && (vec != 8 || type == kFloat32))) return fail(E3B_ERR_ARG, "attention_bwd: bad head layout");
     if (num_dst == 0 && num_edges == 0) return E3B_OK;
     if ((num_dst > 0 && (!q || !grad_out || !out32 || !stats || !grad_q)) || !rowptr || (num_edges > 0 && num_src > 0 && (!k || !v)) || !qk_table ||
-        !v_table || !scratch || !status || (share && !aligned_to(share, 16)) || (buckets && !bias) || !grad_k != !grad_v || (grad_weight && (!edge_weight || !grad_logit)))
+        !v_table || !scratch || !status || (share && !aligned_to(share, 16)) || (buckets && !bias) || !grad_k != !grad_v || (grad_weight && (!edge_weight || !grad_logit)) ||
+        (perm && num_edges > 0 && (share || grad_logit || grad_k) && !edge_dst))
         return fail(E3B_ERR_ARG, "attention_bwd: null pointer");
     if (scratch_bytes < e3b_attention_bwd_scratch_bytes(num_dst, num_edges, dqk))
         return fail(E3B_ERR_ARG, "attention_bwd: scratch of %lld bytes is too small", static_cast<long long>(scratch_bytes));
@@ -349,6 +374,7 @@ extern "C" int e3b_attention_bwd(const void* q, const void* k, const void* v, co
               {rowptr, num_dst, num_edges, s.per_part, s.parts}, partials_in(scratch, s.parts, dq_slot(dqk)), s.merge, rows, p.depth,
               static_cast<uint32_t>(p.warp_smem)};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (perm && edge_dst) E3B_CUDA_TRY(cudaMemsetAsync(edge_dst, 0xff, sizeof(int32_t) * num_edges, st));      // all -1
     const int rc = by_type_and_vectors(type, vec, p.v, [&](auto t0, auto vec0, auto v0) -> int {
         using T = decltype(t0);
         constexpr int VEC = decltype(vec0)::value, V = decltype(v0)::value;
@@ -373,7 +399,20 @@ extern "C" int e3b_attention_bwd(const void* q, const void* k, const void* v, co
         attn_bwd_dst_join_kernel<T, VEC, V><<<dim3(s.parts, p.groups), 32 * s.join_warps, smem, st>>>(a);
         return check_launch("attention_bwd join");
     });
-    if (rc != E3B_OK || !grad_weight || num_edges == 0) return rc;
+    if (rc != E3B_OK || num_edges == 0) return rc;
+    if (perm && (grad_logit || grad_k)) {
+        const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ceil_div(num_edges, 256), kNumSMs * 8));
+        auto clear = [&](auto t0) {
+            using T = decltype(t0);
+            clear_unvisited_kernel<T><<<grid, 256, 0, st>>>(edge_dst, num_edges, heads, dqk, dv, grad_logit, static_cast<T*>(grad_k), static_cast<T*>(grad_v));
+        };
+        if (type == kFloat32) clear(float());
+        else if (type == kBFloat16) clear(__nv_bfloat16());
+        else clear(__half());
+        const int cleared = check_launch("attention_bwd edges of no row");
+        if (cleared != E3B_OK) return cleared;
+    }
+    if (!grad_weight) return E3B_OK;
     attn_weight_grad_kernel<<<static_cast<unsigned>(std::min<int64_t>(ceil_div(num_edges, 256), kNumSMs * 8)), 256, 0, st>>>(
         grad_logit, edge_weight, heads, num_edges, grad_weight);
     return check_launch("attention_bwd weights");

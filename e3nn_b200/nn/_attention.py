@@ -102,7 +102,8 @@ class _AttentionFunction(torch.autograd.Function):
         gv = torch.empty(S, dv, dtype=q.dtype, device=dev) if need_k or need_v else None
         share = torch.empty(E, (H + 1) // 2 * 2, 2, dtype=torch.float32, device=dev) if per_node else None
         da = torch.empty(E, H, dtype=torch.float32, device=dev) if need_bias or need_weight else None
-        dst = torch.empty(E, dtype=torch.int32, device=dev) if per_node else None
+        # with a permutation the call finds the edges of no row by it
+        dst = torch.empty(E, dtype=torch.int32, device=dev) if per_node or (perm is not None and (per_edge or da is not None)) else None
         gweight = torch.empty(E, dtype=torch.float32, device=dev) if need_weight else None
         nbytes = core.e3b_attention_bwd_scratch_bytes(N, E, dqk)
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
@@ -185,7 +186,9 @@ class NeighborAttention(torch.nn.Module):
         Statistics and sums are fp32.  Gradients (first order, fixed order of summation) of ``q``, ``k``, ``v``, ``bias`` and ``edge_weight``;
         those of node-wise ``k`` and ``v`` need the edges by source, ``transpose = csr_from_dst(edge_src, k.shape[0])``,
         which is built in the backward pass (with a synchronisation: not while a graph is captured) if it is not given.
-        Indices out of range are reported like those of `conv_uvu` and their edges left out.
+        Indices out of range are reported like those of `conv_uvu` and their edges left out.  ``rowptr`` must not decrease.  ``perm`` may
+        leave out edges (their gradients are zero) and name any edge in slots of no node, but none twice in slots of nodes: the
+        forward pass would count it twice, the backward pass reports it.
         """
         if transpose is not None and len(transpose) != 2:
             torch._assert(False, "Incorrect shape for transpose")

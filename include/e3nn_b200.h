@@ -359,8 +359,8 @@ int e3b_relative_bias_bwd(const void* grad_bias, const int32_t* buckets, int num
  *
  * e3b_attention_bwd: grad_q [num_dst, dqk]; k and v per edge (edge_src NULL): grad_k, grad_v per edge (both or neither).  Optional, per
  * edge: share [num_edges, heads rounded up to even, 2] {softmax, its gradient's logit part} (16-byte aligned), grad_logit [num_edges, heads]
- * (the gradient of bias), edge_dst [num_edges] (destination, -1: none),
- * grad_weight [num_edges] (needs grad_logit).
+ * (the gradient of bias), edge_dst [num_edges] (destination, -1: none; needed with share and, where perm is given, with any of the others:
+ * an edge that perm does not name in a row gets zeros, one that it names twice sets *status = 4), grad_weight [num_edges] (needs grad_logit).
  * e3b_attention_bwd_src: grad_k and grad_v of nodes from share and edge_dst and the CSR by source (e3b_csr_from_dst of
  * edge_src: src_perm, src_rowptr).  All sums have a fixed order.
  */

@@ -96,3 +96,58 @@ def test_nodes_of_a_graph_alone(layout):
         _, got = check(layout, x, torch.float32, None if a == b else 0.25)
         want = formula(*LAYOUTS[layout][:1], *LAYOUTS[layout][:2], t, torch.float32)["out"]
         assert ((got["out"].double() - whole[a:b].double()).abs() <= 2 * want[1][a:b]).all()
+
+
+def fill_free_memory():
+    """NaN in what the allocator hands out next: an element that no kernel writes shows."""
+    junk = [torch.full((n,), float("nan"), device="cuda") for n in [64, 256, 1024, 4096, 16384, 65536] * 40]
+    del junk
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+@pytest.mark.parametrize("per_edge", [False, True])
+def test_edges_that_a_permutation_leaves_out(layout, per_edge, dtype):
+    """Bad entries, and a padded permutation whose last slots name any edge: an edge of no row has zeros for gradients, the others are
+    what they are without it."""
+    degrees = DEGREES["ragged"]
+    E = sum(degrees)
+    t = make(*LAYOUTS[layout][:2], degrees, dtype, per_edge, "edges", True, True, behind=40)
+    t["bias"].clamp_(min=-2.0)
+    t["weight"].fill_(1.0)
+    mod = module(layout, dtype, t)
+    zeros = {**t, "perm": t["perm"].clone()}
+    zeros["perm"][E:] = t["perm"][0]                       # padding that names an edge of the rows
+    fill_free_memory()
+    got = run(mod, zeros)
+    compare(got, formula(*LAYOUTS[layout][:1], *LAYOUTS[layout][:2], zeros, dtype))
+    want = run(mod, t)
+    assert all(torch.equal(got[n], want[n]) for n in got)
+    e3nn_b200.check_status()
+
+    bad = torch.tensor([4, 30, 31, E - 1], device="cuda")
+    without = {**t, "weight": t["weight"].clone()}
+    without["weight"][t["perm"][bad]] = 0.0
+    want = run(mod, without)
+    out_of_range = {**t, "perm": t["perm"].clone()}
+    out_of_range["perm"][bad] = torch.tensor([-1, E + 40, 2 ** 40, -2 ** 40], device="cuda")
+    for _ in range(3):
+        fill_free_memory()
+        got = run(mod, out_of_range)
+        with pytest.raises(IndexError):
+            e3nn_b200.check_status()
+        for n in got:
+            assert torch.equal(got[n], want[n]), n
+
+
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+@pytest.mark.parametrize("per_edge", [False, True])
+def test_an_edge_named_twice_is_reported_by_the_backward_pass(layout, per_edge):
+    t = make(*LAYOUTS[layout][:2], DEGREES["hub"], torch.float32, per_edge, "table", False, True)
+    mod = module(layout, torch.float32, t)
+    run(mod, t)
+    e3nn_b200.check_status()
+    t["perm"][3] = t["perm"][650]
+    run(mod, t)
+    with pytest.raises(IndexError, match="twice"):
+        e3nn_b200.check_status()
