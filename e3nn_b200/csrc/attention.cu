@@ -125,6 +125,7 @@ __global__ void __launch_bounds__(256) attn_fwd_kernel(const FwdArgs a) {
 #pragma unroll
                         for (int u = 0; u < U; ++u) {
                             const float w = __expf(dot[u] - ref);
+                            if (w == 0.0f) continue;      // as in the ring: it adds nothing, whatever v holds
                             s.l += w;
 #pragma unroll
                             for (int j = 0; j < V; ++j) {

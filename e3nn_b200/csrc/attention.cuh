@@ -186,7 +186,7 @@ __device__ __forceinline__ void store_row(T* __restrict__ base, int64_t row, int
         if (col[j] < 0) continue;
         float o[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) o[i] = f[j][i] * by;
+        for (int i = 0; i < VEC; ++i) o[i] = by == 0.0f ? 0.0f : f[j][i] * by;      // (a share of zero: whatever the row holds)
         Packed<T, VEC>::store(base + row * stride + col[j], o);
     }
 }

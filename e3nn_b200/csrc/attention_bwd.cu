@@ -168,10 +168,12 @@ __global__ void __launch_bounds__(256) attn_bwd_dst_kernel(const BwdArgs a) {
                                 p = __expf(x - top) * inv;
                                 da = p == 0.0f ? 0.0f : p * (dp - delta);
                             }
+                            if (da != 0.0f) {
 #pragma unroll
-                            for (int j = 0; j < V; ++j)
+                                for (int j = 0; j < V; ++j)
 #pragma unroll
-                                for (int i = 0; i < VEC; ++i) s.a[0][j][i] = fmaf(da, kf[j][i], s.a[0][j][i]);
+                                    for (int i = 0; i < VEC; ++i) s.a[0][j][i] = fmaf(da, kf[j][i], s.a[0][j][i]);
+                            }
                             if (edge[u] < 0) continue;
                             if (leads && a.share) a.share_of(edge[u])[head] = make_float2(p, da);
                             if (leads && a.da) a.da[static_cast<int64_t>(edge[u]) * a.h.heads + head] = da;

@@ -92,9 +92,9 @@ __global__ void __launch_bounds__(256) attn_bwd_src_kernel(const SrcArgs a) {
                                 qq[u][j].unpack(x);
                                 gg[u][j].unpack(y);
 #pragma unroll
-                                for (int i = 0; i < VEC; ++i) {
-                                    s.a[0][j][i] = fmaf(da[u], x[i], s.a[0][j][i]);
-                                    s.a[1][j][i] = fmaf(p[u], y[i], s.a[1][j][i]);
+                                for (int i = 0; i < VEC; ++i) {      // (a share of zero adds nothing, whatever q and the cotangent hold)
+                                    if (da[u] != 0.0f) s.a[0][j][i] = fmaf(da[u], x[i], s.a[0][j][i]);
+                                    if (p[u] != 0.0f) s.a[1][j][i] = fmaf(p[u], y[i], s.a[1][j][i]);
                                 }
                             }
                         }

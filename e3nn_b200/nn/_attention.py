@@ -181,7 +181,8 @@ class NeighborAttention(torch.nn.Module):
         ``bias``: ``[E, num_heads]``, or with ``buckets [E]`` (int32) a table ``[num_buckets, num_heads]`` (`RelativeBias`);
         an entry ``-inf`` of the former masks its edge for that head, whatever ``k`` and ``v`` hold there.  ``edge_weight [E]``
         multiplies the exponentials (a smooth cutoff); an edge with weight zero or below is left out, its rows are not read
-        and its gradients, that of the weight included, are zero.
+        and its gradients, that of the weight included, are zero.  So does an edge whose share is zero in fp32 (below 2^-126): it adds
+        nothing to any sum, infinities and NaN in its ``v`` or in the cotangent of its row included.
 
         Statistics and sums are fp32.  Gradients (first order, fixed order of summation) of ``q``, ``k``, ``v``, ``bias`` and ``edge_weight``;
         those of node-wise ``k`` and ``v`` need the edges by source, ``transpose = csr_from_dst(edge_src, k.shape[0])``,

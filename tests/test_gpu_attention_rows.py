@@ -151,3 +151,67 @@ def test_an_edge_named_twice_is_reported_by_the_backward_pass(layout, per_edge):
     run(mod, t)
     with pytest.raises(IndexError, match="twice"):
         e3nn_b200.check_status()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+@pytest.mark.parametrize("per_edge", [False, True])
+@pytest.mark.parametrize("mask", ["weight", "bias", "share"])
+def test_what_a_masked_edge_may_lie_next_to(layout, per_edge, mask, dtype):
+    """Row 5 holds infinities or NaN in q and in its cotangent, and masked edges: these, and sources that only they lead to, have zeros
+    for gradients.  Masked: by weight, by bias, or by a bias so low that the share is zero in fp32."""
+    degrees = DEGREES["ragged"]
+    t = make(*LAYOUTS[layout][:2], degrees, dtype, per_edge, "edges" if mask != "weight" else None, mask == "weight", sources=60)
+    row = torch.arange(int(t["rowptr"][5]), int(t["rowptr"][6]), device="cuda")
+    masked = row[::2]
+    if t["src"] is not None:                               # sources of their own
+        t["src"] %= 30
+        t["src"][masked] = 30 + torch.arange(len(masked), device="cuda")
+    if mask == "weight":
+        t["weight"][row] = 0.5
+        t["weight"][masked] = 0.0
+    else:
+        t["bias"].clamp_(min=-2.0)
+        t["bias"][masked] = -math.inf if mask == "bias" else -1000.0
+    mod = module(layout, dtype, t)
+    clean = run(mod, t)
+    reached = masked if per_edge else t["src"][masked]
+    for value in (float("inf"), float("nan")):
+        for name in ("g",) if mask == "share" else ("g", "q"):      # (of a NaN in q nothing is masked by a low bias)
+            x = {**t, name: t[name].clone()}
+            x[name][5] = value
+            got = run(mod, x)
+            for n in ("k", "v"):
+                assert not got[n][reached].any(), (name, n)
+            if mask != "weight":
+                assert not got["bias"][masked].any()
+            else:
+                assert not got["weight"][masked].any()
+            others = [n for n in range(len(degrees)) if n != 5]
+            assert torch.equal(got["out"][others], clean["out"][others]) and torch.equal(got["q"][others], clean["q"][others])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+@pytest.mark.parametrize("per_edge", [False, True])
+def test_a_share_of_zero_adds_nothing(layout, per_edge, dtype):
+    """Infinities and NaN in v (and, for the gradients of others, in k) behind a share that is zero in fp32: as without the edge."""
+    degrees = DEGREES["ragged"]
+    t = make(*LAYOUTS[layout][:2], degrees, dtype, per_edge, "edges", sources=60)
+    edges = torch.tensor([0, 5, 20, 60], device="cuda")
+    rows = edges
+    if t["src"] is not None:
+        t["src"] %= 30
+        rows = t["src"][edges] = 30 + torch.arange(4, device="cuda")
+    t["bias"].clamp_(min=-2.0)
+    mod = module(layout, dtype, t)
+    gone = {**t, "bias": t["bias"].clone()}
+    gone["bias"][edges] = -math.inf
+    want = run(mod, gone)
+    t["bias"][edges] = torch.finfo(torch.float32).min
+    for value in (float("inf"), -float("inf"), float("nan")):
+        x = {**t, "v": t["v"].clone()}
+        x["v"][rows] = value
+        got = run(mod, x)
+        for n in got:
+            assert torch.equal(got[n], want[n]), n
