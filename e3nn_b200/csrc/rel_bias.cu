@@ -21,7 +21,8 @@ namespace e3b {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxBuckets = 1024;
+constexpr int kMaxBuckets = 1024;      // of the distance buckets (their thresholds lie in shared memory); a table may have more
+constexpr int64_t kMostCells = INT32_MAX - 32;      // of a table
 constexpr int kSumThreads = 512;       // of a block of the table gradient, at most
 
 __global__ void __launch_bounds__(kThreads) distance_buckets_kernel(const float* __restrict__ pos, const int64_t* __restrict__ src,
@@ -103,14 +104,14 @@ __global__ void __launch_bounds__(kThreads) bias_fwd_kernel(const T* __restrict_
 }
 
 // Thread t of a block: HV heads from HV (t % lanes) on (lanes = width / HV), slice t / lanes; its block's edges in turns of `slices`.
-// Shared memory: [slices][num_buckets][width].
+// Shared memory: [slices][window][width]: the buckets from blockIdx.z * window on (all of them, unless the table is large).
 template <typename T, int HV>
 __global__ void __launch_bounds__(kSumThreads, 1) bias_bwd_kernel(const T* __restrict__ grad, const int32_t* __restrict__ buckets, int num_buckets,
-                                                                  int heads, int width, int slices, int64_t edges, int64_t edges_per_block,
+                                                                  int window, int heads, int width, int slices, int64_t edges, int64_t edges_per_block,
                                                                   float* __restrict__ partial, int32_t* status) {
     extern __shared__ __align__(16) float acc[];
     const int lanes = width / HV, h = threadIdx.x % lanes * HV, slice = threadIdx.x / lanes, head = blockIdx.y * width + h;
-    const int cells = num_buckets * width;
+    const int first = blockIdx.z * window, here = min(window, num_buckets - first), cells = here * width;
     for (int i = threadIdx.x; i < slices * cells; i += blockDim.x) acc[i] = 0.0f;
     __syncthreads();
     const int64_t begin = static_cast<int64_t>(blockIdx.x) * edges_per_block;
@@ -133,18 +134,19 @@ __global__ void __launch_bounds__(kSumThreads, 1) bias_bwd_kernel(const T* __res
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (e0 + u * slices >= count) break;
-                if (b[u] < 0 || b[u] >= num_buckets) {
-                    bad = true;
+                const int at = b[u] - first;
+                if (static_cast<unsigned>(at) >= static_cast<unsigned>(here)) {
+                    bad = bad || b[u] < 0 || b[u] >= num_buckets;
                     continue;
                 }
                 float x[HV], y[HV];
                 Packed<float, HV> sum;
-                sum.load(mine + b[u] * width);
+                sum.load(mine + at * width);
                 sum.unpack(x);
                 g[u].unpack(y);
 #pragma unroll
                 for (int i = 0; i < HV; ++i) x[i] += y[i];
-                Packed<float, HV>::store(mine + b[u] * width, x);
+                Packed<float, HV>::store(mine + at * width, x);
             }
         }
         if (bad) *status = 2;
@@ -155,7 +157,7 @@ __global__ void __launch_bounds__(kSumThreads, 1) bias_bwd_kernel(const T* __res
         if (static_cast<int>(blockIdx.y) * width + hh >= heads) continue;
         float s = 0.0f;
         for (int k = 0; k < slices; ++k) s += acc[k * cells + i];
-        partial[(static_cast<int64_t>(blockIdx.x) * num_buckets + b) * heads + blockIdx.y * width + hh] = s;
+        partial[(static_cast<int64_t>(blockIdx.x) * num_buckets + first + b) * heads + blockIdx.y * width + hh] = s;
     }
 }
 
@@ -176,10 +178,10 @@ __global__ void __launch_bounds__(1024) bias_sum_kernel(const float* __restrict_
     if (threadIdx.x == 0 && cell < cells) out[cell] = from_float<T>(t);
 }
 
-// How the table gradient is split: heads a thread and a block take, slices of a block's edges, thread blocks.  The tables of the
+// How the table gradient is split: heads a thread and a block take, buckets and slices of edges of a block, thread blocks.  The tables of the
 // slices fill the shared memory of an SM; a wide vector of heads a thread keeps the loads in flight when that leaves few threads.
 struct BiasSplit {
-    int vec, width, slices, groups, parts;
+    int vec, width, slices, groups, parts, window;
     int64_t per_block;
     size_t smem;
 };
@@ -188,8 +190,8 @@ BiasSplit bias_split(int64_t edges, int heads, int num_buckets, int element) {
     constexpr size_t kMostSmem = 208 * 1024;
     s.vec = element == 2 && heads % 8 == 0 ? 8 : heads % 4 == 0 ? 4 : 1;
     s.width = std::min(heads, 32);
-    while (s.width > s.vec && sizeof(float) * num_buckets * s.width > kMostSmem) s.width = static_cast<int>(ceil_div(s.width / 2, s.vec)) * s.vec;
-    const size_t table = sizeof(float) * num_buckets * s.width;
+    s.window = static_cast<int>(std::min<size_t>(num_buckets, kMostSmem / (sizeof(float) * s.width)));      // every block reads the buckets of its edges, whatever its window
+    const size_t table = sizeof(float) * s.window * s.width;
     s.groups = static_cast<int>(ceil_div(heads, s.width));
     // a block clears, sums and writes its tables: every slice takes at least some edges
     const int64_t a_block = ceil_div(edges, kNumSMs);
@@ -226,8 +228,10 @@ int bias_bwd(const void* grad, const int32_t* buckets, int num_buckets, int head
         constexpr int HV = decltype(v0)::value;
         const int allowed = allow_smem(bias_bwd_kernel<T, HV>, s.smem);
         if (allowed != E3B_OK) return allowed;
-        bias_bwd_kernel<T, HV><<<dim3(s.parts, s.groups), s.width / HV * s.slices, s.smem, st>>>(
-            static_cast<const T*>(grad), buckets, num_buckets, heads, s.width, s.slices, edges, s.per_block, partial, status);
+        const unsigned windows = static_cast<unsigned>(ceil_div(num_buckets, s.window));
+        if (windows > 65535 || s.groups > 65535) return fail(E3B_ERR_UNSUPPORTED, "relative_bias_bwd: a table of %d buckets and %d heads", num_buckets, heads);
+        bias_bwd_kernel<T, HV><<<dim3(s.parts, s.groups, windows), s.width / HV * s.slices, s.smem, st>>>(
+            static_cast<const T*>(grad), buckets, num_buckets, s.window, heads, s.width, s.slices, edges, s.per_block, partial, status);
         return check_launch("relative_bias_bwd");
     };
     if (!aligned_to(grad, s.vec * sizeof(T))) return fail(E3B_ERR_ARG, "relative_bias_bwd: the gradient must start on %d bytes", static_cast<int>(s.vec * sizeof(T)));
@@ -263,7 +267,8 @@ extern "C" int e3b_distance_buckets(const float* pos, const int64_t* edge_src, c
 
 extern "C" int e3b_relative_bias_fwd(const void* table, const int32_t* buckets, int num_buckets, int num_heads, int64_t num_edges, int type,
                                      void* bias, int32_t* status, void* stream) {
-    if (num_edges < 0 || num_buckets < 1 || num_buckets > kMaxBuckets || num_heads < 1 || !known_type(type)) return fail(E3B_ERR_ARG, "relative_bias_fwd: bad size or type");
+    if (num_edges < 0 || num_buckets < 1 || num_heads < 1 || !known_type(type)) return fail(E3B_ERR_ARG, "relative_bias_fwd: bad size or type");
+    if (static_cast<int64_t>(num_buckets) * num_heads > kMostCells) return fail(E3B_ERR_UNSUPPORTED, "relative_bias_fwd: a table of %d buckets and %d heads", num_buckets, num_heads);
     if (num_edges == 0) return E3B_OK;
     if (!table || !buckets || !bias || !status) return fail(E3B_ERR_ARG, "relative_bias_fwd: null pointer");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -273,15 +278,16 @@ extern "C" int e3b_relative_bias_fwd(const void* table, const int32_t* buckets, 
 }
 
 extern "C" int64_t e3b_relative_bias_scratch_bytes(int64_t num_edges, int num_buckets, int num_heads) {
-    if (num_edges < 0 || num_buckets < 1 || num_buckets > kMaxBuckets || num_heads < 1) return 0;
+    if (num_edges < 0 || num_buckets < 1 || num_heads < 1) return 0;
     const int parts = std::max(bias_split(num_edges, num_heads, num_buckets, 2).parts, bias_split(num_edges, num_heads, num_buckets, 4).parts);
     return sizeof(float) * static_cast<int64_t>(parts) * num_buckets * num_heads;
 }
 
 extern "C" int e3b_relative_bias_bwd(const void* grad_bias, const int32_t* buckets, int num_buckets, int num_heads, int64_t num_edges, int type,
                                      void* grad_table, int table_type, void* scratch, int64_t scratch_bytes, int32_t* status, void* stream) {
-    if (num_edges < 0 || num_buckets < 1 || num_buckets > kMaxBuckets || num_heads < 1 || !known_type(type) || !known_type(table_type))
+    if (num_edges < 0 || num_buckets < 1 || num_heads < 1 || !known_type(type) || !known_type(table_type))
         return fail(E3B_ERR_ARG, "relative_bias_bwd: bad size or type");
+    if (static_cast<int64_t>(num_buckets) * num_heads > kMostCells) return fail(E3B_ERR_UNSUPPORTED, "relative_bias_bwd: a table of %d buckets and %d heads", num_buckets, num_heads);
     if (!grad_table) return fail(E3B_ERR_ARG, "relative_bias_bwd: null pointer");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (num_edges == 0) {

@@ -178,7 +178,7 @@ class NeighborAttention(torch.nn.Module):
         without it they are rows of edges.  Slots before ``rowptr[0]`` and from ``rowptr[N]`` on belong to no node (``rowptr[a:b+1]`` gives
         the nodes ``a .. b-1`` of a graph alone); their gradients are zero.  A node without edges gets zeros.
 
-        ``bias``: ``[E, num_heads]``, or with ``buckets [E]`` (int32) a table ``[num_buckets, num_heads]`` (`RelativeBias`);
+        ``bias``: ``[E, num_heads]``, or with ``buckets [E]`` (int32) a table ``[num_buckets, num_heads]`` of any length (`RelativeBias`);
         an entry ``-inf`` of the former masks its edge for that head, whatever ``k`` and ``v`` hold there.  ``edge_weight [E]``
         multiplies the exponentials (a smooth cutoff); an edge with weight zero or below is left out, its rows are not read
         and its gradients, that of the weight included, are zero.  So does an edge whose share is zero in fp32 (below 2^-126): it adds

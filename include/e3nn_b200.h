@@ -330,7 +330,7 @@ int e3b_norm_gate_residual_bwd(const void* residual, const void* y, const void* 
  * in fp64 from fp32 coordinates; shift may be NULL; an index out of range sets *status = 2 and gives bucket 0.
  * e3b_relative_bias_fwd: bias[e, h] = table[buckets[e], h], both of `type`; a bucket out of range sets *status = 2 and gives 0.
  * e3b_relative_bias_bwd: grad_table[b, h] = sum over the edges of bucket b of grad_bias[e, h], in fp32 and in a fixed order, with
- * e3b_relative_bias_scratch_bytes(...) bytes of scratch; grad_bias is 16-byte aligned.  At most 1,024 buckets.
+ * e3b_relative_bias_scratch_bytes(...) bytes of scratch; grad_bias is 16-byte aligned.  A table has fewer than 2^31 - 32 entries.
  */
 int e3b_distance_buckets(const float* pos, const int64_t* edge_src, const int64_t* edge_dst, const float* shift,
                          const double* thresholds_squared, int num_thresholds, int64_t num_edges, int64_t num_nodes,

@@ -215,3 +215,36 @@ def test_a_share_of_zero_adds_nothing(layout, per_edge, dtype):
         got = run(mod, x)
         for n in got:
             assert torch.equal(got[n], want[n]), n
+
+
+@pytest.mark.parametrize("layout", ["bulk", "loads"])
+@pytest.mark.parametrize("num", [1025, 3000, 60000])
+def test_tables_of_many_buckets(layout, num):
+    """More than the 1,024 that RelativeBias makes: the gradient takes them in windows."""
+    gen = torch.Generator().manual_seed(num)
+    t = make(*LAYOUTS[layout][:2], DEGREES["hub"], torch.float32, False, "table", True)
+    t["bias"] = torch.randn(num, LAYOUTS[layout][1], generator=gen).cuda()
+    t["buckets"] = torch.randint(num, t["buckets"].shape, generator=gen, dtype=torch.int32).cuda()
+    t["buckets"][:50], t["buckets"][50:60] = num - 1, 0
+    check(layout, t, torch.float32)
+    t["buckets"][7], t["buckets"][300] = num, -1
+    run(module(layout, torch.float32, t), t)
+    with pytest.raises(IndexError):
+        e3nn_b200.check_status()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("num,heads,edges", [(1665, 32, 5000), (6000, 8, 20011), (1700, 70, 301), (54000, 1, 4000)])
+def test_gradient_of_a_large_table(num, heads, edges, dtype):
+    """Sums of n terms in fp32, one rounding each, and one to the table's type."""
+    from e3nn_b200.nn._relative_bias import bias_table_grad
+
+    gen = torch.Generator().manual_seed(num)
+    b = torch.randint(num, (edges,), generator=gen, dtype=torch.int32)
+    b[: edges // 2] %= 3
+    g = torch.randn(edges, heads, generator=gen).to(dtype)
+    got = bias_table_grad(g.cuda(), b.cuda(), num, dtype).cpu()
+    add = lambda x: torch.zeros(num, heads, dtype=torch.float64).index_add_(0, b.long(), x)
+    ref, n = add(g.double()), torch.bincount(b.long(), minlength=num)[:, None]
+    bound = (0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2) * ref.abs() + n * 2.0 ** -24 * add(g.double().abs()) + torch.finfo(dtype).tiny
+    assert ((got.double() - ref).abs() <= bound).all()
