@@ -232,6 +232,8 @@ class NeighborAttention(torch.nn.Module):
                 raise ValueError("buckets need the table they index: bias=[num_buckets, num_heads]")
             if buckets.dtype != torch.int32:
                 raise TypeError("buckets must be int32")
+            if bias.shape[0] * H > 2 ** 31 - 33:
+                raise NotImplementedError("a table of biases has fewer than 2^31 - 32 entries")
         for t, name in ((bias, "bias"), (edge_weight, "edge_weight")):
             if t is not None:
                 _lib.element_type(t, name)

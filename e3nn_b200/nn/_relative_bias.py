@@ -95,6 +95,8 @@ class RelativeBias(torch.nn.Module):
         r_linear = r_max if r_linear is None else r_linear
         if not 1 <= num_buckets <= 1024 or num_heads < 1:
             raise ValueError(f"num_buckets must be 1 .. 1024 and num_heads positive, got {num_buckets} and {num_heads}")
+        if num_buckets * num_heads > 2 ** 31 - 33:
+            raise NotImplementedError(f"a table has fewer than 2^31 - 32 entries, got {num_buckets} buckets and {num_heads} heads")
         if not 0.0 < r_linear <= r_max < float("inf"):
             raise ValueError(f"0 < r_linear <= r_max is needed, got r_linear={r_linear} and r_max={r_max}")
         self.num_buckets, self.num_heads, self.r_max, self.r_linear = num_buckets, num_heads, float(r_max), float(r_linear)

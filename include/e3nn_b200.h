@@ -348,7 +348,7 @@ int e3b_relative_bias_bwd(const void* grad_bias, const int32_t* buckets, int num
  * over the slots s of row n (rowptr[n] <= s < rowptr[n+1]; rowptr[0] may be above 0), e = perm[s] (perm NULL: s), r = edge_src[e]
  * (edge_src NULL: e).  q [num_dst, .], k and v [num_src, .] of `type`, rows q_stride, k_stride, v_stride elements apart;
  * out [num_dst, dv] dense.  bias NULL, [num_edges, heads] (-inf: masked, k and v unread), or with buckets [num_edges] a table
- * [num_buckets, heads].  edge_weight NULL or [num_edges]; an edge with a weight <= 0 is left out and its rows are unread.
+ * [num_buckets, heads] of fewer than 2^31 - 32 entries.  edge_weight NULL or [num_edges]; an edge with a weight <= 0 is left out and its rows are unread.
  * A row without edges (or all left out) is zero.  An index out of range sets *status = 2, its edge is left out.
  * layout: HOST array {vector width 1, 4 or (16-bit types) 8, heads, vectors of a head of q and k, of v, columns of q and k, of v}; qk_table, v_table:
  * per vector {column of head 0, columns from one head to the next}; a width

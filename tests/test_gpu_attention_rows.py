@@ -248,3 +248,10 @@ def test_gradient_of_a_large_table(num, heads, edges, dtype):
     ref, n = add(g.double()), torch.bincount(b.long(), minlength=num)[:, None]
     bound = (0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2) * ref.abs() + n * 2.0 ** -24 * add(g.double().abs()) + torch.finfo(dtype).tiny
     assert ((got.double() - ref).abs() <= bound).all()
+
+
+def test_tables_that_32_bits_do_not_index_are_refused():
+    t = make("6x0e+3x1o", 3, DEGREES["one edge"], torch.float32, False, "table")
+    mod = bnn.NeighborAttention("6x0e+3x1o", "6x0e+3x1o", 3).cuda()
+    with pytest.raises(NotImplementedError):
+        mod(t["q"], t["k"], t["v"], t["rowptr"], t["src"], bias=torch.zeros(1, 3, device="cuda").expand(2 ** 30, 3), buckets=t["buckets"])

@@ -124,3 +124,8 @@ def test_calls_that_someone_follows_go_through_autograd():
         torch.func.jvp(f, (x,), (x,))
         torch.func.vmap(f)(x)
     assert seen == [True] * 3 and not _lib.wants_function(x)
+
+
+def test_tables_are_indexed_in_32_bits():
+    with pytest.raises(NotImplementedError, match="entries"):
+        bnn.RelativeBias(1024, 2 ** 21, 5.0)
