@@ -72,6 +72,11 @@ def _aligned(t: torch.Tensor, width: int) -> torch.Tensor:
     return t if t.data_ptr() % (width * t.element_size()) == 0 else t.clone()
 
 
+def _aligned_wide(t: torch.Tensor) -> torch.Tensor:
+    """Rows of more than 4,096 columns are taken by vectors of four only."""
+    return t if t.shape[1] <= 4096 else _aligned(t, 4)
+
+
 def _flat_rows(x: torch.Tensor, dim: int, name: str) -> torch.Tensor:
     if x.dim() < 1 or x.shape[-1] != dim:
         torch._assert(False, f"Incorrect last dimension for {name}")
@@ -156,7 +161,7 @@ class _RMSNormFunction(torch.autograd.Function):
             gw = torch.empty(nch, dtype=torch.float32, device=x.device)
             nbytes = core.e3b_norm_scratch_bytes(rows, nch)
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        grad = grad.contiguous()
+        grad = _aligned_wide(grad.contiguous())
         with _lib.device_of(x):
             rc = core.e3b_rms_norm_bwd(x.data_ptr(), grad.data_ptr(), _lib.address(weight), tbl.data_ptr(), inv.data_ptr(), channels.data_ptr(), nch,
                                        inv.shape[0], fours, eps, _lib.address(gx), _lib.address(gw), _lib.address(scratch), nbytes, rows, dim,
@@ -202,7 +207,7 @@ class RMSNorm(torch.nn.Module):
         tables = (buffers["_tbl"], buffers["_inv_bits"], buffers["_channels"])
         _on_device_of(x, self, tables[0], weight)
         _lib.element_type(x, "x")
-        rows = _flat_rows(x, self._dim, "x")
+        rows = _aligned_wide(_flat_rows(x, self._dim, "x"))
         _lib.check_earlier(x)
         weight = _fp32(weight)
         if _lib.wants_function(rows, weight):
