@@ -187,6 +187,8 @@ class RMSNorm(torch.nn.Module):
         blocks = _blocks(self.irreps_in)
         self._dim = self.irreps_in.dim
         self._fours = int(_fours(blocks))
+        if self._dim > (8192 if self._fours else 4096):
+            raise _lib.E3BError(f"rows of {self._dim} columns are not supported, at most 4096, 8192 where no vector of four straddles two blocks")
         cols = _column_blocks(blocks)
         tbl = torch.tensor([(b, c, 0, 0) for b, c in cols], dtype=torch.int32).reshape(-1, 4)
         self.register_buffer("_tbl", tbl, persistent=False)

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import e3nn_b200
 from e3nn_b200 import nn as bnn
 from e3nn_b200 import o3
 from e3nn_b200.nn._attention import _head_vectors
@@ -129,3 +130,11 @@ def test_calls_that_someone_follows_go_through_autograd():
 def test_tables_are_indexed_in_32_bits():
     with pytest.raises(NotImplementedError, match="entries"):
         bnn.RelativeBias(1024, 2 ** 21, 5.0)
+
+
+def test_rows_that_no_kernel_takes_are_refused_when_the_norm_is_made():
+    for irreps in ("4097x0e", "8196x0e", "9000x0e", "1367x1o", "4095x0e+2x0o"):
+        with pytest.raises(e3nn_b200.E3BError, match="columns"):
+            bnn.RMSNorm(irreps)
+    for irreps in ("4096x0e", "8192x0e", "4095x0e", "4093x0e+1x1o", "4100x0e"):
+        assert bnn.RMSNorm(irreps)._dim == o3.Irreps(irreps).dim
