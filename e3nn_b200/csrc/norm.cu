@@ -109,10 +109,11 @@ template <typename T, int VEC, int K>
 __global__ void __launch_bounds__(kMaxThreads) rms_bwd_kernel(const T* __restrict__ x, const T* __restrict__ gh, const float* __restrict__ weight,
                                                               const int32_t* __restrict__ tbl, const float* __restrict__ inv_n,
                                                               const int32_t* __restrict__ chan, int nchan, float eps, T* __restrict__ gx,
-                                                              float* __restrict__ partial, int64_t rows, int dim, int nblk, int nw) {
+                                                              float* __restrict__ partial, int64_t rows, int dim, int nblk, int nw, int turns) {
     extern __shared__ float smem[];
-    float* red = smem;                           // [2 turns][2 sums][nblk][nw]
-    float* buf = smem + 4 * nblk * nw;           // [dim]
+    // two rows' shares in turn; of rows with so many blocks that they do not fit twice one row's, which the weights' sums replace at the end
+    float* red = smem;                                            // [turns][2 sums][nblk][nw]
+    float* buf = smem + (turns == 2 ? 4 * nblk * nw : 0);         // [dim]
     Columns<VEC, K> c;
     c.init(tbl, dim);
     float w[K][VEC], inv[K], acc[K][VEC];
@@ -125,14 +126,14 @@ __global__ void __launch_bounds__(kMaxThreads) rms_bwd_kernel(const T* __restric
             acc[k][i] = 0.0f;
         }
     }
-    for (int i = threadIdx.x; i < 4 * nblk * nw; i += blockDim.x) red[i] = 0.0f;
+    for (int i = threadIdx.x; i < turns * 2 * nblk * nw; i += blockDim.x) red[i] = 0.0f;
     __syncthreads();
     Packed<T, VEC> nx[K], ng[K];
     int64_t z = blockIdx.x;
 #pragma unroll
     for (int k = 0; k < K; ++k)
         if (c.col[k] >= 0) { nx[k].load(x + z * dim + c.col[k]); ng[k].load(gh + z * dim + c.col[k]); }
-    for (int turn = 0; z < rows; z += gridDim.x, turn ^= 1) {
+    for (int turn = 0; z < rows; z += gridDim.x, turn ^= turns - 1) {
         float v[K][VEC], g[K][VEC], sq[K], dot[K];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -168,6 +169,7 @@ __global__ void __launch_bounds__(kMaxThreads) rms_bwd_kernel(const T* __restric
             }
             if (gx) Packed<T, VEC>::store(gx + z * dim + c.col[k], o);
         }
+        if (turns == 1) __syncthreads();
     }
     if (!partial) return;
 #pragma unroll
@@ -217,6 +219,7 @@ int by_type(int type, const Shape& s, F&& f) {
     return by_shape<__half>(s, f);
 }
 
+constexpr size_t kMostSmem = 226 * 1024;      // that allow_smem allows
 bool row_fits(int widest, bool vec4) { return widest <= (vec4 ? 4 * 4 : 8) * kMaxThreads; }      // of RMSNorm
 
 }  // namespace
@@ -264,7 +267,10 @@ extern "C" int e3b_rms_norm_bwd(const void* x, const void* grad_h, const float* 
     const bool v4 = vec4 && dim % 4 == 0 && aligned_to(x, bytes) && aligned_to(grad_h, bytes) && aligned_to(grad_x, bytes);
     if (!row_fits(dim, v4)) return fail(E3B_ERR_UNSUPPORTED, "rms_norm_bwd: %d columns", dim);
     const Shape s = row_shape(dim, v4);
-    const size_t smem = sizeof(float) * (4 * num_blocks * s.nw + dim);
+    // what the forward kernel takes fits here too: with one row's shares at a time, as many bytes as two rows' there
+    const size_t twice = sizeof(float) * (4 * static_cast<size_t>(num_blocks) * s.nw + dim);
+    const int turns = twice <= kMostSmem ? 2 : 1;
+    const size_t smem = turns == 2 ? twice : std::max(sizeof(float) * 2 * static_cast<size_t>(num_blocks) * s.nw, sizeof(float) * static_cast<size_t>(dim));
     int grid = 0;
     const int rc = by_type(type, s, [&](auto t0, auto v0, auto k0) -> int {
         using T = decltype(t0);
@@ -273,7 +279,7 @@ extern "C" int e3b_rms_norm_bwd(const void* x, const void* grad_h, const float* 
         if (r != E3B_OK) return r;
         rms_bwd_kernel<T, VEC, K><<<grid, s.threads, smem, st>>>(
             static_cast<const T*>(x), static_cast<const T*>(grad_h), weight, table, inv_count, channels, num_channels, eps,
-            static_cast<T*>(grad_x), grad_weight ? static_cast<float*>(scratch) : nullptr, rows, dim, num_blocks, s.nw);
+            static_cast<T*>(grad_x), grad_weight ? static_cast<float*>(scratch) : nullptr, rows, dim, num_blocks, s.nw, turns);
         return check_launch("rms_norm_bwd");
     });
     if (rc != E3B_OK || !grad_weight || num_channels == 0) return rc;

@@ -176,7 +176,7 @@ class RMSNorm(torch.nn.Module):
 
     ``affine=False``: without the weights (one per channel, ones at the start).  Input ``[..., irreps.dim]`` in float32,
     bfloat16 or float16; the output has its type.  Blocks are normalised as they are written: ``"16x0e+16x0e"`` has two.
-    At most 4,096 columns, 8,192 where no vector of four straddles two blocks."""
+    At most 4,096 columns, 8,192 where no vector of four straddles two blocks, and 1,808 blocks."""
 
     def __init__(self, irreps, eps: float = 1e-5, affine: bool = True) -> None:
         super().__init__()

@@ -305,7 +305,7 @@ int e3b_fill_columns(float* out, int64_t num_rows, int row_stride, int col0, int
  * taken by one warp each.
  * e3b_norm_gate_residual_bwd: grad_z or grad_h may be NULL, each of the gradients too; grad_params [channels in + 2 channels out] =
  * gradients of weight_post, scale, weight_pre, with e3b_norm_scratch_bytes(rows, its length) bytes of scratch.
- * e3b_rms_norm: rows of at most 8,192 columns with vec4 and pointers aligned to four elements, else 4,096.
+ * e3b_rms_norm: rows of at most 8,192 columns with vec4 and pointers aligned to four elements, else 4,096; at most 1,808 blocks.
  */
 int64_t e3b_norm_scratch_bytes(int64_t rows, int num_params);
 int e3b_rms_norm_fwd(const void* x, const float* weight, const int32_t* table, const float* inv_count, int num_blocks, int vec4,

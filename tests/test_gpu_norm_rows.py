@@ -31,3 +31,24 @@ def test_wide_rows_that_start_anywhere(irreps, dtype):
     assert torch.equal(h, want)
     for a, b in zip(torch.autograd.grad(h, (moved, mod.weight), shifted(g)), torch.autograd.grad(want, (plain, mod.weight), g.cuda())):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("irreps", ["+".join(["1x0e"] * 1001), "+".join(["1x0e", "1x1o"] * 904), "+".join(["4x0e"] * 1808)], ids=["1001 of one", "904 of two", "1808 of four"])
+def test_rows_of_many_blocks(irreps):
+    """As many as the forward pass takes: the gradient's two sums a block have to fit as well."""
+    gen = torch.Generator().manual_seed(0)
+    irreps, rows = o3.Irreps(irreps), 700
+    mod = bnn.RMSNorm(irreps, eps=0.1).cuda()
+    x, g = rows_of(rows, irreps.dim, torch.float32, gen), rows_of(rows, irreps.dim, torch.float32, gen)
+    xd = x.cuda().requires_grad_()
+    h = mod(xd)
+    gx, gw = torch.autograd.grad(h, (xd, mod.weight), g.cuda())
+    at, col = torch.tensor([b for b, (mul, ir) in enumerate(irreps) for _ in range(mul * ir.dim)]), torch.tensor([1.0 / (mul * ir.dim) for mul, ir in irreps]).double()
+    mean = lambda t: torch.zeros(rows, len(irreps), dtype=torch.float64).index_add_(1, at, t) * col
+    rstd = (mean(x.double() ** 2) + 0.1).rsqrt()[:, at]
+    n = x.double() * rstd
+    close(h.detach(), n, torch.float32)
+    close(gx, rstd * (g.double() - n * mean(g.double() * n)[:, at]), torch.float32, size=(rstd * (g.double().abs() + n.abs() * mean((g.double() * n).abs())[:, at])))
+    chan = torch.tensor([c for c, d in enumerate([ir.dim for mul, ir in irreps for _ in range(mul)]) for _ in range(d)])
+    add = lambda t: torch.zeros(irreps.num_irreps, dtype=torch.float64).index_add_(0, chan, t.sum(0))
+    close(gw, add(g.double() * n), torch.float32, terms=64 + rows, size=add((g.double() * n).abs()))
