@@ -119,6 +119,8 @@ class _AttentionFunction(torch.autograd.Function):
             _lib.check(rc, "e3b_attention_bwd")
         if per_node:
             if perm_t is None:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("the edges by source cannot be built while a graph is captured: give NeighborAttention transpose=csr_from_dst(edge_src, k.shape[0])")
                 perm_t, rowptr_t = csr_from_dst(src, S)
             nbytes = core.e3b_attention_bwd_src_scratch_bytes(S, E, dqk, dv)
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)

@@ -131,3 +131,25 @@ def test_gradients_come_in_the_types_of_the_inputs():
     full = torch.autograd.grad(mod(q, k, v, rowptr, bias=exact[0], edge_weight=exact[1]).pow(2).sum(), exact)
     for a, b, t in zip(grads, full, (bias, weight)):
         assert a.dtype == t.dtype and torch.equal(a, b.to(t.dtype))
+
+
+def test_edges_by_source_are_not_built_in_a_capture():
+    mod, (q, k, v, rowptr, src), _ = modules()["attention"]
+    mod = mod.cuda()
+    transpose = e3nn_b200.csr_from_dst(src, k.shape[0])
+    k = k.requires_grad_()
+    def step(**kw):
+        return torch.autograd.grad(mod(q, k, v, rowptr, src, **kw).sum(), k)[0]
+    want = step()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step(transpose=transpose)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="transpose=csr_from_dst"):
+            step()
+        got = step(transpose=transpose)           # the capture goes on
+    graph.replay()
+    assert torch.equal(got, want)
