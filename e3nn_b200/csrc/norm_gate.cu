@@ -1,7 +1,8 @@
 // Norm, gate, residual and norm, forward (norm_gate.cuh: the formula and the layout of a row).
 //
-// A row of 1,216 + 1,024 columns is read once and written twice, but what bounds both forms is instructions: sums per irreps block,
-// conversions and activations of about 2,000 warp instructions a row.  By thread blocks: two rows are under way per block while
+// A row of 1,216 + 1,024 columns is read once and written twice; sums per irreps block, conversions and activations take about 2,000 warp
+// instructions a row, which fill about half of the issue slots.  The rest is latency: at most 16 warps an SM by warps, each with two row
+// sums after one another, and barriers by thread blocks.  By thread blocks: two rows are under way per block while
 // one is computed, three barriers a row.  By warps (below): 262,144 rows of 1,216 + 1,024 columns in bf16 858 us = 2.6 TB/s (by thread blocks
 // 1,080), 16,384 rows in fp32 85 us = 3.3 TB/s (105).
 #include "norm_gate.cuh"
@@ -372,7 +373,6 @@ extern "C" int e3b_norm_gate_residual_fwd(const void* residual, const void* y, c
             const int64_t per_warp = 4 * spread + kStage;
             int warps = static_cast<int>(std::min<int64_t>(row_warps(VEC, K), (112 * 1024 - 4 * padded) / per_warp));      // two blocks an SM
             if (warps < 1) warps = 1;
-            while (warps > 1 && rows < static_cast<int64_t>(warps) * kNumSMs) warps /= 2;
             const size_t smem = 4 * padded + warps * per_warp;
             int grid = 0;
             const int e = resident_blocks(norm_gate_fwd_row_kernel<T, VEC, NW, K, M>, 32 * warps, smem, ceil_div(rows, warps), &grid);

@@ -203,8 +203,10 @@ inline bool row_plan(const int32_t* host, const int32_t* in_count, const int32_t
     return true;
 }
 
-// Activations of a narrow item: silu and sigmoid on the hardware's exponential and division (relative error below 2^-22 + |x| 2^-23, where
-// gate_act costs five times the instructions), the others as in gate_act.
+// Activations of a narrow item: silu and sigmoid on the hardware's exponential and division, the others as in gate_act (which costs five times the
+// instructions, and whose last bits differ).  From the documented errors (__expf 2 + 1.173 |x| ulp, __fdividef 2 ulp for divisors to 2^126,
+// an ulp at most 2^-23) and the three roundings around them: relative error below (6 + 1.2 |x|) 2^-23 for x > -87; below that, where a
+// sigmoid is less than 2^-125, the result may be zero.
 template <int N>
 __device__ __forceinline__ void activate(int act, float cst, const float (&x)[N], float (&y)[N]) {
     if (act == kGSilu || act == kGSigmoid) {

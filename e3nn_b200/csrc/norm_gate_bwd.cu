@@ -4,8 +4,8 @@
 // gg = gz' scale goes through the gate (a gate's cotangent is the sum of gg n over its components, times the derivative of its activation),
 // then through the first norm like the second.  z and both statistics are computed again from residual and y: that costs no traffic,
 // and z is not rounded.  Parameter gradients are summed over the rows of a thread block in registers, one entry a column,
-// added up per channel at its end and over the thread blocks in their order.  Bound by instructions (one row takes
-// 8 warps about 800 each) and the five barriers a row: 16,384 rows of 1,216 + 1,024 columns in fp32 231 us = 1.9 TB/s, in bf16 204 us.  Measured
+// added up per channel at its end and over the thread blocks in their order.  Bound by the five barriers a row and the latency between
+// them (one row takes 8 warps about 800 instructions each, under half of the issue slots): 16,384 rows of 1,216 + 1,024 columns in fp32 231 us = 1.9 TB/s, in bf16 204 us.  Measured
 // and not taken: two items a thread with half the threads (402 us: twelve warps an SM no longer hide the barriers).
 #include "norm_gate.cuh"
 

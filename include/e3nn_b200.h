@@ -301,8 +301,8 @@ int e3b_fill_columns(float* out, int64_t num_rows, int row_stride, int col0, int
  * channels with the same number of components: {w, n, wide slots, narrow slots, din, dout, blocks in, blocks out, length of the row of gates per
  * column}, per wide slot ten integers {first input column, first output column, items, blocks of both, place of the first column's gate
  * or -1}, per narrow slot {kind, first input column, first output column or -1, items, blocks of both, activation, constant, place of the
- * first gate, components}, the columns of the blocks in, of the blocks out.  Rows of at most 9 wide and 8 narrow slots and 8 blocks are
- * taken by one warp each.
+ * first gate, components}, the columns of the blocks in, of the blocks out.  From 1,184 rows on one warp
+ * takes a row of at most 8 blocks and, with w = 8, 5 wide and 4 narrow slots, with w = 4, 9 and 4, with w = 1, 9 and 8.
  * e3b_norm_gate_residual_bwd: grad_z or grad_h may be NULL, each of the gradients too; grad_params [channels in + 2 channels out] =
  * gradients of weight_post, scale, weight_pre, with e3b_norm_scratch_bytes(rows, its length) bytes of scratch.
  * e3b_rms_norm: rows of at most 8,192 columns with vec4 and pointers aligned to four elements, else 4,096; at most 1,808 blocks.

@@ -52,3 +52,21 @@ def test_rows_of_many_blocks(irreps):
     chan = torch.tensor([c for c, d in enumerate([ir.dim for mul, ir in irreps for _ in range(mul)]) for _ in range(d)])
     add = lambda t: torch.zeros(irreps.num_irreps, dtype=torch.float64).index_add_(0, chan, t.sum(0))
     close(gw, add(g.double() * n), torch.float32, terms=64 + rows, size=add((g.double() * n).abs()))
+
+
+@pytest.mark.parametrize("rows,columns", [(3, 2048), (1200, 256)])       # a row by thread blocks, by warps
+@pytest.mark.parametrize("act", ["silu", "sigmoid"])
+def test_activations_far_from_zero(act, rows, columns):
+    """Columns of ones, so that the activation's argument is the weight: relative error below (6 + 1.2 |x|) 2^-23 above -87, one more rounding for
+    the scale and one for the sum with a residual of zero; below that an absolute error of 2^-125 |x|."""
+    f = {"silu": torch.nn.functional.silu, "sigmoid": torch.sigmoid}[act]
+    gate = bnn.Activation(f"{columns}x0e", [f])
+    cst = gate._in_cst.double()
+    mod = bnn.NormGateResidual(gate, eps=0.0, pre_norm=False).cuda()
+    w = torch.linspace(-130.0, 130.0, columns)
+    with torch.no_grad():
+        mod.weight_post.copy_(w)
+        z = mod(torch.zeros(rows, columns, device="cuda"), torch.ones(rows, columns, device="cuda")).cpu().double()
+    ref, x = cst * f(w.double()), w.double().abs()
+    bound = torch.where(w > -87, (6 + 1.2 * x + 2) * 2.0 ** -23 * ref.abs(), 2.0 ** -125 * x * cst) + 2.0 ** -149
+    assert ((z - ref).abs() <= bound).all()
