@@ -4,12 +4,12 @@
     dp = <g, v>      delta = <g, out>      da = p (dp - delta)
     grad q = scale sum da k      grad k = scale sum da q      grad v = sum p g      grad bias = da      grad w = sum_h da / w
 
-Bounds, with u = 2^-24, d columns a head, n edges a row, L the largest sum of magnitudes behind a logit of the row (scale <|q|, |k|> +
+Bounds, with u = 2^-24, d = min(columns a head, 38) (a lane adds at most 32 of them, five shuffles the lanes), n edges a row, L the largest sum of magnitudes behind a logit of the row (scale <|q|, |k|> +
 |bias| + |log w|).  A logit is off by (d + 3) u L; an exponential by 2 (2 + 1.18 * 2L) u of itself (its documented error) and by the
 logit's error, its own and the one in the row's sum; the sum adds n u, every rise of the running maximum (at most n) 4 u and, all
 together, 5 L u.  So a share is within  eps = (16 + 5n + (4d + 32) L) u  of itself.  The rest are sums of products, one rounding each,
 of terms whose magnitudes are added up here one by one: sum p |v| for the output, P = p (<|g|, |v|> + <|g|, sum p |v|>) for da.  A result is
-rounded once to its type, by half a step at most.
+rounded once to its type, by half a step at most (below the normal numbers, half the step there); shares below 2^-126 may be zero.
 """
 import math
 
@@ -30,9 +30,10 @@ def head_columns(irreps, heads):
     return torch.tensor(cols)
 
 
-def formula(irreps_qk, irreps_v, heads, t, dtype):
+def formula(irreps_qk, irreps_v, heads, t, dtype, steps=None):
     """``{name: (value, bound)}`` of out and the gradients of q, k, v, bias and weight (where `t` has them), on the device of `t`.
-    `t`: q, k, v, g, rowptr and, or None, src, perm, bias, buckets, weight."""
+    `t`: q, k, v, g, rowptr and, or None, src, perm, bias, buckets, weight.  `steps`: additions that follow one another in any sum, at most
+    (default: as many as it has terms); long sums are split."""
     dev = t["q"].device
     cq, cv = head_columns(irreps_qk, heads).to(dev), head_columns(irreps_v, heads).to(dev)
     (H, d), dv, scale = cq.shape, cv.shape[1], cq.shape[1] ** -0.5
@@ -72,14 +73,16 @@ def formula(irreps_qk, irreps_v, heads, t, dtype):
     out_abs = rows(p[:, :, None] * V.abs(), dst, N)
     Gd = where(G[dst])
     da = p * ((Gd * V).sum(2) - (Gd * out[dst]).sum(2))
-    n = (rowptr[1:] - rowptr[:-1]).double()[:, None]
+    at_most = lambda x: x if steps is None else x.clamp(max=steps)
+    n = at_most((rowptr[1:] - rowptr[:-1]).double()[:, None])
     L = amax(scale * (Q.abs() * K.abs()).sum(2) + b.abs() + lw.abs()).clamp(min=0.0)
-    eps = U32 * (16 + 5 * n + (4 * d + 32) * L)
+    d_steps, v_steps = min(d, 38), min(dv, 38)
+    eps = U32 * (16 + 5 * n + (4 * d_steps + 32) * L)
     P = p * ((Gd.abs() * V.abs()).sum(2) + (Gd.abs() * out_abs[dst]).sum(2))
-    e_da = 2 * eps[dst] + (dv + 2 * n[dst] + 6) * U32       # relative to P; with the roundings of a sum over the row
+    e_da = 2 * eps[dst] + (v_steps + 2 * n[dst] + 6) * U32       # relative to P; with the roundings of a sum over the row
 
     per = dst if t["src"] is None else r
-    n_out = 1.0 if t["src"] is None else torch.bincount(r, minlength=S).double()[r][:, None] if len(r) else 1.0
+    n_out = 1.0 if t["src"] is None else at_most(torch.bincount(r, minlength=S).double()[r][:, None]) if len(r) else 1.0
     e_out = U32 * n_out
     value, bound = {}, {}
     value["out"], bound["out"] = columns(out, cv, v.shape[1]), columns(out_abs * (eps + (n + 2) * U32)[:, :, None], cv, v.shape[1])
@@ -94,7 +97,7 @@ def formula(irreps_qk, irreps_v, heads, t, dtype):
             value["bias"], bound["bias"] = rows(da, e, E), rows(P * e_da, e, E)
         else:
             bucket, num = t["buckets"][e].long(), t["bias"].shape[0]
-            count = torch.bincount(bucket, minlength=num).double()[bucket][:, None] if len(e) else 1.0
+            count = at_most(torch.bincount(bucket, minlength=num).double()[bucket][:, None]) if len(e) else 1.0
             value["bias"], bound["bias"] = rows(da, bucket, num), rows(P * (e_da + count * U32), bucket, num)
     if t["weight"] is not None:
         inv = torch.where(w > 0, 1 / torch.where(w > 0, w, 1.0), 0.0)
@@ -102,7 +105,7 @@ def formula(irreps_qk, irreps_v, heads, t, dtype):
     result = {}
     for name, x in value.items():
         to = torch.float32 if name in ("bias", "weight") else dtype
-        result[name] = (x, bound[name] + torch.finfo(to).eps / 2 * x.abs() + torch.finfo(to).tiny, to)
+        result[name] = (x, bound[name] + torch.finfo(to).eps / 2 * (x.abs() + torch.finfo(to).tiny) + 2.0 ** -120, to)
     return result
 
 

@@ -255,3 +255,199 @@ def test_tables_that_32_bits_do_not_index_are_refused():
     mod = bnn.NeighborAttention("6x0e+3x1o", "6x0e+3x1o", 3).cuda()
     with pytest.raises(NotImplementedError):
         mod(t["q"], t["k"], t["v"], t["rowptr"], t["src"], bias=torch.zeros(1, 3, device="cuda").expand(2 ** 30, 3), buckets=t["buckets"])
+
+
+ALL_DEGREES = {**DEGREES, "many empty": [0] * 300 + [4] + [0] * 100, "long row": [700], "no edges": [0, 0, 0]}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+@pytest.mark.parametrize("degrees", list(ALL_DEGREES))
+@pytest.mark.parametrize("per_edge", [False, True])
+def test_lengths_biases_weights_and_permuted_edges(degrees, per_edge, layout, dtype):
+    for i, (bias, weight, perm) in enumerate(((None, False, False), ("table", False, True), ("edges", True, True), ("edges", False, False))):
+        t = make(*LAYOUTS[layout][:2], ALL_DEGREES[degrees], dtype, per_edge, bias, weight, perm, seed=i)
+        check(layout, t, dtype, 0.25 if sum(ALL_DEGREES[degrees]) > 20 else None)      # (of a handful of edges most gradients cancel)
+
+
+WIDE = [("256x0e+256x1o", 1), ("1023x0e", 1), ("64x0e+64x1o+64x2e+64x3o", 8), ("64x0e+64x1o+64x2e+64x3o", 16), ("20x0e+20x1o+20x2e", 2), ("4096x0e", 8),
+        ("40x0e+20x1o", 20), ("34x0e", 34), ("64x0e+64x1o", 64)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("irreps,heads", WIDE)
+@pytest.mark.parametrize("per_edge", [False, True])
+def test_gradients_of_wide_and_of_many_heads(irreps, heads, per_edge, dtype):
+    """Up to the 1,024 columns a head that there may be (32 single columns a lane), and more heads than a warp has lanes."""
+    t = make(irreps, heads, [3, 0, 40, 1], dtype, per_edge, "table", True, True)
+    t["q"] *= 0.3                                          # logits of a few units
+    got = run(bnn.NeighborAttention(irreps, irreps, heads).cuda(), t)
+    compare(got, formula(irreps, irreps, heads, t, dtype))
+    e3nn_b200.check_status()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("irreps,heads", [("16x0e+16x1o", 2), ("8x0e+8x1o+8x2e", 2), ("6x0e+3x1o", 3), ("64x0e+64x1o+64x2e+64x3o", 8)])
+@pytest.mark.parametrize("per_edge", [False, True])
+def test_large_graph(irreps, heads, per_edge, dtype):
+    """Enough edges for whole blocks of warps, uneven rows and a hub."""
+    gen = torch.Generator().manual_seed(heads)
+    degrees = (torch.rand(900, generator=gen) ** 3 * 40).long()
+    degrees[17], degrees[400:420] = 900, 0
+    t = make(irreps, heads, degrees.tolist(), dtype, per_edge, "table", True, sources=700)
+    compare(run(bnn.NeighborAttention(irreps, irreps, heads).cuda(), t), formula(irreps, irreps, heads, t, dtype))
+    e3nn_b200.check_status()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+@pytest.mark.parametrize("shape", ["one query", "one query, nodes", "a popular source", "two hubs"])
+def test_rows_over_many_blocks(layout, shape, dtype):
+    """Parts inside one row are added up in blocks first, in all three passes: one destination, one source."""
+    E = 30011
+    degrees = {"one query": [E], "one query, nodes": [E], "a popular source": [101] * 297, "two hubs": [14000, 0, 16000] + [1] * 5}[shape]
+    t = make(*LAYOUTS[layout][:2], degrees, dtype, shape == "one query", "table", False, sources=900)
+    if shape == "a popular source":                        # 95 of 100 edges leave from it
+        t["k"], t["v"], t["src"] = t["k"][:2], t["v"][:2], (torch.arange(len(t["src"]), device="cuda") % 20 == 0).long()
+    t["q"] *= 0.5
+    mod = module(layout, dtype, t)
+    got = run(mod, t)
+    # a part has at most 30,308 items / 592 warps = 52 edges; up to 16 of them are added in a block, the blocks' sums by 16 warps, at most
+    # 1,895 parts / 16 after one another, then the 16: below 52 + 16 + 119 + 16
+    compare(got, formula(*LAYOUTS[layout][:1], *LAYOUTS[layout][:2], t, dtype, steps=203), sharp=1.0)
+    again = run(mod, t)
+    assert all(torch.equal(got[n], again[n]) for n in got)
+    e3nn_b200.check_status()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+def test_one_edge_has_share_one_and_no_gradient_through_it(layout, dtype):
+    irreps, heads = LAYOUTS[layout][:2]
+    N = 50
+    for per_edge in (True, False):
+        t = make(irreps, heads, [1] * N, dtype, per_edge, sources=N)
+        if not per_edge:
+            t["src"] = torch.randperm(N, generator=torch.Generator().manual_seed(0)).cuda()
+        t["weight"] = torch.logspace(-30, 0, N).cuda()
+        got = run(module(layout, dtype, t), t)
+        assert torch.equal(got["out"], t["v"] if per_edge else t["v"][t["src"]])
+        assert not got["q"].any() and not got["k"].any() and not got["weight"].any()
+        assert torch.equal(got["v"] if per_edge else got["v"][t["src"]], t["g"])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+@pytest.mark.parametrize("per_edge", [False, True])
+def test_masked_places_may_hold_anything(layout, per_edge, dtype):
+    irreps, heads = LAYOUTS[layout][:2]
+    E = 40
+    t = make(irreps, heads, [10, 30], dtype, per_edge, sources=E)
+    if not per_edge:
+        t["src"] = torch.randperm(E, generator=torch.Generator().manual_seed(1)).cuda()
+    bad = torch.zeros(E, dtype=torch.bool, device="cuda")
+    bad[[0, 3, 11, 25, 39]] = True
+    mod = module(layout, dtype, t)
+    for mask in ({"weight": torch.where(bad, 0.0, 1.0)}, {"bias": torch.where(bad, -math.inf, 0.0)[:, None].repeat(1, heads)},
+                 {"weight": torch.zeros(E, device="cuda")}, {"bias": torch.full((E, heads), -math.inf, device="cuda")}):
+        clean = run(mod, {**t, **mask})
+        if bool((mask["weight"] == 0).all() if "weight" in mask else (mask["bias"] < 0).all()):      # a row whose mask leaves nothing
+            assert not any(x.any() for x in clean.values())
+        for value in (float("nan"), float("inf"), -float("inf")):
+            x = {**t, **mask, "k": t["k"].clone(), "v": t["v"].clone()}
+            rows = bad if per_edge else t["src"][bad]
+            x["k"][rows], x["v"][rows] = value, value
+            got = run(mod, x)
+            assert all(torch.equal(got[n], clean[n]) for n in got)
+    low = {**t, "bias": torch.full((E, heads), torch.finfo(torch.float32).min, device="cuda")}      # the type's lowest value everywhere: all alike
+    v = t["v"] if per_edge else t["v"][t["src"]]
+    mean = torch.stack([v[:10].double().mean(0), v[10:].double().mean(0)])
+    err = (run(mod, low)["out"].double() - mean).abs()
+    assert (err <= torch.finfo(dtype).eps / 2 * mean.abs() + 100 * 2.0 ** -24 * v.double().abs().max()).all()
+
+
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+@pytest.mark.parametrize("per_edge", [False, True])
+def test_bad_indices_are_reported_and_left_out_of_gradients(layout, per_edge):
+    t = make(*LAYOUTS[layout][:2], DEGREES["ragged"], torch.float32, per_edge, "table", True)
+    bad = torch.tensor([2, 20, 41, 80], device="cuda")
+    t["weight"].fill_(1.0)
+    mod = module(layout, torch.float32, t)
+    without = {**t, "weight": t["weight"].clone()}
+    without["weight"][bad] = 0.0
+    want = run(mod, without)
+    e3nn_b200.check_status()
+    cases = [("buckets", torch.tensor([9, -1, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32))]
+    if not per_edge:
+        cases.append(("src", torch.tensor([23, -1, 2 ** 40, -2 ** 40])))
+    for name, values in cases:
+        x = {**t, name: t[name].clone()}
+        x[name][bad] = values.cuda()
+        leaves = {n: x[n].detach().requires_grad_() for n in NAMES if x[n] is not None}
+        # (the edges by source of the graph as it should be: building them refuses such a source)
+        out = mod(leaves["q"], leaves["k"], leaves["v"], x["rowptr"], x["src"], bias=leaves["bias"], buckets=x["buckets"], edge_weight=leaves["weight"],
+                  transpose=None if per_edge else e3nn_b200.csr_from_dst(t["src"], 23))
+        got = {"out": out.detach(), **dict(zip(leaves, torch.autograd.grad(out, list(leaves.values()), t["g"])))}
+        with pytest.raises(IndexError):
+            e3nn_b200.check_status()
+        assert all(torch.equal(got[n], want[n]) for n in got)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+def test_packed_rows_broadcast_rows_and_unaligned_ones(layout, dtype):
+    irreps, heads, wide, narrow = LAYOUTS[layout]
+    t = make(irreps, heads, DEGREES["ragged"], dtype, False, sources=10)
+    D = t["q"].shape[1]
+    mod, want = module(layout, dtype, t), None
+    want = run(mod, t)
+    packed = torch.cat([t["q"], t["k"], t["v"]], 1).requires_grad_()
+    out = mod(*packed.split([D, D, D], 1), t["rowptr"], t["src"], transpose=e3nn_b200.csr_from_dst(t["src"], 10))
+    (gp,) = torch.autograd.grad(out, packed, t["g"])
+    if (3 * D) % (wide if dtype == torch.float32 else narrow) == 0:                        # the same vectors
+        assert torch.equal(out, want["out"]) and torch.equal(gp, torch.cat([want["q"], want["k"], want["v"]], 1))
+    exact = formula(irreps, irreps, heads, t, dtype)
+    odd = torch.zeros(10, 3 * D + 3, dtype=dtype, device="cuda")
+    odd[:, 1:3 * D + 1] = packed.detach()
+    odd.requires_grad_()
+    out = mod(*odd[:, 1:3 * D + 1].split([D, D, D], 1), t["rowptr"], t["src"])
+    (go,) = torch.autograd.grad(out, odd, t["g"])
+    compare({"out": out.detach(), **dict(zip("qkv", go[:, 1:3 * D + 1].split([D, D, D], 1)))}, exact)
+    one = t["q"][:1].expand(10, D)
+    got, dense = run(mod, {**t, "q": one}), run(mod, {**t, "q": one.contiguous()})
+    assert all(torch.equal(got[n], dense[n]) for n in got)
+    shifted = torch.zeros(10 * D + 1, dtype=dtype, device="cuda")[1:].view(10, D).copy_(t["g"])      # a cotangent that is not aligned
+    got = run(mod, {**t, "g": shifted})
+    assert all(torch.equal(got[n], want[n]) for n in got)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+@pytest.mark.parametrize("perm", [False, True])
+def test_captured_and_replayed(layout, perm, dtype):
+    t = make(*LAYOUTS[layout][:2], DEGREES["hub"], dtype, False, "table", True, perm)
+    mod = module(layout, dtype, t)
+    transpose = e3nn_b200.csr_from_dst(t["src"], 23)
+    def step(values):
+        leaves = [x.detach().requires_grad_() for x in values]
+        out = mod(*leaves[:3], t["rowptr"], t["src"], perm=t["perm"], bias=leaves[3], buckets=t["buckets"], edge_weight=leaves[4], transpose=transpose)
+        return (out.detach(), *torch.autograd.grad(out, leaves, t["g"]))
+    static = [t[n].clone() for n in NAMES]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        aside = step(static)
+    torch.cuda.current_stream().wait_stream(stream)
+    assert all(torch.equal(a, b) for a, b in zip(aside, step(static)))
+    graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            outs.append(step(static))
+    for s in static[:3]:
+        s.mul_(0.75)
+    want = step(static)
+    for _ in range(2):                                     # (a second replay finds what the first has left)
+        graphs[0].replay()
+        graphs[1].replay()
+        assert all(torch.equal(a, b) for out in outs for a, b in zip(out, want))
+    e3nn_b200.check_status()
