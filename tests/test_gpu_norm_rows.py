@@ -4,7 +4,7 @@ import torch
 
 from e3nn_b200 import nn as bnn
 from e3nn_b200 import o3
-from test_gpu_norm import close, norm64, rows_of
+from test_gpu_norm import ACT64, U32, close, gate64, gates, norm64, rows_of
 
 pytestmark = pytest.mark.gpu
 
@@ -70,3 +70,112 @@ def test_activations_far_from_zero(act, rows, columns):
     ref, x = cst * f(w.double()), w.double().abs()
     bound = torch.where(w > -87, (6 + 1.2 * x + 2) * 2.0 ** -23 * ref.abs(), 2.0 ** -125 * x * cst) + 2.0 ** -149
     assert ((z - ref).abs() <= bound).all()
+
+
+def parameter_terms(mod, r, y, gz, gh, gate):
+    """Gradients of the norm-gate-residual in 64 bits, written out, and per parameter the sum of the magnitudes of what is added."""
+    ins, outs = mod.irreps_in, mod.irreps_out
+    def channels(irreps):
+        return torch.tensor([c for c, d in enumerate([ir.dim for mul, ir in irreps for _ in range(mul)]) for _ in range(d)])
+    def blocks(irreps):
+        return torch.tensor([b for b, (mul, ir) in enumerate(irreps) for _ in range(mul * ir.dim)])
+    ci, co, bi, bo = channels(ins), channels(outs), blocks(ins), blocks(outs)
+    def mean(x, b):
+        n = torch.bincount(b).double()
+        return (torch.zeros(x.shape[0], len(n), dtype=torch.float64).index_add(1, b, x) / n)[:, b]
+    wp, sc, wn = mod.weight_post.detach().cpu().double()[ci], mod.scale.detach().cpu().double()[co], mod.weight_pre.detach().cpu().double()[co]
+    y, r, gz, gh = (t.double() for t in (y, r, gz, gh))
+    n = y * (mean(y * y, bi) + mod.eps).rsqrt()
+    pre = (n * wp).requires_grad_()
+    val = gate64(gate, pre) if gate is not None else pre * 1.0
+    x, val_abs = pre.detach(), pre.detach().abs()
+    if gate is not None:
+        parts = []
+        for (src, gcol, act), cst in zip(gate._out_tbl.tolist(), gate._out_cst.tolist()):
+            arg = x[:, src] if gcol < 0 else x[:, gcol]
+            parts.append(cst * (ACT64[act](arg).abs() + arg.abs()) * (1.0 if gcol < 0 else x[:, src].abs()))
+        val_abs = torch.stack(parts, 1)
+    z, z_abs = r + sc * val.detach(), r.abs() + sc.abs() * val_abs
+    rz = (mean(z * z, bo) + mod.eps).rsqrt()
+    t = gh * wn
+    gz2 = gz + rz * (t - z * rz * rz * mean(t * z, bo))
+    gz_abs = gz.abs() + rz * (t.abs() + z_abs * rz * rz * mean(t.abs() * z_abs, bo))
+    (g_pre,) = torch.autograd.grad(val, pre, gz2 * sc, retain_graph=True)
+    # the same chain with magnitudes: a gate's cotangent adds the products of its components; a slope is at most `steep` and what it is the
+    # difference of; an argument that is off by a part of itself moves function and slope (whose own slopes are at most one) by as much of it
+    steep = {0: lambda x: torch.sigmoid(x) * (1 + x.abs()), 1: torch.ones_like, 2: torch.ones_like, 3: torch.ones_like, 4: torch.sigmoid, 5: torch.ones_like}
+    def jacobian_abs(g):
+        if gate is None:
+            return g
+        out = torch.zeros_like(pre)
+        rows = gate._out_tbl.tolist()
+        for j, (src, gcol, act) in enumerate(rows):
+            cst = float(gate._out_cst[j])
+            arg = x[:, src] if gcol < 0 else x[:, gcol]
+            f, d = ACT64[act](arg).abs() + arg.abs(), steep[act](arg) + arg.abs()
+            if gcol < 0:
+                out[:, src] += cst * d * g[:, j]
+            else:
+                out[:, src] += cst * f * g[:, j]
+                out[:, gcol] += cst * d * x[:, src].abs() * g[:, j]
+        return out.detach()
+    pre_abs = jacobian_abs(gz_abs * sc.abs())
+    add = lambda x, c, num: torch.zeros(num, dtype=torch.float64).index_add(0, c, x.sum(0))
+    num_in, num_out = ins.num_irreps, outs.num_irreps
+    values = add(g_pre * n, ci, num_in), add(gz2 * val.detach(), co, num_out), add(gh * z * rz, co, num_out)
+    sizes = add(pre_abs * n.abs(), ci, num_in), add(gz_abs * val_abs, co, num_out), add(gh.abs() * z_abs * rz, co, num_out)
+    s = (mean(y * y, bi) + mod.eps).rsqrt()
+    gx = s * (g_pre * wp - n * mean(g_pre * wp * n, bi))
+    gx_abs = s * (pre_abs * wp.abs() + n.abs() * mean(pre_abs * wp.abs() * n.abs(), bi))
+    return (gz2, gx, *values), (gz_abs, gx_abs, *sizes)
+
+
+# Of what is added, each part is off by: a root mean square (a tree of sums of at most 32 + 5 + 16 additions, its root) 60 roundings, used twice for z,
+# twice for y; the two means of products 60 each; activations 30 (an exponential with an argument that the norm keeps below the root of the
+# columns, a division); the products on the way 40.  Where a cotangent is a difference its parts count with their magnitudes, and z with those
+# of the residual and of what is added to it.
+ROUNDINGS = 450
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", ["l2", "odd", "odd gates", "no scalars", "activation", "wide", "wide odd", "none", "l3"])
+@pytest.mark.parametrize("rows", [3, 1301])
+def test_gradients_with_a_bound_on_every_number(name, rows, dtype):
+    if name.startswith("wide") and rows > 3:
+        rows = 400                                         # several rows a thread block all the same
+    gen = torch.Generator().manual_seed(len(name) + rows)
+    gate = gates()[name]
+    mod = bnn.NormGateResidual(gate, irreps="6x0e+3x1o" if gate is None else None, eps=1e-3, scale_init=0.7).cuda()
+    din, dout = mod.irreps_in.dim, mod.irreps_out.dim
+    r, y, gz, gh = (rows_of(rows, d, dtype, gen) for d in (dout, din, dout, dout))
+    params = [mod.weight_post, mod.scale, mod.weight_pre]
+    with torch.no_grad():
+        for p in params:
+            p.copy_(1 + 0.3 * torch.randn(p.shape, generator=gen))
+    rd, yd = r.cuda().requires_grad_(), y.cuda().requires_grad_()
+    got = torch.autograd.grad(mod(rd, yd), [rd, yd] + params, (gz.cuda(), gh.cuda()))
+    refs, sizes = parameter_terms(mod, r, y, gz, gh, gate)
+    # a thread block adds its rows one by one, at most 148 blocks' sums by 32 threads, a channel up to 7 components
+    adds = rows // 148 + 2 + 148 * 4 // 32 + 32 + 7
+    for a, ref, size, what in zip(got, refs, sizes, ("residual", "y", "weight_post", "scale", "weight_pre")):
+        to = dtype if what in ("residual", "y") else torch.float32
+        assert a.dtype == to and a.shape == ref.shape
+        bound = torch.finfo(to).eps / 2 * ref.abs() + (ROUNDINGS + (0 if what in ("residual", "y") else adds)) * U32 * size + torch.finfo(to).tiny
+        excess = ((a.cpu().double() - ref).abs() / bound).max().item()
+        assert excess <= 1.0, f"{what}: {excess:.2f} x the bound"
+        assert bound.mean() < 0.05 * ref.abs().mean(), what
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("irreps", ["4096x0e", "4095x0e", "4093x0e activated", "4096x0e activated"])
+def test_gradients_of_the_widest_rows(irreps, dtype):
+    act = bnn.Activation(irreps.split()[0], [torch.nn.functional.silu]) if "activated" in irreps else None
+    mod = bnn.NormGateResidual(act, irreps=None if act else irreps, eps=1e-3).cuda()
+    gen = torch.Generator().manual_seed(0)
+    r, y, gz, gh = (rows_of(3, mod.irreps_out.dim, dtype, gen) for _ in range(4))
+    rd, yd = r.cuda().requires_grad_(), y.cuda().requires_grad_()
+    got = torch.autograd.grad(mod(rd, yd), (rd, yd, mod.weight_post, mod.scale, mod.weight_pre), (gz.cuda(), gh.cuda()))
+    refs, sizes = parameter_terms(mod, r, y, gz, gh, act)
+    for a, ref, size, to in zip(got, refs, sizes, (dtype, dtype) + (torch.float32,) * 3):
+        bound = torch.finfo(to).eps / 2 * ref.abs() + (ROUNDINGS + 3) * U32 * size + torch.finfo(to).tiny
+        assert ((a.cpu().double() - ref).abs() <= bound).all() and bound.mean() < 0.05 * ref.abs().mean()

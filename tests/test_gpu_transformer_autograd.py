@@ -153,3 +153,53 @@ def test_edges_by_source_are_not_built_in_a_capture():
         got = step(transpose=transpose)           # the capture goes on
     graph.replay()
     assert torch.equal(got, want)
+
+
+def test_every_parameter_of_a_block_against_differences():
+    """Norm, bias, attention with a cutoff, norm-gate-residual and a convolution block: the slope along a direction in each parameter
+    and input against a difference quotient."""
+    import math
+
+    from e3nn_b200 import o3
+
+    torch.manual_seed(0)
+    gen = torch.Generator().manual_seed(0)
+    irreps, heads, N = o3.Irreps("8x0e+8x1o+4x2e"), 4, 40
+    pos = (12.0 * torch.rand(N, 3, generator=gen)).cuda()
+    src, dst, shift, rowptr = bnn.neighbor_list_pbc(pos, 15.0, 5.0)
+    pre, bias = bnn.RMSNorm(irreps).cuda(), bnn.RelativeBias(8, heads, 5.0, r_linear=2.5).cuda()
+    block = bnn.AttentionBlock(irreps, heads, linear_math_mode="fp32", scale_init=0.5).cuda()
+    conv = bnn.InteractionBlock(irreps, lmax=1, num_basis=4, hidden=32, r_max=5.0, num_neighbors=5.0, linear_math_mode="fp32", radial_math_mode="fp32").cuda()
+    post = bnn.NormGateResidual(irreps=irreps).cuda()
+    with torch.no_grad():
+        bias.weight.normal_(0, 0.5)
+    buckets = bias.buckets(pos, src, dst, shift)
+    cutoff = 0.5 * (torch.cos(math.pi * (pos[src] - pos[dst] + shift).norm(dim=1) / 5.0) + 1)
+    x, c1, c2 = (torch.randn(N, irreps.dim, generator=gen).cuda() for _ in range(3))
+    transpose = e3nn_b200.csr_from_dst(src, N)
+    def loss(x):
+        z, h = block(x, pre(x), rowptr, src, bias=bias.weight, buckets=buckets, edge_weight=cutoff, transpose=transpose)
+        z, h = post(z, conv(pos, h, src, dst, rowptr, shift))
+        return (z.double() * c1).sum() + (h.double() * c2).sum()
+    leaves = {"x": x, **{f"{i}.{n}": p for i, m in enumerate((pre, bias, block, conv, post)) for n, p in m.named_parameters()}}
+    x.requires_grad_()
+    grads = dict(zip(leaves, torch.autograd.grad(loss(x), list(leaves.values()))))
+    for name, leaf in leaves.items():
+        direction = torch.randn(leaf.shape, generator=gen).cuda()
+        direction *= leaf.detach().pow(2).mean().sqrt() / direction.pow(2).mean().sqrt()
+        slope = (grads[name].double() * direction).sum().item()
+        size = grads[name].double().norm().item() * direction.double().norm().item() / leaf.numel() ** 0.5      # of a slope along a random direction
+        def at(s):
+            with torch.no_grad():
+                start = leaf.clone()
+                leaf.add_(direction, alpha=s)
+                value = loss(x).item()
+                leaf.copy_(start)
+            return value
+        # central differences at three steps: truncation falls with the square, the rounding of z and h (2^-24 of a few units, some thousand numbers of
+        # either sign) grows with the inverse; the two larger ones give the truncation (Richardson)
+        d = [(at(s) - at(-s)) / (2 * s) for s in (2.0 ** -5, 2.0 ** -6)]
+        best, doubt = (4 * d[1] - d[0]) / 3, abs(d[1] - d[0])
+        noise = 2.0 ** -24 * 4 * (x.numel() * 2) ** 0.5 * 32 / 2.0 ** -6
+        assert abs(best - slope) <= doubt + noise, (name, best, slope, doubt, noise)
+        assert doubt + noise < 0.5 * max(size, abs(slope)), (name, slope, doubt, noise, size)
