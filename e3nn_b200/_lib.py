@@ -173,6 +173,23 @@ def require_operand(t: torch.Tensor, like: torch.Tensor, name: str, numel: Optio
         torch._assert(t.numel() == numel, f"Invalid {name} shape: expected {numel} elements, got {t.numel()}")
 
 
+class HostInts:
+    """A host array of int32 for an entry point, made once and kept by a module, which can be copied and pickled with it."""
+
+    def __init__(self, values) -> None:
+        self._array = (c_int32 * len(values))(*values)
+        self._as_parameter_ = ctypes.addressof(self._array)      # (what ctypes passes)
+
+    def __getitem__(self, i):
+        return self._array[i]
+
+    def __len__(self) -> int:
+        return len(self._array)
+
+    def __reduce__(self):
+        return HostInts, (list(self._array),)
+
+
 _ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 

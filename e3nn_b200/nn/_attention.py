@@ -8,8 +8,6 @@ from __future__ import annotations
 
 from typing import List, Optional, Tuple
 
-import ctypes
-
 import torch
 
 from .. import _lib
@@ -164,7 +162,7 @@ class NeighborAttention(torch.nn.Module):
             tables = [_head_vectors(irreps, self.num_heads, vec) for irreps in (self.irreps_qk, self.irreps_v)]
             self.register_buffer(f"_qk{vec}", tables[0], persistent=False)
             self.register_buffer(f"_v{vec}", tables[1], persistent=False)
-            self._layouts[vec] = (ctypes.c_int32 * 6)(vec, self.num_heads, tables[0].shape[0], tables[1].shape[0], *self._dims)
+            self._layouts[vec] = _lib.HostInts([vec, self.num_heads, tables[0].shape[0], tables[1].shape[0], *self._dims])
 
     def __repr__(self) -> str:
         return f"{self.__class__.__name__}(q, k: {self.irreps_qk}, v: {self.irreps_v}, {self.num_heads} heads)"

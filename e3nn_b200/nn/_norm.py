@@ -93,7 +93,7 @@ def _on_device_of(x: torch.Tensor, module: torch.nn.Module, table: torch.Tensor,
 
 
 def _row_plan(wides, narrows, back, ins, outs, width: int, narrow: int):
-    """The items of `_gate_items` as slots of at most 32 neighbours (see ``plan`` of ``e3b_norm_gate_residual_fwd``), a ctypes array."""
+    """The items of `_gate_items` as slots of at most 32 neighbours (see ``plan`` of ``e3b_norm_gate_residual_fwd``)."""
     place, length = {}, 0                             # gate column -> place of its copies, one per component
     for c, row in enumerate(back):
         if row[0] == 2:
@@ -127,7 +127,7 @@ def _row_plan(wides, narrows, back, ins, outs, width: int, narrow: int):
     din, dout = (sum(mul * d for mul, d in b) for b in (ins, outs))
     flat = [width, narrow, num_wide, len(slots) - num_wide, din, dout, len(ins), len(outs), length]
     flat += [x for slot in slots for x in slot] + [mul * d for mul, d in ins] + [mul * d for mul, d in outs]
-    return (ctypes.c_int32 * len(flat))(*flat)
+    return _lib.HostInts(flat)
 
 
 def _rms_norm(x, weight, fours: int, eps: float, tbl, inv, _channels) -> torch.Tensor:
@@ -355,7 +355,7 @@ class NormGateResidual(torch.nn.Module):
                 self.register_buffer(f"_narrow{width}{narrow}", items[1], persistent=False)
                 self._table_names[width, narrow] = (f"_wide{width}{narrow}", f"_narrow{width}{narrow}", "_in", "_out", "_in_channels", "_out_channels",
                                                     "_in_inv_bits", "_out_inv_bits")
-                sizes = (ctypes.c_int32 * 11)(width, narrow, len(items[0]), len(items[1]), items[2], din, dout, len(ins), len(outs), n_in, n_out)
+                sizes = _lib.HostInts([width, narrow, len(items[0]), len(items[1]), items[2], din, dout, len(ins), len(outs), n_in, n_out])
                 pair = 2 if width == 4 else narrow        # by warps, two columns an item where rows are wide enough for it
                 rows = items if pair == narrow else _gate_items(back, const, forth, ins, outs, width, pair)
                 plan = None if rows is None else _row_plan(rows[0].tolist(), rows[1].tolist(), back, ins, outs, width, pair)

@@ -203,3 +203,15 @@ def test_every_parameter_of_a_block_against_differences():
         noise = 2.0 ** -24 * 4 * (x.numel() * 2) ** 0.5 * 32 / 2.0 ** -6
         assert abs(best - slope) <= doubt + noise, (name, best, slope, doubt, noise)
         assert doubt + noise < 0.5 * max(size, abs(slope)), (name, slope, doubt, noise, size)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_a_pickled_module_computes(name):
+    import copy
+    import pickle
+
+    mod, inputs, _ = modules()[name]
+    mod = mod.cuda()
+    want = flat(mod(*inputs))
+    for other in (pickle.loads(pickle.dumps(mod)), copy.deepcopy(mod)):
+        assert all(torch.equal(a, b) for a, b in zip(flat(other(*inputs)), want))

@@ -138,3 +138,21 @@ def test_rows_that_no_kernel_takes_are_refused_when_the_norm_is_made():
             bnn.RMSNorm(irreps)
     for irreps in ("4096x0e", "8192x0e", "4095x0e", "4093x0e+1x1o", "4100x0e"):
         assert bnn.RMSNorm(irreps)._dim == o3.Irreps(irreps).dim
+
+
+def test_modules_are_copied_and_pickled():
+    import copy
+    import pickle
+
+    gate = bnn.Gate("4x0e", [torch.tanh], "4x0e", [torch.sigmoid], "4x1o")
+    for mod in (bnn.RMSNorm("4x0e"), bnn.NormGateResidual(gate), bnn.RelativeBias(4, 2, 5.0), bnn.NeighborAttention("4x0e+4x1o", "4x0e", 2),
+                bnn.AttentionBlock("4x0e+4x1o", 2)):
+        for other in (copy.deepcopy(mod), pickle.loads(pickle.dumps(mod))):
+            assert repr(other) == repr(mod)
+            for a, b in zip(list(mod.parameters()) + list(mod.buffers()), list(other.parameters()) + list(other.buffers())):
+                assert torch.equal(a, b)
+            for name in ("_layouts", "_sizes"):
+                for key, value in getattr(mod, name, {}).items():
+                    mine, theirs = value if isinstance(value, tuple) else (value,), getattr(other, name)[key]
+                    for a, b in zip(mine, theirs if isinstance(theirs, tuple) else (theirs,)):
+                        assert (a is None and b is None) or (list(a) == list(b) and a._as_parameter_ != b._as_parameter_)
