@@ -205,7 +205,7 @@ class RMSNorm(torch.nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if not x.is_cuda:
             raise NotImplementedError("RMSNorm runs on CUDA tensors only")
-        buffers, weight = self._buffers, self._parameters["weight"]
+        buffers, weight = self._buffers, self.weight
         tables = (buffers["_tbl"], buffers["_inv_bits"], buffers["_channels"])
         _on_device_of(x, self, tables[0], weight)
         _lib.element_type(x, "x")
@@ -380,8 +380,7 @@ class NormGateResidual(torch.nn.Module):
         if residual.dtype != y.dtype:
             raise TypeError(f"residual and y must have one type, got {residual.dtype} and {y.dtype}")
         _lib.element_type(y, "y")
-        buffers, parameters = self._buffers, self._parameters
-        w_post, scale, w_pre = parameters["weight_post"], parameters["scale"], parameters["weight_pre"]
+        buffers, w_post, scale, w_pre = self._buffers, self.weight_post, self.scale, self.weight_pre
         _on_device_of(y, self, buffers["_in"], residual, w_post, scale, w_pre)
         (din, dout), sizes = self._dims, self._sizes
         # vectors of 16 bytes if the row falls into such

@@ -133,7 +133,7 @@ class RelativeBias(torch.nn.Module):
     def forward(self, buckets: torch.Tensor) -> torch.Tensor:
         if not buckets.is_cuda:
             raise NotImplementedError("RelativeBias runs on CUDA tensors only")
-        weight = self._parameters["weight"]
+        weight = self.weight
         if weight.get_device() != buckets.get_device():
             raise RuntimeError(f"Expected all tensors to be on the same device, but weight is on {weight.device} and buckets on {buckets.device}")
         if buckets.dtype != torch.int32:

@@ -215,3 +215,38 @@ def test_a_pickled_module_computes(name):
     want = flat(mod(*inputs))
     for other in (pickle.loads(pickle.dumps(mod)), copy.deepcopy(mod)):
         assert all(torch.equal(a, b) for a, b in zip(flat(other(*inputs)), want))
+
+
+@pytest.mark.parametrize("how", ["parametrized", "pruned", "plain attributes"])
+def test_parameters_that_something_else_provides(how):
+    """Parametrisations, pruning and wrappers that put views of one flat tensor in the place of parameters take them out of the module's table."""
+    import copy
+
+    from torch.nn.utils import parametrize, prune
+
+    class Double(torch.nn.Module):
+        def forward(self, w):
+            return 2 * w
+
+    buckets = torch.tensor([0, 3, 1], dtype=torch.int32, device="cuda")
+    cases = [(*modules()[n][:2], names) for n, names in (("rms", ["weight"]), ("norm", ["weight_post", "scale", "weight_pre"]))]
+    cases.append((bnn.RelativeBias(4, 2, 5.0), (buckets,), ["weight"]))
+    for mod, inputs, names in cases:
+        mod = mod.cuda()
+        changed = copy.deepcopy(mod)
+        for name in names:
+            value = getattr(mod, name)
+            if how == "parametrized":
+                parametrize.register_parametrization(changed, name, Double())
+            elif how == "pruned":
+                prune.custom_from_mask(changed, name, (torch.arange(value.numel(), device="cuda") % 2).reshape(value.shape))
+            else:
+                delattr(changed, name)
+                setattr(changed, name, (3 * value.detach()).requires_grad_())
+            with torch.no_grad():
+                value.mul_({"parametrized": 2, "plain attributes": 3}.get(how, 1))
+                if how == "pruned":
+                    value.mul_((torch.arange(value.numel(), device="cuda") % 2).reshape(value.shape))
+        got, want = flat(changed(*inputs)), flat(mod(*inputs))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert all(a.requires_grad for a in got)
