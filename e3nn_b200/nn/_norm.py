@@ -22,7 +22,8 @@ import torch
 from .. import _lib
 from ..o3 import Irreps
 from ._activation import Activation
-from ._gate import Gate
+from ._fc import normalize2mom_constant
+from ._gate import _ACT_CODE, Gate
 
 
 def _blocks(irreps: Irreps) -> List[Tuple[int, int]]:
@@ -334,7 +335,11 @@ class NormGateResidual(torch.nn.Module):
             back, const = [[0, j, 1, 0, 3] for j in range(din)], [1.0] * din
             forth = [[j, -1, 3] for j in range(dout)]
         else:
-            back, const, forth = gate._in_tbl.tolist(), gate._in_cst.tolist(), gate._out_tbl.tolist()
+            back, forth = gate._in_tbl.tolist(), gate._out_tbl.tolist()
+            # (not the gate's own table of them, which .half() and the like round)
+            names = {code: name for name, code in _ACT_CODE.items()}
+            constants = {code: 1.0 if names[code] is None else normalize2mom_constant(names[code]) for code in {row[4] for row in back}}
+            const = [0.0 if row[0] == 3 else constants[row[4]] for row in back]
         comps = [(row[1], row[2]) if row[0] == 2 else (0, 0) for row in back]
         tables = {"_in": [(*bc, *n) for bc, n in zip(_column_blocks(ins), comps)], "_out": [(*bc, 0, 0) for bc in _column_blocks(outs)]}
         for name, value in tables.items():

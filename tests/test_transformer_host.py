@@ -156,3 +156,15 @@ def test_modules_are_copied_and_pickled():
                     mine, theirs = value if isinstance(value, tuple) else (value,), getattr(other, name)[key]
                     for a, b in zip(mine, theirs if isinstance(theirs, tuple) else (theirs,)):
                         assert (a is None and b is None) or (list(a) == list(b) and a._as_parameter_ != b._as_parameter_)
+
+
+def test_constants_of_a_gate_in_half_precision():
+    for make in (lambda: bnn.Gate("4x0e+2x0o", [torch.nn.functional.silu, torch.tanh], "3x0e", [torch.sigmoid], "2x1o+1x2e"),
+                 lambda: bnn.Activation("4x0e+2x0o+4x1o", [torch.nn.functional.silu, torch.abs, None])):
+        full, half = bnn.NormGateResidual(make()), bnn.NormGateResidual(make().half())
+        assert full._in_channels.tolist() == half._in_channels.tolist()
+        for name, value in full.named_buffers():
+            assert torch.equal(value, dict(half.named_buffers())[name]), name
+        narrow = full._narrow11.tolist()
+        for kind, col, _, _, _, act, bits, _ in narrow:
+            assert torch.tensor(bits, dtype=torch.int32).view(torch.float32) == make()._in_cst[col]
