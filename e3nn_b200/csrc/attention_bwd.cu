@@ -356,7 +356,8 @@ extern "C" int e3b_attention_bwd(const void* q, const void* k, const void* v, co
         return fail(E3B_ERR_ARG, "attention_bwd: bad size or type");
     const int vec = layout[0], heads = layout[1], nqk = layout[2], nv = layout[3], dqk = layout[4], dv = layout[5];
     if (heads < 1 || (vec != 1 && vec != 4 && (vec != 8 || type == kFloat32))) return fail(E3B_ERR_ARG, "attention_bwd: bad head layout");
-    if (buckets && (num_buckets < 0 || static_cast<int64_t>(num_buckets) * heads > INT32_MAX - 32))
+    if (buckets && num_buckets < 1) return fail(E3B_ERR_ARG, "attention_bwd: an empty table of biases");      // (the kernels read its first row in the place of a bad one)
+    if (buckets && static_cast<int64_t>(num_buckets) * heads > INT32_MAX - 32)
         return fail(E3B_ERR_UNSUPPORTED, "attention_bwd: a table of %d buckets and %d heads", num_buckets, heads);
     if (num_dst == 0 && num_edges == 0) return E3B_OK;
     if ((num_dst > 0 && (!q || !grad_out || !out32 || !stats || !grad_q)) || !rowptr || (num_edges > 0 && num_src > 0 && (!k || !v)) || !qk_table ||

@@ -451,3 +451,23 @@ def test_captured_and_replayed(layout, perm, dtype):
         graphs[1].replay()
         assert all(torch.equal(a, b) for out in outs for a, b in zip(out, want))
     e3nn_b200.check_status()
+
+
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+@pytest.mark.parametrize("per_edge", [False, True])
+@pytest.mark.parametrize("perm", [False, True])
+def test_no_rows_and_no_sources(layout, per_edge, perm):
+    irreps, heads = LAYOUTS[layout][:2]
+    t = make(irreps, heads, [], torch.float32, per_edge, "edges", True, perm, behind=50)      # edges, but no node
+    fill_free_memory()
+    got = run(bnn.NeighborAttention(irreps, irreps, heads).cuda(), t)
+    assert got["out"].shape == (0, t["q"].shape[1]) and not any(got[n].any() for n in got)
+    e3nn_b200.check_status()
+    if per_edge or perm:
+        return
+    t = make(irreps, heads, [3, 4], torch.float32, False, None, True)                         # sources out of range: there is none
+    mod = bnn.NeighborAttention(irreps, irreps, heads).cuda()
+    out = mod(t["q"], t["k"][:0], t["v"][:0], t["rowptr"], t["src"], edge_weight=t["weight"])
+    with pytest.raises(IndexError):
+        e3nn_b200.check_status()
+    assert not out.any()

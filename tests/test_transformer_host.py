@@ -168,3 +168,17 @@ def test_constants_of_a_gate_in_half_precision():
         narrow = full._narrow11.tolist()
         for kind, col, _, _, _, act, bits, _ in narrow:
             assert torch.tensor(bits, dtype=torch.int32).view(torch.float32) == make()._in_cst[col]
+
+
+def test_tables_of_biases_that_the_entry_points_refuse():
+    """Refused before anything is launched or read: the addresses are not looked at."""
+    from e3nn_b200 import _lib
+
+    core, p, layout = _lib.core(), 256, _lib.HostInts([1, 4, 2, 2, 8, 8])
+    def fwd(num_buckets):
+        return core.e3b_attention_fwd(p, p, p, 8, 8, 8, p, 0, p, p, p, num_buckets, 0, p, p, layout, 1.0, 1, 1, 1, 0, p, 0, 0, p, 0, p, 0)
+    def bwd(num_buckets):
+        return core.e3b_attention_bwd(p, p, p, p, 8, 8, 8, p, p, p, 0, p, p, p, num_buckets, 0, p, p, layout, 1.0, 1, 1, 1, 0, p, 0, 0, 0, 0, 0, 0, p, 0, p, 0)
+    for call in (fwd, bwd):
+        assert call(0) == call(-1) == -1 and call(2 ** 29) == -3
+        assert call(2 ** 20) == -1 and b"scratch" in core.e3b_last_error()       # (with such a table the next check is reached)
