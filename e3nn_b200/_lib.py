@@ -178,7 +178,7 @@ class HostInts:
 
     def __init__(self, values) -> None:
         self._array = (c_int32 * len(values))(*values)
-        self._as_parameter_ = ctypes.addressof(self._array)      # (what ctypes passes)
+        self.address = self._as_parameter_ = ctypes.addressof(self._array)      # (what ctypes passes; an integer costs it least)
 
     def __getitem__(self, i):
         return self._array[i]
@@ -189,6 +189,8 @@ class HostInts:
     def __reduce__(self):
         return HostInts, (list(self._array),)
 
+
+_grad_enabled, _transforms_active, _tracing_state = torch.is_grad_enabled, torch._C._are_functorch_transforms_active, torch._C._get_tracing_state
 
 _ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -228,13 +230,15 @@ def wants_function(*tensors: Optional[torch.Tensor]) -> bool:
     """Whether a call has to go through its autograd function: it is recorded for a backward pass, or someone else follows it.  A
     kernel launched past the function leaves no trace for a forward-mode level (the result would lose its tangent; the
     function raises), a transform of `torch.func`, or the tracer of `torch.jit` (which would record the empty output alone)."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return True
-    return _forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active() or is_tracing()
+    if _grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return _forward_ad._current_level >= 0 or _transforms_active() or _tracing_state() is not None
 
 
 def is_tracing() -> bool:
-    return torch._C._get_tracing_state() is not None
+    return _tracing_state() is not None
 
 
 _no_switch = contextlib.nullcontext()

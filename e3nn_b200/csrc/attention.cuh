@@ -179,14 +179,15 @@ __device__ __forceinline__ void load_row_f(float (&f)[V][VEC], const T* __restri
 #pragma unroll
     for (int j = 0; j < V; ++j) p[j].unpack(f[j]);
 }
-template <typename T, int VEC, int V>
+// SHARE: a factor of zero gives zeros, whatever the row holds.
+template <typename T, int VEC, int V, bool SHARE = false>
 __device__ __forceinline__ void store_row(T* __restrict__ base, int64_t row, int64_t stride, const int (&col)[V], const float (&f)[V][VEC], float by) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         if (col[j] < 0) continue;
         float o[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) o[i] = by == 0.0f ? 0.0f : f[j][i] * by;      // (a share of zero: whatever the row holds)
+        for (int i = 0; i < VEC; ++i) o[i] = SHARE && by == 0.0f ? 0.0f : f[j][i] * by;
         Packed<T, VEC>::store(base + row * stride + col[j], o);
     }
 }

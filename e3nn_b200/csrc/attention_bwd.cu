@@ -20,7 +20,7 @@ struct BwdArgs {
     void *grad_q, *grad_k, *grad_v;      // grad_k, grad_v: per edge, or null
     float2* share;                       // [edges, even(heads)] {p, da} or null
     float* da;                           // [edges, heads] or null
-    int32_t* dst;                        // [edges] or null: destination of every edge; with a permutation -1 beforehand
+    int32_t* dst;                        // [edges] or null: destination of every edge; with a permutation below zero beforehand
     float scale;
     Heads h;
     Edges e;
@@ -31,11 +31,6 @@ struct BwdArgs {
     int depth;
     uint32_t warp_smem;
     __device__ __forceinline__ float2* share_of(int64_t edge) const { return share + edge * ((h.heads + 1) & ~1); }
-    // Notes the destination of an edge.  A permutation may name an edge twice: two rows would write its gradients.
-    __device__ __forceinline__ void visit(int edge, int row) const {
-        if (!e.perm) dst[edge] = row;
-        else if (atomicCAS(dst + edge, -1, row) != -1) *e.status = 4;
-    }
 };
 
 // q, cotangent and statistics of a row; returns delta.  The output enters unrounded, in the order of the dots g v of the kernel (PAIRS: of
@@ -71,8 +66,9 @@ __device__ __forceinline__ float open_row(const BwdArgs& a, int64_t n, const int
 // edges that no row has visited are cleared afterwards (clear_unvisited_kernel): slots outside may name any edge, and not every
 // edge need be named.
 template <typename T, int VEC, int V>
-__device__ __forceinline__ void clear_outside(const BwdArgs& a, const Part& range, const int (&cq)[V], const int (&cv)[V], int head, bool leads) {
-    if (a.e.perm || (range.first >= range.e0 && range.behind >= range.e1)) return;
+__device__ __forceinline__ void clear_outside(const BwdArgs& a, int part, const int (&cq)[V], const int (&cv)[V], int head, bool leads) {
+    if (a.e.perm || (a.r.num > 0 && a.r.begin(0) == 0 && a.r.end(a.r.num - 1) == a.r.edges)) return;
+    const Part range = find_part(a.r, part);      // (found again: kept from the walk it costs registers there)
     float zero[V][VEC];
 #pragma unroll
     for (int j = 0; j < V; ++j)
@@ -124,7 +120,7 @@ __global__ void __launch_bounds__(256) attn_bwd_dst_kernel(const BwdArgs a) {
                 for (int64_t base = first; base < last; base += 32) {
                     EdgeMeta meta;
                     meta.load(a.e, base + lane, last);
-                    if (a.dst && blockIdx.y == 0 && meta.edge >= 0) a.visit(meta.edge, row_now);
+                    if (a.dst && blockIdx.y == 0 && meta.edge >= 0) a.dst[meta.edge] = row_now;
                     const int count = static_cast<int>(min(last - base, int64_t{32}));
                     for (int u0 = 0; u0 < count; u0 += U) {
                         Packed<T, VEC> kk[U][V], vv[U][V];
@@ -178,8 +174,8 @@ __global__ void __launch_bounds__(256) attn_bwd_dst_kernel(const BwdArgs a) {
                             if (leads && a.share) a.share_of(edge[u])[head] = make_float2(p, da);
                             if (leads && a.da) a.da[static_cast<int64_t>(edge[u]) * a.h.heads + head] = da;
                             if (a.grad_k) {
-                                store_row<T, VEC, V>(static_cast<T*>(a.grad_k), edge[u], a.h.dqk, cq, qf, a.scale * da);
-                                store_row<T, VEC, V>(static_cast<T*>(a.grad_v), edge[u], a.h.dv, cv, gf, p);
+                                store_row<T, VEC, V, true>(static_cast<T*>(a.grad_k), edge[u], a.h.dqk, cq, qf, a.scale * da);
+                                store_row<T, VEC, V, true>(static_cast<T*>(a.grad_v), edge[u], a.h.dv, cv, gf, p);
                             }
                         }
                     }
@@ -195,7 +191,7 @@ __global__ void __launch_bounds__(256) attn_bwd_dst_kernel(const BwdArgs a) {
                     ended = static_cast<int>(n);
                 }
             });
-        clear_outside<T, VEC, V>(a, range, cq, cv, head, leads);
+        clear_outside<T, VEC, V>(a, part, cq, cv, head, leads);
         if (blockIdx.y == 0 && lane == 0) a.parts.ended[part] = ended;
     }
     leave_part(a.merge, s, goes_on, part, a.r.parts, a.parts, a.h, cq, cv, head, leads, smem);
@@ -230,7 +226,7 @@ __global__ void __launch_bounds__(384, 1) attn_bwd_dst_ring_kernel(const BwdArgs
                 s.clear();
             },
             [&](const EdgeMeta& meta, int at, int m) {
-                if (a.dst && lane >= at && lane < at + m && meta.edge >= 0) a.visit(meta.edge, row_now);
+                if (a.dst && lane >= at && lane < at + m && meta.edge >= 0) a.dst[meta.edge] = row_now;
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     const int from = (at + u) & 31;
@@ -268,8 +264,8 @@ __global__ void __launch_bounds__(384, 1) attn_bwd_dst_ring_kernel(const BwdArgs
                     if (leads && a.share) a.share_of(edge[u])[head] = make_float2(p, da);
                     if (leads && a.da) a.da[static_cast<int64_t>(edge[u]) * a.h.heads + head] = da;
                     if (a.grad_k) {
-                        store_row<T, VEC, V>(static_cast<T*>(a.grad_k), edge[u], a.h.dqk, cq, qf, a.scale * da);
-                        store_row<T, VEC, V>(static_cast<T*>(a.grad_v), edge[u], a.h.dv, cv, gf, p);
+                        store_row<T, VEC, V, true>(static_cast<T*>(a.grad_k), edge[u], a.h.dqk, cq, qf, a.scale * da);
+                        store_row<T, VEC, V, true>(static_cast<T*>(a.grad_v), edge[u], a.h.dv, cv, gf, p);
                     }
                 }
             },
@@ -283,7 +279,7 @@ __global__ void __launch_bounds__(384, 1) attn_bwd_dst_ring_kernel(const BwdArgs
                     ended = static_cast<int>(n);
                 }
             });
-        clear_outside<T, VEC, V>(a, range, cq, cv, head, leads);
+        clear_outside<T, VEC, V>(a, part, cq, cv, head, leads);
         if (lane == 0) a.parts.ended[part] = ended;
     }
     leave_part(a.merge, s, goes_on, part, a.r.parts, a.parts, a.h, cq, cv, head, leads, reinterpret_cast<float*>(memory));
@@ -302,7 +298,17 @@ __global__ void __launch_bounds__(512) attn_bwd_dst_join_kernel(const BwdArgs a)
     if (join_parts(s, a.r, blockIdx.x, a.parts, a.h, cq, cq, head, live, smem, &n)) store_row<T, VEC, V>(static_cast<T*>(a.grad_q), n, a.h.dqk, cq, s.a[0], a.scale);
 }
 
-// Gradients of the edges that no row has visited (dst -1) are zero.  A warp looks at 32 edges.
+// With a permutation, before the rows are walked: every edge that a slot of a row names is claimed (-1 -> -2).  One that is named twice would
+// get its gradients from two rows.  (An exchange in the kernel that walks the rows costs it 2 % without a permutation too.)
+__global__ void __launch_bounds__(256) claim_edges_kernel(const Rows r, const int64_t* __restrict__ perm, int32_t* __restrict__ dst, int32_t* status) {
+    const int64_t last = r.num > 0 ? r.end(r.num - 1) : 0;
+    for (int64_t s = (r.num > 0 ? r.begin(0) : 0) + static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; s < last; s += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+        const int64_t e = perm[s];
+        if (e >= 0 && e < r.edges && atomicCAS(dst + e, -1, -2) != -1) *status = 4;
+    }
+}
+
+// Gradients of the edges that no row has visited (dst below zero) are zero.  A warp looks at 32 edges.
 template <typename T>
 __global__ void __launch_bounds__(256) clear_unvisited_kernel(const int32_t* __restrict__ dst, int64_t edges, int heads, int dqk, int dv, float* __restrict__ da,
                                                               T* __restrict__ grad_k, T* __restrict__ grad_v) {
@@ -379,7 +385,13 @@ extern "C" int e3b_attention_bwd(const void* q, const void* k, const void* v, co
               {rowptr, num_dst, num_edges, s.per_part, s.parts}, partials_in(scratch, s.parts, dq_slot(dqk)), s.merge, rows, p.depth,
               static_cast<uint32_t>(p.warp_smem)};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (perm && edge_dst) E3B_CUDA_TRY(cudaMemsetAsync(edge_dst, 0xff, sizeof(int32_t) * num_edges, st));      // all -1
+    const unsigned edge_grid = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(ceil_div(num_edges, 256), kNumSMs * 8)));
+    if (perm && edge_dst) {
+        E3B_CUDA_TRY(cudaMemsetAsync(edge_dst, 0xff, sizeof(int32_t) * num_edges, st));      // all -1
+        claim_edges_kernel<<<edge_grid, 256, 0, st>>>(a.r, perm, edge_dst, status);
+        const int claimed = check_launch("attention_bwd edges");
+        if (claimed != E3B_OK) return claimed;
+    }
     const int rc = by_type_and_vectors(type, vec, p.v, [&](auto t0, auto vec0, auto v0) -> int {
         using T = decltype(t0);
         constexpr int VEC = decltype(vec0)::value, V = decltype(v0)::value;
@@ -406,10 +418,9 @@ extern "C" int e3b_attention_bwd(const void* q, const void* k, const void* v, co
     });
     if (rc != E3B_OK || num_edges == 0) return rc;
     if (perm && (grad_logit || grad_k)) {
-        const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ceil_div(num_edges, 256), kNumSMs * 8));
         auto clear = [&](auto t0) {
             using T = decltype(t0);
-            clear_unvisited_kernel<T><<<grid, 256, 0, st>>>(edge_dst, num_edges, heads, dqk, dv, grad_logit, static_cast<T*>(grad_k), static_cast<T*>(grad_v));
+            clear_unvisited_kernel<T><<<edge_grid, 256, 0, st>>>(edge_dst, num_edges, heads, dqk, dv, grad_logit, static_cast<T*>(grad_k), static_cast<T*>(grad_v));
         };
         if (type == kFloat32) clear(float());
         else if (type == kBFloat16) clear(__nv_bfloat16());
@@ -418,7 +429,7 @@ extern "C" int e3b_attention_bwd(const void* q, const void* k, const void* v, co
         if (cleared != E3B_OK) return cleared;
     }
     if (!grad_weight) return E3B_OK;
-    attn_weight_grad_kernel<<<static_cast<unsigned>(std::min<int64_t>(ceil_div(num_edges, 256), kNumSMs * 8)), 256, 0, st>>>(
+    attn_weight_grad_kernel<<<edge_grid, 256, 0, st>>>(
         grad_logit, edge_weight, heads, num_edges, grad_weight);
     return check_launch("attention_bwd weights");
 }

@@ -63,7 +63,7 @@ def _attend(c: _Call, keep: bool):
         rc = core.e3b_attention_fwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), k.stride(0), v.stride(0), c.rowptr.data_ptr(), address(c.perm), address(c.src),
             address(c.bias), address(c.buckets), c.bias.shape[0] if c.buckets is not None else 0, address(c.weight), c.qk_tbl.data_ptr(), c.v_tbl.data_ptr(),
-            c.layout, c.scale, N, k.shape[0], c.edges, type_code, out.data_ptr(), address(out32), address(stats), scratch.data_ptr(), nbytes,
+            c.layout.address, c.scale, N, k.shape[0], c.edges, type_code, out.data_ptr(), address(out32), address(stats), scratch.data_ptr(), nbytes,
             _lib.status_address(q), _lib.raw_stream(q))
     if rc:
         _lib.check(rc, "e3b_attention_fwd")
@@ -110,7 +110,7 @@ class _AttentionFunction(torch.autograd.Function):
             rc = core.e3b_attention_bwd(
                 address(q), address(k), address(v), address(grad), q.stride(0), k.stride(0), v.stride(0), address(out32), address(stats),
                 address(rowptr), address(perm), address(src), address(bias), address(buckets), bias.shape[0] if buckets is not None else 0, address(weight),
-                address(qk_tbl), address(v_tbl), layout, scale, N, S, E, type_code, address(gq), address(gk) if per_edge else None,
+                address(qk_tbl), address(v_tbl), layout.address, scale, N, S, E, type_code, address(gq), address(gk) if per_edge else None,
                 address(gv) if per_edge else None, address(share), address(da), address(dst), address(gweight), address(scratch), nbytes, status,
                 _lib.raw_stream(q))
         if rc:
@@ -125,7 +125,7 @@ class _AttentionFunction(torch.autograd.Function):
             with _lib.device_of(q):
                 rc = core.e3b_attention_bwd_src(
                     address(q), address(grad), q.stride(0), address(share), address(dst), address(perm_t), address(rowptr_t), address(qk_tbl), address(v_tbl),
-                    layout, scale, N, S, E, type_code, address(gk), address(gv), address(scratch), nbytes, status, _lib.raw_stream(q))
+                    layout.address, scale, N, S, E, type_code, address(gk), address(gv), address(scratch), nbytes, status, _lib.raw_stream(q))
             if rc:
                 _lib.check(rc, "e3b_attention_bwd_src")
         gbias = None

@@ -81,7 +81,7 @@ def _aligned_wide(t: torch.Tensor) -> torch.Tensor:
 def _flat_rows(x: torch.Tensor, dim: int, name: str) -> torch.Tensor:
     if x.dim() < 1 or x.shape[-1] != dim:
         torch._assert(False, f"Incorrect last dimension for {name}")
-    if x.dim() == 2 and x.is_contiguous() and not _lib.is_tracing():      # (a tracer has to see the calls: its next input may lie otherwise)
+    if x.dim() == 2 and x.is_contiguous():
         return x
     return x.reshape(-1, dim).contiguous() if dim > 0 else x.reshape(x.shape[:-1].numel(), 0)
 
@@ -132,7 +132,6 @@ def _row_plan(wides, narrows, back, ins, outs, width: int, narrow: int):
 
 
 def _rms_norm(x, weight, fours: int, eps: float, tbl, inv, _channels) -> torch.Tensor:
-    torch._assert(x.shape[1] == tbl.shape[0], "Incorrect last dimension for x")      # (of a traced call: checked nowhere else)
     h = torch.empty_like(x)
     with _lib.device_of(x):
         rc = _lib.core().e3b_rms_norm_fwd(x.data_ptr(), _lib.address(weight), tbl.data_ptr(), inv.data_ptr(), inv.shape[0], fours, eps, h.data_ptr(),
@@ -145,6 +144,10 @@ def _rms_norm(x, weight, fours: int, eps: float, tbl, inv, _channels) -> torch.T
 class _RMSNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, fours, eps, *tables):
+        # a traced call comes here with its next input: what `RMSNorm.forward` saw was another one
+        if x.shape[1] != tables[0].shape[0]:
+            torch._assert(False, "Incorrect last dimension for x")
+        x = x.contiguous()
         ctx.save_for_backward(x, weight)
         ctx.meta = (tables, fours, eps)
         return _rms_norm(x, weight, fours, eps, *tables)
@@ -259,14 +262,12 @@ def _gate_items(back, const, forth, ins, outs, width: int, narrow: int):
 def _norm_gate(residual, y, w_post, scale, w_pre, shape, eps: float, *tables):
     sizes, plan = shape
     wide, narrow, in_tbl, out_tbl, _, _, in_inv, out_inv = tables
-    if residual.shape != (y.shape[0], out_tbl.shape[0]) or y.shape[1] != in_tbl.shape[0] or residual.dtype != y.dtype:      # (a traced call)
-        torch._assert(False, "residual and y do not fit the module")
     z = torch.empty_like(residual)
     h = torch.empty_like(residual) if w_pre is not None else None
     with _lib.device_of(y):
         rc = _lib.core().e3b_norm_gate_residual_fwd(
             residual.data_ptr(), y.data_ptr(), w_post.data_ptr(), scale.data_ptr(), _lib.address(w_pre), wide.data_ptr(), narrow.data_ptr(),
-            in_tbl.data_ptr(), out_tbl.data_ptr(), in_inv.data_ptr(), out_inv.data_ptr(), sizes, plan, eps, z.data_ptr(), _lib.address(h), y.shape[0],
+            in_tbl.data_ptr(), out_tbl.data_ptr(), in_inv.data_ptr(), out_inv.data_ptr(), sizes.address, 0 if plan is None else plan.address, eps, z.data_ptr(), _lib.address(h), y.shape[0],
             _lib.element_type(y), _lib.raw_stream(y))
     if rc:
         _lib.check(rc, "e3b_norm_gate_residual_fwd")
@@ -276,6 +277,10 @@ def _norm_gate(residual, y, w_post, scale, w_pre, shape, eps: float, *tables):
 class _NormGateFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, residual, y, w_post, scale, w_pre, shape, eps, *tables):
+        # (a traced call comes here with its next inputs)
+        if residual.shape != (y.shape[0], tables[3].shape[0]) or y.shape[1] != tables[2].shape[0] or residual.dtype != y.dtype:
+            torch._assert(False, "residual and y do not fit the module")
+        residual, y = residual.contiguous(), y.contiguous()
         ctx.save_for_backward(residual, y, w_post, scale, w_pre)
         ctx.meta = (tables, shape, eps)
         ctx.set_materialize_grads(False)
@@ -301,7 +306,7 @@ class _NormGateFunction(torch.autograd.Function):
         with _lib.device_of(y):
             rc = core.e3b_norm_gate_residual_bwd(
                 residual.data_ptr(), y.data_ptr(), address(grad_z), address(grad_h), w_post.data_ptr(), scale.data_ptr(), address(w_pre),
-                *(t.data_ptr() for t in tables), sizes, eps, address(g_residual), address(gy), address(params), address(scratch), nbytes, rows,
+                *(t.data_ptr() for t in tables), sizes.address, eps, address(g_residual), address(gy), address(params), address(scratch), nbytes, rows,
                 _lib.element_type(y), _lib.raw_stream(y))
         if rc:
             _lib.check(rc, "e3b_norm_gate_residual_bwd")
@@ -385,7 +390,11 @@ class NormGateResidual(torch.nn.Module):
         if residual.dtype != y.dtype:
             raise TypeError(f"residual and y must have one type, got {residual.dtype} and {y.dtype}")
         _lib.element_type(y, "y")
-        buffers, w_post, scale, w_pre = self._buffers, self.weight_post, self.scale, self.weight_pre
+        buffers, parameters = self._buffers, self._parameters
+        try:
+            w_post, scale, w_pre = parameters["weight_post"], parameters["scale"], parameters["weight_pre"]
+        except KeyError:      # provided by something else
+            w_post, scale, w_pre = self.weight_post, self.scale, self.weight_pre
         _on_device_of(y, self, buffers["_in"], residual, w_post, scale, w_pre)
         (din, dout), sizes = self._dims, self._sizes
         # vectors of 16 bytes if the row falls into such

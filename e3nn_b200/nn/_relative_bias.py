@@ -18,8 +18,6 @@ from .. import _lib
 
 def _distance_buckets(pos, edge_src, edge_dst, shift, squares):
     E = edge_src.shape[0]
-    if pos.shape[1] != 3 or edge_dst.shape != (E,) or (shift is not None and shift.shape != (E, 3)):      # (of a traced call: checked nowhere else)
-        torch._assert(False, "Incorrect shape for pos, edge_src, edge_dst or shift")
     out = torch.empty(E, dtype=torch.int32, device=pos.device)
     with _lib.device_of(pos):
         rc = _lib.core().e3b_distance_buckets(pos.data_ptr(), edge_src.data_ptr(), edge_dst.data_ptr(), _lib.address(shift), squares.data_ptr(),
@@ -33,8 +31,11 @@ class _DistanceBucketsFunction(torch.autograd.Function):
     """What a tracer records: whole numbers have no derivatives."""
 
     @staticmethod
-    def forward(ctx, *args):
-        out = _distance_buckets(*args)
+    def forward(ctx, pos, edge_src, edge_dst, shift, squares):
+        E = edge_src.shape[0]
+        if pos.shape[1] != 3 or edge_dst.shape != (E,) or (shift is not None and shift.shape != (E, 3)):      # (of its next graph)
+            torch._assert(False, "Incorrect shape for pos, edge_src, edge_dst or shift")
+        out = _distance_buckets(pos, edge_src, edge_dst, shift, squares)
         ctx.mark_non_differentiable(out)
         return out
 
@@ -133,7 +134,9 @@ class RelativeBias(torch.nn.Module):
     def forward(self, buckets: torch.Tensor) -> torch.Tensor:
         if not buckets.is_cuda:
             raise NotImplementedError("RelativeBias runs on CUDA tensors only")
-        weight = self.weight
+        weight = self._parameters.get("weight")
+        if weight is None:      # provided by something else
+            weight = self.weight
         if weight.get_device() != buckets.get_device():
             raise RuntimeError(f"Expected all tensors to be on the same device, but weight is on {weight.device} and buckets on {buckets.device}")
         if buckets.dtype != torch.int32:
