@@ -71,22 +71,22 @@ def _attend(c: _Call, keep: bool):
 
 
 class _AttentionFunction(torch.autograd.Function):
-    """Every tensor of a call is an argument: what the backward pass reads again is watched for changes in between, and a traced call
-    takes its next graph."""
+    """What the backward pass reads again is saved, so that changes in between are noticed.  ``edges``: rowptr, edge_src, perm, buckets and the
+    transpose in one tuple; for a tracer, whose replay brings other graphs, one by one."""
 
     @staticmethod
-    def forward(ctx, module, *tensors):
-        c = module._checked(*tensors)
+    def forward(ctx, module, q, k, v, bias, weight, *edges):
+        c = module._checked(q, k, v, bias, weight, *(edges if len(edges) > 1 else edges[0]))
         out, out32, stats = _attend(c, True)
         ctx.save_for_backward(c.q, c.k, c.v, c.bias, c.weight, out32, stats, c.rowptr, c.src, c.perm, c.buckets, c.perm_t, c.rowptr_t)
-        ctx.call = (c.vec, c.layout, c.qk_tbl, c.v_tbl, c.scale, c.edges)
+        ctx.call = (c.vec, c.layout, c.qk_tbl, c.v_tbl, c.scale, c.edges, len(edges))
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         q, k, v, bias, weight, out32, stats, rowptr, src, perm, buckets, perm_t, rowptr_t = ctx.saved_tensors
-        vec, layout, qk_tbl, v_tbl, scale, E = ctx.call
+        vec, layout, qk_tbl, v_tbl, scale, E, others = ctx.call
         _, H, _, _, dqk, dv = list(layout)
         N, S, dev, type_code, core, address = q.shape[0], k.shape[0], q.device, _lib.element_type(q), _lib.core(), _lib.address
         _, need_k, need_v, need_bias, need_weight = ctx.needs_input_grad[1:6]
@@ -131,7 +131,7 @@ class _AttentionFunction(torch.autograd.Function):
         gbias = None
         if need_bias:
             gbias = bias_table_grad(da, buckets, bias.shape[0], torch.float32) if buckets is not None else da
-        return None, gq, gk if need_k else None, gv if need_v else None, gbias, gweight, *(None,) * 6
+        return None, gq, gk if need_k else None, gv if need_v else None, gbias, gweight, *(None,) * others
 
 
 class NeighborAttention(torch.nn.Module):
@@ -193,11 +193,11 @@ class NeighborAttention(torch.nn.Module):
         """
         if transpose is not None and len(transpose) != 2:
             torch._assert(False, "Incorrect shape for transpose")
-        tensors = (q, k, v, bias, edge_weight, rowptr, edge_src, perm, buckets, *(transpose or (None, None)))
+        edges = (rowptr, edge_src, perm, buckets, *(transpose or (None, None)))
         if _lib.wants_function(q, k, v, bias, edge_weight):
-            out = _AttentionFunction.apply(self, *tensors)
+            out = _AttentionFunction.apply(self, q, k, v, bias, edge_weight, *(edges if _lib.is_tracing() else (edges,)))
         else:
-            out = _attend(self._checked(*tensors), False)[0]
+            out = _attend(self._checked(q, k, v, bias, edge_weight, *edges), False)[0]
         if check_indices:
             _lib.check_status(q.device, "NeighborAttention")
         return out

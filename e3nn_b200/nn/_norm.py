@@ -131,10 +131,10 @@ def _row_plan(wides, narrows, back, ins, outs, width: int, narrow: int):
     return _lib.HostInts(flat)
 
 
-def _rms_norm(x, weight, fours: int, eps: float, tbl, inv, _channels) -> torch.Tensor:
+def _rms_norm(x, weight, fours: int, eps: float, num_blocks: int, tbl, inv, _channels) -> torch.Tensor:
     h = torch.empty_like(x)
     with _lib.device_of(x):
-        rc = _lib.core().e3b_rms_norm_fwd(x.data_ptr(), _lib.address(weight), tbl.data_ptr(), inv.data_ptr(), inv.shape[0], fours, eps, h.data_ptr(),
+        rc = _lib.core().e3b_rms_norm_fwd(x.data_ptr(), _lib.address(weight), tbl.data_ptr(), inv.data_ptr(), num_blocks, fours, eps, h.data_ptr(),
                                           x.shape[0], x.shape[1], _lib.element_type(x), _lib.raw_stream(x))
     if rc:
         _lib.check(rc, "e3b_rms_norm_fwd")
@@ -143,14 +143,16 @@ def _rms_norm(x, weight, fours: int, eps: float, tbl, inv, _channels) -> torch.T
 
 class _RMSNormFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, fours, eps, *tables):
-        # a traced call comes here with its next input: what `RMSNorm.forward` saw was another one
-        if x.shape[1] != tables[0].shape[0]:
+    def forward(ctx, x, weight, module):
+        tables, fours, eps = module._tables(), module._fours, module.eps
+        # a traced call comes here with its next input: what `RMSNorm.forward` saw was another one.  (No shapes of the tables: to a tracer
+        # they are tensors from outside.)
+        if x.shape[1] != module._dim:
             torch._assert(False, "Incorrect last dimension for x")
         x = x.contiguous()
         ctx.save_for_backward(x, weight)
         ctx.meta = (tables, fours, eps)
-        return _rms_norm(x, weight, fours, eps, *tables)
+        return _rms_norm(x, weight, fours, eps, module._num_blocks, *tables)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -172,7 +174,7 @@ class _RMSNormFunction(torch.autograd.Function):
                                        _lib.element_type(x), _lib.raw_stream(x))
         if rc:
             _lib.check(rc, "e3b_rms_norm_bwd")
-        return gx, gw, *(None,) * 5
+        return gx, gw, None
 
 
 class RMSNorm(torch.nn.Module):
@@ -189,7 +191,7 @@ class RMSNorm(torch.nn.Module):
         if not self.eps >= 0.0:
             raise ValueError(f"eps must not be negative, got {eps}")
         blocks = _blocks(self.irreps_in)
-        self._dim = self.irreps_in.dim
+        self._dim, self._num_blocks = self.irreps_in.dim, len(blocks)
         self._fours = int(_fours(blocks))
         if self._dim > (8192 if self._fours else 4096):
             raise _lib.E3BError(f"rows of {self._dim} columns are not supported, at most 4096, 8192 where no vector of four straddles two blocks")
@@ -206,20 +208,23 @@ class RMSNorm(torch.nn.Module):
     def __repr__(self) -> str:
         return f"{self.__class__.__name__}({self.irreps_in}, eps={self.eps})"
 
+    def _tables(self):
+        buffers = self._buffers
+        return buffers["_tbl"], buffers["_inv_bits"], buffers["_channels"]
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if not x.is_cuda:
             raise NotImplementedError("RMSNorm runs on CUDA tensors only")
-        buffers, weight = self._buffers, self.weight
-        tables = (buffers["_tbl"], buffers["_inv_bits"], buffers["_channels"])
+        tables, weight = self._tables(), self.weight
         _on_device_of(x, self, tables[0], weight)
         _lib.element_type(x, "x")
         rows = _aligned_wide(_flat_rows(x, self._dim, "x"))
         _lib.check_earlier(x)
         weight = _fp32(weight)
         if _lib.wants_function(rows, weight):
-            out = _RMSNormFunction.apply(rows, weight, self._fours, self.eps, *tables)
+            out = _RMSNormFunction.apply(rows, weight, self)
         else:
-            out = _rms_norm(rows, weight, self._fours, self.eps, *tables)
+            out = _rms_norm(rows, weight, self._fours, self.eps, self._num_blocks, *tables)
         return out if x.dim() == 2 else out.reshape(x.shape)
 
 
@@ -276,9 +281,10 @@ def _norm_gate(residual, y, w_post, scale, w_pre, shape, eps: float, *tables):
 
 class _NormGateFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, residual, y, w_post, scale, w_pre, shape, eps, *tables):
+    def forward(ctx, residual, y, w_post, scale, w_pre, module, key):
+        tables, shape, eps = module._tables(key), module._sizes[key], module.eps
         # (a traced call comes here with its next inputs)
-        if residual.shape != (y.shape[0], tables[3].shape[0]) or y.shape[1] != tables[2].shape[0] or residual.dtype != y.dtype:
+        if residual.shape != (y.shape[0], module._dims[1]) or y.shape[1] != module._dims[0] or residual.dtype != y.dtype:
             torch._assert(False, "residual and y do not fit the module")
         residual, y = residual.contiguous(), y.contiguous()
         ctx.save_for_backward(residual, y, w_post, scale, w_pre)
@@ -292,7 +298,7 @@ class _NormGateFunction(torch.autograd.Function):
         residual, y, w_post, scale, w_pre = ctx.saved_tensors
         tables, (sizes, plan), eps = ctx.meta
         if grad_z is None and grad_h is None:
-            return (None,) * 15
+            return (None,) * 7
         core, rows, address = _lib.core(), y.shape[0], _lib.address
         grad_z, grad_h = (None if g is None else _aligned(g.contiguous(), sizes[0]) for g in (grad_z, grad_h))
         g_residual = torch.empty_like(residual) if ctx.needs_input_grad[0] else None
@@ -311,7 +317,7 @@ class _NormGateFunction(torch.autograd.Function):
         if rc:
             _lib.check(rc, "e3b_norm_gate_residual_bwd")
         gw = params.split([n_in, n_out, n_out]) if params is not None else (None, None, None)
-        return (g_residual, gy, gw[0], gw[1], gw[2] if w_pre is not None else None, *(None,) * 10)
+        return (g_residual, gy, gw[0], gw[1], gw[2] if w_pre is not None else None, None, None)
 
 
 class NormGateResidual(torch.nn.Module):
@@ -382,6 +388,10 @@ class NormGateResidual(torch.nn.Module):
     def __repr__(self) -> str:
         return f"{self.__class__.__name__}({self.irreps_in} -> {self.irreps_out}, eps={self.eps})"
 
+    def _tables(self, key):
+        buffers = self._buffers
+        return [buffers[name] for name in self._table_names[key]]
+
     def forward(self, residual: torch.Tensor, y: torch.Tensor):
         if not (residual.is_cuda and y.is_cuda):
             raise NotImplementedError("NormGateResidual runs on CUDA tensors only")
@@ -403,10 +413,11 @@ class NormGateResidual(torch.nn.Module):
                 break
         r, x = _aligned(_flat_rows(residual, dout, "residual"), key[0]), _aligned(_flat_rows(y, din, "y"), key[0])
         _lib.check_earlier(y)
-        tables = (*(buffers[name] for name in self._table_names[key]),)
         args = (r, x, _fp32(w_post), _fp32(scale), _fp32(w_pre))
-        apply = _NormGateFunction.apply if _lib.wants_function(*args) else _norm_gate
-        z, h = apply(*args, sizes[key], self.eps, *tables)
+        if _lib.wants_function(*args):
+            z, h = _NormGateFunction.apply(*args, self, key)
+        else:
+            z, h = _norm_gate(*args, sizes[key], self.eps, *self._tables(key))
         if residual.dim() == 2:
             return (z, h) if self.pre_norm else z
         return (z.reshape(residual.shape), h.reshape(residual.shape)) if self.pre_norm else z.reshape(residual.shape)
