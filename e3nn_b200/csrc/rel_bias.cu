@@ -135,11 +135,13 @@ __global__ void __launch_bounds__(kSumThreads, 1) bias_bwd_kernel(const T* __res
             for (int u = 0; u < U; ++u) {
                 if (e0 + u * slices >= count) break;
                 const int at = b[u] - first;
-                if (at < 0 || at >= here) {
-                    if (!WINDOWS || b[u] < 0 || b[u] >= num_buckets) bad = true;
+                float x[HV], y[HV];
+                if (at < 0 || at >= here) {      // bad, if there is anything to add: slots of no row may name any bucket
+                    g[u].unpack(y);
+#pragma unroll
+                    for (int i = 0; i < HV; ++i) bad = bad || (y[i] != 0.0f && (!WINDOWS || b[u] < 0 || b[u] >= num_buckets));
                     continue;
                 }
-                float x[HV], y[HV];
                 Packed<float, HV> sum;
                 sum.load(mine + at * width);
                 sum.unpack(x);

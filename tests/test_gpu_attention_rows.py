@@ -471,3 +471,17 @@ def test_no_rows_and_no_sources(layout, per_edge, perm):
     with pytest.raises(IndexError):
         e3nn_b200.check_status()
     assert not out.any()
+
+
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+@pytest.mark.parametrize("per_edge", [False, True])
+def test_padding_may_hold_any_bucket(layout, per_edge):
+    """Buckets of slots that belong to no row are looked at in neither direction."""
+    t = make(*LAYOUTS[layout][:2], DEGREES["ragged"], torch.float32, per_edge, "table", True, front=9, behind=40)
+    want = run(module(layout, torch.float32, t), t)
+    e3nn_b200.check_status()
+    padded = {**t, "buckets": t["buckets"].clone()}
+    padded["buckets"][:9], padded["buckets"][-40:] = 2 ** 31 - 1, -1
+    got = run(module(layout, torch.float32, t), padded)
+    e3nn_b200.check_status()
+    assert all(torch.equal(got[n], want[n]) for n in got)
