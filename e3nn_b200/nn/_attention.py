@@ -93,7 +93,7 @@ class _AttentionFunction(torch.autograd.Function):
         grad = grad.contiguous()
         if not _fits(grad, vec):
             grad = grad.clone()
-        per_node = src is not None and (need_k or need_v)
+        per_node = src is not None and (need_k or need_v) and S > 0
         per_edge = src is None and (need_k or need_v)
         gq = torch.empty(N, dqk, dtype=q.dtype, device=dev)
         gk = torch.empty(S, dqk, dtype=q.dtype, device=dev) if need_k or need_v else None
@@ -119,7 +119,8 @@ class _AttentionFunction(torch.autograd.Function):
             if perm_t is None:
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("the edges by source cannot be built while a graph is captured: give NeighborAttention transpose=csr_from_dst(edge_src, k.shape[0])")
-                perm_t, rowptr_t = csr_from_dst(src, S)
+                # (slots of no row may name any source, bad ones of rows have been reported: neither adds anything, wherever it is sorted to)
+                perm_t, rowptr_t = csr_from_dst(src.clamp(0, S - 1), S)
             nbytes = core.e3b_attention_bwd_src_scratch_bytes(S, E, dqk, dv)
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
             with _lib.device_of(q):

@@ -467,10 +467,12 @@ def test_no_rows_and_no_sources(layout, per_edge, perm):
         return
     t = make(irreps, heads, [3, 4], torch.float32, False, None, True)                         # sources out of range: there is none
     mod = bnn.NeighborAttention(irreps, irreps, heads).cuda()
-    out = mod(t["q"], t["k"][:0], t["v"][:0], t["rowptr"], t["src"], edge_weight=t["weight"])
+    q, k, v = t["q"].requires_grad_(), t["k"][:0].requires_grad_(), t["v"][:0].requires_grad_()
+    out = mod(q, k, v, t["rowptr"], t["src"], edge_weight=t["weight"])
+    gq, gk, gv = torch.autograd.grad(out, (q, k, v), t["g"])
     with pytest.raises(IndexError):
         e3nn_b200.check_status()
-    assert not out.any()
+    assert not out.any() and not gq.any() and gk.shape == gv.shape == k.shape
 
 
 @pytest.mark.parametrize("layout", list(LAYOUTS))
@@ -484,4 +486,29 @@ def test_padding_may_hold_any_bucket(layout, per_edge):
     padded["buckets"][:9], padded["buckets"][-40:] = 2 ** 31 - 1, -1
     got = run(module(layout, torch.float32, t), padded)
     e3nn_b200.check_status()
+    assert all(torch.equal(got[n], want[n]) for n in got)
+
+
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+def test_padding_may_hold_any_source(layout):
+    """So may the sources of such slots, where the backward pass builds the edges by source itself; a bad source in a row is reported and left out there too."""
+    t = make(*LAYOUTS[layout][:2], DEGREES["ragged"], torch.float32, False, "table", True, front=9, behind=40)
+    mod = module(layout, torch.float32, t)
+    want = run(mod, t)
+    padded = {**t, "src": t["src"].clone()}
+    padded["src"][:9], padded["src"][-40:-20], padded["src"][-20:] = -1, 23, 2 ** 40
+    got = run(mod, padded, transposed=False)
+    e3nn_b200.check_status()
+    compare(got, formula(*LAYOUTS[layout][:1], *LAYOUTS[layout][:2], t, torch.float32))
+    assert all(torch.equal(got[n], want[n]) for n in ("out", "q", "bias", "weight"))
+    bad = torch.tensor([12, 30], device="cuda")
+    t["weight"][bad] = 1.0
+    without = {**t, "weight": t["weight"].clone()}
+    without["weight"][bad] = 0.0
+    t["src"][bad] = torch.tensor([-1, 23], device="cuda")
+    got = run(mod, t, transposed=False)
+    with pytest.raises(IndexError):
+        e3nn_b200.check_status()
+    without["src"] = t["src"].clamp(0, 22)
+    want = run(mod, without)
     assert all(torch.equal(got[n], want[n]) for n in got)
