@@ -4,12 +4,14 @@
 //   out[n]_h = sum_e softmax_e(a[e, h]) v[src]_h           over the edges e of row n; a row without edges is zero
 //
 // One pass: the maximum and the sum of a row run along with the sum of the values.  k and v are rows of nodes (gathered by src) or of
-// edges.  An edge moves (dqk + dv) elements from L2 or HBM and costs 2 (dqk + dv) operations on a row of q that no other edge shares
-// its k with, so the matrix units have nothing to do; what counts is bytes in flight (fp32) and instructions an edge (16 bits).
+// edges.  An edge moves (dqk + dv) elements from L2 or HBM and costs 2 (dqk + dv) operations.  All edges of a row share its q, but each has a
+// row of k and of v of its own, gathered for a few operations an element, so these run on the FP32 pipe.  What counts is bytes in flight in
+// fp32; in 16 bits latency at 12 to 16 warps an SM (42 to 45 % of the issue slots are used) and reads of the ring: a row of 1,024 columns in
+// bf16 and 8 heads takes 36 shared-memory wavefronts where 16 are the least, one of 576 in fp32 36 for 18.
 // Layout of heads, ring, split into parts and their joining: attention.cuh.  Logits, statistics and sums are fp32; the output is
 // rounded once.  2,097,152 edges over 65,536 nodes, 576 columns, 8 heads: fp32 1,126 us = 8.6 TB/s of gathered rows (302 MB of k and v, L2
-// holds 126 MB), bf16 910 us; 425,984 edges of 1,024 columns in bf16 265 us = 6.6 TB/s; one query over 50,021 edges of 576 columns in bf16
-// 31 us and 22 us for the join.
+// holds 126 MB), bf16 890 us; 425,984 edges of 1,024 columns in bf16 265 us = 6.6 TB/s; one query over 50,021 edges of 576 columns in bf16
+// 33 us and 22 us for the join, in fp32 55 and 26 us.
 #include "attention.cuh"
 
 namespace e3b {
@@ -44,7 +46,8 @@ __device__ __forceinline__ void finish_row(const FwdArgs& a, const Sums<VEC, V, 
 }
 
 // Rows by loads into registers, for rows that cannot be copied in units of 16 bytes and for heads of several warps: the k and v rows of
-// several edges (about 80 registers) are under way before the first is used.  (On the bf16 case above, before the ring: 1,065 us.)
+// several edges (about 80 registers) are under way before the first is used.  425,984 edges of 576 columns on 16 heads (four channels a head)
+// in bf16 507 us where the ring takes 192 us for twice the bytes in fp32: latency.
 template <typename T, int VEC, int V>
 __global__ void __launch_bounds__(256) attn_fwd_kernel(const FwdArgs a) {
     extern __shared__ float smem[];

@@ -6,8 +6,8 @@
 // delta is taken from the unrounded fp32 output: dp - delta cancels, and in a row with one edge it is exactly zero.
 // k and v per edge: their gradients are written here, row by row.  k and v per node: p and da of every edge are kept and
 // attention_bwd_src.cu adds the terms of every source over its outgoing edges.  Like the forward kernel with three products
-// a column in place of two: 425,984 edges of 1,024 columns in bf16 450 us = 3.9 TB/s of gathered rows (instructions; twelve warps an SM, whose
-// registers hold q, g and the sums of q's gradient); 150,001 edges with k and v per edge, 180 columns in fp32, 102 us (432 MB read and written).
+// a column in place of two: 425,984 edges of 1,024 columns in bf16 450 us = 3.9 TB/s of gathered rows (latency and shared-memory reads at 42 %
+// of the issue slots: the registers, q, g and the sums of q's gradient, allow twelve warps an SM), in fp32 1,127 us; 150,001 edges with k and v per edge, 180 columns in fp32, 102 us (432 MB read and written).
 #include "attention.cuh"
 
 namespace e3b {

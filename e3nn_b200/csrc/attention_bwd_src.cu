@@ -4,7 +4,7 @@
 // with p and da from attention_bwd.cu.  The edges of a source come from the CSR by source (perm, rowptr: the stable sort of
 // edge_src), so every row is summed in a fixed order, without atomics (which would move two rows an edge twice, read and
 // written).  The same parts, lanes and ring as in the forward kernel, with the edge's p and da as a third copy: 425,984 edges of
-// 1,024 columns in bf16 211 us = 8.3 TB/s of gathered rows.
+// 1,024 columns in bf16 211 us = 8.3 TB/s of gathered rows, in fp32 432 us.
 #include "attention.cuh"
 
 namespace e3b {

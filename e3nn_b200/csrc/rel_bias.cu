@@ -4,14 +4,15 @@
 //   bias[e, h] = table[bucket[e], h];     grad_table[b, h] = sum over the edges of bucket b of grad[e, h]
 //
 // Buckets: squared distances and squared thresholds are compared in fp64, where the fp32 inputs and their differences are
-// exact to 2^-53, so that a distance next to a border falls on the side that it is on.  Bound by HBM (28 bytes of edge data in,
-// 4 out; the positions come from L2).
-// 2,097,152 edges: 27 us (92 MB of edge data, 3.4 TB/s).
-// Bias: bound by the write of 4 H bytes an edge (2 H in 16 bits): 2,097,152 edges of 16 heads in fp32 36 us = 4.0 TB/s.
+// exact to 2^-53, so that a distance next to a border falls on the side that it is on.  28 bytes of edge data in, 4 out, and two
+// positions from L2 that wait for the indices: 2,097,152 edges 27 us (67 MB, 2.5 TB/s), bound by those dependent loads.
+// Bias: writes 4 H bytes an edge (2 H in 16 bits): 2,097,152 edges of 16 heads in fp32 36 us = 4.0 TB/s, in bf16 36 us too: a table entry is
+// looked up per output.
 // Gradient: every thread keeps its heads and walks edges of its own; it adds into cells of a table in shared memory that no other
 // thread touches, so the order of the additions is fixed by the grid; slices, then thread blocks, are added in order.  No atomics.
 // Bound by the loads in flight: a table per slice limits the threads, sixteen 16-byte loads each make up for it: 2,097,152 edges, 16 heads, 64 buckets
-// in fp32 60 us = 2.4 TB/s (one head a thread: 98 us); 8 heads, 256 buckets in bf16, where only 26 slices fit, 79 us.
+// in fp32 60 us = 2.4 TB/s (one head a thread: 98 us), in bf16 54 us; 8 heads, 256 buckets in bf16, where only 26 slices fit, 79 us.  Tables that do
+// not fit (more than 1,664 buckets of 32 heads) are taken in windows of buckets, each of which reads all edges.
 #include <algorithm>
 
 #include "common.cuh"

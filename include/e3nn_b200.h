@@ -329,7 +329,8 @@ int e3b_norm_gate_residual_bwd(const void* residual, const void* y, const void* 
  * e3b_distance_buckets: buckets[e] = number of squared thresholds (ascending, at most 1,023) that are <= |pos[src] - pos[dst] + shift|^2,
  * in fp64 from fp32 coordinates; shift may be NULL; an index out of range sets *status = 2 and gives bucket 0.
  * e3b_relative_bias_fwd: bias[e, h] = table[buckets[e], h], both of `type`; a bucket out of range sets *status = 2 and gives 0.
- * e3b_relative_bias_bwd: grad_table[b, h] = sum over the edges of bucket b of grad_bias[e, h], in fp32 and in a fixed order, with
+ * e3b_relative_bias_bwd: grad_table[b, h] = sum over the edges of bucket b of grad_bias[e, h], in fp32 and in a fixed order (an edge whose
+ * bucket is out of range is left out, and sets *status = 2 if its grad_bias is not zero), with
  * e3b_relative_bias_scratch_bytes(...) bytes of scratch; grad_bias is 16-byte aligned.  A table has fewer than 2^31 - 32 entries.
  */
 int e3b_distance_buckets(const float* pos, const int64_t* edge_src, const int64_t* edge_dst, const float* shift,
@@ -359,7 +360,7 @@ int e3b_relative_bias_bwd(const void* grad_bias, const int32_t* buckets, int num
  *
  * e3b_attention_bwd: grad_q [num_dst, dqk]; k and v per edge (edge_src NULL): grad_k, grad_v per edge (both or neither).  Optional, per
  * edge: share [num_edges, heads rounded up to even, 2] {softmax, its gradient's logit part} (16-byte aligned), grad_logit [num_edges, heads]
- * (the gradient of bias), edge_dst [num_edges] (destination, -1: none; needed with share and, where perm is given, with any of the others:
+ * (the gradient of bias), edge_dst [num_edges] (destination, below 0: none; needed with share and, where perm is given, with any of the others:
  * an edge that perm does not name in a row gets zeros, one that it names twice sets *status = 4), grad_weight [num_edges] (needs grad_logit).
  * e3b_attention_bwd_src: grad_k and grad_v of nodes from share and edge_dst and the CSR by source (e3b_csr_from_dst of
  * edge_src: src_perm, src_rowptr).  All sums have a fixed order.
