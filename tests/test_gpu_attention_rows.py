@@ -512,3 +512,28 @@ def test_padding_may_hold_any_source(layout):
     without["src"] = t["src"].clamp(0, 22)
     want = run(mod, without)
     assert all(torch.equal(got[n], want[n]) for n in got)
+
+
+@pytest.mark.parametrize("kind", ["per node", "per edge", "per edge, permuted"])
+def test_gradients_beyond_32_bit_offsets(kind):
+    """Keys and values whose last rows start past 2^31 elements, and their gradients; all rows but forty belong to nothing."""
+    irreps, heads, d, E = "256x0e", 8, 256, 40
+    S = 2 ** 31 // d + 1000
+    gen = torch.Generator().manual_seed(0)
+    small = {n: torch.randn(r, d, generator=gen).bfloat16().cuda() for n, r in (("q", 2), ("k", E), ("v", E), ("g", 2))}
+    k, v = torch.zeros(S, d, dtype=torch.bfloat16, device="cuda"), torch.zeros(S, d, dtype=torch.bfloat16, device="cuda")
+    rows = torch.arange(S - E, S, device="cuda")
+    k[rows], v[rows] = small["k"], small["v"]
+    q, k, v = small["q"].clone().requires_grad_(), k.requires_grad_(), v.requires_grad_()
+    rowptr, perm = torch.tensor([0, 17, E], device="cuda"), None
+    if kind == "per edge":
+        rowptr = rowptr + S - E
+    elif kind == "per edge, permuted":
+        perm = torch.arange(S, device="cuda").roll(E)
+    mod = bnn.NeighborAttention(irreps, irreps, heads).cuda()
+    out = mod(q, k, v, rowptr, rows if kind == "per node" else None, perm=perm)
+    gq, gk, gv = torch.autograd.grad(out, (q, k, v), small["g"])
+    e3nn_b200.check_status()
+    t = {**small, "rowptr": torch.tensor([0, 17, E], device="cuda"), "src": None, "perm": None, "bias": None, "buckets": None, "weight": None}
+    compare({"out": out.detach(), "q": gq, "k": gk[-E:], "v": gv[-E:]}, formula(irreps, irreps, heads, t, torch.bfloat16))
+    assert not gk[:-E].any() and not gv[:-E].any()
